@@ -1,10 +1,11 @@
 /*
  * kermac_amd.h -- C ABI of libkermac_amd.so, the MI355X (gfx950) implementation
- * of kermac's fused distance hot path.
+ * of kermac's fused distance hot path, and of attention beside it.
  *
  * Everything here is plain C: device pointers travel as `const float *`, the
  * HIP stream as `void *` (a hipStream_t; NULL = the default stream).  All
- * tensors are fp32 and already resident in device memory.  Launches are
+ * tensors are fp32 (attention: also fp16 and bf16, as `const void *`) and
+ * already resident in device memory.  Launches are
  * asynchronous on the given stream; no entry point synchronises or allocates.
  *
  * Every entry point returns 0 on success.  A non-zero return is one of the
@@ -25,7 +26,7 @@
 extern "C" {
 #endif
 
-#define KMC_ABI_VERSION 2
+#define KMC_ABI_VERSION 3
 
 enum kmc_status {
     KMC_OK = 0,
@@ -453,6 +454,39 @@ typedef struct kmc_matrix_coefficients_params {
     int64_t out_split_stride;
 } kmc_matrix_coefficients_params;
 int kmc_matrix_times_coefficients(const kmc_matrix_coefficients_params *params, void *stream);
+
+/* ---- attention: exp(scale <q, k>) with rows divided by their sums, times values ----
+ * No counterpart in the reference; the operands are tensors of rank 4 in fp32, fp16 or bf16, all of one type, the last
+ * dimension contiguous and every other one with a stride of its own, in elements (0: broadcast).  Sums, maxima and
+ * exponentials are fp32 throughout. */
+enum kmc_element_type { KMC_FP32 = 0, KMC_FP16 = 1, KMC_BF16 = 2 };
+
+typedef struct kmc_attention_params {
+    int32_t type;               /* kmc_element_type */
+    int32_t flags;              /* KMC_FLAG_FORCE_SCALAR_ACCESS or 0 */
+    int32_t l, m, n;            /* batch entries, queries and keys of each */
+    int32_t h, g;               /* heads of queries, heads of keys and values; h a multiple of g */
+    int32_t k, o;               /* features of queries and keys, of values; 1 .. 256 */
+    float scale;
+    const void *q; int64_t q_ls, q_ms, q_hs;                    /* [l, m, h, k] */
+    const void *key; int64_t key_ls, key_ns, key_gs;            /* [l, n, g, k] */
+    const void *value; int64_t value_ls, value_ns, value_gs;    /* [l, n, g, o] */
+    void *out; int64_t out_ls, out_ms, out_hs;                  /* [l, m, h, o] */
+    float *lse;                 /* [l, m, h] contiguous, log sum exp of a row (-inf for one without keys), or NULL */
+    const int32_t *key_lengths; /* [l]: the keys of an entry that take part, taken as 0 .. n where outside; or NULL: all */
+    const uint8_t *key_mask; int64_t key_mask_ls, key_mask_ns;  /* [l, n]: not 0 where a key takes part; or NULL */
+    /* prefix_n > 0 or causal: every query also meets prefix_n keys common to all entries, and query i of an entry is token
+     * key_lengths - m + i of its own keys, of which it meets those up to itself (key_lengths needed, no key_mask). */
+    int32_t prefix_n, causal;
+    const void *prefix_key; int64_t prefix_key_ns, prefix_key_gs;       /* [prefix_n, g, k] */
+    const void *prefix_value; int64_t prefix_value_ns, prefix_value_gs; /* [prefix_n, g, o] */
+    /* What kmc_attention_workspace_bytes asks for, 16-byte aligned: partial results, where the keys are cut over workgroups
+     * or the prefix is walked once for all entries.  Less than that, or NULL: one pass over the keys per tile of rows. */
+    void *workspace; int64_t workspace_bytes;
+} kmc_attention_params;
+int kmc_attention(const kmc_attention_params *params, void *stream);
+/* Bytes of workspace that kmc_attention uses for this call (0: none). */
+int kmc_attention_workspace_bytes(const kmc_attention_params *params, int64_t *bytes);
 
 /* ---- run-time compilation (stands in for cuda.core Program / ObjectCode:
  *      src/kermac/module_cache/module_cache.py:13-51, 219-239) ---- */

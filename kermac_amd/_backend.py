@@ -17,7 +17,7 @@ from typing import List, Optional, Sequence, Tuple
 # KERMAC_AMD_LIBRARY points at another build of the same ABI (e.g. an experimental one).
 LIB_PATH = Path(os.environ.get("KERMAC_AMD_LIBRARY") or Path(__file__).resolve().parent / "_lib" / "libkermac_amd.so")
 
-ABI_VERSION = 2
+ABI_VERSION = 3
 
 # enum kmc_status
 OK = 0
@@ -53,6 +53,10 @@ FLAG_DIRECT_PANELS = 2048
 FLAG_GRAM_OWN_CENTRE = 4096
 FLAG_PRODUCT_PIECES = 8192
 FLAG_PRODUCT_ACCUMULATE = 16384
+# enum kmc_element_type
+FP32 = 0
+FP16 = 1
+BF16 = 2
 SAMPLE_BYTES = 1024             # KMC_SAMPLE_BYTES: what the sample in front of a matrix-core launch takes of the workspace
 
 _float_p = c_void_p  # device pointers are passed as integers
@@ -118,6 +122,26 @@ class MatrixCoefficientsParams(Structure):
     ]
 
 
+class AttentionParams(Structure):
+    """struct kmc_attention_params"""
+    _fields_ = [
+        ("type", c_int32), ("flags", c_int32),
+        ("l", c_int32), ("m", c_int32), ("n", c_int32), ("h", c_int32), ("g", c_int32), ("k", c_int32), ("o", c_int32),
+        ("scale", c_float),
+        ("q", c_void_p), ("q_ls", c_int64), ("q_ms", c_int64), ("q_hs", c_int64),
+        ("key", c_void_p), ("key_ls", c_int64), ("key_ns", c_int64), ("key_gs", c_int64),
+        ("value", c_void_p), ("value_ls", c_int64), ("value_ns", c_int64), ("value_gs", c_int64),
+        ("out", c_void_p), ("out_ls", c_int64), ("out_ms", c_int64), ("out_hs", c_int64),
+        ("lse", c_void_p),
+        ("key_lengths", c_void_p),
+        ("key_mask", c_void_p), ("key_mask_ls", c_int64), ("key_mask_ns", c_int64),
+        ("prefix_n", c_int32), ("causal", c_int32),
+        ("prefix_key", c_void_p), ("prefix_key_ns", c_int64), ("prefix_key_gs", c_int64),
+        ("prefix_value", c_void_p), ("prefix_value_ns", c_int64), ("prefix_value_gs", c_int64),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
 # Every exported symbol of include/kermac_amd.h: name -> (restype, argtypes).
 SIGNATURES = {
     "kmc_abi_version": (ctypes.c_int, []),
@@ -141,6 +165,8 @@ SIGNATURES = {
     "kmc_kernel_coefficients_workspace_bytes": (ctypes.c_int, [POINTER(KernelCoefficientsParams), POINTER(c_int64)]),
     "kmc_kernel_times_coefficients_has_variant": (ctypes.c_int, [c_int32, c_int32]),
     "kmc_kernel_times_coefficients_jit": (ctypes.c_int, [c_void_p, POINTER(KernelCoefficientsParams), c_void_p]),
+    "kmc_attention": (ctypes.c_int, [POINTER(AttentionParams), c_void_p]),
+    "kmc_attention_workspace_bytes": (ctypes.c_int, [POINTER(AttentionParams), POINTER(c_int64)]),
     "kmc_jit_compile": (ctypes.c_int, [
         c_char_p, c_char_p,
         ctypes.c_int, POINTER(c_char_p), POINTER(c_char_p),
@@ -289,6 +315,21 @@ def matrix_times_coefficients(params: MatrixCoefficientsParams, stream: int) -> 
 
 def kernel_times_coefficients_has_variant(inner_operator: int, inner_power: int) -> bool:
     return bool(library().kmc_kernel_times_coefficients_has_variant(inner_operator, inner_power))
+
+
+def attention(params: AttentionParams, stream: int) -> None:
+    status = library().kmc_attention(byref(params), stream)
+    if status != OK:
+        check(status)
+
+
+def attention_workspace_bytes(params: AttentionParams) -> int:
+    """Bytes of workspace that kmc_attention uses for these parameters (0: none)."""
+    needed = c_int64(0)
+    status = library().kmc_attention_workspace_bytes(byref(params), byref(needed))
+    if status != OK:
+        check(status)
+    return needed.value
 
 
 def dispatch_rules() -> dict:

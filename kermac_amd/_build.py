@@ -47,6 +47,7 @@ HOST_SOURCES = [
     "host/launcher_table.cpp",
     "host/norm_gradient_launch.cpp",
     "host/kernel_coefficients_launch.cpp",
+    "host/attention_launch.cpp",
 ]
 
 
@@ -80,6 +81,9 @@ def _jobs():
     inst = CSRC / "kernels" / "gram_bf16_kernel_inst.hip"
     for same_points in (0, 1):
         jobs.append((inst, OBJ_DIR / f"gram_bf16_kernel_inst_{same_points}.o", [f"-DKMC_SAME_POINTS={same_points}"]))
+    inst = CSRC / "kernels" / "attention_inst.hip"
+    for element_type in (0, 1, 2):
+        jobs.append((inst, OBJ_DIR / f"attention_inst_{element_type}.o", [f"-DKMC_ATT_TYPE={element_type}"]))
     for rel in EXTRA_DEVICE_SOURCES:
         src = CSRC / rel
         jobs.append((src, OBJ_DIR / (src.stem + ".o"), []))

@@ -1,0 +1,227 @@
+// C-ABI entry points for attention.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "host_common.hpp"
+#include "../kernels/attention_args.hpp"
+
+using namespace kmc_host;
+
+namespace kmc_host {
+#define KMC_DECLARE_ATTENTION(type) hipError_t launch_attention_forward_##type(const kmc::AttentionArgs &, int, bool, hipStream_t);
+KMC_DECLARE_ATTENTION(0)
+KMC_DECLARE_ATTENTION(1)
+KMC_DECLARE_ATTENTION(2)
+#undef KMC_DECLARE_ATTENTION
+}  // namespace kmc_host
+
+namespace {
+
+constexpr int MAX_WIDTH = 256;
+constexpr int MAX_KEYS = 0x7fffffff - 1024;         // a tile behind the last key still has a number
+constexpr int MAX_SLOTS = 128;
+
+int element_size(int type) { return type == KMC_FP32 ? 4 : 2; }
+
+// Whether rows can be read and written 16 bytes at a time: the address, and the stride of every dimension that is walked.
+struct Layout {
+    int size;
+    bool aligned = true;
+    void operand(const void *p, int width)
+    {
+        if (p) aligned = aligned && aligned16(p) && width * size % 16 == 0;
+    }
+    void stride(int extent, int64_t stride)
+    {
+        if (extent > 1) aligned = aligned && stride * size % 16 == 0;
+    }
+};
+
+int check_extents(int type, int l, int m, int n, int h, int g, int k, int o, float scale)
+{
+    if (type != KMC_FP32 && type != KMC_FP16 && type != KMC_BF16) return fail(KMC_ERR_INVALID_ARGUMENT, "element type %d is none of 0, 1, 2", type);
+    if (l < 0 || m < 0 || n < 0 || h < 0 || g < 0) return fail(KMC_ERR_INVALID_ARGUMENT, "negative extent l=%d m=%d n=%d h=%d g=%d", l, m, n, h, g);
+    if (n > MAX_KEYS) return fail(KMC_ERR_INVALID_ARGUMENT, "n=%d is beyond %d keys", n, MAX_KEYS);
+    if (h > 0 && (g == 0 || h % g != 0)) return fail(KMC_ERR_INVALID_ARGUMENT, "h=%d is no multiple of g=%d", h, g);
+    if (k < 1 || k > MAX_WIDTH || o < 1 || o > MAX_WIDTH)
+        return fail(KMC_ERR_INVALID_ARGUMENT, "k=%d and o=%d must be in 1 .. %d", k, o, MAX_WIDTH);
+    if (!std::isfinite(scale)) return fail(KMC_ERR_INVALID_ARGUMENT, "scale must be finite");
+    // rows of a head of keys over the batch, and rows times heads over the batch, are numbered in 31 bits
+    if (static_cast<double>(l) * m * h > 2.0e9) return fail(KMC_ERR_INVALID_ARGUMENT, "l m h = %.0f is beyond 2e9 rows", static_cast<double>(l) * m * h);
+    return KMC_OK;
+}
+
+// The scale to base 2 is kept positive, so that the largest score has the largest product; its sign moves into the queries.
+void set_scale(float scale, float *scale_log2, float *query_factor)
+{
+    const float to_base_2 = std::fabs(scale) * 1.4426950408889634f;
+    *scale_log2 = to_base_2 > 0.0f ? to_base_2 : 1.0f;
+    *query_factor = to_base_2 > 0.0f ? (scale < 0.0f ? -1.0f : 1.0f) : 0.0f;
+}
+
+// Workgroups that one launch wants before its keys are cut no further: two per CU.
+constexpr int WANTED_WORKGROUPS = 512;
+constexpr int ROWS_OF_OWN_KEYS = 32;                // up to here every wave walks keys of its own
+constexpr int ROWS_PER_WORKGROUP = 128;
+constexpr int MIN_KEYS_OWN = 128, MIN_KEYS_SHARED = 256;
+
+// false: more workgroups than a launch holds
+bool plan_job(kmc::AttentionJob *job, int first_segment, int last_segment, int64_t entries, int64_t rows, int heads, int keys, bool may_cut)
+{
+    job->first_segment = first_segment;
+    job->last_segment = last_segment;
+    job->rows = static_cast<int>(rows);
+    job->own_keys = rows <= ROWS_OF_OWN_KEYS;
+    job->row_tiles = job->own_keys ? 1 : static_cast<int>((rows + ROWS_PER_WORKGROUP - 1) / ROWS_PER_WORKGROUP);
+    const int64_t base = entries * heads * job->row_tiles;
+    int64_t splits = 1;
+    if (may_cut && base > 0) {
+        const int least = job->own_keys ? MIN_KEYS_OWN : MIN_KEYS_SHARED;
+        splits = std::min<int64_t>({(WANTED_WORKGROUPS + base / 2) / base, (static_cast<int64_t>(keys) + least - 1) / least, MAX_SLOTS / 2});
+        splits = std::max<int64_t>(splits, 1);
+    }
+    job->splits = static_cast<int>(splits);
+    const int64_t workgroups = base * splits;
+    if (workgroups > 0x7fffff00ll / 2) return false;
+    job->workgroups = static_cast<int>(workgroups);
+    job->grid = static_cast<int>((workgroups + 7) / 8 * 8);
+    job->slot = 0;
+    job->partial = 0;
+    return true;
+}
+
+struct Plan {
+    kmc::AttentionArgs args;
+    bool aligned, empty;
+    int64_t bytes;              // of workspace
+};
+
+int64_t partial_bytes(const kmc::AttentionArgs &args) { return args.slots * args.rows_total * (4ll * args.partial_width + 4); }
+
+int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
+{
+    if (!p) return fail(KMC_ERR_INVALID_ARGUMENT, "null parameter block");
+    const int status = check_extents(p->type, p->l, p->m, p->n, p->h, p->g, p->k, p->o, p->scale);
+    if (status != KMC_OK) return status;
+    if (p->prefix_n < 0 || p->prefix_n > MAX_KEYS) return fail(KMC_ERR_INVALID_ARGUMENT, "prefix_n=%d is outside 0 .. %d", p->prefix_n, MAX_KEYS);
+    if (p->causal && !p->key_lengths) return fail(KMC_ERR_INVALID_ARGUMENT, "causal needs key_lengths");
+    if ((p->causal || p->prefix_n > 0) && p->key_mask) return fail(KMC_ERR_INVALID_ARGUMENT, "key_mask does not go with a prefix");
+    const int64_t strides[] = {p->q_ls, p->q_ms, p->q_hs, p->key_ls, p->key_ns, p->key_gs, p->value_ls, p->value_ns, p->value_gs,
+                               p->out_ls, p->out_ms, p->out_hs, p->key_mask_ls, p->key_mask_ns, p->prefix_key_ns, p->prefix_key_gs,
+                               p->prefix_value_ns, p->prefix_value_gs};
+    for (const int64_t stride : strides)
+        if (stride < 0) return fail(KMC_ERR_INVALID_ARGUMENT, "negative stride");
+    plan->bytes = 0;
+    plan->empty = p->l == 0 || p->m == 0 || p->h == 0;
+    if (plan->empty) return KMC_OK;
+    if (!p->q || !p->out) return fail(KMC_ERR_INVALID_ARGUMENT, "null q / out pointer");
+    if (p->n > 0 && (!p->key || !p->value)) return fail(KMC_ERR_INVALID_ARGUMENT, "null key / value pointer");
+    if (p->prefix_n > 0 && (!p->prefix_key || !p->prefix_value)) return fail(KMC_ERR_INVALID_ARGUMENT, "null prefix_key / prefix_value pointer");
+
+    kmc::AttentionArgs &args = plan->args;
+    args = kmc::AttentionArgs{};
+    args.q = p->q; args.q_ls = p->q_ls; args.q_ms = p->q_ms; args.q_hs = p->q_hs;
+    args.out = p->out; args.out_ls = p->out_ls; args.out_ms = p->out_ms; args.out_hs = p->out_hs;
+    args.lse = p->lse;
+    args.m = p->m; args.g = p->g; args.r = p->h / p->g; args.k = p->k; args.o = p->o;
+    set_scale(p->scale, &args.scale_log2, &args.query_factor);
+    args.rows_total = static_cast<int64_t>(p->l) * p->m * p->h;
+    args.partial_width = (p->o + 3) / 4 * 4;
+
+    const bool prefixed = p->prefix_n > 0;
+    kmc::AttentionKeys &prefix = args.keys[0], &own = args.keys[prefixed ? 1 : 0];
+    if (prefixed) {
+        prefix.k = p->prefix_key; prefix.k_ns = p->prefix_key_ns; prefix.k_gs = p->prefix_key_gs;
+        prefix.v = p->prefix_value; prefix.v_ns = p->prefix_value_ns; prefix.v_gs = p->prefix_value_gs;
+        prefix.n = p->prefix_n;
+    }
+    own.k = p->key; own.k_ls = p->key_ls; own.k_ns = p->key_ns; own.k_gs = p->key_gs;
+    own.v = p->value; own.v_ls = p->value_ls; own.v_ns = p->value_ns; own.v_gs = p->value_gs;
+    own.lengths = p->key_lengths;
+    own.mask = p->key_mask; own.mask_ls = p->key_mask_ls; own.mask_ns = p->key_mask_ns;
+    own.n = p->n;
+    own.causal = p->causal != 0;
+
+    const int64_t rows = static_cast<int64_t>(p->m) * args.r;
+    bool fits = true;
+    if (with_workspace && prefixed) {
+        // the prefix as one problem of the rows of all entries, the entries' own keys as another
+        fits = plan_job(&args.job[0], 0, 1, 1, p->l * rows, p->g, p->prefix_n, true);
+        fits = fits && plan_job(&args.job[1], 1, 2, p->l, rows, p->g, p->n, true);
+        args.job[0].partial = args.job[1].partial = 1;
+        args.job[1].slot = args.job[0].splits;
+        args.slots = args.job[0].splits + args.job[1].splits;
+    } else {
+        fits = plan_job(&args.job[0], 0, prefixed ? 2 : 1, p->l, rows, p->g, p->n, with_workspace);
+        if (args.job[0].splits > 1) {
+            args.job[0].partial = 1;
+            args.slots = args.job[0].splits;
+        }
+    }
+    if (!fits) return fail(KMC_ERR_INVALID_ARGUMENT, "more workgroups than a launch holds");
+    plan->bytes = partial_bytes(args);
+
+    Layout layout{element_size(p->type)};
+    layout.operand(p->q, p->k);
+    layout.operand(p->out, p->o);
+    layout.stride(p->l, p->q_ls); layout.stride(p->m, p->q_ms); layout.stride(p->h, p->q_hs);
+    layout.stride(p->l, p->out_ls); layout.stride(p->m, p->out_ms); layout.stride(p->h, p->out_hs);
+    if (p->n > 0) {
+        layout.operand(p->key, p->k);
+        layout.operand(p->value, p->o);
+        layout.stride(p->l, p->key_ls); layout.stride(p->n, p->key_ns); layout.stride(p->g, p->key_gs);
+        layout.stride(p->l, p->value_ls); layout.stride(p->n, p->value_ns); layout.stride(p->g, p->value_gs);
+    }
+    if (prefixed) {
+        layout.operand(p->prefix_key, p->k);
+        layout.operand(p->prefix_value, p->o);
+        layout.stride(p->prefix_n, p->prefix_key_ns); layout.stride(p->g, p->prefix_key_gs);
+        layout.stride(p->prefix_n, p->prefix_value_ns); layout.stride(p->g, p->prefix_value_gs);
+    }
+    plan->aligned = layout.aligned && !(p->flags & KMC_FLAG_FORCE_SCALAR_ACCESS);
+    return KMC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kmc_attention_workspace_bytes(const kmc_attention_params *params, int64_t *bytes)
+{
+    if (!bytes) return fail(KMC_ERR_INVALID_ARGUMENT, "bytes: null pointer");
+    Plan plan;
+    const int status = prepare(params, true, &plan);
+    if (status != KMC_OK) return status;
+    *bytes = plan.bytes;
+    return KMC_OK;
+}
+
+int kmc_attention(const kmc_attention_params *params, void *stream)
+{
+    Plan plan;
+    int status = prepare(params, true, &plan);
+    if (status != KMC_OK) return status;
+    if (plan.empty) return KMC_OK;
+    if (plan.bytes > 0 && (!params->workspace || params->workspace_bytes < plan.bytes)) {
+        status = prepare(params, false, &plan);
+        if (status != KMC_OK) return status;
+    }
+    status = require_gfx950();
+    if (status != KMC_OK) return status;
+    kmc::AttentionArgs &args = plan.args;
+    if (plan.bytes > 0) {
+        if (!aligned16(params->workspace)) return fail(KMC_ERR_INVALID_ARGUMENT, "workspace is not aligned to 16 bytes");
+        args.partial_out = static_cast<float *>(params->workspace);
+        args.partial_lse = args.partial_out + args.slots * args.rows_total * args.partial_width;
+    }
+    const int width = std::max(params->k, params->o);
+    const hipStream_t on = static_cast<hipStream_t>(stream);
+    const hipError_t e = params->type == KMC_FP32   ? launch_attention_forward_0(args, width, plan.aligned, on)
+                         : params->type == KMC_FP16 ? launch_attention_forward_1(args, width, plan.aligned, on)
+                                                    : launch_attention_forward_2(args, width, plan.aligned, on);
+    if (e != hipSuccess) return fail_hip(e, "attention launch");
+    return KMC_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,563 @@
+// Attention: a kernel matrix exp(scale <q, k>) whose rows are divided by their sums, times values.
+//
+//   s[m, n] = scale sum_k q[m, k] k[n, k],   lse[m] = log sum_n exp s[m, n],   out[m, o] = sum_n exp(s[m, n] - lse[m]) v[n, o]
+//
+// over the keys n that take part.  One pass over keys and values: a running maximum and a running sum per query, the
+// output rescaled when the maximum grows (both in fp32; exponentials to base 2 with log2(e) folded into the scale).
+//
+// Queries of the heads that share a head of keys are the rows of one problem: row r is query r / R of head r % R
+// (R heads per head of keys), so keys and values are read once for all of them.  Queries of all batch entries
+// against one common set of keys are one problem in the same way.
+//
+// The products run on the 32 x 32 matrix instruction with the scores transposed, s^T[n, row] = K Q^T: a lane then owns one
+// row of the softmax (two lanes, for alternating groups of four keys), its statistics are one register each, and the
+// registers that hold s^T are, in the order in which they stand, the operand of out^T[o, row] = V^T P^T if the
+// contraction takes the keys of a step as 4 h + {0..3}, 8 + 4 h + {0..3} for half wave h.  V^T comes from row-major tiles in
+// LDS by the transposing read (16-bit types) or by 32-bit reads (fp32).  P is rounded to the type of the values: the error of
+// a sum of many rounded weights stays below the rounding of the result itself; fp32 keeps every bit.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "attention_args.hpp"
+
+namespace kmc {
+
+typedef float att_f32x16 __attribute__((ext_vector_type(16)));
+typedef float att_f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned att_u32x4 __attribute__((ext_vector_type(4)));
+typedef short att_s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned long long att_u64;
+
+template <typename T> struct AttVector { typedef T type __attribute__((ext_vector_type(8))); };
+template <typename T> using att_vec8 = typename AttVector<T>::type;
+
+constexpr float ATT_LOG2_E = 1.4426950408889634f;
+constexpr float ATT_LN_2 = 0.6931471805599453f;
+
+// c += a b over 16 k: lane l holds row (of a) or column (of b) l % 32 and 8 of the k, those of half wave l / 32.
+__device__ __forceinline__ att_f32x16 att_mma(att_vec8<__bf16> a, att_vec8<__bf16> b, att_f32x16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ att_f32x16 att_mma(att_vec8<_Float16> a, att_vec8<_Float16> b, att_f32x16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ att_f32x16 att_mma(att_vec8<float> a, att_vec8<float> b, att_f32x16 c)
+{
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+
+// Register i of a 32 x 32 result holds row att_row(i, half wave) of column lane % 32.
+__device__ __forceinline__ constexpr int att_row(int i, int half) { return 8 * (i / 4) + 4 * half + i % 4; }
+
+// The sum or maximum of a value over the two lanes of a column.
+__device__ __forceinline__ float att_other_half(float x) { return __shfl_xor(x, 32); }
+
+// Rows of D elements of a tile in LDS.  Read as they are (16 bytes of a row per lane): 16 bytes of padding put consecutive rows
+// into consecutive groups of four banks.  Read transposed: a 16-bit read touches 4 rows x 64 bytes per half wave, which 64
+// bytes of padding put side by side; an fp32 read touches a row each at a distance of 4 rows, 32 banks apart with 32 bytes.
+template <typename T, int DP> constexpr int ATT_STRIDE = DP + 16 / static_cast<int>(sizeof(T));
+template <typename T, int DP> constexpr int ATT_STRIDE_T = DP + (sizeof(T) == 2 ? 32 : 8);
+
+template <typename T, int DP>
+__device__ __forceinline__ att_vec8<T> att_read_row(const T *tile, int stride, int row, int k)
+{
+    const T *p = tile + row * stride + k;
+    att_vec8<T> x;
+    if constexpr (sizeof(T) == 2) {
+        x = *reinterpret_cast<const att_vec8<T> *>(p);
+    } else {
+        const att_f32x4 low = reinterpret_cast<const att_f32x4 *>(p)[0], high = reinterpret_cast<const att_f32x4 *>(p)[1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { x[j] = low[j]; x[4 + j] = high[j]; }
+    }
+    return x;
+}
+
+// Lane l gets column `column` + l % 32 of the 16 rows from `row` on, in the order 4 h + {0..3}, 8 + 4 h + {0..3}.
+template <typename T>
+__device__ __forceinline__ att_vec8<T> att_read_transposed(const T *tile, int stride, int row, int column, int lane)
+{
+    const int half = lane >> 5;
+    att_vec8<T> x;
+    if constexpr (sizeof(T) == 2) {
+        const T *p = tile + (row + 4 * half + (lane % 16) / 4) * stride + column + 16 * (lane / 16 % 2) + 4 * (lane % 4);
+        typedef __attribute__((address_space(3))) att_s16x4 lds_s16x4;
+        union { att_s16x4 part[2]; att_vec8<T> whole; } u;
+        u.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p));
+        u.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 8 * stride));
+        x = u.whole;
+    } else {
+        const T *p = tile + (row + 4 * half) * stride + column + lane % 32;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { x[j] = p[j * stride]; x[4 + j] = p[(8 + j) * stride]; }
+    }
+    return x;
+}
+
+// Eight fp32 values of a result, registers 8 step .. 8 step + 7, rounded to the operand type.
+template <typename T>
+__device__ __forceinline__ att_vec8<T> att_operand(const att_f32x16 &x, int step)
+{
+    att_vec8<T> y;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = static_cast<T>(x[8 * step + j]);
+    return y;
+}
+
+// 16 bytes of a row of `width` elements from element `at` on; what lies behind the row reads as zero.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ att_u32x4 att_load16(const T *row, int at, int width)
+{
+    constexpr int COUNT = 16 / sizeof(T);
+    att_u32x4 x = {0, 0, 0, 0};
+    if constexpr (ALIGNED) {
+        if (at < width) x = *reinterpret_cast<const att_u32x4 *>(row + at);       // width is a multiple of COUNT
+    } else {
+        union { T value[COUNT]; att_u32x4 whole; } u;
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j) u.value[j] = at + j < width ? row[at + j] : static_cast<T>(0.0f);
+        x = u.whole;
+    }
+    return x;
+}
+
+// Eight elements of a row, for an operand that is kept in registers.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ att_vec8<T> att_load8(const T *row, int at, int width)
+{
+    union { att_u32x4 part[sizeof(T) / 2]; att_vec8<T> whole; } u;
+#pragma unroll
+    for (unsigned j = 0; j < sizeof(T) / 2; ++j) u.part[j] = att_load16<T, ALIGNED>(row, at + j * (16 / static_cast<int>(sizeof(T))), width);
+    return u.whole;
+}
+
+// A tile of ROWS rows of DP elements on its way from memory to LDS through the registers of THREADS threads.
+template <typename T, int DP, int ROWS, int THREADS, bool ALIGNED>
+struct AttTile {
+    static constexpr int CHUNK = 16 / sizeof(T);                    // elements of a 16-byte piece
+    static constexpr int CHUNKS = DP / CHUNK;                       // pieces of a row
+    static constexpr int PER_THREAD = ROWS * CHUNKS / THREADS;
+    static_assert(ROWS * CHUNKS % THREADS == 0 && THREADS % CHUNKS == 0, "whole rows per step");
+    static constexpr int ROW_STEP = THREADS / CHUNKS;
+    att_u32x4 held[PER_THREAD];
+
+    // Rows 0 .. rows - 1 of base (rows of `width` elements, `stride` apart); rows behind them read as zero.
+    __device__ __forceinline__ void load(const T *base, i64 stride, int rows, int width, int thread)
+    {
+        const int row = thread / CHUNKS, at = thread % CHUNKS * CHUNK;
+        const T *p = base + row * stride;
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; ++j) {
+            held[j] = att_u32x4{0, 0, 0, 0};
+            if (row + j * ROW_STEP < rows) held[j] = att_load16<T, ALIGNED>(p, at, width);
+            p += ROW_STEP * stride;
+        }
+    }
+
+    // Rows whose bit in `kept` is not set are stored as zeros.
+    template <int STRIDE>
+    __device__ __forceinline__ void store(T *tile, int thread, bool all_kept, att_u64 kept) const
+    {
+        const int row = thread / CHUNKS, at = thread % CHUNKS * CHUNK;
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; ++j) {
+            att_u32x4 x = held[j];
+            if (!all_kept && !(kept >> (row + j * ROW_STEP) & 1)) x = att_u32x4{0, 0, 0, 0};
+            *reinterpret_cast<att_u32x4 *>(tile + (row + j * ROW_STEP) * STRIDE + at) = x;
+        }
+    }
+};
+
+// One bit per key n0 .. n0 + 63: the key exists and takes part.  The same in all waves of a workgroup.
+__device__ __forceinline__ att_u64 att_kept_keys(const AttentionKeys &keys, int entry, int n0, int end, int lane)
+{
+    const int n = n0 + lane;
+    bool kept = n < end;
+    if (kept && keys.mask) kept = keys.mask[entry * keys.mask_ls + n * keys.mask_ns] != 0;
+    return __ballot(kept);
+}
+
+__device__ __forceinline__ int att_length(const AttentionKeys &keys, int entry)
+{
+    if (!keys.lengths) return keys.n;
+    const int length = keys.lengths[entry];
+    return length < 0 ? 0 : length < keys.n ? length : keys.n;
+}
+
+// Writes of a wave to LDS are seen by its other lanes: LDS serves a wave in order, the compiler has to keep that order.
+__device__ __forceinline__ void att_wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// What a wave carries along the keys for its 32 rows.
+template <int DP>
+struct AttState {
+    att_f32x16 out[DP / 32];
+    float top, sum;              // the largest score so far and the sum of this lane's exponentials below it, to base 2
+};
+
+// One tile of KT keys in LDS against the 32 rows whose queries are in `query`.  `kept` has a bit per key for this lane's row.
+template <typename T, int DP, int KT>
+__device__ __forceinline__ void att_forward_tile(AttState<DP> &state, const att_vec8<T> (&query)[DP / 16], const T *keys, const T *values, float scale_log2,
+                                                 att_u64 kept, int lane)
+{
+    const int half = lane >> 5;
+    att_f32x16 s[KT / 32];
+#pragma unroll
+    for (int b = 0; b < KT / 32; ++b) {
+        s[b] = att_f32x16{0};
+#pragma unroll
+        for (int step = 0; step < DP / 16; ++step)
+            s[b] = att_mma(att_read_row<T, DP>(keys, ATT_STRIDE<T, DP>, 32 * b + lane % 32, 16 * step + 8 * half), query[step], s[b]);
+    }
+    const att_u64 all = KT == 64 ? ~0ull : (1ull << KT) - 1;
+    if (!__all((kept & all) == all)) {
+#pragma unroll
+        for (int b = 0; b < KT / 32; ++b) {
+            const unsigned mine = static_cast<unsigned>(kept >> (32 * b)) >> (4 * half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][i] = mine >> att_row(i, 0) & 1 ? s[b][i] : -__builtin_inff();
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < KT / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+    top = fmaxf(top, att_other_half(top));
+    top = fmaxf(state.top, top * scale_log2);
+    const float base = top == -__builtin_inff() ? 0.0f : top;          // no key of this row yet: every exponential below is 0
+    const float shrink = __builtin_amdgcn_exp2f(state.top - base);
+    state.top = top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int b = 0; b < KT / 32; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale_log2, -base));
+            sum += s[b][i];
+        }
+    state.sum = state.sum * shrink + sum;
+    if (!__all(shrink == 1.0f)) {
+#pragma unroll
+        for (int o = 0; o < DP / 32; ++o) state.out[o] *= shrink;
+    }
+#pragma unroll
+    for (int b = 0; b < KT / 32; ++b)
+#pragma unroll
+        for (int step = 0; step < 2; ++step) {
+            const att_vec8<T> weights = att_operand<T>(s[b], step);
+#pragma unroll
+            for (int o = 0; o < DP / 32; ++o)
+                state.out[o] = att_mma(att_read_transposed(values, ATT_STRIDE_T<T, DP>, 32 * b + 16 * step, 32 * o, lane), weights, state.out[o]);
+        }
+}
+
+// Keys [begin, end) of a segment for split `split` of `splits`, in whole tiles.
+__device__ __forceinline__ void att_range(int length, int tile, int split, int splits, int *begin, int *end)
+{
+    const int tiles = (length + tile - 1) / tile;
+    const i64 per_split = static_cast<i64>((tiles + splits - 1) / splits) * tile;
+    const i64 first = split * per_split;
+    *begin = first < length ? static_cast<int>(first) : length;
+    *end = length - *begin < per_split ? length : static_cast<int>(*begin + per_split);
+}
+
+// The low `count` bits, count clamped to 0 .. 64.
+__device__ __forceinline__ att_u64 att_low_bits(int count)
+{
+    return count >= 64 ? ~0ull : count <= 0 ? 0ull : (1ull << count) - 1;
+}
+
+// Where row `row` of a problem's entry lives.
+struct AttRow { int entry, query, head; };
+__device__ __forceinline__ AttRow att_find_row(const AttentionArgs &args, int first_entry, int g, int row)
+{
+    const int token = row / args.r;
+    AttRow at;
+    at.head = g * args.r + row % args.r;
+    at.entry = first_entry + token / args.m;
+    at.query = token % args.m;
+    return at;
+}
+
+template <typename T, int DP>
+struct AttForwardShape {
+    // Rows per workgroup and keys per tile where waves share the keys; waves and keys per tile where each wave has keys of its own.
+    static constexpr int ROW_WAVES = 4;
+    static constexpr int SHARED_KEYS = DP * sizeof(T) <= 512 ? 64 : 32;
+    static constexpr int OWN_KEYS = 32;
+    static constexpr int OWN_WAVES = DP * sizeof(T) <= 512 ? 4 : 2;      // 1 KB rows: two waves' tiles fill LDS
+    static constexpr int WAVES_PER_SIMD = DP * sizeof(T) <= 256 ? 2 : 1;
+    static constexpr int TILE_BYTES_PER_KEY = (ATT_STRIDE<T, DP> + ATT_STRIDE_T<T, DP>) * static_cast<int>(sizeof(T));
+    static constexpr int SHARED_BYTES = SHARED_KEYS * TILE_BYTES_PER_KEY;
+    static constexpr int OWN_BYTES = OWN_WAVES * OWN_KEYS * TILE_BYTES_PER_KEY;
+    static constexpr int JOIN_BYTES = (OWN_WAVES - 1) * (DP * 32 + 64) * 4 + 512;
+    static constexpr int BYTES_1 = SHARED_BYTES > OWN_BYTES ? SHARED_BYTES : OWN_BYTES;
+    static constexpr int BYTES = BYTES_1 > JOIN_BYTES ? BYTES_1 : JOIN_BYTES;
+};
+
+// Writes a wave's 32 rows: the result itself, or a partial result and its lse (to base 2) for att_join.
+template <typename T, int DP, bool ALIGNED>
+__device__ __forceinline__ void att_forward_write(const AttentionArgs &args, const AttentionJob &job, const AttState<DP> &state, float sum, int entry, int g,
+                                                  int row, int split, int lane)
+{
+    if (row >= job.rows) return;
+    const int half = lane >> 5;
+    const AttRow at = att_find_row(args, entry, g, row);
+    const i64 id = (static_cast<i64>(at.entry) * args.m + at.query) * (static_cast<i64>(args.g) * args.r) + at.head;
+    const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;      // a row without keys gets zeros, not a number stays
+    const float lse2 = sum == 0.0f ? -__builtin_inff() : state.top + __builtin_amdgcn_logf(sum);
+    if (job.partial) {
+        const i64 slot = static_cast<i64>(job.slot + split) * args.rows_total + id;
+        if (half == 0) args.partial_lse[slot] = lse2;
+        if (sum == 0.0f) return;                                                    // nobody reads it
+        float *to = args.partial_out + slot * args.partial_width;
+#pragma unroll
+        for (int o = 0; o < DP / 32; ++o)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int column = 32 * o + 8 * q + 4 * half;
+                if (column < args.partial_width) {
+                    const att_f32x4 x = {state.out[o][4 * q] * inverse, state.out[o][4 * q + 1] * inverse, state.out[o][4 * q + 2] * inverse,
+                                         state.out[o][4 * q + 3] * inverse};
+                    *reinterpret_cast<att_f32x4 *>(to + column) = x;
+                }
+            }
+        return;
+    }
+    if (args.lse && half == 0) args.lse[id] = lse2 * ATT_LN_2;
+    T *to = static_cast<T *>(args.out) + at.entry * args.out_ls + at.query * args.out_ms + at.head * args.out_hs;
+#pragma unroll
+    for (int o = 0; o < DP / 32; ++o)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int column = 32 * o + 8 * q + 4 * half;
+            typedef T four __attribute__((ext_vector_type(4)));
+            four x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = static_cast<T>(state.out[o][4 * q + j] * inverse);
+            if (ALIGNED) {
+                if (column < args.o) *reinterpret_cast<four *>(to + column) = x;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (column + j < args.o) to[column + j] = x[j];
+            }
+        }
+}
+
+template <typename T, int DP, bool ALIGNED>
+__device__ __forceinline__ void att_load_queries(const AttentionArgs &args, const AttentionJob &job, int entry, int g, int row, int lane, att_vec8<T> (&query)[DP / 16])
+{
+    const int half = lane >> 5;
+    const AttRow at = att_find_row(args, entry, g, row < job.rows ? row : 0);
+    const T *from = static_cast<const T *>(args.q) + at.entry * args.q_ls + at.query * args.q_ms + at.head * args.q_hs;
+#pragma unroll
+    for (int step = 0; step < DP / 16; ++step) {
+        query[step] = att_load8<T, ALIGNED>(from, 16 * step + 8 * half, args.k);
+        if (args.query_factor != 1.0f)                                              // -1 or 0: exact
+#pragma unroll
+            for (int j = 0; j < 8; ++j) query[step][j] = static_cast<T>(static_cast<float>(query[step][j]) * args.query_factor);
+    }
+}
+
+// A workgroup per (batch entry, head of keys, range of keys, tile of rows).
+//
+// More than 32 rows: ROW_WAVES waves of 32 rows each share the tiles of keys and values.  At most 32 rows (single tokens): reading keys
+// and values is all the work, so every wave walks tiles of its own without waiting for the others, and the waves' results are joined at the end.
+template <typename T, int DP, bool ALIGNED>
+__global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void attention_forward(const AttentionArgs args)
+{
+    typedef AttForwardShape<T, DP> Shape;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[Shape::BYTES];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    // XCD x gets a contiguous part of the list, in which the tiles of rows of one set of keys stand together: they share its L2.
+    int id = blockIdx.x;
+    const bool second = id >= args.job[0].grid;
+    const AttentionJob &job = args.job[second];
+    if (second) id -= args.job[0].grid;
+    id = (id & 7) * (job.grid >> 3) + (id >> 3);
+    if (id >= job.workgroups) return;
+    const int row_tile = id % job.row_tiles;
+    id /= job.row_tiles;
+    const int split = id % job.splits;
+    id /= job.splits;
+    const int g = id % args.g, entry = id / args.g;
+
+    AttState<DP> state;
+#pragma unroll
+    for (int o = 0; o < DP / 32; ++o) state.out[o] = att_f32x16{0};
+    state.top = -__builtin_inff();
+    state.sum = 0.0f;
+    att_vec8<T> query[DP / 16];
+
+    if (!job.own_keys) {
+        constexpr int KT = Shape::SHARED_KEYS;
+        T *key_tile = reinterpret_cast<T *>(lds);
+        T *value_tile = key_tile + KT * ATT_STRIDE<T, DP>;
+        const int first_row = row_tile * 32 * Shape::ROW_WAVES + 32 * wave;
+        const int row = first_row + lane % 32;
+        const bool works = first_row < job.rows;
+        att_load_queries<T, DP, ALIGNED>(args, job, entry, g, row, lane, query);
+        for (int segment = job.first_segment; segment < job.last_segment; ++segment) {
+            const AttentionKeys &keys = args.keys[segment];
+            const int length = att_length(keys, entry);
+            int begin, end;
+            att_range(length, KT, split, job.splits, &begin, &end);
+            // query i of a sequence's last m tokens sees the tokens up to its own
+            int limit = 0x7fffffff;
+            if (keys.causal) {
+                limit = length - args.m + 1 + row / args.r % args.m;
+                int last_row = (row_tile + 1) * 32 * Shape::ROW_WAVES - 1;
+                last_row = last_row < job.rows ? last_row : job.rows - 1;
+                const int last_limit = length - args.m + 1 + last_row / args.r;
+                end = end < last_limit ? end : last_limit;
+            }
+            const T *k = static_cast<const T *>(keys.k) + entry * keys.k_ls + g * keys.k_gs;
+            const T *v = static_cast<const T *>(keys.v) + entry * keys.v_ls + g * keys.v_gs;
+            AttTile<T, DP, KT, 256, ALIGNED> next_k, next_v;
+            if (begin < end) {
+                next_k.load(k + begin * keys.k_ns, keys.k_ns, end - begin, args.k, threadIdx.x);
+                next_v.load(v + begin * keys.v_ns, keys.v_ns, end - begin, args.o, threadIdx.x);
+            }
+            for (int n = begin; n < end; n += KT) {
+                const att_u64 kept = att_kept_keys(keys, entry, n, end, lane);
+                __syncthreads();
+                next_k.template store<ATT_STRIDE<T, DP>>(key_tile, threadIdx.x, true, 0);
+                next_v.template store<ATT_STRIDE_T<T, DP>>(value_tile, threadIdx.x, !keys.mask, kept);
+                __syncthreads();
+                if (n + KT < end) {
+                    const i64 at = n + KT;
+                    next_k.load(k + at * keys.k_ns, keys.k_ns, end - static_cast<int>(at), args.k, threadIdx.x);
+                    next_v.load(v + at * keys.v_ns, keys.v_ns, end - static_cast<int>(at), args.o, threadIdx.x);
+                }
+                if (works) att_forward_tile<T, DP, KT>(state, query, key_tile, value_tile, args.scale_log2, kept & att_low_bits(limit - n), lane);
+            }
+        }
+        if (!works) return;
+        const float sum = state.sum + att_other_half(state.sum);
+        att_forward_write<T, DP, ALIGNED>(args, job, state, sum, entry, g, row, split, lane);
+    } else {
+        constexpr int KT = Shape::OWN_KEYS, WAVES = Shape::OWN_WAVES;
+        T *key_tile = reinterpret_cast<T *>(lds + wave * KT * Shape::TILE_BYTES_PER_KEY);
+        T *value_tile = key_tile + KT * ATT_STRIDE<T, DP>;
+        const int row = lane % 32;                                      // at most 32 rows: one tile
+        if (wave < WAVES) {
+            att_load_queries<T, DP, ALIGNED>(args, job, entry, g, row, lane, query);
+            for (int segment = job.first_segment; segment < job.last_segment; ++segment) {
+                const AttentionKeys &keys = args.keys[segment];
+                const int length = att_length(keys, entry);
+                int begin, end;
+                att_range(length, KT, split, job.splits, &begin, &end);
+                const int limit = keys.causal ? length - args.m + 1 + row / args.r % args.m : 0x7fffffff;
+                const T *k = static_cast<const T *>(keys.k) + entry * keys.k_ls + g * keys.k_gs;
+                const T *v = static_cast<const T *>(keys.v) + entry * keys.v_ls + g * keys.v_gs;
+                AttTile<T, DP, KT, 64, ALIGNED> next_k, next_v;
+                i64 n = begin + wave * KT;
+                if (n < end) {
+                    next_k.load(k + n * keys.k_ns, keys.k_ns, end - static_cast<int>(n), args.k, lane);
+                    next_v.load(v + n * keys.v_ns, keys.v_ns, end - static_cast<int>(n), args.o, lane);
+                }
+                for (; n < end; n += KT * WAVES) {
+                    const att_u64 kept = att_kept_keys(keys, entry, static_cast<int>(n), end, lane);
+                    next_k.template store<ATT_STRIDE<T, DP>>(key_tile, lane, true, 0);
+                    next_v.template store<ATT_STRIDE_T<T, DP>>(value_tile, lane, !keys.mask, kept);
+                    att_wave_sync();
+                    const i64 at = n + KT * WAVES;
+                    if (at < end) {
+                        next_k.load(k + at * keys.k_ns, keys.k_ns, end - static_cast<int>(at), args.k, lane);
+                        next_v.load(v + at * keys.v_ns, keys.v_ns, end - static_cast<int>(at), args.o, lane);
+                    }
+                    att_forward_tile<T, DP, KT>(state, query, key_tile, value_tile, args.scale_log2, kept & att_low_bits(limit - static_cast<int>(n)), lane);
+                    att_wave_sync();
+                }
+            }
+        }
+        // join the waves: sums and outputs below one common maximum, added in the order of the waves
+        float sum = state.sum + att_other_half(state.sum);
+        float *tops = reinterpret_cast<float *>(lds);                   // [WAVES][32], then (WAVES - 1) waves' sums and outputs
+        float *others = tops + 128;
+        __syncthreads();
+        static_assert(WAVES * 32 <= 128, "room for the tops");
+        if (wave < WAVES && lane < 32) tops[wave * 32 + lane] = state.top;
+        __syncthreads();
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, tops[w * 32 + lane % 32]);
+        __syncthreads();
+        const float shrink = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(state.top - top);
+        state.top = top;
+        sum *= shrink;
+#pragma unroll
+        for (int o = 0; o < DP / 32; ++o) state.out[o] *= shrink;
+        if (wave > 0 && wave < WAVES) {
+            float *mine = others + (wave - 1) * (DP * 32 + 64);
+#pragma unroll
+            for (int o = 0; o < DP / 32; ++o)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mine[(16 * o + i) * 64 + lane] = state.out[o][i];
+            mine[DP * 32 + lane] = sum;
+        }
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 0; w < WAVES - 1; ++w) {
+            const float *from = others + w * (DP * 32 + 64);
+#pragma unroll
+            for (int o = 0; o < DP / 32; ++o)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) state.out[o][i] += from[(16 * o + i) * 64 + lane];
+            sum += from[DP * 32 + lane];
+        }
+        att_forward_write<T, DP, ALIGNED>(args, job, state, sum, entry, g, row, split, lane);
+    }
+}
+
+// The partial results of one row, weighted by exp(lse of the part - lse of all).  A wave per row, the parts in their order.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_join(const AttentionArgs args)
+{
+    const int lane = threadIdx.x & 63;
+    const i64 id = static_cast<i64>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (id >= args.rows_total) return;
+    float top = -__builtin_inff();
+    for (int part = lane; part < args.slots; part += 64) top = fmaxf(top, args.partial_lse[part * args.rows_total + id]);
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1) top = fmaxf(top, __shfl_xor(top, step));
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    float sum = 0.0f;
+    float out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int part = 0; part < args.slots; ++part) {
+        const i64 slot = part * args.rows_total + id;
+        const float lse2 = args.partial_lse[slot];
+        if (lse2 == -__builtin_inff()) continue;                        // a part without keys wrote nothing
+        const float weight = __builtin_amdgcn_exp2f(lse2 - base);
+        sum += weight;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (64 * j + lane < args.o) out[j] += weight * args.partial_out[slot * args.partial_width + 64 * j + lane];
+    }
+    const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+    const i64 token = id / (static_cast<i64>(args.g) * args.r);
+    const int head = static_cast<int>(id % (static_cast<i64>(args.g) * args.r));
+    if (args.lse && lane == 0) args.lse[id] = sum == 0.0f ? -__builtin_inff() : (base + __builtin_amdgcn_logf(sum)) * ATT_LN_2;
+    T *to = static_cast<T *>(args.out) + token / args.m * args.out_ls + token % args.m * args.out_ms + head * args.out_hs;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (64 * j + lane < args.o) to[64 * j + lane] = static_cast<T>(out[j] * inverse);
+}
+
+}  // namespace kmc

@@ -1,0 +1,44 @@
+// Arguments of the attention kernels, shared by the device code and the host side that fills them.
+#pragma once
+
+namespace kmc {
+
+typedef long long i64;
+
+// Keys and values of one segment; strides in elements.
+struct AttentionKeys {
+    const void *k, *v;
+    i64 k_ls, k_ns, k_gs, v_ls, v_ns, v_gs;
+    const int *lengths;                     // per batch entry, or null: all n take part
+    const unsigned char *mask;              // per batch entry and key, or null
+    i64 mask_ls, mask_ns;
+    int n;
+    int causal;                             // the queries are the last m of `lengths` tokens
+};
+
+// A list of workgroups: (batch entry, head of keys, range of keys, tile of rows), the tile of rows fastest.
+struct AttentionJob {
+    int first_segment, last_segment;
+    int rows, row_tiles, splits;
+    int slot;                               // of its first partial result
+    int partial, own_keys;
+    int workgroups, grid;                   // grid: workgroups rounded up to a multiple of the 8 XCDs
+};
+
+struct AttentionArgs {
+    const void *q;
+    i64 q_ls, q_ms, q_hs;
+    void *out;
+    i64 out_ls, out_ms, out_hs;
+    float *lse;                             // [l, m, g r], or null
+    AttentionKeys keys[2];
+    AttentionJob job[2];
+    int m, g, r, k, o;
+    float scale_log2;                       // |scale| log2(e), above 0
+    float query_factor;                     // 1; -1 for a negative scale; 0 for a scale of 0
+    float *partial_out, *partial_lse;       // [slots, rows_total, partial_width], [slots, rows_total] to base 2
+    int slots, partial_width;
+    i64 rows_total;                         // l m g r
+};
+
+}  // namespace kmc

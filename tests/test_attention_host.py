@@ -1,0 +1,148 @@
+"""Attention operators without a GPU: what they refuse, and the parameters that they hand to the library."""
+import ctypes
+import math
+import re
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+import kermac_amd as kermac
+from kermac_amd import _backend
+from kermac_amd.attention import _plan_attention
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+def make(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def plan(q, k, v, out=None, scale=None, key_lengths=None, key_mask=None, return_lse=False, prefix=None):
+    return _plan_attention(q, k, v, out, scale, key_lengths, key_mask, return_lse, prefix=prefix, require_device=False)
+
+
+def test_operands_on_the_cpu_are_refused():
+    q = make(1, 2, 2, 8)
+    with pytest.raises(ValueError, match="CUDA device"):
+        kermac.cross_attention(q, q, q)
+    with pytest.raises(ValueError, match="CUDA device"):
+        kermac.prefix_attention(q, q[0], q[0], q, q, torch.zeros(1, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("error, match, change", [
+    (TypeError, "PyTorch tensor", dict(q=3.0)),
+    (TypeError, "PyTorch tensor", dict(k=[1.0])),
+    (TypeError, "dtype", dict(q=make(2, 5, 4, 16, dtype=torch.float64))),
+    (TypeError, "dtype", dict(k=make(2, 7, 2, 16, dtype=torch.bfloat16))),
+    (TypeError, "dtype", dict(v=make(2, 7, 2, 24, dtype=torch.float16))),
+    (ValueError, "3-dimensional or 4-dimensional", dict(q=make(5, 16))),
+    (ValueError, "3-dimensional or 4-dimensional", dict(v=make(1, 2, 7, 2, 24))),
+    (ValueError, "batch size", dict(k=make(3, 7, 2, 16), v=make(3, 7, 2, 24))),
+    (ValueError, "batch size", dict(k=make(1, 7, 2, 16))),
+    (ValueError, "batch size", dict(q=make(1, 5, 4, 16))),
+    (ValueError, "features", dict(k=make(2, 7, 2, 17))),
+    (ValueError, "tokens and heads", dict(v=make(2, 8, 2, 24))),
+    (ValueError, "tokens and heads", dict(v=make(2, 7, 4, 24))),
+    (ValueError, "multiple of the heads", dict(q=make(2, 5, 3, 16))),
+    (ValueError, "multiple of the heads", dict(k=make(2, 7, 0, 16), v=make(2, 7, 0, 24))),
+    (ValueError, "1 .. 256", dict(q=make(2, 5, 4, 257), k=make(2, 7, 2, 257))),
+    (ValueError, "1 .. 256", dict(v=make(2, 7, 2, 0))),
+    (ValueError, "stride 1", dict(q=make(2, 5, 16, 4).transpose(2, 3))),
+    (ValueError, "finite", dict(scale=math.inf)),
+    (ValueError, "finite", dict(scale=math.nan)),
+    (TypeError, "torch.int32", dict(key_lengths=torch.zeros(2, dtype=torch.int64))),
+    (ValueError, "key_lengths", dict(key_lengths=torch.zeros(1, dtype=torch.int32))),
+    (ValueError, "key_lengths", dict(key_lengths=torch.zeros(4, dtype=torch.int32)[::2])),
+    (TypeError, "torch.bool", dict(key_mask=torch.zeros(2, 7))),
+    (ValueError, "key_mask", dict(key_mask=torch.zeros(2, 8, dtype=torch.bool))),
+    (ValueError, "key_mask", dict(key_mask=torch.zeros(3, 7, dtype=torch.bool))),
+    (TypeError, "dtype", dict(out=make(2, 5, 4, 24, dtype=torch.float16))),
+    (ValueError, "shape", dict(out=make(2, 5, 4, 16))),
+    (ValueError, "stride 1", dict(out=make(2, 5, 24, 4).transpose(2, 3))),
+    (ValueError, "expanded", dict(out=make(1, 5, 4, 24).expand(2, 5, 4, 24))),
+], ids=lambda x: None if isinstance(x, type) else str(x) if isinstance(x, str) else "-".join(x))
+def test_refusals(error, match, change):
+    arguments = dict(q=make(2, 5, 4, 16), k=make(2, 7, 2, 16), v=make(2, 7, 2, 24))
+    plan(**arguments)
+    arguments.update(change)
+    with pytest.raises(error, match=match):
+        plan(**arguments)
+
+
+@pytest.mark.parametrize("error, match, change", [
+    (ValueError, "no batch mode", dict(prefix=(make(1, 9, 2, 16), make(9, 2, 24)))),
+    (ValueError, "prefix_keys", dict(prefix=(make(9, 1, 16), make(9, 2, 24)))),
+    (ValueError, "prefix_keys", dict(prefix=(make(9, 2, 8), make(9, 2, 24)))),
+    (ValueError, "prefix_values", dict(prefix=(make(9, 2, 16), make(8, 2, 24)))),
+    (ValueError, "prefix_values", dict(prefix=(make(9, 2, 16), make(9, 2, 16)))),
+    (TypeError, "dtype", dict(prefix=(make(9, 2, 16, dtype=torch.float16), make(9, 2, 24)))),
+    (ValueError, "batch size", dict(k=make(1, 7, 2, 16), v=make(1, 7, 2, 24))),
+    (ValueError, "lengths", dict(key_lengths=torch.zeros(3, dtype=torch.int32))),
+], ids=lambda x: None if isinstance(x, type) else str(x) if isinstance(x, str) else "-".join(x))
+def test_prefix_refusals(error, match, change):
+    arguments = dict(q=make(2, 5, 4, 16), k=make(2, 7, 2, 16), v=make(2, 7, 2, 24), prefix=(make(9, 2, 16), make(9, 2, 24)),
+                     key_lengths=torch.zeros(2, dtype=torch.int32))
+    plan(**arguments)
+    arguments.update(change)
+    with pytest.raises(error, match=match):
+        plan(**arguments)
+
+
+def test_parameters_of_views():
+    both = make(2, 7, 2, 3, 16)
+    q = make(2, 4, 5, 16).transpose(1, 2)
+    out = make(2, 5, 4, 20)[..., :16]
+    params = plan(q, both[:, :, 0, :2], both[:, :, 1, :2], out=out, scale=0.5).params
+    assert (params.type, params.l, params.m, params.n, params.h, params.g, params.k, params.o) == (_backend.FP32, 2, 5, 7, 4, 2, 16, 16)
+    assert (params.q_ls, params.q_ms, params.q_hs) == (320, 16, 80)
+    assert (params.key_ls, params.key_ns, params.key_gs) == (672, 96, 16)
+    assert params.value == params.key + 48 * 4 and params.scale == 0.5
+    assert (params.out_ls, params.out_ms, params.out_hs) == (400, 80, 20)
+    params = plan(q, both[:1, :, 0, :2], both[:1, :, 1, :2], key_mask=torch.ones(7, dtype=torch.bool)).params
+    assert params.key_ls == params.value_ls == params.key_mask_ls == 0 and params.key_mask_ns == 1
+    assert params.scale == 0.25
+
+
+def library_parameters(**change):
+    params = plan(make(2, 5, 4, 16), make(2, 7, 2, 16), make(2, 7, 2, 24), key_lengths=torch.zeros(2, dtype=torch.int32),
+                  prefix=(make(9, 2, 16), make(9, 2, 24))).params
+    for name, value in change.items():
+        setattr(params, name, value)
+    return params
+
+
+@pytest.mark.parametrize("change", [
+    dict(type=3), dict(l=-1), dict(n=-1), dict(n=2**31 - 1), dict(h=5), dict(g=0), dict(k=0), dict(k=257), dict(o=257), dict(scale=math.nan),
+    dict(q_ms=-1), dict(prefix_value_gs=-1), dict(prefix_n=-1), dict(q=None), dict(out=None), dict(key=None), dict(prefix_value=None),
+    dict(key_lengths=None), dict(key_mask=1), dict(l=2**20, m=2**20),
+], ids=lambda c: "-".join(f"{k}={v}" for k, v in c.items()))
+def test_the_library_refuses_before_any_device_call(change):
+    assert _backend.attention_workspace_bytes(library_parameters()) > 0
+    params = library_parameters(**change)
+    for call in (lambda: _backend.attention(params, None), lambda: _backend.attention_workspace_bytes(params)):
+        with pytest.raises(_backend.BackendError) as info:
+            call()
+        assert info.value.status == _backend.ERR_INVALID_ARGUMENT
+
+
+def test_header_and_binding_agree(tmp_path):
+    gcc = shutil.which("gcc")
+    if gcc is None:
+        pytest.skip("no C compiler")
+    structs = {"kmc_attention_params": _backend.AttentionParams}
+    lines = ['#include "kermac_amd.h"', "#include <stddef.h>", "#include <stdio.h>", "int main(void) {"]
+    for c_name, binding in structs.items():
+        lines.append(f'  printf("{c_name} size %zu\\n", sizeof({c_name}));')
+        lines += [f'  printf("{c_name} {field} %zu\\n", offsetof({c_name}, {field}));' for field, _ in binding._fields_]
+    lines += ['  printf("types %d %d %d\\n", KMC_FP32, KMC_FP16, KMC_BF16);', "  return 0;", "}"]
+    (tmp_path / "probe.c").write_text("\n".join(lines))
+    subprocess.run([gcc, "-std=c11", "-Wall", "-Werror", f"-I{ROOT / 'include'}", str(tmp_path / "probe.c"), "-o", str(tmp_path / "probe")], check=True)
+    printed = subprocess.run([str(tmp_path / "probe")], check=True, capture_output=True, text=True).stdout
+    for c_name, binding in structs.items():
+        assert f"{c_name} size {ctypes.sizeof(binding)}\n" in printed
+        for field, _ in binding._fields_:
+            assert re.search(rf"^{c_name} {field} {getattr(binding, field).offset}$", printed, re.M), f"{c_name}.{field}"
+    assert f"types {_backend.FP32} {_backend.FP16} {_backend.BF16}\n" in printed
