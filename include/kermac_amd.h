@@ -488,6 +488,28 @@ int kmc_attention(const kmc_attention_params *params, void *stream);
 /* Bytes of workspace that kmc_attention uses for this call (0: none). */
 int kmc_attention_workspace_bytes(const kmc_attention_params *params, int64_t *bytes);
 
+/* The gradient of kmc_attention without a prefix.  out and lse are what it returned for the same q, key, value, lengths, mask
+ * and scale; the gradients are contiguous, those of masked keys are 0. */
+typedef struct kmc_attention_gradient_params {
+    int32_t type, flags;
+    int32_t l, m, n, h, g, k, o;
+    int32_t key_entries;        /* l, or 1: one source for all entries (key_ls and value_ls 0), whose gradients are summed over them */
+    float scale;
+    const void *q; int64_t q_ls, q_ms, q_hs;
+    const void *key; int64_t key_ls, key_ns, key_gs;
+    const void *value; int64_t value_ls, value_ns, value_gs;
+    const void *out; int64_t out_ls, out_ms, out_hs;
+    const void *grad_out; int64_t grad_out_ls, grad_out_ms, grad_out_hs;    /* [l, m, h, o] */
+    const float *lse;           /* [l, m, h] contiguous */
+    const int32_t *key_lengths;
+    const uint8_t *key_mask; int64_t key_mask_ls, key_mask_ns;
+    void *grad_q, *grad_key, *grad_value;       /* [l, m, h, k], [key_entries, n, g, k], [key_entries, n, g, o] */
+    /* What kmc_attention_gradient_workspace_bytes asks for, 16-byte aligned; at least 4 l m h bytes, with which no work is cut. */
+    void *workspace; int64_t workspace_bytes;
+} kmc_attention_gradient_params;
+int kmc_attention_gradient(const kmc_attention_gradient_params *params, void *stream);
+int kmc_attention_gradient_workspace_bytes(const kmc_attention_gradient_params *params, int64_t *bytes);
+
 /* ---- run-time compilation (stands in for cuda.core Program / ObjectCode:
  *      src/kermac/module_cache/module_cache.py:13-51, 219-239) ---- */
 

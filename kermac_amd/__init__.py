@@ -16,12 +16,12 @@ from .build_a_kernel import (InnerOperator, KernelDescriptor, KernelType, PowerT
 from .cdist import cdist
 from ._scratch import scratch, set_max_scratch_bytes, get_max_scratch_bytes
 from .cdist_grad import cdist_grad
-from .attention import cross_attention, prefix_attention
+from .attention import cross_attention, cross_attention_grad, prefix_attention
 
 __version__ = "0.1.0"
 
 __all__ = [
-    "cdist", "cdist_grad", "cross_attention", "prefix_attention", "KernelDescriptor", "run_kernel", "PowerType", "InnerOperator", "KernelType",
+    "cdist", "cdist_grad", "cross_attention", "cross_attention_grad", "prefix_attention", "KernelDescriptor", "run_kernel", "PowerType", "InnerOperator", "KernelType",
     "Symmetry", "kernel_descriptor_laplace_l1", "kernel_descriptor_laplace_l2", "kernel_descriptor_p_norm",
     "kernel_descriptor_l1_norm", "kernel_descriptor_l2_norm", "kernel_descriptor_mma",
     "pre_compile_descriptors", "ModuleCache", "CudaTimer", "PyTorchStreamWrapper", "TensorStats",

@@ -142,6 +142,25 @@ class AttentionParams(Structure):
     ]
 
 
+class AttentionGradientParams(Structure):
+    """struct kmc_attention_gradient_params"""
+    _fields_ = [
+        ("type", c_int32), ("flags", c_int32),
+        ("l", c_int32), ("m", c_int32), ("n", c_int32), ("h", c_int32), ("g", c_int32), ("k", c_int32), ("o", c_int32),
+        ("key_entries", c_int32), ("scale", c_float),
+        ("q", c_void_p), ("q_ls", c_int64), ("q_ms", c_int64), ("q_hs", c_int64),
+        ("key", c_void_p), ("key_ls", c_int64), ("key_ns", c_int64), ("key_gs", c_int64),
+        ("value", c_void_p), ("value_ls", c_int64), ("value_ns", c_int64), ("value_gs", c_int64),
+        ("out", c_void_p), ("out_ls", c_int64), ("out_ms", c_int64), ("out_hs", c_int64),
+        ("grad_out", c_void_p), ("grad_out_ls", c_int64), ("grad_out_ms", c_int64), ("grad_out_hs", c_int64),
+        ("lse", c_void_p),
+        ("key_lengths", c_void_p),
+        ("key_mask", c_void_p), ("key_mask_ls", c_int64), ("key_mask_ns", c_int64),
+        ("grad_q", c_void_p), ("grad_key", c_void_p), ("grad_value", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
 # Every exported symbol of include/kermac_amd.h: name -> (restype, argtypes).
 SIGNATURES = {
     "kmc_abi_version": (ctypes.c_int, []),
@@ -167,6 +186,8 @@ SIGNATURES = {
     "kmc_kernel_times_coefficients_jit": (ctypes.c_int, [c_void_p, POINTER(KernelCoefficientsParams), c_void_p]),
     "kmc_attention": (ctypes.c_int, [POINTER(AttentionParams), c_void_p]),
     "kmc_attention_workspace_bytes": (ctypes.c_int, [POINTER(AttentionParams), POINTER(c_int64)]),
+    "kmc_attention_gradient": (ctypes.c_int, [POINTER(AttentionGradientParams), c_void_p]),
+    "kmc_attention_gradient_workspace_bytes": (ctypes.c_int, [POINTER(AttentionGradientParams), POINTER(c_int64)]),
     "kmc_jit_compile": (ctypes.c_int, [
         c_char_p, c_char_p,
         ctypes.c_int, POINTER(c_char_p), POINTER(c_char_p),
@@ -329,6 +350,17 @@ def attention_workspace_bytes(params: AttentionParams) -> int:
     status = library().kmc_attention_workspace_bytes(byref(params), byref(needed))
     if status != OK:
         check(status)
+    return needed.value
+
+
+def attention_gradient(params: AttentionGradientParams, stream: int) -> None:
+    check(library().kmc_attention_gradient(byref(params), stream))
+
+
+def attention_gradient_workspace_bytes(params: AttentionGradientParams) -> int:
+    """Bytes of workspace that kmc_attention_gradient uses for these parameters."""
+    needed = c_int64(0)
+    check(library().kmc_attention_gradient_workspace_bytes(byref(params), byref(needed)))
     return needed.value
 
 

@@ -81,9 +81,9 @@ def _jobs():
     inst = CSRC / "kernels" / "gram_bf16_kernel_inst.hip"
     for same_points in (0, 1):
         jobs.append((inst, OBJ_DIR / f"gram_bf16_kernel_inst_{same_points}.o", [f"-DKMC_SAME_POINTS={same_points}"]))
-    inst = CSRC / "kernels" / "attention_inst.hip"
-    for element_type in (0, 1, 2):
-        jobs.append((inst, OBJ_DIR / f"attention_inst_{element_type}.o", [f"-DKMC_ATT_TYPE={element_type}"]))
+    for name in ("attention_grad_inst", "attention_inst"):
+        for element_type in (0, 1, 2):          # enum kmc_element_type
+            jobs.append((CSRC / "kernels" / f"{name}.hip", OBJ_DIR / f"{name}_{element_type}.o", [f"-DKMC_ATT_TYPE={element_type}"]))
     for rel in EXTRA_DEVICE_SOURCES:
         src = CSRC / rel
         jobs.append((src, OBJ_DIR / (src.stem + ".o"), []))

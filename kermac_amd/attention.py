@@ -32,8 +32,7 @@ def _check_tensors(named, device, dtype, require_device):
         if not isinstance(x, torch.Tensor):
             raise TypeError(f"{name} must be a PyTorch tensor")
         if x.dtype is not dtype:
-            raise TypeError(f"{name} must have dtype {dtype}, got {x.dtype}" if dtype in _TYPES else
-                            f"{name} must have dtype torch.float32, torch.float16 or torch.bfloat16, got {x.dtype}")
+            raise TypeError(f"{name} must have dtype {dtype}, got {x.dtype}")
         if require_device and not x.is_cuda:
             raise ValueError(f"{name} must be on a CUDA device")
         if x.device != device:
@@ -211,6 +210,81 @@ def cross_attention(
     plan = _plan_attention(queries, keys, values, out, scale, key_lengths, key_mask, return_lse)
     _launch(plan, queries.device, debug)
     return (plan.out, plan.lse) if return_lse else plan.out
+
+
+def _plan_attention_grad(grad_out, queries, keys, values, out, lse, scale, key_lengths, key_mask, require_device=True):
+    """The checks of the forward call, whose result `out` and `lse` are, and the gradient's parameters."""
+    forward = _plan_attention(queries, keys, values, out, scale, key_lengths, key_mask, False, require_device=require_device)
+    of = forward.params
+    device = queries.device
+    shape = (of.l, of.m, of.h, of.o)
+    _check_tensors((("grad_out", grad_out),), device, queries.dtype, require_device)
+    if tuple(grad_out.shape) != shape and not (grad_out.dim() == 3 and of.l == 1 and tuple(grad_out.shape) == shape[1:]):
+        raise ValueError(f"grad_out must have shape {shape}, got {tuple(grad_out.shape)}")
+    _, _, _, _, d_ls, d_ms, d_hs = _layout("grad_out", grad_out)
+    _check_tensors((("lse", lse),), device, torch.float32, require_device)
+    if tuple(lse.shape) != shape[:3] or not lse.is_contiguous():
+        raise ValueError(f"lse must be contiguous with shape {shape[:3]}, got {tuple(lse.shape)}")
+    make = torch.zeros if queries.numel() == 0 else torch.empty         # no query: nothing is launched
+    key_entries = keys.size(0) if keys.dim() == 4 else 1
+    grads = (torch.empty(queries.shape, dtype=queries.dtype, device=device), make(keys.shape, dtype=keys.dtype, device=device),
+             make(values.shape, dtype=values.dtype, device=device))
+    params = _backend.AttentionGradientParams(
+        of.type, 0, of.l, of.m, of.n, of.h, of.g, of.k, of.o, key_entries, of.scale, of.q, of.q_ls, of.q_ms, of.q_hs, of.key, of.key_ls, of.key_ns, of.key_gs,
+        of.value, of.value_ls, of.value_ns, of.value_gs, of.out, of.out_ls, of.out_ms, of.out_hs, grad_out.data_ptr(), d_ls, d_ms, d_hs, lse.data_ptr(),
+        of.key_lengths, of.key_mask, of.key_mask_ls, of.key_mask_ns, grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr())
+    plan = _AttentionPlan()
+    plan.params, plan.out, plan.lse = params, grads, None
+    plan.keepalive = [forward, grad_out, lse]
+    return plan
+
+
+@_scratch.operator
+def cross_attention_grad(
+    grad_out: torch.Tensor,                 # [L?, M, H, O]
+    queries: torch.Tensor,                  # [L?, M, H, K]
+    keys: torch.Tensor,                     # [L?, N, G, K]
+    values: torch.Tensor,                   # [L?, N, G, O]
+    out: torch.Tensor,                      # [L?, M, H, O]
+    lse: torch.Tensor,                      # [L, M, H]
+    *,
+    scale: Optional[float] = None,
+    key_lengths: Optional[torch.Tensor] = None,
+    key_mask: Optional[torch.Tensor] = None,
+    debug=False,
+):
+    """Gradients of ``cross_attention`` with respect to queries, keys and values, given the gradient of its result.
+
+    ``out`` and ``lse`` are what ``cross_attention(..., return_lse=True)`` returned for the same tensors, scale, lengths and
+    mask.  The gradient of a head of keys and values is the sum over the heads of queries that share it; that of keys and
+    values of batch size 1 is the sum over the batch.  Keys that do not take part have a gradient of zero, and so has a query without
+    keys.  Sums are fp32 in an order that does not depend on timing; in fp16 the products of weights and gradients are
+    numbers of that type, so gradients far below 1e-4 want a loss scale.
+
+    Returns ``(grad_queries, grad_keys, grad_values)``, new contiguous tensors with the shapes of the inputs.  Takes 4 bytes of
+    scratch memory per row at least.
+
+    Raises:
+        TypeError: non-tensor inputs or a wrong dtype.
+        ValueError: bad shapes, strides, batch sizes or devices, a scale that is not finite.
+        RuntimeError: the limit on scratch memory, or the supplied buffer, does not allow those bytes.
+    """
+    plan = _plan_attention_grad(grad_out, queries, keys, values, out, lse, scale, key_lengths, key_mask)
+    params, device = plan.params, queries.device
+    stream = _current_stream_for(device)
+    needed = _backend.attention_gradient_workspace_bytes(params)
+    if needed:
+        workspace = _scratch.allocate(needed, device)
+        if workspace is None:           # refused: uncut launches, with room for one sum per row
+            needed = -(-4 * params.l * params.m * params.h // 16) * 16
+            workspace = _scratch.allocate(needed, device)
+        if workspace is None:
+            raise RuntimeError(f"cross_attention_grad needs {needed} bytes of scratch memory: the limit, the supplied buffer or the device does not allow them")
+        params.workspace, params.workspace_bytes = workspace.data_ptr(), needed
+    if debug:
+        print("(Kermac Debug) Launching kernel: attention_grad_queries, attention_grad_keys")
+    _backend.attention_gradient(params, stream)
+    return plan.out
 
 
 @_scratch.operator

@@ -9,7 +9,9 @@
 using namespace kmc_host;
 
 namespace kmc_host {
-#define KMC_DECLARE_ATTENTION(type) hipError_t launch_attention_forward_##type(const kmc::AttentionArgs &, int, bool, hipStream_t);
+#define KMC_DECLARE_ATTENTION(type)                                                                    \
+    hipError_t launch_attention_forward_##type(const kmc::AttentionArgs &, int, bool, hipStream_t);     \
+    hipError_t launch_attention_gradient_##type(const kmc::AttentionGradArgs &, int, bool, hipStream_t);
 KMC_DECLARE_ATTENTION(0)
 KMC_DECLARE_ATTENTION(1)
 KMC_DECLARE_ATTENTION(2)
@@ -183,6 +185,98 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
     return KMC_OK;
 }
 
+// Parts that `base` workgroups of `extent` steps each are cut into, `least` steps to a part.
+int parts(int64_t base, int64_t extent, int64_t least)
+{
+    if (base == 0) return 1;
+    const int64_t wanted = std::min<int64_t>({(WANTED_WORKGROUPS + base / 2) / base, (extent + least - 1) / least, MAX_SLOTS});
+    return static_cast<int>(std::max<int64_t>(wanted, 1));
+}
+
+struct GradPlan {
+    kmc::AttentionGradArgs args;
+    bool aligned, empty;
+    int64_t delta_bytes, q_bytes, k_bytes, v_bytes;
+    int64_t bytes() const { return delta_bytes + q_bytes + k_bytes + v_bytes; }
+};
+
+constexpr int MIN_ROW_TILES = 4;                    // tiles of rows that a part of the keys' kernel walks at least
+
+int prepare(const kmc_attention_gradient_params *p, bool may_cut, GradPlan *plan)
+{
+    if (!p) return fail(KMC_ERR_INVALID_ARGUMENT, "null parameter block");
+    const int status = check_extents(p->type, p->l, p->m, p->n, p->h, p->g, p->k, p->o, p->scale);
+    if (status != KMC_OK) return status;
+    if (p->key_entries != p->l && p->key_entries != 1) return fail(KMC_ERR_INVALID_ARGUMENT, "key_entries=%d is neither l=%d nor 1", p->key_entries, p->l);
+    const int64_t strides[] = {p->q_ls, p->q_ms, p->q_hs, p->key_ls, p->key_ns, p->key_gs, p->value_ls, p->value_ns, p->value_gs, p->out_ls, p->out_ms,
+                               p->out_hs, p->grad_out_ls, p->grad_out_ms, p->grad_out_hs, p->key_mask_ls, p->key_mask_ns};
+    for (const int64_t stride : strides)
+        if (stride < 0) return fail(KMC_ERR_INVALID_ARGUMENT, "negative stride");
+    if (p->key_entries != p->l && (p->key_ls != 0 || p->value_ls != 0))
+        return fail(KMC_ERR_INVALID_ARGUMENT, "one source for all entries has key_ls and value_ls 0");
+    *plan = GradPlan{};
+    plan->empty = p->l == 0 || p->m == 0 || p->h == 0;
+    if (plan->empty) return KMC_OK;
+    if (!p->q || !p->out || !p->grad_out || !p->lse || !p->grad_q) return fail(KMC_ERR_INVALID_ARGUMENT, "null q / out / grad_out / lse / grad_q pointer");
+    if (p->n > 0 && (!p->key || !p->value || !p->grad_key || !p->grad_value))
+        return fail(KMC_ERR_INVALID_ARGUMENT, "null key / value / grad_key / grad_value pointer");
+
+    kmc::AttentionGradArgs &args = plan->args;
+    args.q = p->q; args.q_ls = p->q_ls; args.q_ms = p->q_ms; args.q_hs = p->q_hs;
+    args.out = p->out; args.out_ls = p->out_ls; args.out_ms = p->out_ms; args.out_hs = p->out_hs;
+    args.grad_out = p->grad_out; args.grad_out_ls = p->grad_out_ls; args.grad_out_ms = p->grad_out_ms; args.grad_out_hs = p->grad_out_hs;
+    args.lse = p->lse;
+    kmc::AttentionKeys &keys = args.keys;
+    keys.k = p->key; keys.k_ls = p->key_ls; keys.k_ns = p->key_ns; keys.k_gs = p->key_gs;
+    keys.v = p->value; keys.v_ls = p->value_ls; keys.v_ns = p->value_ns; keys.v_gs = p->value_gs;
+    keys.lengths = p->key_lengths;
+    keys.mask = p->key_mask; keys.mask_ls = p->key_mask_ls; keys.mask_ns = p->key_mask_ns;
+    keys.n = p->n;
+    args.grad_q = p->grad_q; args.grad_k = p->grad_key; args.grad_v = p->grad_value;
+    args.l = p->l; args.m = p->m; args.g = p->g; args.r = p->h / p->g; args.k = p->k; args.o = p->o;
+    args.key_entries = p->key_entries;
+    args.scale = p->scale;
+    set_scale(p->scale, &args.scale_log2, &args.query_factor);
+    args.partial_k_width = (p->k + 3) / 4 * 4;
+    args.partial_o_width = (p->o + 3) / 4 * 4;
+
+    const int64_t rows = static_cast<int64_t>(p->m) * args.r;
+    args.q_row_tiles = static_cast<int>((rows + 127) / 128);
+    const int64_t q_base = static_cast<int64_t>(p->l) * p->g * args.q_row_tiles;
+    args.q_splits = may_cut ? parts(q_base, p->n, MIN_KEYS_SHARED) : 1;
+    args.key_tiles = (p->n + 127) / 128;
+    const int64_t k_base = static_cast<int64_t>(p->key_entries) * p->g * args.key_tiles;
+    const int64_t tiles_of_rows = static_cast<int64_t>(args.r) * ((p->m + 31) / 32) * (p->key_entries == p->l ? 1 : p->l);
+    args.k_splits = may_cut ? parts(k_base, tiles_of_rows, MIN_ROW_TILES) : 1;
+    const int64_t q_workgroups = q_base * args.q_splits, k_workgroups = k_base * args.k_splits;
+    if (std::max(q_workgroups, k_workgroups) > 0x7ffffff0ll) return fail(KMC_ERR_INVALID_ARGUMENT, "more workgroups than a launch holds");
+    args.q_workgroups = static_cast<int>(q_workgroups);
+    args.q_grid = static_cast<int>((q_workgroups + 7) / 8 * 8);
+    args.k_workgroups = static_cast<int>(k_workgroups);
+    args.k_grid = static_cast<int>((k_workgroups + 7) / 8 * 8);
+
+    const int64_t q_rows = static_cast<int64_t>(p->l) * p->m * p->h, k_rows = static_cast<int64_t>(p->key_entries) * p->n * p->g;
+    plan->delta_bytes = (4 * q_rows + 15) / 16 * 16;
+    if (args.q_splits > 1) plan->q_bytes = 4ll * args.q_splits * q_rows * args.partial_k_width;
+    if (args.k_splits > 1) {
+        plan->k_bytes = 4ll * args.k_splits * k_rows * args.partial_k_width;
+        plan->v_bytes = 4ll * args.k_splits * k_rows * args.partial_o_width;
+    }
+
+    Layout layout{element_size(p->type)};
+    layout.operand(p->q, p->k); layout.operand(p->out, p->o); layout.operand(p->grad_out, p->o); layout.operand(p->grad_q, p->k);
+    layout.stride(p->l, p->q_ls); layout.stride(p->m, p->q_ms); layout.stride(p->h, p->q_hs);
+    layout.stride(p->l, p->out_ls); layout.stride(p->m, p->out_ms); layout.stride(p->h, p->out_hs);
+    layout.stride(p->l, p->grad_out_ls); layout.stride(p->m, p->grad_out_ms); layout.stride(p->h, p->grad_out_hs);
+    if (p->n > 0) {
+        layout.operand(p->key, p->k); layout.operand(p->value, p->o); layout.operand(p->grad_key, p->k); layout.operand(p->grad_value, p->o);
+        layout.stride(p->l, p->key_ls); layout.stride(p->n, p->key_ns); layout.stride(p->g, p->key_gs);
+        layout.stride(p->l, p->value_ls); layout.stride(p->n, p->value_ns); layout.stride(p->g, p->value_gs);
+    }
+    plan->aligned = layout.aligned && !(p->flags & KMC_FLAG_FORCE_SCALAR_ACCESS);
+    return KMC_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -221,6 +315,46 @@ int kmc_attention(const kmc_attention_params *params, void *stream)
                          : params->type == KMC_FP16 ? launch_attention_forward_1(args, width, plan.aligned, on)
                                                     : launch_attention_forward_2(args, width, plan.aligned, on);
     if (e != hipSuccess) return fail_hip(e, "attention launch");
+    return KMC_OK;
+}
+
+int kmc_attention_gradient_workspace_bytes(const kmc_attention_gradient_params *params, int64_t *bytes)
+{
+    if (!bytes) return fail(KMC_ERR_INVALID_ARGUMENT, "bytes: null pointer");
+    GradPlan plan;
+    const int status = prepare(params, true, &plan);
+    if (status != KMC_OK) return status;
+    *bytes = plan.bytes();
+    return KMC_OK;
+}
+
+int kmc_attention_gradient(const kmc_attention_gradient_params *params, void *stream)
+{
+    GradPlan plan;
+    int status = prepare(params, true, &plan);
+    if (status != KMC_OK) return status;
+    if (plan.empty) return KMC_OK;
+    if (!params->workspace || params->workspace_bytes < plan.bytes()) {
+        status = prepare(params, false, &plan);
+        if (status != KMC_OK) return status;
+        if (!params->workspace || params->workspace_bytes < plan.bytes())
+            return fail(KMC_ERR_INVALID_ARGUMENT, "the gradient of attention needs a workspace of %lld bytes", static_cast<long long>(plan.bytes()));
+    }
+    if (!aligned16(params->workspace)) return fail(KMC_ERR_INVALID_ARGUMENT, "workspace is not aligned to 16 bytes");
+    status = require_gfx950();
+    if (status != KMC_OK) return status;
+    kmc::AttentionGradArgs &args = plan.args;
+    char *at = static_cast<char *>(params->workspace);
+    args.delta = reinterpret_cast<float *>(at);
+    args.partial_q = reinterpret_cast<float *>(at += plan.delta_bytes);
+    args.partial_k = reinterpret_cast<float *>(at += plan.q_bytes);
+    args.partial_v = reinterpret_cast<float *>(at += plan.k_bytes);
+    const int width = std::max(params->k, params->o);
+    const hipStream_t on = static_cast<hipStream_t>(stream);
+    const hipError_t e = params->type == KMC_FP32   ? launch_attention_gradient_0(args, width, plan.aligned, on)
+                         : params->type == KMC_FP16 ? launch_attention_gradient_1(args, width, plan.aligned, on)
+                                                    : launch_attention_gradient_2(args, width, plan.aligned, on);
+    if (e != hipSuccess) return fail_hip(e, "attention gradient launch");
     return KMC_OK;
 }
 

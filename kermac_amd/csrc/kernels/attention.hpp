@@ -307,6 +307,29 @@ struct AttForwardShape {
     static constexpr int BYTES = BYTES_1 > JOIN_BYTES ? BYTES_1 : JOIN_BYTES;
 };
 
+// A lane's column of results [DP, 32] as the row of `width` elements that it is in memory, times a factor.
+template <typename T, int DP, bool ALIGNED>
+__device__ __forceinline__ void att_store_columns(T *to, const att_f32x16 (&x)[DP / 32], float factor, int width, int half)
+{
+#pragma unroll
+    for (int o = 0; o < DP / 32; ++o)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int column = 32 * o + 8 * q + 4 * half;
+            typedef T four __attribute__((ext_vector_type(4)));
+            four y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = static_cast<T>(x[o][4 * q + j] * factor);
+            if (ALIGNED) {
+                if (column < width) *reinterpret_cast<four *>(to + column) = y;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (column + j < width) to[column + j] = y[j];
+            }
+        }
+}
+
 // Writes a wave's 32 rows: the result itself, or a partial result and its lse (to base 2) for att_join.
 template <typename T, int DP, bool ALIGNED>
 __device__ __forceinline__ void att_forward_write(const AttentionArgs &args, const AttentionJob &job, const AttState<DP> &state, float sum, int entry, int g,
@@ -337,24 +360,8 @@ __device__ __forceinline__ void att_forward_write(const AttentionArgs &args, con
         return;
     }
     if (args.lse && half == 0) args.lse[id] = lse2 * ATT_LN_2;
-    T *to = static_cast<T *>(args.out) + at.entry * args.out_ls + at.query * args.out_ms + at.head * args.out_hs;
-#pragma unroll
-    for (int o = 0; o < DP / 32; ++o)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int column = 32 * o + 8 * q + 4 * half;
-            typedef T four __attribute__((ext_vector_type(4)));
-            four x;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = static_cast<T>(state.out[o][4 * q + j] * inverse);
-            if (ALIGNED) {
-                if (column < args.o) *reinterpret_cast<four *>(to + column) = x;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (column + j < args.o) to[column + j] = x[j];
-            }
-        }
+    att_store_columns<T, DP, ALIGNED>(static_cast<T *>(args.out) + at.entry * args.out_ls + at.query * args.out_ms + at.head * args.out_hs, state.out, inverse,
+                                      args.o, half);
 }
 
 template <typename T, int DP, bool ALIGNED>

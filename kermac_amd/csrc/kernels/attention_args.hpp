@@ -41,4 +41,29 @@ struct AttentionArgs {
     i64 rows_total;                         // l m g r
 };
 
+struct AttentionGradArgs {
+    const void *q, *out, *grad_out;
+    i64 q_ls, q_ms, q_hs, out_ls, out_ms, out_hs, grad_out_ls, grad_out_ms, grad_out_hs;
+    const float *lse;                       // [l, m, g r]
+    AttentionKeys keys;
+    void *grad_q, *grad_k, *grad_v;         // contiguous [l, m, g r, k], [key_entries, n, g, k], [key_entries, n, g, o]
+    int l, m, g, r, k, o;
+    int key_entries;                        // l, or 1: one source for all entries
+    float scale, scale_log2, query_factor;
+    float *delta;                           // [l, m, g r]: sum_o out grad_out, written by the first kernel for the second
+    int q_row_tiles, q_splits, q_workgroups, q_grid;
+    int key_tiles, k_splits, k_workgroups, k_grid;
+    float *partial_q, *partial_k, *partial_v;   // [splits, rows, width rounded up to 4], where the work is cut
+    int partial_k_width, partial_o_width;
+};
+
+// The sum of partial results, times a factor, in the operands' type.
+struct AttentionSumArgs {
+    const float *partial;
+    void *out;
+    i64 rows;
+    int splits, width, partial_width;
+    float factor;
+};
+
 }  // namespace kmc

@@ -1,0 +1,61 @@
+// Instantiations of attention's gradient for one element type (KMC_ATT_TYPE: 0 fp32, 1 fp16, 2 bf16).
+#include "attention_grad.hpp"
+#include "launch.hpp"
+
+namespace kmc_host {
+
+namespace {
+
+#if KMC_ATT_TYPE == 0
+typedef float Element;
+#elif KMC_ATT_TYPE == 1
+typedef _Float16 Element;
+#else
+typedef __bf16 Element;
+#endif
+
+template <int DP, bool ALIGNED>
+hipError_t gradient(const kmc::AttentionGradArgs &args, hipStream_t stream)
+{
+    // the queries' kernel writes delta, which the keys' kernel reads
+    const hipError_t status = launch(kmc::attention_grad_queries<Element, DP, ALIGNED>, dim3(args.q_grid), dim3(256), stream, args);
+    if (status != hipSuccess || args.k_grid == 0) return status;
+    return launch(kmc::attention_grad_keys<Element, DP, ALIGNED>, dim3(args.k_grid), dim3(256), stream, args);
+}
+
+template <int DP>
+hipError_t gradient(const kmc::AttentionGradArgs &args, bool aligned, hipStream_t stream)
+{
+    return aligned ? gradient<DP, true>(args, stream) : gradient<DP, false>(args, stream);
+}
+
+hipError_t sum(const float *partial, void *out, kmc::i64 rows, int splits, int width, int partial_width, float factor, hipStream_t stream)
+{
+    const kmc::AttentionSumArgs args = {partial, out, rows, splits, width, partial_width, factor};
+    const kmc::i64 blocks = (rows * width + 255) / 256;
+    return launch(kmc::attention_sum<Element>, dim3(static_cast<unsigned>(blocks < 16384 ? blocks : 16384)), dim3(256), stream, args);
+}
+
+}  // namespace
+
+#define KMC_ATT_NAME_2(name, type) name##_##type
+#define KMC_ATT_NAME_1(name, type) KMC_ATT_NAME_2(name, type)
+#define KMC_ATT_NAME(name) KMC_ATT_NAME_1(name, KMC_ATT_TYPE)
+
+hipError_t KMC_ATT_NAME(launch_attention_gradient)(const kmc::AttentionGradArgs &args, int width, bool aligned, hipStream_t stream)
+{
+    hipError_t status = width <= 64    ? gradient<64>(args, aligned, stream)
+                        : width <= 128 ? gradient<128>(args, aligned, stream)
+                                       : gradient<256>(args, aligned, stream);
+    const kmc::i64 q_rows = static_cast<kmc::i64>(args.l) * args.m * args.g * args.r;
+    const kmc::i64 k_rows = static_cast<kmc::i64>(args.key_entries) * args.keys.n * args.g;
+    if (status == hipSuccess && args.q_splits > 1)
+        status = sum(args.partial_q, args.grad_q, q_rows, args.q_splits, args.k, args.partial_k_width, args.scale, stream);
+    if (status == hipSuccess && args.k_splits > 1)
+        status = sum(args.partial_k, args.grad_k, k_rows, args.k_splits, args.k, args.partial_k_width, args.scale, stream);
+    if (status == hipSuccess && args.k_splits > 1)
+        status = sum(args.partial_v, args.grad_v, k_rows, args.k_splits, args.o, args.partial_o_width, 1.0f, stream);
+    return status;
+}
+
+}  // namespace kmc_host

@@ -59,6 +59,51 @@ def forward(q, k, v, keep, scale):
     return out.transpose(1, 2), lse.transpose(1, 2), bound.transpose(1, 2), lse_bound.transpose(1, 2)
 
 
+def gradients(grad_out, q, k, v, keep, scale):
+    """(grad_q, grad_k, grad_v) and their bounds.  On top of the forward's errors: lse is off by its bound, the result that delta is
+    made of by its own, ds is rounded to the operands' type in front of the two products with keys and queries, p in front of the one with d."""
+    unit, floor = UNIT[q.dtype], FLOOR[q.dtype]
+    L, M, H, K = q.shape
+    N, G, O = v.shape[1:]
+    R, shared = H // G, k.shape[0] == 1 and L > 1
+    out, lse, out_bound, lse_bound = forward(q, k, v, keep, scale)
+    q, k, v, d = (x.detach().cpu().double() for x in (q, k, v, grad_out))
+    used = keep.any(1)[..., None, None]
+    k, v = (torch.where(used, x.expand(L, *x.shape[1:]), torch.zeros(()).double()).repeat_interleave(R, 2) for x in (k, v))
+    q, k, v, d, out, out_bound = (x.transpose(1, 2).contiguous() for x in (q, k, v, d, out, out_bound))
+    lse, lse_bound = lse.transpose(1, 2)[..., None], lse_bound.transpose(1, 2)[..., None]
+    s = torch.matmul(q, k.transpose(2, 3)) * scale
+    S = torch.matmul(q.abs(), k.abs().transpose(2, 3)) * abs(scale)
+    p = torch.exp(s - lse).masked_fill(~keep[:, None], 0.0)
+    p_error = p * 2 * (2 * (K + 4) * E32 * S + 16 * E32 + lse_bound + 4 * E32 * lse.abs().nan_to_num(posinf=0.0))
+    dp = torch.matmul(d, v.transpose(2, 3))
+    dp_magnitude = torch.matmul(d.abs(), v.abs().transpose(2, 3))
+    delta = (d * out).sum(-1, keepdim=True)
+    delta_error = (d.abs() * out_bound).sum(-1, keepdim=True) + (O + 16) * E32 * (d.abs() * out.abs()).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    ds_error = p_error * (dp - delta).abs() + p * ((O + 16) * E32 * dp_magnitude + delta_error)
+    ds_error = ds_error + unit * 1.01 * (ds.abs() + ds_error) + floor * keep[:, None]
+    p_rounded_error = p_error + unit * 1.01 * p + floor * keep[:, None]
+
+    def result(value, bound):
+        return value, bound + unit * 1.01 * (value.abs() + bound) + floor
+
+    def over_rows(x):
+        """[L, H, N, D] -> [L or 1, N, G, D]: the sum over heads and entries that share the keys"""
+        x = x.reshape(L, G, R, N, -1).sum(2).transpose(1, 2)
+        return x.sum(0, keepdim=True) if shared else x
+
+    rows = M * R * (L if shared else 1) + 16
+    grad_q = (scale * torch.matmul(ds, k)).transpose(1, 2)
+    grad_q_bound = (abs(scale) * (torch.matmul(ds_error, k.abs()) + (N + 16) * E32 * torch.matmul(ds.abs(), k.abs()))).transpose(1, 2)
+    grad_k = over_rows(scale * torch.matmul(ds.transpose(2, 3), q))
+    grad_k_bound = over_rows(abs(scale) * (torch.matmul(ds_error.transpose(2, 3), q.abs()) + rows * E32 * torch.matmul(ds.abs().transpose(2, 3), q.abs())))
+    grad_v = over_rows(torch.matmul(p.transpose(2, 3), d))
+    grad_v_bound = over_rows(torch.matmul(p_rounded_error.transpose(2, 3), d.abs()) + rows * E32 * torch.matmul(p.transpose(2, 3), d.abs()))
+    results = [result(*x) for x in ((grad_q, grad_q_bound), (grad_k, grad_k_bound), (grad_v, grad_v_bound))]
+    return [value for value, _ in results], [bound for _, bound in results]
+
+
 def prefix(q, pk, pv, k, v, lengths, scale):
     """(out, bound) of prefix_attention: the prefix and the own keys of an entry as one sequence of keys."""
     L, M = q.shape[:2]

@@ -11,7 +11,7 @@ import torch
 
 import kermac_amd as kermac
 from kermac_amd import _backend
-from kermac_amd.attention import _plan_attention
+from kermac_amd.attention import _plan_attention, _plan_attention_grad
 
 ROOT = Path(__file__).resolve().parents[1]
 
@@ -128,11 +128,53 @@ def test_the_library_refuses_before_any_device_call(change):
         assert info.value.status == _backend.ERR_INVALID_ARGUMENT
 
 
+@pytest.mark.parametrize("error, match, change", [
+    (TypeError, "grad_out", dict(grad_out=None)),
+    (TypeError, "grad_out", dict(grad_out=make(2, 5, 4, 24, dtype=torch.float16))),
+    (ValueError, "grad_out", dict(grad_out=make(2, 5, 4, 16))),
+    (ValueError, "grad_out", dict(grad_out=make(2, 5, 24, 4).transpose(2, 3))),
+    (ValueError, "out", dict(out=make(2, 5, 4, 16))),
+    (TypeError, "lse", dict(lse=make(2, 5, 4, dtype=torch.float64))),
+    (ValueError, "lse", dict(lse=make(2, 4, 5))),
+    (ValueError, "lse", dict(lse=make(2, 4, 5).transpose(1, 2))),
+    (ValueError, "batch size", dict(keys=make(1, 7, 2, 16))),
+    (TypeError, "torch.int32", dict(key_lengths=torch.zeros(2))),
+], ids=lambda x: None if isinstance(x, type) else str(x) if isinstance(x, str) else "-".join(x))
+def test_gradient_refusals(error, match, change):
+    arguments = dict(grad_out=make(2, 5, 4, 24), queries=make(2, 5, 4, 16), keys=make(2, 7, 2, 16), values=make(2, 7, 2, 24), out=make(2, 5, 4, 24),
+                     lse=make(2, 5, 4), scale=None, key_lengths=None, key_mask=None, require_device=False)
+    plan = _plan_attention_grad(**arguments)
+    assert [tuple(x.shape) for x in plan.out] == [(2, 5, 4, 16), (2, 7, 2, 16), (2, 7, 2, 24)]
+    arguments.update(change)
+    with pytest.raises(error, match=match):
+        _plan_attention_grad(**arguments)
+
+
+@pytest.mark.parametrize("change", [
+    dict(type=-1), dict(m=-1), dict(h=3), dict(k=0), dict(o=257), dict(scale=math.inf), dict(key_entries=3), dict(key_entries=1), dict(grad_out_ls=-1),
+    dict(lse=None), dict(grad_q=None), dict(grad_value=None), dict(value=None), dict(out=None),
+], ids=lambda c: "-".join(f"{k}={v}" for k, v in c.items()))
+def test_the_library_refuses_gradients_before_any_device_call(change):
+    params = _plan_attention_grad(make(2, 5, 4, 24), make(2, 5, 4, 16), make(2, 7, 2, 16), make(2, 7, 2, 24), make(2, 5, 4, 24), make(2, 5, 4), None, None, None,
+                                  require_device=False).params
+    needed = _backend.attention_gradient_workspace_bytes(params)
+    assert needed >= 4 * 2 * 5 * 4
+    for workspace, nbytes in ((None, needed), (1 << 20, 4 * 2 * 5 * 4 - 1), ((1 << 20) + 4, needed)):
+        params.workspace, params.workspace_bytes = workspace, nbytes
+        with pytest.raises(_backend.BackendError, match="workspace"):
+            _backend.attention_gradient(params, None)
+    for name, value in change.items():
+        setattr(params, name, value)
+    with pytest.raises(_backend.BackendError) as info:
+        _backend.attention_gradient_workspace_bytes(params)
+    assert info.value.status == _backend.ERR_INVALID_ARGUMENT
+
+
 def test_header_and_binding_agree(tmp_path):
     gcc = shutil.which("gcc")
     if gcc is None:
         pytest.skip("no C compiler")
-    structs = {"kmc_attention_params": _backend.AttentionParams}
+    structs = {"kmc_attention_params": _backend.AttentionParams, "kmc_attention_gradient_params": _backend.AttentionGradientParams}
     lines = ['#include "kermac_amd.h"', "#include <stddef.h>", "#include <stdio.h>", "int main(void) {"]
     for c_name, binding in structs.items():
         lines.append(f'  printf("{c_name} size %zu\\n", sizeof({c_name}));')
