@@ -184,10 +184,10 @@ SIGNATURES = {
     "kmc_kernel_coefficients_workspace_bytes": (ctypes.c_int, [POINTER(KernelCoefficientsParams), POINTER(c_int64)]),
     "kmc_kernel_times_coefficients_has_variant": (ctypes.c_int, [c_int32, c_int32]),
     "kmc_kernel_times_coefficients_jit": (ctypes.c_int, [c_void_p, POINTER(KernelCoefficientsParams), c_void_p]),
-    "kmc_attention": (ctypes.c_int, [POINTER(AttentionParams), c_void_p]),
-    "kmc_attention_workspace_bytes": (ctypes.c_int, [POINTER(AttentionParams), POINTER(c_int64)]),
-    "kmc_attention_gradient": (ctypes.c_int, [POINTER(AttentionGradientParams), c_void_p]),
-    "kmc_attention_gradient_workspace_bytes": (ctypes.c_int, [POINTER(AttentionGradientParams), POINTER(c_int64)]),
+    "kmc_attention": (ctypes.c_int, [c_void_p, c_void_p]),
+    "kmc_attention_workspace_bytes": (ctypes.c_int, [c_void_p, POINTER(c_int64)]),
+    "kmc_attention_gradient": (ctypes.c_int, [c_void_p, c_void_p]),
+    "kmc_attention_gradient_workspace_bytes": (ctypes.c_int, [c_void_p, POINTER(c_int64)]),
     "kmc_jit_compile": (ctypes.c_int, [
         c_char_p, c_char_p,
         ctypes.c_int, POINTER(c_char_p), POINTER(c_char_p),
@@ -338,29 +338,37 @@ def kernel_times_coefficients_has_variant(inner_operator: int, inner_power: int)
     return bool(library().kmc_kernel_times_coefficients_has_variant(inner_operator, inner_power))
 
 
-def attention(params: AttentionParams, stream: int) -> None:
-    status = library().kmc_attention(byref(params), stream)
+def struct_format(block) -> str:
+    """The format with which the struct module packs the fields of a flat parameter block, in the C compiler's alignment."""
+    codes = {c_int32: "i", c_float: "f", c_int64: "q", c_void_p: "P"}
+    return "@" + "".join(codes[kind] for _, kind in block._fields_)
+
+
+# (`params` is a structure, or its bytes as struct_format packs them)
+
+def attention(params, stream: int) -> None:
+    status = library().kmc_attention(params if type(params) is bytes else byref(params), stream)
     if status != OK:
         check(status)
 
 
-def attention_workspace_bytes(params: AttentionParams) -> int:
+def attention_workspace_bytes(params) -> int:
     """Bytes of workspace that kmc_attention uses for these parameters (0: none)."""
     needed = c_int64(0)
-    status = library().kmc_attention_workspace_bytes(byref(params), byref(needed))
-    if status != OK:
-        check(status)
+    check(library().kmc_attention_workspace_bytes(params if type(params) is bytes else byref(params), byref(needed)))
     return needed.value
 
 
-def attention_gradient(params: AttentionGradientParams, stream: int) -> None:
-    check(library().kmc_attention_gradient(byref(params), stream))
+def attention_gradient(params, stream: int) -> None:
+    status = library().kmc_attention_gradient(params if type(params) is bytes else byref(params), stream)
+    if status != OK:
+        check(status)
 
 
-def attention_gradient_workspace_bytes(params: AttentionGradientParams) -> int:
+def attention_gradient_workspace_bytes(params) -> int:
     """Bytes of workspace that kmc_attention_gradient uses for these parameters."""
     needed = c_int64(0)
-    check(library().kmc_attention_gradient_workspace_bytes(byref(params), byref(needed)))
+    check(library().kmc_attention_gradient_workspace_bytes(params if type(params) is bytes else byref(params), byref(needed)))
     return needed.value
 
 

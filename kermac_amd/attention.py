@@ -14,7 +14,9 @@ step calls ``cross_attention_grad`` with the result and the row sums that ``cros
 """
 from __future__ import annotations
 
+import functools
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -25,28 +27,49 @@ from .build_a_kernel import _current_stream_for
 
 _TYPES = {torch.float32: _backend.FP32, torch.float16: _backend.FP16, torch.bfloat16: _backend.BF16}
 _MAX_WIDTH = 256
+_MAX_EXTENT = 2_000_000_000
+
+# A call on one token costs the GPU a few microseconds, so its host side counts: the parameter blocks are packed in one step (a field by
+# field structure takes four times as long), and what a shape asks of the workspace is asked of the library once.
+_PARAMS = struct.Struct(_backend.struct_format(_backend.AttentionParams))
+_GRADIENT_PARAMS = struct.Struct(_backend.struct_format(_backend.AttentionGradientParams))
 
 
-def _check_tensors(named, device, dtype, require_device):
-    for name, x in named:
-        if not isinstance(x, torch.Tensor):
-            raise TypeError(f"{name} must be a PyTorch tensor")
-        if x.dtype is not dtype:
-            raise TypeError(f"{name} must have dtype {dtype}, got {x.dtype}")
-        if require_device and not x.is_cuda:
-            raise ValueError(f"{name} must be on a CUDA device")
-        if x.device != device:
-            raise ValueError(f"{name} must be on the same CUDA device as inputs: got {x.device}, expected {device}")
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(L, M, N, H, G, K, O, P, causal):
+    """kmc_attention_workspace_bytes: a function of the extents alone."""
+    one = 16                            # stands for any address: nothing is read
+    return _backend.attention_workspace_bytes(_backend.AttentionParams(
+        _backend.FP32, 0, L, M, N, H, G, K, O, 1.0, q=one, key=one, value=one, out=one, key_lengths=one, prefix_n=P, causal=causal,
+        prefix_key=one, prefix_value=one))
 
 
-def _layout(name, x):
+@functools.lru_cache(maxsize=4096)
+def _gradient_workspace_bytes(L, M, N, H, G, K, O, key_entries):
+    one = 16
+    return _backend.attention_gradient_workspace_bytes(_backend.AttentionGradientParams(
+        _backend.FP32, 0, L, M, N, H, G, K, O, key_entries, 1.0, q=one, key=one, value=one, out=one, grad_out=one, lse=one, grad_q=one, grad_key=one,
+        grad_value=one))
+
+
+def _check(name, x, device, dtype):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a PyTorch tensor")
+    if x.dtype is not dtype:
+        raise TypeError(f"{name} must have dtype {dtype}, got {x.dtype}")
+    if x.device != device:
+        raise ValueError(f"{name} must be on the same CUDA device as inputs: got {x.device}, expected {device}")
+
+
+def _operand(name, x, device, dtype):
     """(batch entries, tokens, heads, features, strides of the first three) of a [tokens, heads, features] tensor or a batch of them."""
+    _check(name, x, device, dtype)
     shape, strides = x.shape, x.stride()
-    if len(shape) == 4:
+    if len(strides) == 4:
         (L, tokens, heads, width), (ls, ts, hs, ws) = shape, strides
         if L == 1:
             ls = 0
-    elif len(shape) == 3:
+    elif len(strides) == 3:
         (tokens, heads, width), (ts, hs, ws) = shape, strides
         L, ls = 1, 0
     else:
@@ -58,116 +81,121 @@ def _layout(name, x):
     return L, tokens, heads, width, ls, ts, hs
 
 
-def _result(name, out, shape, like, require_device):
-    """`out`, checked, or a new tensor of `shape`."""
-    if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
-    _check_tensors(((name, out),), like.device, like.dtype, require_device)
-    if tuple(out.shape) != tuple(shape) and not (out.dim() == 3 and shape[0] == 1 and tuple(out.shape) == tuple(shape[1:])):
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(out.shape)}")
-    if any(stride == 0 and extent > 1 for extent, stride in zip(out.shape, out.stride())):
+def _strides_of_result(name, out, shape, device, dtype):
+    _check(name, out, device, dtype)
+    if tuple(out.shape) != shape and not (out.dim() == 3 and shape[0] == 1 and tuple(out.shape) == shape[1:]):
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(out.shape)}")
+    strides = out.stride()
+    if any(stride == 0 and extent > 1 for extent, stride in zip(out.shape, strides)):
         raise ValueError(f"{name} must not be an expanded tensor")
-    return out
+    if strides[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"{name} must have stride 1 in last dimension")
+    return strides[0] if len(strides) == 4 else 0, strides[-3], strides[-2]
 
 
-def _scale(scale, width):
-    scale = width ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
-    return scale
-
-
-def _lengths(name, lengths, L, device, require_device):
-    _check_tensors(((name, lengths),), device, torch.int32, require_device)
-    if tuple(lengths.shape) != (L,) or (L > 1 and lengths.stride(0) != 1):
-        raise ValueError(f"{name} must be contiguous with shape (L={L},), got {tuple(lengths.shape)}")
-    return lengths.data_ptr()
-
-
-def _check_types(x):
-    if not isinstance(x, torch.Tensor):
-        raise TypeError("queries must be a PyTorch tensor")
-    if x.dtype not in _TYPES:
-        raise TypeError(f"queries must have dtype torch.float32, torch.float16 or torch.bfloat16, got {x.dtype}")
+def _mask(key_mask, L, N, device):
+    """(address, stride of an entry, stride of a key)"""
+    _check("key_mask", key_mask, device, torch.bool)
+    if tuple(key_mask.shape) not in ((N,), (1, N), (L, N)):
+        raise ValueError(f"key_mask must have shape (N={N},) or (L={L}, N={N}), got {tuple(key_mask.shape)}")
+    return key_mask.data_ptr(), key_mask.stride(0) if key_mask.dim() == 2 and key_mask.size(0) > 1 else 0, key_mask.stride(-1)
 
 
 class _AttentionPlan:
-    __slots__ = ("params", "out", "lse", "keepalive")
+    """A checked call: `fields` are those of the parameter block in front of the workspace's."""
+    __slots__ = ("fields", "extents", "out", "lse", "device")
+
+    @property
+    def params(self) -> _backend.AttentionParams:
+        """The block as a structure."""
+        return _backend.AttentionParams.from_buffer_copy(_PARAMS.pack(*self.fields, 0, 0))
 
 
 def _plan_attention(queries, keys, values, out, scale, key_lengths, key_mask, return_lse, prefix=None, require_device=True) -> _AttentionPlan:
     """Validation and parameter marshalling, without the launch.  `prefix`: the prefix's keys and values; the queries are then
     the last tokens of `key_lengths`."""
-    _check_types(queries)
+    if not isinstance(queries, torch.Tensor):
+        raise TypeError("queries must be a PyTorch tensor")
     device, dtype = queries.device, queries.dtype
-    inputs = [("queries", queries), ("keys", keys), ("values", values)]
-    if prefix is not None:
-        inputs += [("prefix_keys", prefix[0]), ("prefix_values", prefix[1])]
-    _check_tensors(inputs, device, dtype, require_device)
-    L, M, H, K, q_ls, q_ms, q_hs = _layout("queries", queries)
-    L_k, N, G, K_k, k_ls, k_ns, k_gs = _layout("keys", keys)
-    L_v, N_v, G_v, O, v_ls, v_ns, v_gs = _layout("values", values)
+    element = _TYPES.get(dtype)
+    if element is None:
+        raise TypeError(f"queries must have dtype torch.float32, torch.float16 or torch.bfloat16, got {dtype}")
+    if require_device and not queries.is_cuda:
+        raise ValueError("queries must be on a CUDA device")
+    L, M, H, K, q_ls, q_ms, q_hs = _operand("queries", queries, device, dtype)
+    L_k, N, G, K_k, k_ls, k_ns, k_gs = _operand("keys", keys, device, dtype)
+    L_v, N_v, G_v, O, v_ls, v_ns, v_gs = _operand("values", values, device, dtype)
     if L_k != L_v or (L_k != L and (L_k != 1 or prefix is not None)):
         raise ValueError(f"keys and values must both have the batch size of queries (L={L})"
                          + (" or both 1" if prefix is None else "") + f", got {L_k} and {L_v}")
     if K_k != K:
         raise ValueError(f"keys must have as many features as queries (K={K}), got {K_k}")
-    if (N_v, G_v) != (N, G):
+    if N_v != N or G_v != G:
         raise ValueError(f"values must have as many tokens and heads as keys (N={N}, G={G}), got {N_v} and {G_v}")
     if G == 0 and H > 0 or G > 0 and H % G != 0:
         raise ValueError(f"the heads of queries (H={H}) must be a multiple of the heads of keys (G={G})")
-    scale = _scale(scale, K)
-
-    params = _backend.AttentionParams(_TYPES[dtype], 0, L, M, N, H, G, K, O, scale, queries.data_ptr(), q_ls, q_ms, q_hs,
-                                      keys.data_ptr(), k_ls, k_ns, k_gs, values.data_ptr(), v_ls, v_ns, v_gs)
-    plan = _AttentionPlan()
-    plan.keepalive = [queries, keys, values, key_lengths, key_mask, prefix]
+    if L * M * H > _MAX_EXTENT or max(L, M, N, H) > _MAX_EXTENT:
+        raise ValueError(f"at most {_MAX_EXTENT} keys, and rows over the batch and the heads: got N={N}, L={L}, M={M}, H={H}")
+    scale = K ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
+    lengths_ptr = mask_ptr = mask_ls = mask_ns = 0
     if key_lengths is not None:
-        params.key_lengths = _lengths("lengths" if prefix is not None else "key_lengths", key_lengths, L, device, require_device)
+        name = "key_lengths" if prefix is None else "lengths"
+        _check(name, key_lengths, device, torch.int32)
+        if key_lengths.dim() != 1 or key_lengths.size(0) != L or (L > 1 and key_lengths.stride(0) != 1):
+            raise ValueError(f"{name} must be contiguous with shape (L={L},), got {tuple(key_lengths.shape)}")
+        lengths_ptr = key_lengths.data_ptr()
     if key_mask is not None:
-        _check_tensors((("key_mask", key_mask),), device, torch.bool, require_device)
-        if tuple(key_mask.shape) not in ((N,), (1, N), (L, N)):
-            raise ValueError(f"key_mask must have shape (N={N},) or (L={L}, N={N}), got {tuple(key_mask.shape)}")
-        batched = key_mask.dim() == 2 and key_mask.size(0) > 1
-        params.key_mask, params.key_mask_ls, params.key_mask_ns = key_mask.data_ptr(), key_mask.stride(0) if batched else 0, key_mask.stride(-1)
+        mask_ptr, mask_ls, mask_ns = _mask(key_mask, L, N, device)
+    P = causal = pk_ptr = pk_ns = pk_gs = pv_ptr = pv_ns = pv_gs = 0
     if prefix is not None:
         prefix_k, prefix_v = prefix
+        L_p, P, G_p, K_p, _, pk_ns, pk_gs = _operand("prefix_keys", prefix_k, device, dtype)
+        L_pv, P_v, G_pv, O_p, _, pv_ns, pv_gs = _operand("prefix_values", prefix_v, device, dtype)
         if prefix_k.dim() != 3 or prefix_v.dim() != 3:
             raise ValueError("prefix_keys and prefix_values must be 3-dimensional: they have no batch mode")
-        _, P, G_p, K_p, _, pk_ns, pk_gs = _layout("prefix_keys", prefix_k)
-        _, P_v, G_pv, O_p, _, pv_ns, pv_gs = _layout("prefix_values", prefix_v)
-        if (G_p, K_p) != (G, K):
+        if G_p != G or K_p != K:
             raise ValueError(f"prefix_keys must have the heads and features of keys (G={G}, K={K}), got {G_p} and {K_p}")
-        if (P_v, G_pv, O_p) != (P, G, O):
+        if P > _MAX_EXTENT:
+            raise ValueError(f"at most {_MAX_EXTENT} keys: got P={P}")
+        if P_v != P or G_pv != G or O_p != O:
             raise ValueError(f"prefix_values must have the tokens of prefix_keys and the heads and features of values (P={P}, G={G}, O={O}), "
                              f"got {P_v}, {G_pv} and {O_p}")
-        params.prefix_n, params.causal = P, 1
-        params.prefix_key, params.prefix_key_ns, params.prefix_key_gs = prefix_k.data_ptr(), pk_ns, pk_gs
-        params.prefix_value, params.prefix_value_ns, params.prefix_value_gs = prefix_v.data_ptr(), pv_ns, pv_gs
+        causal, pk_ptr, pv_ptr = 1, prefix_k.data_ptr(), prefix_v.data_ptr()
 
-    plan.out = out = _result("out", out, (L, M, H, O), queries, require_device)
-    strides = out.stride()
-    if strides[-1] != 1 and O > 1:
-        raise ValueError("out must have stride 1 in last dimension")
-    params.out, params.out_ls, params.out_ms, params.out_hs = out.data_ptr(), strides[0] if len(strides) == 4 else 0, strides[-3], strides[-2]
-    plan.lse = None
+    if out is None:
+        # (a dense tensor of that shape either way; the first form is the quicker call)
+        out = torch.empty_like(queries, memory_format=torch.contiguous_format) if O == K and len(queries.shape) == 4 else torch.empty(
+            (L, M, H, O), dtype=dtype, device=device)
+        o_hs = O
+        o_ms = H * o_hs
+        o_ls = M * o_ms
+    else:
+        o_ls, o_ms, o_hs = _strides_of_result("out", out, (L, M, H, O), device, dtype)
+    plan = _AttentionPlan()
+    plan.lse, lse_ptr = None, 0
     if return_lse:
         plan.lse = torch.empty((L, M, H), dtype=torch.float32, device=device)
-        params.lse = plan.lse.data_ptr()
-    plan.params = params
+        lse_ptr = plan.lse.data_ptr()
+    plan.out, plan.device = out, device
+    plan.extents = (L, M, N, H, G, K, O, P, causal)
+    plan.fields = (element, 0, L, M, N, H, G, K, O, scale, queries.data_ptr(), q_ls, q_ms, q_hs, keys.data_ptr(), k_ls, k_ns, k_gs,
+                   values.data_ptr(), v_ls, v_ns, v_gs, out.data_ptr(), o_ls, o_ms, o_hs, lse_ptr, lengths_ptr, mask_ptr, mask_ls, mask_ns, P, causal,
+                   pk_ptr, pk_ns, pk_gs, pv_ptr, pv_ns, pv_gs)
     return plan
 
 
-def _launch(plan, device, debug):
-    stream = _current_stream_for(device)
-    params = plan.params
-    needed = _backend.attention_workspace_bytes(params)
-    workspace = _scratch.allocate(needed, device) if needed else None
-    if workspace is not None:           # refused: one pass over the keys per tile of rows
-        params.workspace, params.workspace_bytes = workspace.data_ptr(), needed
+def _launch(plan, debug):
+    stream = _current_stream_for(plan.device)
+    needed = _workspace_bytes(*plan.extents)
+    workspace = _scratch.allocate(needed, plan.device) if needed else None
     if debug:
         print(f"(Kermac Debug) Launching kernel: attention_forward{' and attention_join' if workspace is not None else ''}")
-    _backend.attention(params, stream)
+    if workspace is not None:
+        _backend.attention(_PARAMS.pack(*plan.fields, workspace.data_ptr(), needed), stream)
+    else:                               # none needed, or refused: one pass over the keys per tile of rows
+        _backend.attention(_PARAMS.pack(*plan.fields, 0, 0), stream)
     # the launches are queued: the allocator hands the workspace on in stream order
 
 
@@ -208,34 +236,42 @@ def cross_attention(
         ValueError: bad shapes, strides, batch sizes or devices, a scale that is not finite.
     """
     plan = _plan_attention(queries, keys, values, out, scale, key_lengths, key_mask, return_lse)
-    _launch(plan, queries.device, debug)
+    _launch(plan, debug)
     return (plan.out, plan.lse) if return_lse else plan.out
 
 
-def _plan_attention_grad(grad_out, queries, keys, values, out, lse, scale, key_lengths, key_mask, require_device=True):
+class _GradientPlan:
+    __slots__ = ("fields", "extents", "out", "device")
+
+    @property
+    def params(self) -> _backend.AttentionGradientParams:
+        return _backend.AttentionGradientParams.from_buffer_copy(_GRADIENT_PARAMS.pack(*self.fields, 0, 0))
+
+
+def _plan_attention_grad(grad_out, queries, keys, values, out, lse, scale, key_lengths, key_mask, require_device=True) -> _GradientPlan:
     """The checks of the forward call, whose result `out` and `lse` are, and the gradient's parameters."""
-    forward = _plan_attention(queries, keys, values, out, scale, key_lengths, key_mask, False, require_device=require_device)
-    of = forward.params
-    device = queries.device
-    shape = (of.l, of.m, of.h, of.o)
-    _check_tensors((("grad_out", grad_out),), device, queries.dtype, require_device)
-    if tuple(grad_out.shape) != shape and not (grad_out.dim() == 3 and of.l == 1 and tuple(grad_out.shape) == shape[1:]):
-        raise ValueError(f"grad_out must have shape {shape}, got {tuple(grad_out.shape)}")
-    _, _, _, _, d_ls, d_ms, d_hs = _layout("grad_out", grad_out)
-    _check_tensors((("lse", lse),), device, torch.float32, require_device)
-    if tuple(lse.shape) != shape[:3] or not lse.is_contiguous():
-        raise ValueError(f"lse must be contiguous with shape {shape[:3]}, got {tuple(lse.shape)}")
-    make = torch.zeros if queries.numel() == 0 else torch.empty         # no query: nothing is launched
+    if out is None:
+        raise TypeError("out must be a PyTorch tensor")
+    of = _plan_attention(queries, keys, values, out, scale, key_lengths, key_mask, False, require_device=require_device)
+    L, M, N, H, G, K, O, _, _ = of.extents
+    device, dtype = of.device, queries.dtype
+    L_d, M_d, H_d, O_d, d_ls, d_ms, d_hs = _operand("grad_out", grad_out, device, dtype)
+    if (L_d, M_d, H_d, O_d) != (L, M, H, O):
+        raise ValueError(f"grad_out must have shape {(L, M, H, O)}, got {tuple(grad_out.shape)}")
+    _check("lse", lse, device, torch.float32)
+    if tuple(lse.shape) != (L, M, H) or not lse.is_contiguous():
+        raise ValueError(f"lse must be contiguous with shape {(L, M, H)}, got {tuple(lse.shape)}")
     key_entries = keys.size(0) if keys.dim() == 4 else 1
-    grads = (torch.empty(queries.shape, dtype=queries.dtype, device=device), make(keys.shape, dtype=keys.dtype, device=device),
-             make(values.shape, dtype=values.dtype, device=device))
-    params = _backend.AttentionGradientParams(
-        of.type, 0, of.l, of.m, of.n, of.h, of.g, of.k, of.o, key_entries, of.scale, of.q, of.q_ls, of.q_ms, of.q_hs, of.key, of.key_ls, of.key_ns, of.key_gs,
-        of.value, of.value_ls, of.value_ns, of.value_gs, of.out, of.out_ls, of.out_ms, of.out_hs, grad_out.data_ptr(), d_ls, d_ms, d_hs, lse.data_ptr(),
-        of.key_lengths, of.key_mask, of.key_mask_ls, of.key_mask_ns, grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr())
-    plan = _AttentionPlan()
-    plan.params, plan.out, plan.lse = params, grads, None
-    plan.keepalive = [forward, grad_out, lse]
+    contiguous = torch.contiguous_format
+    make = torch.empty_like if L * M * H else torch.zeros_like         # no query: nothing is launched
+    grad_q = torch.empty_like(queries, memory_format=contiguous)
+    grad_k, grad_v = make(keys, memory_format=contiguous), make(values, memory_format=contiguous)
+    plan = _GradientPlan()
+    plan.out, plan.device = (grad_q, grad_k, grad_v), device
+    plan.extents = (L, M, N, H, G, K, O, key_entries)
+    # type .. o of the forward block, key_entries, scale, then its operands up to out's strides
+    plan.fields = (*of.fields[:9], key_entries, *of.fields[9:26], grad_out.data_ptr(), d_ls, d_ms, d_hs, lse.data_ptr(), *of.fields[27:31],
+                   grad_q.data_ptr(), grad_k.data_ptr(), grad_v.data_ptr())
     return plan
 
 
@@ -261,7 +297,7 @@ def cross_attention_grad(
     keys.  Sums are fp32 in an order that does not depend on timing; in fp16 the products of weights and gradients are
     numbers of that type, so gradients far below 1e-4 want a loss scale.
 
-    Returns ``(grad_queries, grad_keys, grad_values)``, new contiguous tensors with the shapes of the inputs.  Takes 4 bytes of
+    Returns ``(grad_queries, grad_keys, grad_values)``, new contiguous tensors with the shapes of the inputs.  Takes 8 bytes of
     scratch memory per row at least.
 
     Raises:
@@ -270,20 +306,19 @@ def cross_attention_grad(
         RuntimeError: the limit on scratch memory, or the supplied buffer, does not allow those bytes.
     """
     plan = _plan_attention_grad(grad_out, queries, keys, values, out, lse, scale, key_lengths, key_mask)
-    params, device = plan.params, queries.device
-    stream = _current_stream_for(device)
-    needed = _backend.attention_gradient_workspace_bytes(params)
+    stream = _current_stream_for(plan.device)
+    needed, workspace = _gradient_workspace_bytes(*plan.extents), None
     if needed:
-        workspace = _scratch.allocate(needed, device)
-        if workspace is None:           # refused: uncut launches, with room for one sum per row
-            needed = -(-4 * params.l * params.m * params.h // 16) * 16
-            workspace = _scratch.allocate(needed, device)
+        workspace = _scratch.allocate(needed, plan.device)
+        if workspace is None:           # refused: uncut launches, with room for the sums of a row
+            L, M, _, H = plan.extents[:4]
+            needed = -(-8 * L * M * H // 16) * 16
+            workspace = _scratch.allocate(needed, plan.device)
         if workspace is None:
             raise RuntimeError(f"cross_attention_grad needs {needed} bytes of scratch memory: the limit, the supplied buffer or the device does not allow them")
-        params.workspace, params.workspace_bytes = workspace.data_ptr(), needed
     if debug:
         print("(Kermac Debug) Launching kernel: attention_grad_queries, attention_grad_keys")
-    _backend.attention_gradient(params, stream)
+    _backend.attention_gradient(_GRADIENT_PARAMS.pack(*plan.fields, workspace.data_ptr() if needed else 0, needed), stream)
     return plan.out
 
 
@@ -314,5 +349,5 @@ def prefix_attention(
     if not isinstance(lengths, torch.Tensor):
         raise TypeError("lengths must be a PyTorch tensor")
     plan = _plan_attention(queries, keys, values, out, scale, lengths, None, False, prefix=(prefix_keys, prefix_values))
-    _launch(plan, queries.device, debug)
+    _launch(plan, debug)
     return plan.out

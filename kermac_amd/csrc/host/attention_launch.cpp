@@ -196,8 +196,8 @@ int parts(int64_t base, int64_t extent, int64_t least)
 struct GradPlan {
     kmc::AttentionGradArgs args;
     bool aligned, empty;
-    int64_t delta_bytes, q_bytes, k_bytes, v_bytes;
-    int64_t bytes() const { return delta_bytes + q_bytes + k_bytes + v_bytes; }
+    int64_t stats_bytes, q_bytes, k_bytes, v_bytes;
+    int64_t bytes() const { return stats_bytes + q_bytes + k_bytes + v_bytes; }
 };
 
 constexpr int MIN_ROW_TILES = 4;                    // tiles of rows that a part of the keys' kernel walks at least
@@ -256,7 +256,7 @@ int prepare(const kmc_attention_gradient_params *p, bool may_cut, GradPlan *plan
     args.k_grid = static_cast<int>((k_workgroups + 7) / 8 * 8);
 
     const int64_t q_rows = static_cast<int64_t>(p->l) * p->m * p->h, k_rows = static_cast<int64_t>(p->key_entries) * p->n * p->g;
-    plan->delta_bytes = (4 * q_rows + 15) / 16 * 16;
+    plan->stats_bytes = (8 * q_rows + 15) / 16 * 16;
     if (args.q_splits > 1) plan->q_bytes = 4ll * args.q_splits * q_rows * args.partial_k_width;
     if (args.k_splits > 1) {
         plan->k_bytes = 4ll * args.k_splits * k_rows * args.partial_k_width;
@@ -345,8 +345,8 @@ int kmc_attention_gradient(const kmc_attention_gradient_params *params, void *st
     if (status != KMC_OK) return status;
     kmc::AttentionGradArgs &args = plan.args;
     char *at = static_cast<char *>(params->workspace);
-    args.delta = reinterpret_cast<float *>(at);
-    args.partial_q = reinterpret_cast<float *>(at += plan.delta_bytes);
+    args.stats = reinterpret_cast<float *>(at);
+    args.partial_q = reinterpret_cast<float *>(at += plan.stats_bytes);
     args.partial_k = reinterpret_cast<float *>(at += plan.q_bytes);
     args.partial_v = reinterpret_cast<float *>(at += plan.k_bytes);
     const int width = std::max(params->k, params->o);

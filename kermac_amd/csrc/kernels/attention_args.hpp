@@ -50,7 +50,7 @@ struct AttentionGradArgs {
     int l, m, g, r, k, o;
     int key_entries;                        // l, or 1: one source for all entries
     float scale, scale_log2, query_factor;
-    float *delta;                           // [l, m, g r]: sum_o out grad_out, written by the first kernel for the second
+    float *stats;                           // [2, l, m, g r]: lse to base 2 (+inf without keys) and delta, from the first kernel for the second
     int q_row_tiles, q_splits, q_workgroups, q_grid;
     int key_tiles, k_splits, k_workgroups, k_grid;
     float *partial_q, *partial_k, *partial_v;   // [splits, rows, width rounded up to 4], where the work is cut

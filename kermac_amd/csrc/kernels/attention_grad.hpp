@@ -73,16 +73,25 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
         for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(static_cast<float>(grad[step][j]), static_cast<float>(result[j]), delta);
     }
     delta += att_other_half(delta);
-    const float lse2 = att_lse2(args.lse[at]);
-    if (split == 0 && row < rows && half == 0) args.delta[at] = delta;
+    float lse2 = att_lse2(args.lse[at]);
 
     att_f32x16 acc[DP / 32];
 #pragma unroll
     for (int o = 0; o < DP / 32; ++o) acc[o] = att_f32x16{0};
 
     const AttentionKeys &keys = args.keys;
+    const int length = att_length(keys, entry);
     int begin, end;
-    att_range(att_length(keys, entry), KT, split, args.q_splits, &begin, &end);
+    att_range(length, KT, split, args.q_splits, &begin, &end);
+    const bool one_tile = length <= KT;
+    const i64 rows_total = static_cast<i64>(args.l) * args.m * args.g * args.r;
+    auto write_stats = [&]() {
+        if (split == 0 && row < rows && half == 0) {
+            args.stats[at] = lse2;
+            args.stats[rows_total + at] = delta;
+        }
+    };
+    if (!one_tile || begin >= end) write_stats();
     const T *k = static_cast<const T *>(keys.k) + entry * keys.k_ls + g * keys.k_gs;
     const T *v = static_cast<const T *>(keys.v) + entry * keys.v_ls + g * keys.v_gs;
     AttTile<T, DP, KT, 256, ALIGNED> next_k, next_v;
@@ -103,6 +112,35 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
             next_v.load(v + next * keys.v_ns, keys.v_ns, end - static_cast<int>(next), args.o, threadIdx.x);
         }
         if (!works) continue;
+        if (one_tile) {
+            // Few keys: delta from the rounded result would be off by as much as ds is large, so it is summed from the weights themselves,
+            // which are normalised again while they are at hand (a single key's weight is exactly 1, its ds exactly 0).
+            float total = 0.0f, inner = 0.0f;
+#pragma unroll
+            for (int b = 0; b < KT / 32; ++b) {
+                att_f32x16 s = {0}, ds = {0};
+#pragma unroll
+                for (int step = 0; step < DP / 16; ++step) {
+                    s = att_mma(att_read_row<T, DP>(key_tile, ATT_STRIDE<T, DP>, 32 * b + lane % 32, 16 * step + 8 * half), query[step], s);
+                    ds = att_mma(att_read_row<T, DP>(value_tile, ATT_STRIDE<T, DP>, 32 * b + lane % 32, 16 * step + 8 * half), grad[step], ds);
+                }
+                const unsigned mine = static_cast<unsigned>(kept >> (32 * b)) >> (4 * half);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (!(mine >> att_row(i, 0) & 1)) continue;
+                    const float p = length == 1 ? 1.0f : att_weight(s[i], args.scale_log2, lse2);
+                    total += p;
+                    inner = __builtin_fmaf(p, ds[i], inner);
+                }
+            }
+            total += att_other_half(total);
+            inner += att_other_half(inner);
+            if (total > 0.0f) {
+                delta = inner / total;
+                if (length > 1) lse2 += __builtin_amdgcn_logf(total);
+            }
+            write_stats();
+        }
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b) {
             att_f32x16 s = {0}, ds = {0};
@@ -131,7 +169,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     }
     if (row >= rows) return;
     if (args.q_splits > 1) {
-        float *to = args.partial_q + (split * (static_cast<i64>(args.l) * args.m * args.g * args.r) + at) * args.partial_k_width;
+        float *to = args.partial_q + (split * rows_total + at) * args.partial_k_width;
 #pragma unroll
         for (int o = 0; o < DP / 32; ++o)
 #pragma unroll
@@ -212,6 +250,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
         kept = exists && n < att_length(keys, of) && (!keys.mask || keys.mask[of * keys.mask_ls + n * keys.mask_ns] != 0);
         all_kept = __all(kept);
     };
+    const i64 rows_total = static_cast<i64>(args.l) * args.m * args.g * args.r;
     AttTile<T, DP, RT, 256, ALIGNED> next_q, next_d;
     float next_stat = 0.0f;
     auto load = [&]() {
@@ -222,8 +261,8 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
                     some, args.o, threadIdx.x);
         const int i = threadIdx.x % RT;
         const i64 at = (static_cast<i64>(entry) * args.m + m0 + i) * (static_cast<i64>(args.g) * args.r) + h;
-        if (threadIdx.x < RT) next_stat = i < some ? att_lse2(args.lse[at]) : __builtin_inff();
-        else if (threadIdx.x < 2 * RT) next_stat = i < some ? args.delta[at] : 0.0f;
+        if (threadIdx.x < RT) next_stat = i < some ? args.stats[at] : __builtin_inff();
+        else if (threadIdx.x < 2 * RT) next_stat = i < some ? args.stats[rows_total + at] : 0.0f;
     };
     find();
     int kept_entry = -1;
