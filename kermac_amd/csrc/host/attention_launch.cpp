@@ -26,7 +26,8 @@ constexpr int MAX_SLOTS = 128;
 
 int element_size(int type) { return type == KMC_FP32 ? 4 : 2; }
 
-// Whether rows can be read and written 16 bytes at a time: the address, and the stride of every dimension that is walked.
+// Whether rows can be read and written 16 bytes at a time: the address, and the stride of every dimension that is walked.  The tokens of a
+// tile are read through one buffer descriptor, which wants rows that do not overlap and a tile that it can number in 31 bits.
 struct Layout {
     int size;
     bool aligned = true;
@@ -37,6 +38,11 @@ struct Layout {
     void stride(int extent, int64_t stride)
     {
         if (extent > 1) aligned = aligned && stride * size % 16 == 0;
+    }
+    void tokens(int extent, int64_t stride, int width)
+    {
+        this->stride(extent, stride);
+        aligned = aligned && (extent <= 1 || stride >= width) && stride * size < (1 << 24);
     }
 };
 
@@ -172,14 +178,14 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
     if (p->n > 0) {
         layout.operand(p->key, p->k);
         layout.operand(p->value, p->o);
-        layout.stride(p->l, p->key_ls); layout.stride(p->n, p->key_ns); layout.stride(p->g, p->key_gs);
-        layout.stride(p->l, p->value_ls); layout.stride(p->n, p->value_ns); layout.stride(p->g, p->value_gs);
+        layout.stride(p->l, p->key_ls); layout.tokens(p->n, p->key_ns, p->k); layout.stride(p->g, p->key_gs);
+        layout.stride(p->l, p->value_ls); layout.tokens(p->n, p->value_ns, p->o); layout.stride(p->g, p->value_gs);
     }
     if (prefixed) {
         layout.operand(p->prefix_key, p->k);
         layout.operand(p->prefix_value, p->o);
-        layout.stride(p->prefix_n, p->prefix_key_ns); layout.stride(p->g, p->prefix_key_gs);
-        layout.stride(p->prefix_n, p->prefix_value_ns); layout.stride(p->g, p->prefix_value_gs);
+        layout.tokens(p->prefix_n, p->prefix_key_ns, p->k); layout.stride(p->g, p->prefix_key_gs);
+        layout.tokens(p->prefix_n, p->prefix_value_ns, p->o); layout.stride(p->g, p->prefix_value_gs);
     }
     plan->aligned = layout.aligned && !(p->flags & KMC_FLAG_FORCE_SCALAR_ACCESS);
     return KMC_OK;
@@ -265,13 +271,13 @@ int prepare(const kmc_attention_gradient_params *p, bool may_cut, GradPlan *plan
 
     Layout layout{element_size(p->type)};
     layout.operand(p->q, p->k); layout.operand(p->out, p->o); layout.operand(p->grad_out, p->o); layout.operand(p->grad_q, p->k);
-    layout.stride(p->l, p->q_ls); layout.stride(p->m, p->q_ms); layout.stride(p->h, p->q_hs);
+    layout.stride(p->l, p->q_ls); layout.tokens(p->m, p->q_ms, p->k); layout.stride(p->h, p->q_hs);
     layout.stride(p->l, p->out_ls); layout.stride(p->m, p->out_ms); layout.stride(p->h, p->out_hs);
-    layout.stride(p->l, p->grad_out_ls); layout.stride(p->m, p->grad_out_ms); layout.stride(p->h, p->grad_out_hs);
+    layout.stride(p->l, p->grad_out_ls); layout.tokens(p->m, p->grad_out_ms, p->o); layout.stride(p->h, p->grad_out_hs);
     if (p->n > 0) {
         layout.operand(p->key, p->k); layout.operand(p->value, p->o); layout.operand(p->grad_key, p->k); layout.operand(p->grad_value, p->o);
-        layout.stride(p->l, p->key_ls); layout.stride(p->n, p->key_ns); layout.stride(p->g, p->key_gs);
-        layout.stride(p->l, p->value_ls); layout.stride(p->n, p->value_ns); layout.stride(p->g, p->value_gs);
+        layout.stride(p->l, p->key_ls); layout.tokens(p->n, p->key_ns, p->k); layout.stride(p->g, p->key_gs);
+        layout.stride(p->l, p->value_ls); layout.tokens(p->n, p->value_ns, p->o); layout.stride(p->g, p->value_gs);
     }
     plan->aligned = layout.aligned && !(p->flags & KMC_FLAG_FORCE_SCALAR_ACCESS);
     return KMC_OK;

@@ -3,7 +3,7 @@
 //   s[m, n] = scale sum_k q[m, k] k[n, k],   lse[m] = log sum_n exp s[m, n],   out[m, o] = sum_n exp(s[m, n] - lse[m]) v[n, o]
 //
 // over the keys n that take part.  One pass over keys and values: a running maximum and a running sum per query, the
-// output rescaled when the maximum grows (both in fp32; exponentials to base 2 with log2(e) folded into the scale).
+// output rescaled when the maximum has grown (both in fp32; exponentials to base 2 with log2(e) folded into the scale).
 //
 // Queries of the heads that share a head of keys are the rows of one problem: row r is query r / R of head r % R
 // (R heads per head of keys), so keys and values are read once for all of them.  Queries of all batch entries
@@ -138,6 +138,11 @@ __device__ __forceinline__ att_vec8<T> att_load8(const T *row, int at, int width
     return u.whole;
 }
 
+constexpr int ATT_BUFFER_FORMAT = 0x00020000;        // 32-bit data, as raw buffers of this architecture want it
+
+// Keeps the compiler from merging a rare case into the common path as selections.
+__device__ __forceinline__ void att_rare() { asm volatile(""); }
+
 // A tile of ROWS rows of DP elements on its way from memory to LDS through the registers of THREADS threads.
 template <typename T, int DP, int ROWS, int THREADS, bool ALIGNED>
 struct AttTile {
@@ -148,30 +153,47 @@ struct AttTile {
     static constexpr int ROW_STEP = THREADS / CHUNKS;
     att_u32x4 held[PER_THREAD];
 
-    // Rows 0 .. rows - 1 of base (rows of `width` elements, `stride` apart); rows behind them read as zero.
+    // Rows 0 .. rows - 1 of base (rows of `width` elements, `stride` apart); rows behind them read as zero.  Aligned rows are read through
+    // a buffer descriptor that ends behind the last one: what lies outside reads as zero without a branch per load.
     __device__ __forceinline__ void load(const T *base, i64 stride, int rows, int width, int thread)
     {
         const int row = thread / CHUNKS, at = thread % CHUNKS * CHUNK;
-        const T *p = base + row * stride;
+        if constexpr (ALIGNED) {
+            const int some = rows < ROWS ? rows : ROWS, step = static_cast<int>(stride) * static_cast<int>(sizeof(T));
+            const int bytes = some > 0 ? (some - 1) * step + width * static_cast<int>(sizeof(T)) : 0;
+            const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, bytes, ATT_BUFFER_FORMAT);
+            unsigned offset = at < width ? static_cast<unsigned>(row * step + at * static_cast<int>(sizeof(T))) : 0x80000000u;
 #pragma unroll
-        for (int j = 0; j < PER_THREAD; ++j) {
-            held[j] = att_u32x4{0, 0, 0, 0};
-            if (row + j * ROW_STEP < rows) held[j] = att_load16<T, ALIGNED>(p, at, width);
-            p += ROW_STEP * stride;
+            for (int j = 0; j < PER_THREAD; ++j) {
+                held[j] = __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0);
+                offset += ROW_STEP * step;
+            }
+        } else {
+            const T *p = base + row * stride;
+#pragma unroll
+            for (int j = 0; j < PER_THREAD; ++j) {
+                held[j] = att_u32x4{0, 0, 0, 0};
+                if (row + j * ROW_STEP < rows) held[j] = att_load16<T, false>(p, at, width);
+                p += ROW_STEP * stride;
+            }
         }
     }
 
-    // Rows whose bit in `kept` is not set are stored as zeros.
     template <int STRIDE>
-    __device__ __forceinline__ void store(T *tile, int thread, bool all_kept, att_u64 kept) const
+    __device__ __forceinline__ void store(T *tile, int thread) const
     {
         const int row = thread / CHUNKS, at = thread % CHUNKS * CHUNK;
 #pragma unroll
-        for (int j = 0; j < PER_THREAD; ++j) {
-            att_u32x4 x = held[j];
-            if (!all_kept && !(kept >> (row + j * ROW_STEP) & 1)) x = att_u32x4{0, 0, 0, 0};
-            *reinterpret_cast<att_u32x4 *>(tile + (row + j * ROW_STEP) * STRIDE + at) = x;
-        }
+        for (int j = 0; j < PER_THREAD; ++j) *reinterpret_cast<att_u32x4 *>(tile + (row + j * ROW_STEP) * STRIDE + at) = held[j];
+    }
+
+    // Rows whose bit in `kept` is not set become zeros.
+    __device__ __forceinline__ void clear(int thread, att_u64 kept)
+    {
+        const int row = thread / CHUNKS;
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; ++j)
+            if (!(kept >> (row + j * ROW_STEP) & 1)) held[j] = att_u32x4{0, 0, 0, 0};
     }
 };
 
@@ -203,8 +225,12 @@ __device__ __forceinline__ void att_wave_sync()
 template <int DP>
 struct AttState {
     att_f32x16 out[DP / 32];
-    float top, sum;              // the largest score so far and the sum of this lane's exponentials below it, to base 2
+    float top, sum;              // a score near the largest so far and the sum of this lane's exponentials relative to it, to base 2
 };
+
+// Outputs and sums are rescaled only when a score passes the one they are relative to by 2^8: exponentials stay below 256, far inside every type,
+// and after the first tiles the 64 or more multiplications per tile are not made.
+constexpr float ATT_HEADROOM = 8.0f;
 
 // One tile of KT keys in LDS against the 32 rows whose queries are in `query`.  `kept` has a bit per key for this lane's row.
 template <typename T, int DP, int KT>
@@ -222,6 +248,7 @@ __device__ __forceinline__ void att_forward_tile(AttState<DP> &state, const att_
     }
     const att_u64 all = KT == 64 ? ~0ull : (1ull << KT) - 1;
     if (!__all((kept & all) == all)) {
+        att_rare();
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b) {
             const unsigned mine = static_cast<unsigned>(kept >> (32 * b)) >> (4 * half);
@@ -234,11 +261,17 @@ __device__ __forceinline__ void att_forward_tile(AttState<DP> &state, const att_
     for (int b = 0; b < KT / 32; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-    top = fmaxf(top, att_other_half(top));
-    top = fmaxf(state.top, top * scale_log2);
-    const float base = top == -__builtin_inff() ? 0.0f : top;          // no key of this row yet: every exponential below is 0
-    const float shrink = __builtin_amdgcn_exp2f(state.top - base);
-    state.top = top;
+    top = fmaxf(top, att_other_half(top)) * scale_log2;
+    if (!__all(top <= state.top + ATT_HEADROOM)) {
+        att_rare();
+        top = fmaxf(state.top, top);
+        const float shrink = __builtin_amdgcn_exp2f(state.top - (top == -__builtin_inff() ? 0.0f : top));
+        state.top = top;
+        state.sum *= shrink;
+#pragma unroll
+        for (int o = 0; o < DP / 32; ++o) state.out[o] *= shrink;
+    }
+    const float base = state.top == -__builtin_inff() ? 0.0f : state.top;          // no key of this row yet: every exponential below is 0
     float sum = 0.0f;
 #pragma unroll
     for (int b = 0; b < KT / 32; ++b)
@@ -247,11 +280,7 @@ __device__ __forceinline__ void att_forward_tile(AttState<DP> &state, const att_
             s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale_log2, -base));
             sum += s[b][i];
         }
-    state.sum = state.sum * shrink + sum;
-    if (!__all(shrink == 1.0f)) {
-#pragma unroll
-        for (int o = 0; o < DP / 32; ++o) state.out[o] *= shrink;
-    }
+    state.sum += sum;
 #pragma unroll
     for (int b = 0; b < KT / 32; ++b)
 #pragma unroll
@@ -443,8 +472,9 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
             for (int n = begin; n < end; n += KT) {
                 const att_u64 kept = att_kept_keys(keys, entry, n, end, lane);
                 __syncthreads();
-                next_k.template store<ATT_STRIDE<T, DP>>(key_tile, threadIdx.x, true, 0);
-                next_v.template store<ATT_STRIDE_T<T, DP>>(value_tile, threadIdx.x, !keys.mask, kept);
+                next_k.template store<ATT_STRIDE<T, DP>>(key_tile, threadIdx.x);
+                if (keys.mask) next_v.clear(threadIdx.x, kept);
+                next_v.template store<ATT_STRIDE_T<T, DP>>(value_tile, threadIdx.x);
                 __syncthreads();
                 if (n + KT < end) {
                     const i64 at = n + KT;
@@ -480,8 +510,9 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                 }
                 for (; n < end; n += KT * WAVES) {
                     const att_u64 kept = att_kept_keys(keys, entry, static_cast<int>(n), end, lane);
-                    next_k.template store<ATT_STRIDE<T, DP>>(key_tile, lane, true, 0);
-                    next_v.template store<ATT_STRIDE_T<T, DP>>(value_tile, lane, !keys.mask, kept);
+                    next_k.template store<ATT_STRIDE<T, DP>>(key_tile, lane);
+                    if (keys.mask) next_v.clear(lane, kept);
+                    next_v.template store<ATT_STRIDE_T<T, DP>>(value_tile, lane);
                     att_wave_sync();
                     const i64 at = n + KT * WAVES;
                     if (at < end) {

@@ -85,16 +85,51 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     att_range(length, KT, split, args.q_splits, &begin, &end);
     const bool one_tile = length <= KT;
     const i64 rows_total = static_cast<i64>(args.l) * args.m * args.g * args.r;
-    auto write_stats = [&]() {
-        if (split == 0 && row < rows && half == 0) {
-            args.stats[at] = lse2;
-            args.stats[rows_total + at] = delta;
-        }
-    };
-    if (!one_tile || begin >= end) write_stats();
     const T *k = static_cast<const T *>(keys.k) + entry * keys.k_ls + g * keys.k_gs;
     const T *v = static_cast<const T *>(keys.v) + entry * keys.v_ls + g * keys.v_gs;
     AttTile<T, DP, KT, 256, ALIGNED> next_k, next_v;
+    if (one_tile && begin < end) {
+        // Few keys: delta from the rounded result would be off by as much as ds is large, so it is summed from the weights themselves,
+        // which are normalised again while they are at hand (a single key's weight is exactly 1, its ds exactly 0).
+        const att_u64 kept = att_kept_keys(keys, entry, begin, end, lane);
+        next_k.load(k, keys.k_ns, end, args.k, threadIdx.x);
+        next_v.load(v, keys.v_ns, end, args.o, threadIdx.x);
+        if (keys.mask) {
+            next_k.clear(threadIdx.x, kept);
+            next_v.clear(threadIdx.x, kept);
+        }
+        next_k.template store<ATT_STRIDE<T, DP>>(key_tile, threadIdx.x);
+        next_v.template store<ATT_STRIDE<T, DP>>(value_tile, threadIdx.x);
+        __syncthreads();
+        float total = 0.0f, inner = 0.0f;
+#pragma unroll 1
+        for (int b = 0; b < KT / 32; ++b) {
+            att_f32x16 s = {0}, ds = {0};
+#pragma unroll
+            for (int step = 0; step < DP / 16; ++step) {
+                s = att_mma(att_read_row<T, DP>(key_tile, ATT_STRIDE<T, DP>, 32 * b + lane % 32, 16 * step + 8 * half), query[step], s);
+                ds = att_mma(att_read_row<T, DP>(value_tile, ATT_STRIDE<T, DP>, 32 * b + lane % 32, 16 * step + 8 * half), grad[step], ds);
+            }
+            const unsigned mine = static_cast<unsigned>(kept >> (32 * b)) >> (4 * half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const bool counts = mine >> att_row(i, 0) & 1;
+                const float p = !counts ? 0.0f : length == 1 ? 1.0f : att_weight(s[i], args.scale_log2, lse2);
+                total += p;
+                inner = __builtin_fmaf(p, ds[i], inner);
+            }
+        }
+        total += att_other_half(total);
+        inner += att_other_half(inner);
+        if (total > 0.0f) {
+            delta = inner / total;
+            if (length > 1) lse2 += __builtin_amdgcn_logf(total);
+        }
+    }
+    if (split == 0 && row < rows && half == 0) {
+        args.stats[at] = lse2;
+        args.stats[rows_total + at] = delta;
+    }
     if (begin < end) {
         next_k.load(k + begin * keys.k_ns, keys.k_ns, end - begin, args.k, threadIdx.x);
         next_v.load(v + begin * keys.v_ns, keys.v_ns, end - begin, args.o, threadIdx.x);
@@ -102,9 +137,13 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     for (int n = begin; n < end; n += KT) {
         const att_u64 kept = att_kept_keys(keys, entry, n, end, lane);
         __syncthreads();
-        next_k.template store<ATT_STRIDE<T, DP>>(key_tile, threadIdx.x, !keys.mask, kept);
-        next_k.template store<ATT_STRIDE_T<T, DP>>(key_tile_t, threadIdx.x, !keys.mask, kept);
-        next_v.template store<ATT_STRIDE<T, DP>>(value_tile, threadIdx.x, !keys.mask, kept);
+        if (keys.mask) {
+            next_k.clear(threadIdx.x, kept);
+            next_v.clear(threadIdx.x, kept);
+        }
+        next_k.template store<ATT_STRIDE<T, DP>>(key_tile, threadIdx.x);
+        next_k.template store<ATT_STRIDE_T<T, DP>>(key_tile_t, threadIdx.x);
+        next_v.template store<ATT_STRIDE<T, DP>>(value_tile, threadIdx.x);
         __syncthreads();
         if (n + KT < end) {
             const i64 next = n + KT;
@@ -112,35 +151,6 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
             next_v.load(v + next * keys.v_ns, keys.v_ns, end - static_cast<int>(next), args.o, threadIdx.x);
         }
         if (!works) continue;
-        if (one_tile) {
-            // Few keys: delta from the rounded result would be off by as much as ds is large, so it is summed from the weights themselves,
-            // which are normalised again while they are at hand (a single key's weight is exactly 1, its ds exactly 0).
-            float total = 0.0f, inner = 0.0f;
-#pragma unroll
-            for (int b = 0; b < KT / 32; ++b) {
-                att_f32x16 s = {0}, ds = {0};
-#pragma unroll
-                for (int step = 0; step < DP / 16; ++step) {
-                    s = att_mma(att_read_row<T, DP>(key_tile, ATT_STRIDE<T, DP>, 32 * b + lane % 32, 16 * step + 8 * half), query[step], s);
-                    ds = att_mma(att_read_row<T, DP>(value_tile, ATT_STRIDE<T, DP>, 32 * b + lane % 32, 16 * step + 8 * half), grad[step], ds);
-                }
-                const unsigned mine = static_cast<unsigned>(kept >> (32 * b)) >> (4 * half);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if (!(mine >> att_row(i, 0) & 1)) continue;
-                    const float p = length == 1 ? 1.0f : att_weight(s[i], args.scale_log2, lse2);
-                    total += p;
-                    inner = __builtin_fmaf(p, ds[i], inner);
-                }
-            }
-            total += att_other_half(total);
-            inner += att_other_half(inner);
-            if (total > 0.0f) {
-                delta = inner / total;
-                if (length > 1) lse2 += __builtin_amdgcn_logf(total);
-            }
-            write_stats();
-        }
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b) {
             att_f32x16 s = {0}, ds = {0};
@@ -154,6 +164,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
 #pragma unroll
             for (int i = 0; i < 16; ++i) ds[i] = att_weight(s[i], args.scale_log2, lse2) * (ds[i] - delta);
             if (here != ~0u) {
+                att_rare();
                 const unsigned mine = here >> (4 * half);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) ds[i] = mine >> att_row(i, 0) & 1 ? ds[i] : 0.0f;
@@ -273,10 +284,10 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
             kept_entry = entry;
         }
         __syncthreads();
-        next_q.template store<ATT_STRIDE<T, DP>>(q_tile, threadIdx.x, true, 0);
-        next_q.template store<ATT_STRIDE_T<T, DP>>(q_tile_t, threadIdx.x, true, 0);
-        next_d.template store<ATT_STRIDE<T, DP>>(d_tile, threadIdx.x, true, 0);
-        next_d.template store<ATT_STRIDE_T<T, DP>>(d_tile_t, threadIdx.x, true, 0);
+        next_q.template store<ATT_STRIDE<T, DP>>(q_tile, threadIdx.x);
+        next_q.template store<ATT_STRIDE_T<T, DP>>(q_tile_t, threadIdx.x);
+        next_d.template store<ATT_STRIDE<T, DP>>(d_tile, threadIdx.x);
+        next_d.template store<ATT_STRIDE_T<T, DP>>(d_tile_t, threadIdx.x);
         if (threadIdx.x < 2 * RT) stats[threadIdx.x] = next_stat;
         __syncthreads();
         ++item;
@@ -311,6 +322,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
             }
         }
         if (!all_kept) {
+            att_rare();
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 s[i] = kept ? s[i] : 0.0f;
