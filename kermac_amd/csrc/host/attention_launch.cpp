@@ -22,8 +22,6 @@ namespace {
 
 constexpr int MAX_WIDTH = 256;
 constexpr int MAX_KEYS = 0x7fffffff - 1024;         // a tile behind the last key still has a number
-constexpr int MAX_SLOTS = 128;
-
 int element_size(int type) { return type == KMC_FP32 ? 4 : 2; }
 
 // Whether rows can be read and written 16 bytes at a time: the address, and the stride of every dimension that is walked.  The tokens of a
@@ -68,34 +66,69 @@ void set_scale(float scale, float *scale_log2, float *query_factor)
     *query_factor = to_base_2 > 0.0f ? (scale < 0.0f ? -1.0f : 1.0f) : 0.0f;
 }
 
-// Workgroups that one launch wants before its keys are cut no further: two per CU.
-constexpr int WANTED_WORKGROUPS = 512;
 constexpr int ROWS_OF_OWN_KEYS = 32;                // up to here every wave walks keys of its own
 constexpr int ROWS_PER_WORKGROUP = 128;
-constexpr int MIN_KEYS_OWN = 128, MIN_KEYS_SHARED = 256;
+
+// How many parts the keys are cut into: the number with the smallest modelled time, in microseconds, fitted to sweeps of 1 .. 64 parts.
+//   Tiles of rows (bound by the matrix cores): 128 rows meet 64 keys in 2.1 us per 128 features in 16 bits (fp32: 7 times as long) while two
+//   workgroups share a CU, in 0.65 of that alone; a launch of more workgroups than fit waits for half of one at its end.
+//   Beside another job (`beside_us` of its own) the two share the chip.
+//   Single tokens (bound by memory): keys and values at 4.7 TB/s, but no workgroup faster than 4 us and 1.05 us per 128 keys of 128 features, and
+//   3.5 us of its place for a workgroup; the launch waits for the last ones, with lengths that differ for the longest.
+//   Joining the parts costs a launch, 5 us, and writing and reading a partial result per part.
+// 1 token against 32000 keys of 8 heads: 257 us in 1 part, 34.6 in the 32 of this rule, 32.2 in the best number, 16; 200 queries against 3000 keys 49.9 / 16.1;
+// 32 x 4000 x 16 heads of 64 features with lengths 82.9 / 75.7 (4 parts), best 73.3 (6); 128 x 1000 x 16 heads 92.1 uncut, 99.7 in 2 parts.
+double time_of_parts(int splits, int64_t base, int64_t rows_total, int64_t keys, bool own_keys, const kmc_attention_params *p, bool joined, double beside_us)
+{
+    const int features = std::max(p->k, p->o);
+    const double size = p->type == KMC_FP32 ? 4.0 : 2.0, width = features <= 64 ? 64 : features <= 96 ? 96 : features <= 128 ? 128 : 256;
+    const int64_t workgroups = base * splits, least = own_keys ? 128 : 64;
+    const double steps = static_cast<double>((keys + least * splits - 1) / (least * splits));
+    const double join_us = (splits > 1 || joined ? rows_total * p->o * 8.0 / 4.0e6 * splits : 0.0) + (splits > 1 && !joined ? 5.0 : 0.0);
+    if (own_keys) {
+        const double one = 4.0 + steps * 1.05 * width / 128 * (p->type == KMC_FP32 ? 5.5 : 1.0);
+        const double memory = keys * static_cast<double>(base) * (p->k + p->o) * size / 4.7e6 * (p->key_lengths ? 0.75 : 1.0);
+        return join_us + std::max(memory, one) + workgroups * 3.5 / 512 + one * (p->key_lengths ? 1.0 : 0.3);
+    }
+    const double tile_us = 2.1 * width / 128 * (p->type == KMC_FP32 ? 7.0 : 1.0), one = steps * tile_us;
+    if (beside_us > 0) return join_us + std::max(one, workgroups * one / 512 + beside_us);
+    return join_us + (workgroups <= 256 ? 0.65 * one : workgroups <= 512 ? one : workgroups * one / 512 + 0.5 * one);
+}
+
+int choose_parts(int64_t base, int64_t rows_total, int64_t keys, bool own_keys, const kmc_attention_params *p, bool joined, double *us)
+{
+    static const int candidates[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 40, 48, 64};
+    const double beside_us = *us;
+    int best = 0;
+    for (const int splits : candidates) {
+        if (splits > 1 && (splits - 1) * (own_keys ? 128 : 64) >= keys) break;
+        const double time = time_of_parts(splits, base, rows_total, keys, own_keys, p, joined, beside_us);
+        if (best == 0 || time < *us) {
+            *us = time;
+            best = splits;
+        }
+    }
+    return best;
+}
+static_assert(2 * 64 <= kmc::ATT_MAX_SLOTS, "the parts of two jobs");
 
 // false: more workgroups than a launch holds
-bool plan_job(kmc::AttentionJob *job, int first_segment, int last_segment, int64_t entries, int64_t rows, int heads, int keys, bool may_cut)
+bool plan_job(kmc::AttentionJob *job, int first_segment, int last_segment, int64_t entries, int64_t rows, int keys, bool may_cut, bool joined,
+              const kmc_attention_params *p, double *us)
 {
     job->first_segment = first_segment;
     job->last_segment = last_segment;
     job->rows = static_cast<int>(rows);
     job->own_keys = rows <= ROWS_OF_OWN_KEYS;
     job->row_tiles = job->own_keys ? 1 : static_cast<int>((rows + ROWS_PER_WORKGROUP - 1) / ROWS_PER_WORKGROUP);
-    const int64_t base = entries * heads * job->row_tiles;
-    int64_t splits = 1;
-    if (may_cut && base > 0) {
-        const int least = job->own_keys ? MIN_KEYS_OWN : MIN_KEYS_SHARED;
-        splits = std::min<int64_t>({(WANTED_WORKGROUPS + base / 2) / base, (static_cast<int64_t>(keys) + least - 1) / least, MAX_SLOTS / 2});
-        splits = std::max<int64_t>(splits, 1);
-    }
-    job->splits = static_cast<int>(splits);
-    const int64_t workgroups = base * splits;
+    const int64_t base = entries * p->g * job->row_tiles;
+    job->splits = may_cut ? choose_parts(base, static_cast<int64_t>(p->l) * p->m * p->h, keys, job->own_keys, p, joined, us) : 1;
+    const int64_t workgroups = base * job->splits;
     if (workgroups > 0x7fffff00ll / 2) return false;
     job->workgroups = static_cast<int>(workgroups);
     job->grid = static_cast<int>((workgroups + 7) / 8 * 8);
     job->slot = 0;
-    job->partial = 0;
+    job->partial = joined;
     return true;
 }
 
@@ -155,13 +188,14 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
     bool fits = true;
     if (with_workspace && prefixed) {
         // the prefix as one problem of the rows of all entries, the entries' own keys as another
-        fits = plan_job(&args.job[0], 0, 1, 1, p->l * rows, p->g, p->prefix_n, true);
-        fits = fits && plan_job(&args.job[1], 1, 2, p->l, rows, p->g, p->n, true);
-        args.job[0].partial = args.job[1].partial = 1;
+        double us = 0;
+        fits = plan_job(&args.job[1], 1, 2, p->l, rows, p->n, true, true, p, &us);
+        fits = fits && plan_job(&args.job[0], 0, 1, 1, p->l * rows, p->prefix_n, true, true, p, &us);
         args.job[1].slot = args.job[0].splits;
         args.slots = args.job[0].splits + args.job[1].splits;
     } else {
-        fits = plan_job(&args.job[0], 0, prefixed ? 2 : 1, p->l, rows, p->g, p->n, with_workspace);
+        double us = 0;
+        fits = plan_job(&args.job[0], 0, prefixed ? 2 : 1, p->l, rows, p->n, with_workspace, false, p, &us);
         if (args.job[0].splits > 1) {
             args.job[0].partial = 1;
             args.slots = args.job[0].splits;
@@ -191,11 +225,15 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
     return KMC_OK;
 }
 
+constexpr int WANTED_WORKGROUPS = 512;              // two per CU
+constexpr int MIN_KEYS = 256;                       // that a part of the queries' kernel walks at least
+constexpr int MAX_PARTS = 128;
+
 // Parts that `base` workgroups of `extent` steps each are cut into, `least` steps to a part.
 int parts(int64_t base, int64_t extent, int64_t least)
 {
     if (base == 0) return 1;
-    const int64_t wanted = std::min<int64_t>({(WANTED_WORKGROUPS + base / 2) / base, (extent + least - 1) / least, MAX_SLOTS});
+    const int64_t wanted = std::min<int64_t>({(WANTED_WORKGROUPS + base / 2) / base, (extent + least - 1) / least, MAX_PARTS});
     return static_cast<int>(std::max<int64_t>(wanted, 1));
 }
 
@@ -249,7 +287,7 @@ int prepare(const kmc_attention_gradient_params *p, bool may_cut, GradPlan *plan
     const int64_t rows = static_cast<int64_t>(p->m) * args.r;
     args.q_row_tiles = static_cast<int>((rows + 127) / 128);
     const int64_t q_base = static_cast<int64_t>(p->l) * p->g * args.q_row_tiles;
-    args.q_splits = may_cut ? parts(q_base, p->n, MIN_KEYS_SHARED) : 1;
+    args.q_splits = may_cut ? parts(q_base, p->n, MIN_KEYS) : 1;
     args.key_tiles = (p->n + 127) / 128;
     const int64_t k_base = static_cast<int64_t>(p->key_entries) * p->g * args.key_tiles;
     const int64_t tiles_of_rows = static_cast<int64_t>(args.r) * ((p->m + 31) / 32) * (p->key_entries == p->l ? 1 : p->l);

@@ -63,7 +63,7 @@ __device__ __forceinline__ float att_other_half(float x) { return __shfl_xor(x, 
 // into consecutive groups of four banks.  Read transposed: a 16-bit read touches 4 rows x 64 bytes per half wave, which 64
 // bytes of padding put side by side; an fp32 read touches a row each at a distance of 4 rows, 32 banks apart with 32 bytes.
 template <typename T, int DP> constexpr int ATT_STRIDE = DP + 16 / static_cast<int>(sizeof(T));
-template <typename T, int DP> constexpr int ATT_STRIDE_T = DP + (sizeof(T) == 2 ? 32 : 8);
+template <typename T, int DP> constexpr int ATT_STRIDE_T = DP + (sizeof(T) == 2 ? (DP == 96 ? 0 : 32) : 8);       // 16 or 48 banks mod 64
 
 template <typename T, int DP>
 __device__ __forceinline__ att_vec8<T> att_read_row(const T *tile, int stride, int row, int k)
@@ -148,16 +148,17 @@ template <typename T, int DP, int ROWS, int THREADS, bool ALIGNED>
 struct AttTile {
     static constexpr int CHUNK = 16 / sizeof(T);                    // elements of a 16-byte piece
     static constexpr int CHUNKS = DP / CHUNK;                       // pieces of a row
-    static constexpr int PER_THREAD = ROWS * CHUNKS / THREADS;
-    static_assert(ROWS * CHUNKS % THREADS == 0 && THREADS % CHUNKS == 0, "whole rows per step");
-    static constexpr int ROW_STEP = THREADS / CHUNKS;
+    static constexpr int SLOTS = CHUNKS <= 8 ? 8 : CHUNKS <= 16 ? 16 : CHUNKS <= 32 ? 32 : 64;        // threads of a row; those behind CHUNKS have no piece
+    static constexpr int ROW_STEP = THREADS / SLOTS;
+    static constexpr int PER_THREAD = ROWS / ROW_STEP;
+    static_assert(THREADS % SLOTS == 0 && ROWS % ROW_STEP == 0, "whole rows per step");
     att_u32x4 held[PER_THREAD];
 
     // Rows 0 .. rows - 1 of base (rows of `width` elements, `stride` apart); rows behind them read as zero.  Aligned rows are read through
     // a buffer descriptor that ends behind the last one: what lies outside reads as zero without a branch per load.
     __device__ __forceinline__ void load(const T *base, i64 stride, int rows, int width, int thread)
     {
-        const int row = thread / CHUNKS, at = thread % CHUNKS * CHUNK;
+        const int row = thread / SLOTS, at = thread % SLOTS * CHUNK;
         if constexpr (ALIGNED) {
             const int some = rows < ROWS ? rows : ROWS, step = static_cast<int>(stride) * static_cast<int>(sizeof(T));
             const int bytes = some > 0 ? (some - 1) * step + width * static_cast<int>(sizeof(T)) : 0;
@@ -182,7 +183,8 @@ struct AttTile {
     template <int STRIDE>
     __device__ __forceinline__ void store(T *tile, int thread) const
     {
-        const int row = thread / CHUNKS, at = thread % CHUNKS * CHUNK;
+        const int row = thread / SLOTS, at = thread % SLOTS * CHUNK;
+        if (SLOTS != CHUNKS && at >= DP) return;
 #pragma unroll
         for (int j = 0; j < PER_THREAD; ++j) *reinterpret_cast<att_u32x4 *>(tile + (row + j * ROW_STEP) * STRIDE + at) = held[j];
     }
@@ -190,7 +192,7 @@ struct AttTile {
     // Rows whose bit in `kept` is not set become zeros.
     __device__ __forceinline__ void clear(int thread, att_u64 kept)
     {
-        const int row = thread / CHUNKS;
+        const int row = thread / SLOTS;
 #pragma unroll
         for (int j = 0; j < PER_THREAD; ++j)
             if (!(kept >> (row + j * ROW_STEP) & 1)) held[j] = att_u32x4{0, 0, 0, 0};
@@ -420,7 +422,9 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-    // XCD x gets a contiguous part of the list, in which the tiles of rows of one set of keys stand together: they share its L2.
+    // The prefix's workgroups come first: they are bound by the matrix cores and are about as many as fit the chip at most, so those of the sequences'
+    // own keys, bound by memory, run beside and behind them (128 sequences behind 65536 tokens: 233 us, with the two kinds alternating 276).
+    // XCD x gets a contiguous part of a job's list, in which the tiles of rows of one set of keys stand together: they share its L2.
     int id = blockIdx.x;
     const bool second = id >= args.job[0].grid;
     const AttentionJob &job = args.job[second];
@@ -429,9 +433,19 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
     if (id >= job.workgroups) return;
     const int row_tile = id % job.row_tiles;
     id /= job.row_tiles;
-    const int split = id % job.splits;
-    id /= job.splits;
-    const int g = id % args.g, entry = id / args.g;
+    int g, split;
+    if (job.own_keys) {             // the heads of the same tokens, which stand side by side in memory, at the same time
+        g = id % args.g;
+        id /= args.g;
+        split = id % job.splits;
+        id /= job.splits;
+    } else {
+        split = id % job.splits;
+        id /= job.splits;
+        g = id % args.g;
+        id /= args.g;
+    }
+    const int entry = id;
 
     AttState<DP> state;
 #pragma unroll
@@ -564,29 +578,41 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
     }
 }
 
-// The partial results of one row, weighted by exp(lse of the part - lse of all).  A wave per row, the parts in their order.
+// The partial results of one row, weighted by exp(lse of the part - lse of all).  A wave per row, the parts in their order.  The weights come
+// first, a lane per part, so that the loads of the results, eight parts at a time, do not wait for them one by one.
 template <typename T>
 __global__ __launch_bounds__(256) void attention_join(const AttentionArgs args)
 {
     const int lane = threadIdx.x & 63;
     const i64 id = static_cast<i64>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (id >= args.rows_total) return;
-    float top = -__builtin_inff();
-    for (int part = lane; part < args.slots; part += 64) top = fmaxf(top, args.partial_lse[part * args.rows_total + id]);
+    static_assert(ATT_MAX_SLOTS == 128, "two parts per lane");
+    const float first = lane < args.slots ? args.partial_lse[lane * args.rows_total + id] : -__builtin_inff();
+    const float second = 64 + lane < args.slots ? args.partial_lse[(64 + lane) * args.rows_total + id] : -__builtin_inff();
+    float top = fmaxf(first, second);
 #pragma unroll
     for (int step = 32; step > 0; step >>= 1) top = fmaxf(top, __shfl_xor(top, step));
     const float base = top == -__builtin_inff() ? 0.0f : top;
-    float sum = 0.0f;
-    float out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int part = 0; part < args.slots; ++part) {
-        const i64 slot = part * args.rows_total + id;
-        const float lse2 = args.partial_lse[slot];
-        if (lse2 == -__builtin_inff()) continue;                        // a part without keys wrote nothing
-        const float weight = __builtin_amdgcn_exp2f(lse2 - base);
-        sum += weight;
+    const float weight[2] = {__builtin_amdgcn_exp2f(first - base), __builtin_amdgcn_exp2f(second - base)};
+    float sum = weight[0] + weight[1];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (64 * j + lane < args.o) out[j] += weight * args.partial_out[slot * args.partial_width + 64 * j + lane];
+    for (int step = 32; step > 0; step >>= 1) sum += __shfl_xor(sum, step);
+    float out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int AT_ONCE = 8;
+    for (int part = 0; part < args.slots; part += AT_ONCE) {
+        float x[AT_ONCE][4];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const i64 slot = (part + u < args.slots ? part + u : 0) * args.rows_total + id;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[u][j] = 64 * j + lane < args.o ? args.partial_out[slot * args.partial_width + 64 * j + lane] : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const float w = part + u < args.slots ? __shfl(weight[part >= 64], (part + u) & 63) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[j] += w != 0.0f ? w * x[u][j] : 0.0f;         // a part without keys wrote nothing
+        }
     }
     const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
     const i64 token = id / (static_cast<i64>(args.g) * args.r);

@@ -5,6 +5,8 @@ namespace kmc {
 
 typedef long long i64;
 
+constexpr int ATT_MAX_SLOTS = 128;          // partial results of a row
+
 // Keys and values of one segment; strides in elements.
 struct AttentionKeys {
     const void *k, *v;

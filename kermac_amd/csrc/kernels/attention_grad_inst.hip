@@ -45,6 +45,7 @@ hipError_t sum(const float *partial, void *out, kmc::i64 rows, int splits, int w
 hipError_t KMC_ATT_NAME(launch_attention_gradient)(const kmc::AttentionGradArgs &args, int width, bool aligned, hipStream_t stream)
 {
     hipError_t status = width <= 64    ? gradient<64>(args, aligned, stream)
+                        : width <= 96  ? gradient<96>(args, aligned, stream)
                         : width <= 128 ? gradient<128>(args, aligned, stream)
                                        : gradient<256>(args, aligned, stream);
     const kmc::i64 q_rows = static_cast<kmc::i64>(args.l) * args.m * args.g * args.r;

@@ -31,7 +31,7 @@ hipError_t forward(const kmc::AttentionArgs &args, bool aligned, hipStream_t str
 hipError_t KMC_ATT_NAME(launch_attention_forward)(const kmc::AttentionArgs &args, int width, bool aligned, hipStream_t stream)
 {
     if (args.job[0].grid + args.job[1].grid > 0) {
-        const hipError_t status = width <= 64 ? forward<64>(args, aligned, stream) : width <= 128 ? forward<128>(args, aligned, stream)
+        const hipError_t status = width <= 64 ? forward<64>(args, aligned, stream) : width <= 96 ? forward<96>(args, aligned, stream) : width <= 128 ? forward<128>(args, aligned, stream)
                                                                                                   : forward<256>(args, aligned, stream);
         if (status != hipSuccess) return status;
     }
