@@ -59,44 +59,72 @@ __device__ __forceinline__ constexpr int att_row(int i, int half) { return 8 * (
 // The sum or maximum of a value over the two lanes of a column.
 __device__ __forceinline__ float att_other_half(float x) { return __shfl_xor(x, 32); }
 
-// Rows of D elements of a tile in LDS.  Read as they are (16 bytes of a row per lane): 16 bytes of padding put consecutive rows
-// into consecutive groups of four banks.  Read transposed: a 16-bit read touches 4 rows x 64 bytes per half wave, which 64
-// bytes of padding put side by side; an fp32 read touches a row each at a distance of 4 rows, 32 banks apart with 32 bytes.
-template <typename T, int DP> constexpr int ATT_STRIDE = DP + 16 / static_cast<int>(sizeof(T));
-template <typename T, int DP> constexpr int ATT_STRIDE_T = DP + (sizeof(T) == 2 ? (DP == 96 ? 0 : 32) : 8);       // 16 or 48 banks mod 64
-
+// A tile of rows of DP elements in LDS, read both ways: 16 bytes of a row per lane, 16 rows at a time, and transposed, which touches 4 rows x 64 bytes per
+// half wave.  Rows of a power of two of bytes stand side by side, and row r holds its 16-byte piece c in place c ^ swizzle(r) / 16: sixteen consecutive
+// rows then have a given piece in different banks, and four rows a given four pieces.  Rows of 96 elements get 16 bytes of padding instead.
 template <typename T, int DP>
-__device__ __forceinline__ att_vec8<T> att_read_row(const T *tile, int stride, int row, int k)
+struct AttLds {
+    static constexpr int PIECE = 16 / static_cast<int>(sizeof(T));      // elements of 16 bytes
+    static constexpr int ROW_BYTES = DP * static_cast<int>(sizeof(T));
+    static constexpr bool SWIZZLED = (ROW_BYTES & (ROW_BYTES - 1)) == 0;
+    static constexpr int STRIDE = SWIZZLED ? ROW_BYTES : ROW_BYTES + 16;
+    // The bits that the swizzle of row r turns in a byte offset; linear in the bits of r.  Two rows of 128 bytes share a line of banks.
+    static __device__ __forceinline__ constexpr int swizzle(int r)
+    {
+        return !SWIZZLED ? 0 : ROW_BYTES == 128 ? ((r >> 1 & 1) << 2 | (r >> 2 & 3)) << 4 : ((r & 3) << 2 | (r >> 2 & 3)) << 4;
+    }
+    static __device__ __forceinline__ constexpr int offset(int row, int piece) { return row * STRIDE + (16 * piece ^ swizzle(row)); }
+};
+
+typedef unsigned char att_lds_byte;
+
+// Eight elements of row `row` + lane % 32 from element k + 8 (lane / 32) on; row and k multiples of 32 and 16.
+template <typename T, int DP>
+__device__ __forceinline__ att_vec8<T> att_read_row(const att_lds_byte *tile, int row, int k, int lane)
 {
-    const T *p = tile + row * stride + k;
+    typedef AttLds<T, DP> Lds;
+    const int size = static_cast<int>(sizeof(T));
+    const int mine = (lane & 31) * Lds::STRIDE + (8 * size * (lane >> 5) ^ Lds::swizzle(lane & 31));
+    const int here = Lds::SWIZZLED ? mine ^ k * size : mine + k * size;
+    const att_lds_byte *p = tile + row * Lds::STRIDE;
     att_vec8<T> x;
     if constexpr (sizeof(T) == 2) {
-        x = *reinterpret_cast<const att_vec8<T> *>(p);
+        x = *reinterpret_cast<const att_vec8<T> *>(p + here);
     } else {
-        const att_f32x4 low = reinterpret_cast<const att_f32x4 *>(p)[0], high = reinterpret_cast<const att_f32x4 *>(p)[1];
+        const att_f32x4 low = *reinterpret_cast<const att_f32x4 *>(p + here);
+        const att_f32x4 high = *reinterpret_cast<const att_f32x4 *>(p + (Lds::SWIZZLED ? here ^ 16 : here + 16));
 #pragma unroll
         for (int j = 0; j < 4; ++j) { x[j] = low[j]; x[4 + j] = high[j]; }
     }
     return x;
 }
 
-// Lane l gets column `column` + l % 32 of the 16 rows from `row` on, in the order 4 h + {0..3}, 8 + 4 h + {0..3}.
-template <typename T>
-__device__ __forceinline__ att_vec8<T> att_read_transposed(const T *tile, int stride, int row, int column, int lane)
+// Lane l gets column `column` + l % 32 of the 16 rows from `row` on, in the order 4 h + {0..3}, 8 + 4 h + {0..3}; row and column multiples of 16 and 32.
+template <typename T, int DP>
+__device__ __forceinline__ att_vec8<T> att_read_transposed(const att_lds_byte *tile, int row, int column, int lane)
 {
+    typedef AttLds<T, DP> Lds;
     const int half = lane >> 5;
     att_vec8<T> x;
     if constexpr (sizeof(T) == 2) {
-        const T *p = tile + (row + 4 * half + (lane % 16) / 4) * stride + column + 16 * (lane / 16 % 2) + 4 * (lane % 4);
+        const int r = 4 * half + (lane & 15) / 4;
+        const int mine = r * Lds::STRIDE + (((32 * (lane >> 4 & 1) + 8 * (lane & 3)) ^ Lds::swizzle(r)));
+        const att_lds_byte *p = tile + row * Lds::STRIDE + (Lds::SWIZZLED ? mine ^ 2 * column : mine + 2 * column);
         typedef __attribute__((address_space(3))) att_s16x4 lds_s16x4;
         union { att_s16x4 part[2]; att_vec8<T> whole; } u;
         u.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p));
-        u.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 8 * stride));
+        const int behind = Lds::SWIZZLED ? (mine ^ 2 * column ^ Lds::swizzle(8)) : mine + 2 * column;       // the same place of row r + 8
+        u.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(tile + (row + 8) * Lds::STRIDE + behind));
         x = u.whole;
     } else {
-        const T *p = tile + (row + 4 * half) * stride + column + lane % 32;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { x[j] = p[j * stride]; x[4 + j] = p[(8 + j) * stride]; }
+        for (int j = 0; j < 4; ++j) {
+            const int r = 4 * half + j;
+            const int mine = r * Lds::STRIDE + (4 * (lane & 31) ^ Lds::swizzle(r));
+            const int here = Lds::SWIZZLED ? mine ^ 4 * column : mine + 4 * column;
+            x[j] = *reinterpret_cast<const float *>(tile + row * Lds::STRIDE + here);
+            x[4 + j] = *reinterpret_cast<const float *>(tile + (row + 8) * Lds::STRIDE + (here ^ Lds::swizzle(8)));
+        }
     }
     return x;
 }
@@ -143,27 +171,61 @@ constexpr int ATT_BUFFER_FORMAT = 0x00020000;        // 32-bit data, as raw buff
 // Keeps the compiler from merging a rare case into the common path as selections.
 __device__ __forceinline__ void att_rare() { asm volatile(""); }
 
-// A tile of ROWS rows of DP elements on its way from memory to LDS through the registers of THREADS threads.
+typedef int att_s32x4 __attribute__((ext_vector_type(4)));
+
+// The rows of a tile in memory: rows 0 .. rows - 1 of base, `width` elements each, `stride` apart; what lies outside reads as zero without a branch
+// per load.
+template <typename T>
+__device__ __forceinline__ att_s32x4 att_descriptor(const T *base, int step, int rows, int width)
+{
+    const int bytes = rows > 0 ? (rows - 1) * step + width * static_cast<int>(sizeof(T)) : 0;
+    const att_u64 address = reinterpret_cast<att_u64>(base);
+    return att_s32x4{__builtin_amdgcn_readfirstlane(static_cast<int>(address)), __builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32) & 0xffff),
+                     __builtin_amdgcn_readfirstlane(bytes), ATT_BUFFER_FORMAT};
+}
+
+// Nothing that was loaded is outstanding, and the compiler knows: it would otherwise wait, in front of the first use of a register that was loaded
+// before a loop, for everything that is outstanding in every turn of the loop, the tiles on their way to LDS included (a third of the run time).
+__device__ __forceinline__ void att_wait_for_loads()
+{
+    asm volatile("" : : : "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt 0, the other counters as they are
+    asm volatile("" : : : "memory");
+}
+
+// A tile of ROWS rows of DP elements on its way from memory to LDS.  begin() asks for it, finish() has it written.  DIRECT: from memory straight into LDS, 1 KB per
+// wave and instruction, each lane fetching the piece that belongs where its 16 bytes end up; no register waits for it.  Otherwise (rows that are no
+// power of two, unaligned rows, tiles of one wave) through registers.
 template <typename T, int DP, int ROWS, int THREADS, bool ALIGNED>
 struct AttTile {
-    static constexpr int CHUNK = 16 / sizeof(T);                    // elements of a 16-byte piece
-    static constexpr int CHUNKS = DP / CHUNK;                       // pieces of a row
-    static constexpr int SLOTS = CHUNKS <= 8 ? 8 : CHUNKS <= 16 ? 16 : CHUNKS <= 32 ? 32 : 64;        // threads of a row; those behind CHUNKS have no piece
+    typedef AttLds<T, DP> Lds;
+    static constexpr bool DIRECT = ALIGNED && Lds::SWIZZLED && THREADS > 64;
+    static constexpr int PIECES = DP / Lds::PIECE;                      // of a row
+    static constexpr int SLOTS = PIECES <= 8 ? 8 : PIECES <= 16 ? 16 : PIECES <= 32 ? 32 : 64;        // threads of a row; those behind PIECES have no piece
     static constexpr int ROW_STEP = THREADS / SLOTS;
     static constexpr int PER_THREAD = ROWS / ROW_STEP;
-    static_assert(THREADS % SLOTS == 0 && ROWS % ROW_STEP == 0, "whole rows per step");
-    att_u32x4 held[PER_THREAD];
+    static_assert(THREADS % SLOTS == 0 && ROWS % ROW_STEP == 0 && PER_THREAD > 0, "whole rows per step");
+    att_u32x4 held[DIRECT ? 1 : PER_THREAD];
 
-    // Rows 0 .. rows - 1 of base (rows of `width` elements, `stride` apart); rows behind them read as zero.  Aligned rows are read through
-    // a buffer descriptor that ends behind the last one: what lies outside reads as zero without a branch per load.
-    __device__ __forceinline__ void load(const T *base, i64 stride, int rows, int width, int thread)
+    __device__ __forceinline__ void begin(const T *base, i64 stride, int rows, int width, att_lds_byte *tile, int thread)
     {
-        const int row = thread / SLOTS, at = thread % SLOTS * CHUNK;
-        if constexpr (ALIGNED) {
-            const int some = rows < ROWS ? rows : ROWS, step = static_cast<int>(stride) * static_cast<int>(sizeof(T));
-            const int bytes = some > 0 ? (some - 1) * step + width * static_cast<int>(sizeof(T)) : 0;
+        constexpr int SIZE = static_cast<int>(sizeof(T));
+        const int row = thread / SLOTS, step = static_cast<int>(stride) * SIZE;
+        if constexpr (DIRECT) {
+            const att_s32x4 from = att_descriptor(base, step, rows < ROWS ? rows : ROWS, width);
+            const unsigned to = static_cast<unsigned>(reinterpret_cast<size_t>((__attribute__((address_space(3))) att_lds_byte *)tile));
+#pragma unroll
+            for (int j = 0; j < PER_THREAD; ++j) {
+                const int r = row + j * ROW_STEP, at = (16 * (thread % SLOTS) ^ Lds::swizzle(row) ^ Lds::swizzle(j * ROW_STEP)) / SIZE;
+                const unsigned offset = at < width ? static_cast<unsigned>(r * step + at * SIZE) : 0x80000000u;
+                const unsigned lds = __builtin_amdgcn_readfirstlane(to + (thread / 64 * (64 / SLOTS) + j * ROW_STEP) * Lds::STRIDE);
+                asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(offset), "s"(from), "s"(lds) : "memory", "m0");
+            }
+        } else if constexpr (ALIGNED) {
+            const int some = rows < ROWS ? rows : ROWS, bytes = some > 0 ? (some - 1) * step + width * SIZE : 0;
             const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, bytes, ATT_BUFFER_FORMAT);
-            unsigned offset = at < width ? static_cast<unsigned>(row * step + at * static_cast<int>(sizeof(T))) : 0x80000000u;
+            const int at = thread % SLOTS * Lds::PIECE;
+            unsigned offset = at < width ? static_cast<unsigned>(row * step + at * SIZE) : 0x80000000u;
 #pragma unroll
             for (int j = 0; j < PER_THREAD; ++j) {
                 held[j] = __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0);
@@ -174,30 +236,35 @@ struct AttTile {
 #pragma unroll
             for (int j = 0; j < PER_THREAD; ++j) {
                 held[j] = att_u32x4{0, 0, 0, 0};
-                if (row + j * ROW_STEP < rows) held[j] = att_load16<T, false>(p, at, width);
+                if (row + j * ROW_STEP < rows) held[j] = att_load16<T, false>(p, thread % SLOTS * Lds::PIECE, width);
                 p += ROW_STEP * stride;
             }
         }
     }
 
-    template <int STRIDE>
-    __device__ __forceinline__ void store(T *tile, int thread) const
+    // Followed by a barrier.
+    __device__ __forceinline__ void finish(att_lds_byte *tile, int thread) const
     {
-        const int row = thread / SLOTS, at = thread % SLOTS * CHUNK;
-        if (SLOTS != CHUNKS && at >= DP) return;
+        if constexpr (DIRECT) {
+            att_wait_for_loads();
+        } else {
+            const int row = thread / SLOTS, piece = thread % SLOTS;
+            if (SLOTS != PIECES && piece >= PIECES) return;
 #pragma unroll
-        for (int j = 0; j < PER_THREAD; ++j) *reinterpret_cast<att_u32x4 *>(tile + (row + j * ROW_STEP) * STRIDE + at) = held[j];
-    }
-
-    // Rows whose bit in `kept` is not set become zeros.
-    __device__ __forceinline__ void clear(int thread, att_u64 kept)
-    {
-        const int row = thread / SLOTS;
-#pragma unroll
-        for (int j = 0; j < PER_THREAD; ++j)
-            if (!(kept >> (row + j * ROW_STEP) & 1)) held[j] = att_u32x4{0, 0, 0, 0};
+            for (int j = 0; j < PER_THREAD; ++j) *reinterpret_cast<att_u32x4 *>(tile + Lds::offset(row + j * ROW_STEP, piece)) = held[j];
+        }
     }
 };
+
+// Rows of a tile in LDS whose bit in `kept` is not set become zeros.  Between barriers.
+template <typename T, int DP, int ROWS, int THREADS>
+__device__ __forceinline__ void att_clear(att_lds_byte *tile, att_u64 kept, int thread)
+{
+    typedef AttLds<T, DP> Lds;
+    constexpr int PIECES = DP / Lds::PIECE;
+    for (int i = thread; i < ROWS * PIECES; i += THREADS)
+        if (!(kept >> (i / PIECES) & 1)) *reinterpret_cast<att_u32x4 *>(tile + Lds::offset(i / PIECES, i % PIECES)) = att_u32x4{0, 0, 0, 0};
+}
 
 // One bit per key n0 .. n0 + 63: the key exists and takes part.  The same in all waves of a workgroup.
 __device__ __forceinline__ att_u64 att_kept_keys(const AttentionKeys &keys, int entry, int n0, int end, int lane)
@@ -227,33 +294,93 @@ __device__ __forceinline__ void att_wave_sync()
 template <int DP>
 struct AttState {
     att_f32x16 out[DP / 32];
-    float top, sum;              // a score near the largest so far and the sum of this lane's exponentials relative to it, to base 2
+    float base, sum;             // a whole number near the largest score so far and the sum of this lane's exponentials relative to it, to base 2
 };
 
 // Outputs and sums are rescaled only when a score passes the one they are relative to by 2^8: exponentials stay below 256, far inside every type,
 // and after the first tiles the 64 or more multiplications per tile are not made.
 constexpr float ATT_HEADROOM = 8.0f;
 
-// One tile of KT keys in LDS against the 32 rows whose queries are in `query`.  `kept` has a bit per key for this lane's row.
-template <typename T, int DP, int KT>
-__device__ __forceinline__ void att_forward_tile(AttState<DP> &state, const att_vec8<T> (&query)[DP / 16], const T *keys, const T *values, float scale_log2,
-                                                 att_u64 kept, int lane)
+// Fragments are read from LDS a group ahead of the matrix instructions that use them.  The compiler, left alone, reads each one in front of its
+// use and waits for it; these fix the order within a region: READS reads, then the matrix instructions, each followed by VALU vector instructions.
+template <int READS, int MMAS, int VALU>
+__device__ __forceinline__ void att_order()
 {
-    const int half = lane >> 5;
-    att_f32x16 s[KT / 32];
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
 #pragma unroll
-    for (int b = 0; b < KT / 32; ++b) {
-        s[b] = att_f32x16{0};
-#pragma unroll
-        for (int step = 0; step < DP / 16; ++step)
-            s[b] = att_mma(att_read_row<T, DP>(keys, ATT_STRIDE<T, DP>, 32 * b + lane % 32, 16 * step + 8 * half), query[step], s[b]);
+    for (int i = 0; i < MMAS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (VALU > 0) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
     }
+}
+__device__ __forceinline__ void att_region() { __builtin_amdgcn_sched_barrier(0); }
+
+template <typename T, int DP>
+struct AttGroups {
+    static constexpr int STEPS = DP / 16;                               // of a contraction over features
+    static constexpr int GROUP = STEPS % 4 == 0 ? 4 : 3;                // fragments of a group
+    static constexpr int GROUPS = STEPS / GROUP;
+    static constexpr int MMAS = sizeof(T) == 4 ? 8 : 1;                 // matrix instructions per fragment
+    static constexpr int READS_ROW = sizeof(T) == 4 ? 2 : 1;
+    static constexpr int READS_T = sizeof(T) == 4 ? 8 : 2;
+};
+
+template <typename T, int DP, int GROUP>
+__device__ __forceinline__ void att_read_group(att_vec8<T> (&f)[GROUP], const att_lds_byte *tile, int row, int group, int lane)
+{
+#pragma unroll
+    for (int i = 0; i < GROUP; ++i) f[i] = att_read_row<T, DP>(tile, row, 16 * (GROUP * group + i), lane);
+}
+
+// All DP columns of 16 rows, transposed.
+template <typename T, int DP>
+__device__ __forceinline__ void att_read_columns(att_vec8<T> (&f)[DP / 32], const att_lds_byte *tile, int row, int lane)
+{
+#pragma unroll
+    for (int o = 0; o < DP / 32; ++o) f[o] = att_read_transposed<T, DP>(tile, row, 32 * o, lane);
+}
+
+// s^T of a tile of KT keys in LDS and the 32 rows whose queries are in `query`.  Blocks of 32 keys take turns: a matrix instruction that adds to the
+// result of the one before waits for it.
+template <typename T, int DP, int KT>
+__device__ __forceinline__ void att_scores(att_f32x16 (&s)[KT / 32], const att_vec8<T> (&query)[DP / 16], const att_lds_byte *keys, int lane)
+{
+    typedef AttGroups<T, DP> G;
+    constexpr int BLOCKS = KT / 32, AT_ONCE = BLOCKS == 1 ? G::GROUP : 2, ALL = G::STEPS / AT_ONCE;
+    att_vec8<T> f[2][AT_ONCE][BLOCKS];
+    auto read = [&](att_vec8<T> (&to)[AT_ONCE][BLOCKS], int i) {
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j)
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b) to[j][b] = att_read_row<T, DP>(keys, 32 * b, 16 * (AT_ONCE * i + j), lane);
+    };
+    read(f[0], 0);
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) s[b] = att_f32x16{0};
+    att_region();
+#pragma unroll
+    for (int i = 0; i < ALL; ++i) {
+        if (i + 1 < ALL) read(f[(i + 1) & 1], i + 1);
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j)
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b) s[b] = att_mma(f[i & 1][j][b], query[AT_ONCE * i + j], s[b]);
+        att_order<AT_ONCE * BLOCKS * G::READS_ROW, AT_ONCE * BLOCKS * G::MMAS, 0>();
+        att_region();
+    }
+}
+
+// Masks a tile's scores (`kept` has a bit per key for this lane's row) and, where they pass the wave's base by 2^8, moves it.  Bases are whole
+// numbers, so that what was made below the old one is rescaled without rounding: output and sum, and `weights` that wait for their product.
+template <typename T, int DP, int KT>
+__device__ __forceinline__ void att_rebase(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], att_f32x16 (&s)[KT / 32], float scale_log2, att_u64 kept, int lane)
+{
     const att_u64 all = KT == 64 ? ~0ull : (1ull << KT) - 1;
     if (!__all((kept & all) == all)) {
         att_rare();
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b) {
-            const unsigned mine = static_cast<unsigned>(kept >> (32 * b)) >> (4 * half);
+            const unsigned mine = static_cast<unsigned>(kept >> (32 * b)) >> (4 * (lane >> 5));
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[b][i] = mine >> att_row(i, 0) & 1 ? s[b][i] : -__builtin_inff();
         }
@@ -264,35 +391,60 @@ __device__ __forceinline__ void att_forward_tile(AttState<DP> &state, const att_
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
     top = fmaxf(top, att_other_half(top)) * scale_log2;
-    if (!__all(top <= state.top + ATT_HEADROOM)) {
+    if (!__all(top <= state.base + ATT_HEADROOM)) {
         att_rare();
-        top = fmaxf(state.top, top);
-        const float shrink = __builtin_amdgcn_exp2f(state.top - (top == -__builtin_inff() ? 0.0f : top));
-        state.top = top;
+        const float base = fmaxf(state.base, __builtin_ceilf(top));
+        const float shrink = __builtin_amdgcn_exp2f(state.base - (base == -__builtin_inff() ? 0.0f : base));
+        state.base = base;
         state.sum *= shrink;
 #pragma unroll
         for (int o = 0; o < DP / 32; ++o) state.out[o] *= shrink;
+#pragma unroll
+        for (int step = 0; step < KT / 16; ++step)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) weights[step][j] = static_cast<T>(static_cast<float>(weights[step][j]) * shrink);
     }
-    const float base = state.top == -__builtin_inff() ? 0.0f : state.top;          // no key of this row yet: every exponential below is 0
-    float sum = 0.0f;
-#pragma unroll
-    for (int b = 0; b < KT / 32; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale_log2, -base));
-            sum += s[b][i];
-        }
-    state.sum += sum;
-#pragma unroll
-    for (int b = 0; b < KT / 32; ++b)
-#pragma unroll
-        for (int step = 0; step < 2; ++step) {
-            const att_vec8<T> weights = att_operand<T>(s[b], step);
-#pragma unroll
-            for (int o = 0; o < DP / 32; ++o)
-                state.out[o] = att_mma(att_read_transposed(values, ATT_STRIDE_T<T, DP>, 32 * b + 16 * step, 32 * o, lane), weights, state.out[o]);
-        }
 }
+
+// exp(s - base) of 16 keys, in the operands' type.
+template <typename T, int DP, int KT>
+__device__ __forceinline__ att_vec8<T> att_weights(AttState<DP> &state, const att_f32x16 (&s)[KT / 32], int step, float scale_log2, float base)
+{
+    float p[8], sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[step / 2][8 * (step % 2) + j], scale_log2, -base));
+        sum += p[j];
+    }
+    state.sum += sum;
+    att_vec8<T> weights;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) weights[j] = static_cast<T>(p[j]);
+    return weights;
+}
+
+// out^T += V^T p^T over the KT keys of a tile; with NEXT, the weights give way to those of the scores s.
+template <typename T, int DP, int KT, bool NEXT>
+__device__ __forceinline__ void att_add_values(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], const att_lds_byte *values, att_vec8<T> (&first)[DP / 32],
+                                               const att_f32x16 (&s)[KT / 32], float scale_log2, float base, int lane)
+{
+    typedef AttGroups<T, DP> G;
+    att_vec8<T> f[2][DP / 32];
+#pragma unroll
+    for (int o = 0; o < DP / 32; ++o) f[0][o] = first[o];
+#pragma unroll
+    for (int step = 0; step < KT / 16; ++step) {
+        if (step + 1 < KT / 16) att_read_columns<T, DP>(f[(step + 1) & 1], values, 16 * (step + 1), lane);
+#pragma unroll
+        for (int o = 0; o < DP / 32; ++o) state.out[o] = att_mma(f[step & 1][o], weights[step], state.out[o]);
+        if (NEXT) weights[step] = att_weights<T, DP, KT>(state, s, step, scale_log2, base);
+        att_order<DP / 32 * G::READS_T, DP / 32 * G::MMAS, NEXT ? (DP <= 64 ? 14 : DP <= 128 ? 7 : 4) : 0>();
+        att_region();
+    }
+}
+
+// Below a base of -inf (no key of this row yet) every exponential is that of -inf, 0.
+__device__ __forceinline__ float att_finite_base(float base) { return base == -__builtin_inff() ? 0.0f : base; }
 
 // Keys [begin, end) of a segment for split `split` of `splits`, in whole tiles.
 __device__ __forceinline__ void att_range(int length, int tile, int split, int splits, int *begin, int *end)
@@ -330,9 +482,9 @@ struct AttForwardShape {
     static constexpr int OWN_KEYS = 32;
     static constexpr int OWN_WAVES = DP * sizeof(T) <= 512 ? 4 : 2;      // 1 KB rows: two waves' tiles fill LDS
     static constexpr int WAVES_PER_SIMD = DP * sizeof(T) <= 256 ? 2 : 1;
-    static constexpr int TILE_BYTES_PER_KEY = (ATT_STRIDE<T, DP> + ATT_STRIDE_T<T, DP>) * static_cast<int>(sizeof(T));
-    static constexpr int SHARED_BYTES = SHARED_KEYS * TILE_BYTES_PER_KEY;
-    static constexpr int OWN_BYTES = OWN_WAVES * OWN_KEYS * TILE_BYTES_PER_KEY;
+    static constexpr int KEY_BYTES = AttLds<T, DP>::STRIDE;
+    static constexpr int SHARED_BYTES = 4 * SHARED_KEYS * KEY_BYTES;     // keys and values, two tiles of each
+    static constexpr int OWN_BYTES = 2 * OWN_WAVES * OWN_KEYS * KEY_BYTES;
     static constexpr int JOIN_BYTES = (OWN_WAVES - 1) * (DP * 32 + 64) * 4 + 512;
     static constexpr int BYTES_1 = SHARED_BYTES > OWN_BYTES ? SHARED_BYTES : OWN_BYTES;
     static constexpr int BYTES = BYTES_1 > JOIN_BYTES ? BYTES_1 : JOIN_BYTES;
@@ -371,7 +523,7 @@ __device__ __forceinline__ void att_forward_write(const AttentionArgs &args, con
     const AttRow at = att_find_row(args, entry, g, row);
     const i64 id = (static_cast<i64>(at.entry) * args.m + at.query) * (static_cast<i64>(args.g) * args.r) + at.head;
     const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;      // a row without keys gets zeros, not a number stays
-    const float lse2 = sum == 0.0f ? -__builtin_inff() : state.top + __builtin_amdgcn_logf(sum);
+    const float lse2 = sum == 0.0f ? -__builtin_inff() : state.base + __builtin_amdgcn_logf(sum);
     if (job.partial) {
         const i64 slot = static_cast<i64>(job.slot + split) * args.rows_total + id;
         if (half == 0) args.partial_lse[slot] = lse2;
@@ -418,7 +570,7 @@ template <typename T, int DP, bool ALIGNED>
 __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void attention_forward(const AttentionArgs args)
 {
     typedef AttForwardShape<T, DP> Shape;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[Shape::BYTES];
+    __shared__ __attribute__((aligned(1024))) att_lds_byte lds[Shape::BYTES];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -450,18 +602,19 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
     AttState<DP> state;
 #pragma unroll
     for (int o = 0; o < DP / 32; ++o) state.out[o] = att_f32x16{0};
-    state.top = -__builtin_inff();
+    state.base = -__builtin_inff();
     state.sum = 0.0f;
     att_vec8<T> query[DP / 16];
 
     if (!job.own_keys) {
         constexpr int KT = Shape::SHARED_KEYS;
-        T *key_tile = reinterpret_cast<T *>(lds);
-        T *value_tile = key_tile + KT * ATT_STRIDE<T, DP>;
+        constexpr int TILE = KT * Shape::KEY_BYTES;
+        att_lds_byte *key_tile = lds, *value_tile = lds + 2 * TILE;
         const int first_row = row_tile * 32 * Shape::ROW_WAVES + 32 * wave;
         const int row = first_row + lane % 32;
         const bool works = first_row < job.rows;
         att_load_queries<T, DP, ALIGNED>(args, job, entry, g, row, lane, query);
+        att_wait_for_loads();
         for (int segment = job.first_segment; segment < job.last_segment; ++segment) {
             const AttentionKeys &keys = args.keys[segment];
             const int length = att_length(keys, entry);
@@ -478,24 +631,63 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
             }
             const T *k = static_cast<const T *>(keys.k) + entry * keys.k_ls + g * keys.k_gs;
             const T *v = static_cast<const T *>(keys.v) + entry * keys.v_ls + g * keys.v_gs;
+            if (begin >= end) continue;
+            // Iteration i: scores of tile i, then the values of tile i - 1 times their weights while the exponentials of tile i are made: the matrix
+            // cores and the vector units work at the same time.  Keys are staged one tile in front of the values, in two buffers each: one barrier.
             AttTile<T, DP, KT, 256, ALIGNED> next_k, next_v;
-            if (begin < end) {
-                next_k.load(k + begin * keys.k_ns, keys.k_ns, end - begin, args.k, threadIdx.x);
-                next_v.load(v + begin * keys.v_ns, keys.v_ns, end - begin, args.o, threadIdx.x);
-            }
-            for (int n = begin; n < end; n += KT) {
-                const att_u64 kept = att_kept_keys(keys, entry, n, end, lane);
-                __syncthreads();
-                next_k.template store<ATT_STRIDE<T, DP>>(key_tile, threadIdx.x);
-                if (keys.mask) next_v.clear(threadIdx.x, kept);
-                next_v.template store<ATT_STRIDE_T<T, DP>>(value_tile, threadIdx.x);
-                __syncthreads();
+            att_f32x16 s[KT / 32];
+            att_vec8<T> weights[KT / 16], first[DP / 32];
+#pragma unroll
+            for (int step = 0; step < KT / 16; ++step) weights[step] = att_vec8<T>{0};
+            __syncthreads();
+            next_k.begin(k + begin * keys.k_ns, keys.k_ns, end - begin, args.k, key_tile, threadIdx.x);
+            next_k.finish(key_tile, threadIdx.x);
+            __syncthreads();
+            int odd = 0;
+            auto stage = [&](int n) {
                 if (n + KT < end) {
                     const i64 at = n + KT;
-                    next_k.load(k + at * keys.k_ns, keys.k_ns, end - static_cast<int>(at), args.k, threadIdx.x);
-                    next_v.load(v + at * keys.v_ns, keys.v_ns, end - static_cast<int>(at), args.o, threadIdx.x);
+                    next_k.begin(k + at * keys.k_ns, keys.k_ns, end - static_cast<int>(at), args.k, key_tile + (odd ^ 1) * TILE, threadIdx.x);
                 }
-                if (works) att_forward_tile<T, DP, KT>(state, query, key_tile, value_tile, args.scale_log2, kept & att_low_bits(limit - n), lane);
+                next_v.begin(v + n * keys.v_ns, keys.v_ns, end - n, args.o, value_tile + odd * TILE, threadIdx.x);
+            };
+            auto staged = [&](int n, att_u64 kept) {
+                if (n + KT < end) next_k.finish(key_tile + (odd ^ 1) * TILE, threadIdx.x);
+                next_v.finish(value_tile + odd * TILE, threadIdx.x);
+                __syncthreads();
+                if (keys.mask && kept != ~0ull) {
+                    att_rare();
+                    att_clear<T, DP, KT, 256>(value_tile + odd * TILE, kept, threadIdx.x);
+                    __syncthreads();
+                }
+                odd ^= 1;
+            };
+            att_u64 kept = att_kept_keys(keys, entry, begin, end, lane);
+            stage(begin);
+            if (works) {
+                att_scores<T, DP, KT>(s, query, key_tile, lane);
+                att_rebase<T, DP, KT>(state, weights, s, args.scale_log2, kept & att_low_bits(limit - begin), lane);
+                const float base = att_finite_base(state.base);
+#pragma unroll
+                for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, args.scale_log2, base);
+            }
+            staged(begin, kept);
+            for (int n = begin + KT; n < end; n += KT) {
+                kept = att_kept_keys(keys, entry, n, end, lane);
+                stage(n);
+                if (works) {
+                    const att_lds_byte *before = value_tile + (odd ^ 1) * TILE;
+                    att_scores<T, DP, KT>(s, query, key_tile + odd * TILE, lane);
+                    att_read_columns<T, DP>(first, before, 0, lane);
+                    att_rebase<T, DP, KT>(state, weights, s, args.scale_log2, kept & att_low_bits(limit - n), lane);
+                    att_add_values<T, DP, KT, true>(state, weights, before, first, s, args.scale_log2, att_finite_base(state.base), lane);
+                }
+                staged(n, kept);
+            }
+            if (works) {
+                const att_lds_byte *before = value_tile + (odd ^ 1) * TILE;
+                att_read_columns<T, DP>(first, before, 0, lane);
+                att_add_values<T, DP, KT, false>(state, weights, before, first, s, 0.0f, 0.0f, lane);
             }
         }
         if (!works) return;
@@ -503,8 +695,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
         att_forward_write<T, DP, ALIGNED>(args, job, state, sum, entry, g, row, split, lane);
     } else {
         constexpr int KT = Shape::OWN_KEYS, WAVES = Shape::OWN_WAVES;
-        T *key_tile = reinterpret_cast<T *>(lds + wave * KT * Shape::TILE_BYTES_PER_KEY);
-        T *value_tile = key_tile + KT * ATT_STRIDE<T, DP>;
+        att_lds_byte *key_tile = lds + 2 * wave * KT * Shape::KEY_BYTES, *value_tile = key_tile + KT * Shape::KEY_BYTES;
         const int row = lane % 32;                                      // at most 32 rows: one tile
         if (wave < WAVES) {
             att_load_queries<T, DP, ALIGNED>(args, job, entry, g, row, lane, query);
@@ -519,39 +710,51 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                 AttTile<T, DP, KT, 64, ALIGNED> next_k, next_v;
                 i64 n = begin + wave * KT;
                 if (n < end) {
-                    next_k.load(k + n * keys.k_ns, keys.k_ns, end - static_cast<int>(n), args.k, lane);
-                    next_v.load(v + n * keys.v_ns, keys.v_ns, end - static_cast<int>(n), args.o, lane);
+                    next_k.begin(k + n * keys.k_ns, keys.k_ns, end - static_cast<int>(n), args.k, key_tile, lane);
+                    next_v.begin(v + n * keys.v_ns, keys.v_ns, end - static_cast<int>(n), args.o, value_tile, lane);
                 }
                 for (; n < end; n += KT * WAVES) {
                     const att_u64 kept = att_kept_keys(keys, entry, static_cast<int>(n), end, lane);
-                    next_k.template store<ATT_STRIDE<T, DP>>(key_tile, lane);
-                    if (keys.mask) next_v.clear(lane, kept);
-                    next_v.template store<ATT_STRIDE_T<T, DP>>(value_tile, lane);
+                    next_k.finish(key_tile, lane);
+                    next_v.finish(value_tile, lane);
                     att_wave_sync();
+                    if (keys.mask && (kept & 0xffffffffull) != 0xffffffffull) {
+                        att_clear<T, DP, KT, 64>(value_tile, kept, lane);
+                        att_wave_sync();
+                    }
                     const i64 at = n + KT * WAVES;
                     if (at < end) {
-                        next_k.load(k + at * keys.k_ns, keys.k_ns, end - static_cast<int>(at), args.k, lane);
-                        next_v.load(v + at * keys.v_ns, keys.v_ns, end - static_cast<int>(at), args.o, lane);
+                        next_k.begin(k + at * keys.k_ns, keys.k_ns, end - static_cast<int>(at), args.k, key_tile, lane);
+                        next_v.begin(v + at * keys.v_ns, keys.v_ns, end - static_cast<int>(at), args.o, value_tile, lane);
                     }
-                    att_forward_tile<T, DP, KT>(state, query, key_tile, value_tile, args.scale_log2, kept & att_low_bits(limit - static_cast<int>(n)), lane);
+                    att_f32x16 s[KT / 32];
+                    att_vec8<T> weights[KT / 16] = {};
+                    att_scores<T, DP, KT>(s, query, key_tile, lane);
+                    att_rebase<T, DP, KT>(state, weights, s, args.scale_log2, kept & att_low_bits(limit - static_cast<int>(n)), lane);
+                    const float base = att_finite_base(state.base);
+#pragma unroll
+                    for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, args.scale_log2, base);
+                    att_vec8<T> first[DP / 32];
+                    att_read_columns<T, DP>(first, value_tile, 0, lane);
+                    att_add_values<T, DP, KT, false>(state, weights, value_tile, first, s, 0.0f, 0.0f, lane);
                     att_wave_sync();
                 }
             }
         }
         // join the waves: sums and outputs below one common maximum, added in the order of the waves
         float sum = state.sum + att_other_half(state.sum);
-        float *tops = reinterpret_cast<float *>(lds);                   // [WAVES][32], then (WAVES - 1) waves' sums and outputs
-        float *others = tops + 128;
+        float *bases = reinterpret_cast<float *>(lds);                   // [WAVES][32], then (WAVES - 1) waves' sums and outputs
+        float *others = bases + 128;
         __syncthreads();
-        static_assert(WAVES * 32 <= 128, "room for the tops");
-        if (wave < WAVES && lane < 32) tops[wave * 32 + lane] = state.top;
+        static_assert(WAVES * 32 <= 128, "room for the bases");
+        if (wave < WAVES && lane < 32) bases[wave * 32 + lane] = state.base;
         __syncthreads();
-        float top = -__builtin_inff();
+        float base = -__builtin_inff();
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, tops[w * 32 + lane % 32]);
+        for (int w = 0; w < WAVES; ++w) base = fmaxf(base, bases[w * 32 + lane % 32]);
         __syncthreads();
-        const float shrink = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(state.top - top);
-        state.top = top;
+        const float shrink = base == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(state.base - base);
+        state.base = base;
         sum *= shrink;
 #pragma unroll
         for (int o = 0; o < DP / 32; ++o) state.out[o] *= shrink;

@@ -24,7 +24,7 @@ struct AttGradShape {
     static constexpr int WAVES_PER_SIMD = ROW_BYTES <= 256 ? 2 : 1;
     static constexpr int WAVES_PER_SIMD_K = ROW_BYTES <= 128 ? 2 : 1;
     static constexpr int ROWS = 32;                                 // per tile of the keys' kernel
-    static constexpr int BOTH = ATT_STRIDE<T, DP> + ATT_STRIDE_T<T, DP>;        // a row as it is, and one to be read transposed
+    static constexpr int BUFFERS = ROW_BYTES <= 512 ? 3 : 2;        // for its tiles: three of 64 KB do not fit
 };
 
 // ds of a 32 x 32 result from scores, d v^T, and the row's statistics: p comes back in `s`.
@@ -38,8 +38,8 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
 {
     typedef AttGradShape<T, DP> Shape;
     constexpr int KT = Shape::KEYS;
-    __shared__ __attribute__((aligned(16))) T lds[KT * (Shape::BOTH + ATT_STRIDE<T, DP>)];
-    T *key_tile = lds, *value_tile = key_tile + KT * ATT_STRIDE<T, DP>, *key_tile_t = value_tile + KT * ATT_STRIDE<T, DP>;
+    constexpr int TILE = KT * AttLds<T, DP>::STRIDE;
+    __shared__ __attribute__((aligned(1024))) att_lds_byte lds[4 * TILE];       // keys and values, two tiles of each
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int id = (blockIdx.x & 7) * (args.q_grid >> 3) + (blockIdx.x >> 3);
@@ -92,23 +92,24 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
         // Few keys: delta from the rounded result would be off by as much as ds is large, so it is summed from the weights themselves,
         // which are normalised again while they are at hand (a single key's weight is exactly 1, its ds exactly 0).
         const att_u64 kept = att_kept_keys(keys, entry, begin, end, lane);
-        next_k.load(k, keys.k_ns, end, args.k, threadIdx.x);
-        next_v.load(v, keys.v_ns, end, args.o, threadIdx.x);
-        if (keys.mask) {
-            next_k.clear(threadIdx.x, kept);
-            next_v.clear(threadIdx.x, kept);
-        }
-        next_k.template store<ATT_STRIDE<T, DP>>(key_tile, threadIdx.x);
-        next_v.template store<ATT_STRIDE<T, DP>>(value_tile, threadIdx.x);
+        next_k.begin(k, keys.k_ns, end, args.k, lds, threadIdx.x);
+        next_v.begin(v, keys.v_ns, end, args.o, lds + TILE, threadIdx.x);
+        next_k.finish(lds, threadIdx.x);
+        next_v.finish(lds + TILE, threadIdx.x);
         __syncthreads();
+        if (keys.mask && kept != ~0ull) {
+            att_clear<T, DP, KT, 256>(lds, kept, threadIdx.x);
+            att_clear<T, DP, KT, 256>(lds + TILE, kept, threadIdx.x);
+            __syncthreads();
+        }
         float total = 0.0f, inner = 0.0f;
 #pragma unroll 1
         for (int b = 0; b < KT / 32; ++b) {
             att_f32x16 s = {0}, ds = {0};
 #pragma unroll
             for (int step = 0; step < DP / 16; ++step) {
-                s = att_mma(att_read_row<T, DP>(key_tile, ATT_STRIDE<T, DP>, 32 * b + lane % 32, 16 * step + 8 * half), query[step], s);
-                ds = att_mma(att_read_row<T, DP>(value_tile, ATT_STRIDE<T, DP>, 32 * b + lane % 32, 16 * step + 8 * half), grad[step], ds);
+                s = att_mma(att_read_row<T, DP>(lds, 32 * b, 16 * step, lane), query[step], s);
+                ds = att_mma(att_read_row<T, DP>(lds + TILE, 32 * b, 16 * step, lane), grad[step], ds);
             }
             const unsigned mine = static_cast<unsigned>(kept >> (32 * b)) >> (4 * half);
 #pragma unroll
@@ -130,25 +131,29 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
         args.stats[at] = lse2;
         args.stats[rows_total + at] = delta;
     }
+    int odd = 0;
+    att_wait_for_loads();
     if (begin < end) {
-        next_k.load(k + begin * keys.k_ns, keys.k_ns, end - begin, args.k, threadIdx.x);
-        next_v.load(v + begin * keys.v_ns, keys.v_ns, end - begin, args.o, threadIdx.x);
+        __syncthreads();
+        next_k.begin(k + begin * keys.k_ns, keys.k_ns, end - begin, args.k, lds, threadIdx.x);
+        next_v.begin(v + begin * keys.v_ns, keys.v_ns, end - begin, args.o, lds + TILE, threadIdx.x);
     }
-    for (int n = begin; n < end; n += KT) {
+    for (int n = begin; n < end; n += KT, odd ^= 1) {
         const att_u64 kept = att_kept_keys(keys, entry, n, end, lane);
+        att_lds_byte *key_tile = lds + 2 * odd * TILE, *value_tile = key_tile + TILE;
+        next_k.finish(key_tile, threadIdx.x);
+        next_v.finish(value_tile, threadIdx.x);
         __syncthreads();
-        if (keys.mask) {
-            next_k.clear(threadIdx.x, kept);
-            next_v.clear(threadIdx.x, kept);
+        if (keys.mask && kept != ~0ull) {
+            att_clear<T, DP, KT, 256>(key_tile, kept, threadIdx.x);
+            att_clear<T, DP, KT, 256>(value_tile, kept, threadIdx.x);
+            __syncthreads();
         }
-        next_k.template store<ATT_STRIDE<T, DP>>(key_tile, threadIdx.x);
-        next_k.template store<ATT_STRIDE_T<T, DP>>(key_tile_t, threadIdx.x);
-        next_v.template store<ATT_STRIDE<T, DP>>(value_tile, threadIdx.x);
-        __syncthreads();
         if (n + KT < end) {
             const i64 next = n + KT;
-            next_k.load(k + next * keys.k_ns, keys.k_ns, end - static_cast<int>(next), args.k, threadIdx.x);
-            next_v.load(v + next * keys.v_ns, keys.v_ns, end - static_cast<int>(next), args.o, threadIdx.x);
+            att_lds_byte *to = lds + 2 * (odd ^ 1) * TILE;
+            next_k.begin(k + next * keys.k_ns, keys.k_ns, end - static_cast<int>(next), args.k, to, threadIdx.x);
+            next_v.begin(v + next * keys.v_ns, keys.v_ns, end - static_cast<int>(next), args.o, to + TILE, threadIdx.x);
         }
         if (!works) continue;
 #pragma unroll
@@ -156,10 +161,10 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
             att_f32x16 s = {0}, ds = {0};
 #pragma unroll
             for (int step = 0; step < DP / 16; ++step)
-                s = att_mma(att_read_row<T, DP>(key_tile, ATT_STRIDE<T, DP>, 32 * b + lane % 32, 16 * step + 8 * half), query[step], s);
+                s = att_mma(att_read_row<T, DP>(key_tile, 32 * b, 16 * step, lane), query[step], s);
 #pragma unroll
             for (int step = 0; step < DP / 16; ++step)
-                ds = att_mma(att_read_row<T, DP>(value_tile, ATT_STRIDE<T, DP>, 32 * b + lane % 32, 16 * step + 8 * half), grad[step], ds);
+                ds = att_mma(att_read_row<T, DP>(value_tile, 32 * b, 16 * step, lane), grad[step], ds);
             const unsigned here = static_cast<unsigned>(kept >> (32 * b));
 #pragma unroll
             for (int i = 0; i < 16; ++i) ds[i] = att_weight(s[i], args.scale_log2, lse2) * (ds[i] - delta);
@@ -174,7 +179,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
                 const att_vec8<T> x = att_operand<T>(ds, step);
 #pragma unroll
                 for (int o = 0; o < DP / 32; ++o)
-                    acc[o] = att_mma(att_read_transposed(key_tile_t, ATT_STRIDE_T<T, DP>, 32 * b + 16 * step, 32 * o, lane), x, acc[o]);
+                    acc[o] = att_mma(att_read_transposed<T, DP>(key_tile, 32 * b + 16 * step, 32 * o, lane), x, acc[o]);
             }
         }
     }
@@ -192,16 +197,54 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     att_store_columns<T, DP, ALIGNED>(to, acc, args.scale, args.k, half);
 }
 
-// A workgroup per (entry of the keys, head of keys, part of the rows, 128 keys); a wave per 32 keys.
+// s of 32 rows in LDS against a wave's keys and d v^T against its values, by turns.  Between the matrix instructions, with VECTOR, the vector work of the
+// tile before: `quad(q)` makes the weights and gradients of the scores of its rows 8 q + 4 h + 0..3.
+template <typename T, int DP, bool VECTOR, typename Quad>
+__device__ __forceinline__ void att_row_scores(att_f32x16 &s, att_f32x16 &ds, const att_vec8<T> (&key)[DP / 16], const att_vec8<T> (&value)[DP / 16],
+                                               const att_lds_byte *q_tile, const att_lds_byte *d_tile, int lane, Quad quad)
+{
+    typedef AttGroups<T, DP> G;
+    constexpr int AT_ONCE = 2, ALL = G::STEPS / AT_ONCE;
+    att_vec8<T> f[2][2 * AT_ONCE];
+    auto read = [&](att_vec8<T> (&to)[2 * AT_ONCE], int i) {
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            to[2 * j] = att_read_row<T, DP>(q_tile, 0, 16 * (AT_ONCE * i + j), lane);
+            to[2 * j + 1] = att_read_row<T, DP>(d_tile, 0, 16 * (AT_ONCE * i + j), lane);
+        }
+    };
+    read(f[0], 0);
+    s = ds = att_f32x16{0};
+    att_region();
+#pragma unroll
+    for (int i = 0; i < ALL; ++i) {
+        if (i + 1 < ALL) read(f[(i + 1) & 1], i + 1);
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            s = att_mma(f[i & 1][2 * j], key[AT_ONCE * i + j], s);
+            ds = att_mma(f[i & 1][2 * j + 1], value[AT_ONCE * i + j], ds);
+        }
+        if (VECTOR)
+#pragma unroll
+            for (int q = 4 * i / ALL; q < 4 * (i + 1) / ALL; ++q) quad(q);
+        att_order<2 * AT_ONCE * G::READS_ROW, 2 * AT_ONCE * G::MMAS, VECTOR ? (sizeof(T) == 4 ? 1 : 4 * 4 / ALL + 1) : 0>();
+        att_region();
+    }
+}
+
+// A workgroup per (entry of the keys, head of keys, part of the rows, 128 keys); a wave per 32 keys, whose keys and values it keeps in registers.
+//
+// Turn i: the scores of tile i + 1 (32 rows) on the matrix cores while the vector units make the weights and gradients of tile i from its scores, then
+// the two products of tile i.  Three buffers: tile i, tile i + 1, and tile i + 2 on its way.
 template <typename T, int DP, bool ALIGNED>
 __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void attention_grad_keys(const AttentionGradArgs args)
 {
     typedef AttGradShape<T, DP> Shape;
-    constexpr int RT = Shape::ROWS;
-    __shared__ __attribute__((aligned(16))) T lds[2 * RT * Shape::BOTH];
-    __shared__ __attribute__((aligned(16))) float stats[2 * RT];
-    T *q_tile = lds, *d_tile = q_tile + RT * ATT_STRIDE<T, DP>;
-    T *q_tile_t = d_tile + RT * ATT_STRIDE<T, DP>, *d_tile_t = q_tile_t + RT * ATT_STRIDE_T<T, DP>;
+    typedef AttGroups<T, DP> G;
+    constexpr int RT = Shape::ROWS, BUFFERS = Shape::BUFFERS;
+    constexpr int TILE = RT * AttLds<T, DP>::STRIDE;
+    __shared__ __attribute__((aligned(1024))) att_lds_byte lds[2 * BUFFERS * TILE];     // queries and gradients of the result
+    __shared__ __attribute__((aligned(16))) float all_stats[BUFFERS][2 * RT];
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int id = (blockIdx.x & 7) * (args.k_grid >> 3) + (blockIdx.x >> 3);
@@ -226,121 +269,128 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
             for (int j = 0; j < 8; ++j) key[step][j] = static_cast<T>(static_cast<float>(key[step][j]) * args.query_factor);
         value[step] = att_load8<T, ALIGNED>(v, 16 * step + 8 * half, args.o);
     }
+    att_wait_for_loads();
     att_f32x16 acc_k[DP / 32], acc_v[DP / 32];
 #pragma unroll
     for (int o = 0; o < DP / 32; ++o) acc_k[o] = acc_v[o] = att_f32x16{0};
 
-    // the rows: entries that share the keys, their heads, 32 queries at a time; this part of them
+    // the rows: entries that share the keys, their heads, 32 queries at a time; this workgroup's part of them
     const int tiles_m = (args.m + RT - 1) / RT;
     const i64 per_entry = static_cast<i64>(args.r) * tiles_m;
-    const i64 items = per_entry * (args.key_entries == args.l ? 1 : args.l);
-    const i64 per_split = (items + args.k_splits - 1) / args.k_splits;
-    i64 item = split * per_split;
-    const i64 last = item + per_split < items ? item + per_split : items;
-    int entry = key_entry + static_cast<int>(item / per_entry);
-    int head = static_cast<int>(item % per_entry / tiles_m), m0 = static_cast<int>(item % tiles_m) * RT;
-
-    bool kept = false, all_kept = false;            // this lane's key takes part in the current entry; all of this wave's do
-    bool fresh = true;
-    // Goes on to the next tile whose entry meets one of the workgroup's keys; the same decisions in all waves.
-    auto find = [&]() {
-        while (item < last) {
-            if (fresh) {
-                const int length = att_length(keys, entry);
-                const att_u64 low = att_kept_keys(keys, entry, first_key, length, lane), high = att_kept_keys(keys, entry, first_key + 64, length, lane);
-                if (low | high) break;
-                item += per_entry - (static_cast<i64>(head) * tiles_m + m0 / RT);
-                ++entry;
-                head = m0 = 0;
-            } else {
-                break;
-            }
-        }
-    };
-    auto keys_of_entry = [&](int of) {
-        kept = exists && n < att_length(keys, of) && (!keys.mask || keys.mask[of * keys.mask_ls + n * keys.mask_ns] != 0);
-        all_kept = __all(kept);
-    };
+    const int entries = args.key_entries == args.l ? 1 : args.l;
+    const i64 per_split = (per_entry * entries + args.k_splits - 1) / args.k_splits;
+    const i64 part_first = split * per_split, part_last = part_first + per_split;
     const i64 rows_total = static_cast<i64>(args.l) * args.m * args.g * args.r;
-    AttTile<T, DP, RT, 256, ALIGNED> next_q, next_d;
-    float next_stat = 0.0f;
-    auto load = [&]() {
-        const int some = args.m - m0;
-        const int h = g * args.r + head;
-        next_q.load(static_cast<const T *>(args.q) + entry * args.q_ls + m0 * args.q_ms + h * args.q_hs, args.q_ms, some, args.k, threadIdx.x);
-        next_d.load(static_cast<const T *>(args.grad_out) + entry * args.grad_out_ls + m0 * args.grad_out_ms + h * args.grad_out_hs, args.grad_out_ms,
-                    some, args.o, threadIdx.x);
-        const int i = threadIdx.x % RT;
-        const i64 at = (static_cast<i64>(entry) * args.m + m0 + i) * (static_cast<i64>(args.g) * args.r) + h;
-        if (threadIdx.x < RT) next_stat = i < some ? args.stats[at] : __builtin_inff();
-        else if (threadIdx.x < 2 * RT) next_stat = i < some ? args.stats[rows_total + at] : 0.0f;
-    };
-    find();
-    int kept_entry = -1;
-    if (item < last) load();
-    while (item < last) {
-        if (entry != kept_entry) {
-            keys_of_entry(entry);
-            kept_entry = entry;
-        }
-        __syncthreads();
-        next_q.template store<ATT_STRIDE<T, DP>>(q_tile, threadIdx.x);
-        next_q.template store<ATT_STRIDE_T<T, DP>>(q_tile_t, threadIdx.x);
-        next_d.template store<ATT_STRIDE<T, DP>>(d_tile, threadIdx.x);
-        next_d.template store<ATT_STRIDE_T<T, DP>>(d_tile_t, threadIdx.x);
-        if (threadIdx.x < 2 * RT) stats[threadIdx.x] = next_stat;
-        __syncthreads();
-        ++item;
-        fresh = false;
-        m0 += RT;
-        if (m0 >= args.m) {
-            m0 = 0;
-            if (++head == args.r) {
-                head = 0;
-                ++entry;
-                fresh = true;
-            }
-        }
-        find();
-        if (item < last) load();
 
-        att_f32x16 s = {0}, ds = {0};
-#pragma unroll
-        for (int step = 0; step < DP / 16; ++step)
-            s = att_mma(att_read_row<T, DP>(q_tile, ATT_STRIDE<T, DP>, lane % 32, 16 * step + 8 * half), key[step], s);
-#pragma unroll
-        for (int step = 0; step < DP / 16; ++step)
-            ds = att_mma(att_read_row<T, DP>(d_tile, ATT_STRIDE<T, DP>, lane % 32, 16 * step + 8 * half), value[step], ds);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
+    for (int e = static_cast<int>(part_first / per_entry); e < entries && e * per_entry < part_last; ++e) {
+        const int entry = key_entry + e;
+        const int first = static_cast<int>(part_first > e * per_entry ? part_first - e * per_entry : 0);
+        const int count = static_cast<int>((part_last < (e + 1) * per_entry ? part_last - e * per_entry : per_entry) - first);
+        const int length = att_length(keys, entry);
+        if (!(att_kept_keys(keys, entry, first_key, length, lane) | att_kept_keys(keys, entry, first_key + 64, length, lane))) continue;
+        // (the gradient of a key that does not take part is cleared where it would enter the products: what the key holds may be anything)
+        const bool kept = exists && n < length && (!keys.mask || keys.mask[entry * keys.mask_ls + n * keys.mask_ns] != 0);
+        const unsigned keep = kept ? ~0u : 0u;
+
+        AttTile<T, DP, RT, 256, ALIGNED> next_q, next_d;
+        float next_stat = 0.0f;
+        int head = first / tiles_m, m0 = first % tiles_m * RT, to = 0;          // of the next tile to load
+        auto begin = [&]() {
+            const int some = args.m - m0, h = g * args.r + head;
+            att_lds_byte *q_tile = lds + 2 * to * TILE;
+            next_q.begin(static_cast<const T *>(args.q) + entry * args.q_ls + m0 * args.q_ms + h * args.q_hs, args.q_ms, some, args.k, q_tile, threadIdx.x);
+            next_d.begin(static_cast<const T *>(args.grad_out) + entry * args.grad_out_ls + m0 * args.grad_out_ms + h * args.grad_out_hs, args.grad_out_ms, some,
+                         args.o, q_tile + TILE, threadIdx.x);
+            const int i = threadIdx.x % RT, row = i < some ? i : 0;
+            const i64 at = (static_cast<i64>(entry) * args.m + m0 + row) * (static_cast<i64>(args.g) * args.r) + h;
+            if (threadIdx.x < 2 * RT) next_stat = args.stats[threadIdx.x < RT ? at : rows_total + at];
+            if (i >= some) next_stat = threadIdx.x < RT ? __builtin_inff() : 0.0f;      // a row that does not exist has weights of 0
+            m0 += RT;
+            if (m0 >= args.m) {
+                m0 = 0;
+                ++head;
+            }
+        };
+        auto finish = [&]() {
+            att_lds_byte *q_tile = lds + 2 * to * TILE;
+            next_q.finish(q_tile, threadIdx.x);
+            next_d.finish(q_tile + TILE, threadIdx.x);
+            if (threadIdx.x < 2 * RT) all_stats[to][threadIdx.x] = next_stat;
+            to = to + 1 == BUFFERS ? 0 : to + 1;
+        };
+        int now = 0;                    // the buffer of the current tile
+        auto then = [&]() { return now + 1 == BUFFERS ? 0 : now + 1; };
+        att_f32x16 s_a, ds_a, s_b, ds_b;
+        att_vec8<T> p[2], x[2];
+        auto make_quad = [&](const att_f32x16 &s, const att_f32x16 &ds, int q) {
+            const float *stats = all_stats[now];
             const att_f32x4 lse2 = *reinterpret_cast<const att_f32x4 *>(stats + 8 * q + 4 * half);
             const att_f32x4 delta = *reinterpret_cast<const att_f32x4 *>(stats + RT + 8 * q + 4 * half);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                s[4 * q + j] = att_weight(s[4 * q + j], args.scale_log2, lse2[j]);
-                ds[4 * q + j] = s[4 * q + j] * (ds[4 * q + j] - delta[j]);
+                const float weight = att_weight(s[4 * q + j], args.scale_log2, lse2[j]);
+                p[q / 2][4 * (q % 2) + j] = static_cast<T>(weight);
+                x[q / 2][4 * (q % 2) + j] = static_cast<T>(weight * (ds[4 * q + j] - delta[j]));
+            }
+        };
+        auto products = [&]() {
+            const att_lds_byte *q_tile = lds + 2 * now * TILE, *d_tile = q_tile + TILE;
+            typedef unsigned words __attribute__((ext_vector_type(sizeof(att_vec8<T>) / 4)));
+#pragma unroll
+            for (int step = 0; step < 2; ++step) {
+                p[step] = __builtin_bit_cast(att_vec8<T>, __builtin_bit_cast(words, p[step]) & keep);
+                x[step] = __builtin_bit_cast(att_vec8<T>, __builtin_bit_cast(words, x[step]) & keep);
+            }
+            att_vec8<T> f[2][DP / 32];
+            att_read_columns<T, DP>(f[0], d_tile, 0, lane);
+            att_region();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i < 3) att_read_columns<T, DP>(f[(i + 1) & 1], i == 0 ? d_tile : q_tile, i == 1 ? 0 : 16, lane);
+#pragma unroll
+                for (int o = 0; o < DP / 32; ++o) {
+                    if (i < 2) acc_v[o] = att_mma(f[i & 1][o], p[i], acc_v[o]);
+                    else acc_k[o] = att_mma(f[i & 1][o], x[i - 2], acc_k[o]);
+                }
+                att_order<DP / 32 * G::READS_T, DP / 32 * G::MMAS, 0>();
+                att_region();
+            }
+        };
+        auto turn = [&](const att_f32x16 &s, const att_f32x16 &ds, att_f32x16 &next_s, att_f32x16 &next_ds, bool more) {
+            if (BUFFERS == 3 && more) begin();
+            const att_lds_byte *q_tile = lds + 2 * then() * TILE;
+            att_row_scores<T, DP, true>(next_s, next_ds, key, value, q_tile, q_tile + TILE, lane, [&](int q) { make_quad(s, ds, q); });
+            products();
+            if (BUFFERS == 2) {
+                __syncthreads();
+                if (more) begin();
+            }
+            if (more) finish();
+            __syncthreads();
+            now = then();
+        };
+
+        __syncthreads();                // an entry before this one is done with the buffers
+        begin();
+        finish();
+        if (count > 1) {
+            begin();
+            finish();
+        }
+        __syncthreads();
+        att_row_scores<T, DP, false>(s_a, ds_a, key, value, lds, lds + TILE, lane, [](int) {});
+        for (int i = 1; i < count; i += 2) {
+            turn(s_a, ds_a, s_b, ds_b, i + 1 < count);
+            if (i + 1 < count) {
+                turn(s_b, ds_b, s_a, ds_a, i + 2 < count);
+            } else {
+                s_a = s_b;
+                ds_a = ds_b;
             }
         }
-        if (!all_kept) {
-            att_rare();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[i] = kept ? s[i] : 0.0f;
-                ds[i] = kept ? ds[i] : 0.0f;
-            }
-        }
-#pragma unroll
-        for (int step = 0; step < 2; ++step) {
-            const att_vec8<T> p = att_operand<T>(s, step);
-#pragma unroll
-            for (int o = 0; o < DP / 32; ++o) acc_v[o] = att_mma(att_read_transposed(d_tile_t, ATT_STRIDE_T<T, DP>, 16 * step, 32 * o, lane), p, acc_v[o]);
-        }
-#pragma unroll
-        for (int step = 0; step < 2; ++step) {
-            const att_vec8<T> x = att_operand<T>(ds, step);
-#pragma unroll
-            for (int o = 0; o < DP / 32; ++o) acc_k[o] = att_mma(att_read_transposed(q_tile_t, ATT_STRIDE_T<T, DP>, 16 * step, 32 * o, lane), x, acc_k[o]);
-        }
+        for (int q = 0; q < 4; ++q) make_quad(s_a, ds_a, q);
+        products();
     }
     if (!exists) return;
     const i64 at = (static_cast<i64>(key_entry) * keys.n + n) * args.g + g;
