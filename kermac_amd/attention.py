@@ -312,7 +312,7 @@ def cross_attention_grad(
         workspace = _scratch.allocate(needed, plan.device)
         if workspace is None:           # refused: uncut launches, with room for the sums of a row
             L, M, _, H = plan.extents[:4]
-            needed = -(-8 * L * M * H // 16) * 16
+            needed = (8 * L * M * H + 8 + 15) // 16 * 16
             workspace = _scratch.allocate(needed, plan.device)
         if workspace is None:
             raise RuntimeError(f"cross_attention_grad needs {needed} bytes of scratch memory: the limit, the supplied buffer or the device does not allow them")

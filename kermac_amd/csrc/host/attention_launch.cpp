@@ -300,7 +300,7 @@ int prepare(const kmc_attention_gradient_params *p, bool may_cut, GradPlan *plan
     args.k_grid = static_cast<int>((k_workgroups + 7) / 8 * 8);
 
     const int64_t q_rows = static_cast<int64_t>(p->l) * p->m * p->h, k_rows = static_cast<int64_t>(p->key_entries) * p->n * p->g;
-    plan->stats_bytes = (8 * q_rows + 15) / 16 * 16;
+    plan->stats_bytes = (8 * q_rows + 8 + 15) / 16 * 16;
     if (args.q_splits > 1) plan->q_bytes = 4ll * args.q_splits * q_rows * args.partial_k_width;
     if (args.k_splits > 1) {
         plan->k_bytes = 4ll * args.k_splits * k_rows * args.partial_k_width;

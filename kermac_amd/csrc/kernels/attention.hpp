@@ -60,18 +60,16 @@ __device__ __forceinline__ constexpr int att_row(int i, int half) { return 8 * (
 __device__ __forceinline__ float att_other_half(float x) { return __shfl_xor(x, 32); }
 
 // A tile of rows of DP elements in LDS, read both ways: 16 bytes of a row per lane, 16 rows at a time, and transposed, which touches 4 rows x 64 bytes per
-// half wave.  Rows of a power of two of bytes stand side by side, and row r holds its 16-byte piece c in place c ^ swizzle(r) / 16: sixteen consecutive
-// rows then have a given piece in different banks, and four rows a given four pieces.  Rows of 96 elements get 16 bytes of padding instead.
+// half wave.  Row r holds its 16-byte piece c in place c ^ swizzle(r) / 16: sixteen consecutive rows then have a given piece in different banks, and four
+// rows a given four pieces (no bank conflict is counted).  Rows take a power of two of bytes: those of 96 elements the place of 128.
 template <typename T, int DP>
 struct AttLds {
     static constexpr int PIECE = 16 / static_cast<int>(sizeof(T));      // elements of 16 bytes
-    static constexpr int ROW_BYTES = DP * static_cast<int>(sizeof(T));
-    static constexpr bool SWIZZLED = (ROW_BYTES & (ROW_BYTES - 1)) == 0;
-    static constexpr int STRIDE = SWIZZLED ? ROW_BYTES : ROW_BYTES + 16;
+    static constexpr int STRIDE = (DP == 96 ? 128 : DP) * static_cast<int>(sizeof(T));
     // The bits that the swizzle of row r turns in a byte offset; linear in the bits of r.  Two rows of 128 bytes share a line of banks.
     static __device__ __forceinline__ constexpr int swizzle(int r)
     {
-        return !SWIZZLED ? 0 : ROW_BYTES == 128 ? ((r >> 1 & 1) << 2 | (r >> 2 & 3)) << 4 : ((r & 3) << 2 | (r >> 2 & 3)) << 4;
+        return STRIDE == 128 ? ((r >> 1 & 1) << 2 | (r >> 2 & 3)) << 4 : ((r & 3) << 2 | (r >> 2 & 3)) << 4;
     }
     static __device__ __forceinline__ constexpr int offset(int row, int piece) { return row * STRIDE + (16 * piece ^ swizzle(row)); }
 };
@@ -85,14 +83,14 @@ __device__ __forceinline__ att_vec8<T> att_read_row(const att_lds_byte *tile, in
     typedef AttLds<T, DP> Lds;
     const int size = static_cast<int>(sizeof(T));
     const int mine = (lane & 31) * Lds::STRIDE + (8 * size * (lane >> 5) ^ Lds::swizzle(lane & 31));
-    const int here = Lds::SWIZZLED ? mine ^ k * size : mine + k * size;
+    const int here = mine ^ k * size;
     const att_lds_byte *p = tile + row * Lds::STRIDE;
     att_vec8<T> x;
     if constexpr (sizeof(T) == 2) {
         x = *reinterpret_cast<const att_vec8<T> *>(p + here);
     } else {
         const att_f32x4 low = *reinterpret_cast<const att_f32x4 *>(p + here);
-        const att_f32x4 high = *reinterpret_cast<const att_f32x4 *>(p + (Lds::SWIZZLED ? here ^ 16 : here + 16));
+        const att_f32x4 high = *reinterpret_cast<const att_f32x4 *>(p + (here ^ 16));
 #pragma unroll
         for (int j = 0; j < 4; ++j) { x[j] = low[j]; x[4 + j] = high[j]; }
     }
@@ -109,11 +107,11 @@ __device__ __forceinline__ att_vec8<T> att_read_transposed(const att_lds_byte *t
     if constexpr (sizeof(T) == 2) {
         const int r = 4 * half + (lane & 15) / 4;
         const int mine = r * Lds::STRIDE + (((32 * (lane >> 4 & 1) + 8 * (lane & 3)) ^ Lds::swizzle(r)));
-        const att_lds_byte *p = tile + row * Lds::STRIDE + (Lds::SWIZZLED ? mine ^ 2 * column : mine + 2 * column);
+        const att_lds_byte *p = tile + row * Lds::STRIDE + (mine ^ 2 * column);
         typedef __attribute__((address_space(3))) att_s16x4 lds_s16x4;
         union { att_s16x4 part[2]; att_vec8<T> whole; } u;
         u.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p));
-        const int behind = Lds::SWIZZLED ? (mine ^ 2 * column ^ Lds::swizzle(8)) : mine + 2 * column;       // the same place of row r + 8
+        const int behind = mine ^ 2 * column ^ Lds::swizzle(8);       // the same place of row r + 8
         u.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(tile + (row + 8) * Lds::STRIDE + behind));
         x = u.whole;
     } else {
@@ -121,7 +119,7 @@ __device__ __forceinline__ att_vec8<T> att_read_transposed(const att_lds_byte *t
         for (int j = 0; j < 4; ++j) {
             const int r = 4 * half + j;
             const int mine = r * Lds::STRIDE + (4 * (lane & 31) ^ Lds::swizzle(r));
-            const int here = Lds::SWIZZLED ? mine ^ 4 * column : mine + 4 * column;
+            const int here = mine ^ 4 * column;
             x[j] = *reinterpret_cast<const float *>(tile + row * Lds::STRIDE + here);
             x[4 + j] = *reinterpret_cast<const float *>(tile + (row + 8) * Lds::STRIDE + (here ^ Lds::swizzle(8)));
         }
@@ -184,26 +182,35 @@ __device__ __forceinline__ att_s32x4 att_descriptor(const T *base, int step, int
                      __builtin_amdgcn_readfirstlane(bytes), ATT_BUFFER_FORMAT};
 }
 
-// Nothing that was loaded is outstanding, and the compiler knows: it would otherwise wait, in front of the first use of a register that was loaded
+// 4 bytes per lane from memory straight into LDS: lane l's to to + 4 l.
+__device__ __forceinline__ void att_load_words(const float *from, const float *to)
+{
+    typedef const __attribute__((address_space(1))) float *global_float;
+    const unsigned lds = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(reinterpret_cast<size_t>((const __attribute__((address_space(3))) float *)to)));
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"((global_float)from), "s"(lds) : "memory", "m0");
+}
+
+// At most IN_FLIGHT loads are outstanding, and the compiler knows: it would otherwise wait, in front of the first use of a register that was loaded
 // before a loop, for everything that is outstanding in every turn of the loop, the tiles on their way to LDS included (a third of the run time).
+template <int IN_FLIGHT = 0>
 __device__ __forceinline__ void att_wait_for_loads()
 {
+    static_assert(IN_FLIGHT < 64, "the counter has six bits");
     asm volatile("" : : : "memory");
-    __builtin_amdgcn_s_waitcnt(0x0f70);         // vmcnt 0, the other counters as they are
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (IN_FLIGHT & 15) | (IN_FLIGHT >> 4) << 14);         // vmcnt, the other counters as they are
     asm volatile("" : : : "memory");
 }
 
 // A tile of ROWS rows of DP elements on its way from memory to LDS.  begin() asks for it, finish() has it written.  DIRECT: from memory straight into LDS, 1 KB per
-// wave and instruction, each lane fetching the piece that belongs where its 16 bytes end up; no register waits for it.  Otherwise (rows that are no
-// power of two, unaligned rows, tiles of one wave) through registers.
+// wave and instruction, each lane fetching the piece that belongs where its 16 bytes end up; no register waits for it.  Otherwise (unaligned rows,
+// tiles of one wave) through registers.
 template <typename T, int DP, int ROWS, int THREADS, bool ALIGNED>
 struct AttTile {
     typedef AttLds<T, DP> Lds;
-    static constexpr bool DIRECT = ALIGNED && Lds::SWIZZLED && THREADS > 64;
-    static constexpr int PIECES = DP / Lds::PIECE;                      // of a row
-    static constexpr int SLOTS = PIECES <= 8 ? 8 : PIECES <= 16 ? 16 : PIECES <= 32 ? 32 : 64;        // threads of a row; those behind PIECES have no piece
+    static constexpr bool DIRECT = ALIGNED && THREADS > 64;
+    static constexpr int SLOTS = Lds::STRIDE / 16;                      // threads of a row
     static constexpr int ROW_STEP = THREADS / SLOTS;
-    static constexpr int PER_THREAD = ROWS / ROW_STEP;
+    static constexpr int PER_THREAD = ROWS / ROW_STEP;                  // loads of a thread
     static_assert(THREADS % SLOTS == 0 && ROWS % ROW_STEP == 0 && PER_THREAD > 0, "whole rows per step");
     att_u32x4 held[DIRECT ? 1 : PER_THREAD];
 
@@ -242,14 +249,14 @@ struct AttTile {
         }
     }
 
-    // Followed by a barrier.
+    // Followed by a barrier.  IN_FLIGHT: loads that were asked for later and may still be on their way.
+    template <int IN_FLIGHT = 0>
     __device__ __forceinline__ void finish(att_lds_byte *tile, int thread) const
     {
         if constexpr (DIRECT) {
-            att_wait_for_loads();
+            att_wait_for_loads<IN_FLIGHT>();
         } else {
             const int row = thread / SLOTS, piece = thread % SLOTS;
-            if (SLOTS != PIECES && piece >= PIECES) return;
 #pragma unroll
             for (int j = 0; j < PER_THREAD; ++j) *reinterpret_cast<att_u32x4 *>(tile + Lds::offset(row + j * ROW_STEP, piece)) = held[j];
         }

@@ -52,7 +52,7 @@ struct AttentionGradArgs {
     int l, m, g, r, k, o;
     int key_entries;                        // l, or 1: one source for all entries
     float scale, scale_log2, query_factor;
-    float *stats;                           // [2, l, m, g r]: lse to base 2 (+inf without keys) and delta, from the first kernel for the second
+    float *stats;                           // [2, l, g r, m]: lse to base 2 (+inf without keys) and delta, from the first kernel for the second; behind them +inf and 0
     int q_row_tiles, q_splits, q_workgroups, q_grid;
     int key_tiles, k_splits, k_workgroups, k_grid;
     float *partial_q, *partial_k, *partial_v;   // [splits, rows, width rounded up to 4], where the work is cut

@@ -24,7 +24,8 @@ struct AttGradShape {
     static constexpr int WAVES_PER_SIMD = ROW_BYTES <= 256 ? 2 : 1;
     static constexpr int WAVES_PER_SIMD_K = ROW_BYTES <= 128 ? 2 : 1;
     static constexpr int ROWS = 32;                                 // per tile of the keys' kernel
-    static constexpr int BUFFERS = ROW_BYTES <= 512 ? 3 : 2;        // for its tiles: three of 64 KB do not fit
+    static constexpr int PAIR = 2 * ROWS * AttLds<T, DP>::STRIDE;   // bytes of a tile of queries and one of gradients
+    static constexpr int DEEP = PAIR <= 16384 ? 6 : PAIR <= 32768 ? 4 : 2;      // buffers for them that fit LDS (twice, where two workgroups share a CU)
 };
 
 // ds of a 32 x 32 result from scores, d v^T, and the row's statistics: p comes back in `s`.
@@ -127,9 +128,14 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
             if (length > 1) lse2 += __builtin_amdgcn_logf(total);
         }
     }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {          // for rows that do not exist: weights of 0
+        args.stats[2 * rows_total] = __builtin_inff();
+        args.stats[2 * rows_total + 1] = 0.0f;
+    }
     if (split == 0 && row < rows && half == 0) {
-        args.stats[at] = lse2;
-        args.stats[rows_total + at] = delta;
+        float *stats = args.stats + (static_cast<i64>(entry) * args.g * args.r + head) * args.m + token;
+        stats[0] = lse2;
+        stats[rows_total] = delta;
     }
     int odd = 0;
     att_wait_for_loads();
@@ -235,16 +241,20 @@ __device__ __forceinline__ void att_row_scores(att_f32x16 &s, att_f32x16 &ds, co
 // A workgroup per (entry of the keys, head of keys, part of the rows, 128 keys); a wave per 32 keys, whose keys and values it keeps in registers.
 //
 // Turn i: the scores of tile i + 1 (32 rows) on the matrix cores while the vector units make the weights and gradients of tile i from its scores, then
-// the two products of tile i.  Three buffers: tile i, tile i + 1, and tile i + 2 on its way.
+// the two products of tile i.  Behind the buffers of these two tiles stand as many as fit for those on their way: the workgroups of a head walk its rows in step,
+// so every tile comes from far, and one turn is shorter than that takes.
 template <typename T, int DP, bool ALIGNED>
 __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void attention_grad_keys(const AttentionGradArgs args)
 {
     typedef AttGradShape<T, DP> Shape;
     typedef AttGroups<T, DP> G;
-    constexpr int RT = Shape::ROWS, BUFFERS = Shape::BUFFERS;
-    constexpr int TILE = RT * AttLds<T, DP>::STRIDE;
+    constexpr int RT = Shape::ROWS, TILE = RT * AttLds<T, DP>::STRIDE;
+    typedef AttTile<T, DP, RT, 256, ALIGNED> Tile;
+    constexpr int BUFFERS = Tile::DIRECT || Shape::DEEP == 2 ? Shape::DEEP : 3;
+    constexpr int AHEAD = BUFFERS == 2 ? 1 : BUFFERS - 2;              // tiles on their way behind the two in use
+    constexpr int LOADS = 2 * Tile::PER_THREAD + 1;                     // of a wave for a tile
     __shared__ __attribute__((aligned(1024))) att_lds_byte lds[2 * BUFFERS * TILE];     // queries and gradients of the result
-    __shared__ __attribute__((aligned(16))) float all_stats[BUFFERS][2 * RT];
+    __shared__ __attribute__((aligned(256))) float all_stats[BUFFERS][2 * RT];           // lse to base 2 and delta of a tile's rows
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int id = (blockIdx.x & 7) * (args.k_grid >> 3) + (blockIdx.x >> 3);
@@ -292,8 +302,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
         const bool kept = exists && n < length && (!keys.mask || keys.mask[entry * keys.mask_ls + n * keys.mask_ns] != 0);
         const unsigned keep = kept ? ~0u : 0u;
 
-        AttTile<T, DP, RT, 256, ALIGNED> next_q, next_d;
-        float next_stat = 0.0f;
+        Tile next_q, next_d;
         int head = first / tiles_m, m0 = first % tiles_m * RT, to = 0;          // of the next tile to load
         auto begin = [&]() {
             const int some = args.m - m0, h = g * args.r + head;
@@ -301,22 +310,30 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
             next_q.begin(static_cast<const T *>(args.q) + entry * args.q_ls + m0 * args.q_ms + h * args.q_hs, args.q_ms, some, args.k, q_tile, threadIdx.x);
             next_d.begin(static_cast<const T *>(args.grad_out) + entry * args.grad_out_ls + m0 * args.grad_out_ms + h * args.grad_out_hs, args.grad_out_ms, some,
                          args.o, q_tile + TILE, threadIdx.x);
-            const int i = threadIdx.x % RT, row = i < some ? i : 0;
-            const i64 at = (static_cast<i64>(entry) * args.m + m0 + row) * (static_cast<i64>(args.g) * args.r) + h;
-            if (threadIdx.x < 2 * RT) next_stat = args.stats[threadIdx.x < RT ? at : rows_total + at];
-            if (i >= some) next_stat = threadIdx.x < RT ? __builtin_inff() : 0.0f;      // a row that does not exist has weights of 0
+            // (all waves load the same: they count the same loads; rows that do not exist get the pair behind all others)
+            const int i = lane % RT;
+            const i64 at = i < some ? (static_cast<i64>(entry) * args.g * args.r + h) * args.m + m0 + i + (lane < RT ? 0 : rows_total)
+                                    : 2 * rows_total + (lane < RT ? 0 : 1);
+            att_load_words(args.stats + at, all_stats[to]);
             m0 += RT;
             if (m0 >= args.m) {
                 m0 = 0;
                 ++head;
             }
+            if (Tile::DIRECT) to = to + 1 == BUFFERS ? 0 : to + 1;
         };
-        auto finish = [&]() {
-            att_lds_byte *q_tile = lds + 2 * to * TILE;
-            next_q.finish(q_tile, threadIdx.x);
-            next_d.finish(q_tile + TILE, threadIdx.x);
-            if (threadIdx.x < 2 * RT) all_stats[to][threadIdx.x] = next_stat;
-            to = to + 1 == BUFFERS ? 0 : to + 1;
+        // The tile asked for longest ago has arrived; `some`: AHEAD - 1 others are on their way.
+        auto finish = [&](bool some) {
+            if constexpr (Tile::DIRECT) {
+                if (some) att_wait_for_loads<(AHEAD - 1) * LOADS>();
+                else att_wait_for_loads();
+            } else {
+                att_wait_for_loads();
+                att_lds_byte *q_tile = lds + 2 * to * TILE;
+                next_q.finish(q_tile, threadIdx.x);
+                next_d.finish(q_tile + TILE, threadIdx.x);
+                to = to + 1 == BUFFERS ? 0 : to + 1;
+            }
         };
         int now = 0;                    // the buffer of the current tile
         auto then = [&]() { return now + 1 == BUFFERS ? 0 : now + 1; };
@@ -356,33 +373,37 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
                 att_region();
             }
         };
-        auto turn = [&](const att_f32x16 &s, const att_f32x16 &ds, att_f32x16 &next_s, att_f32x16 &next_ds, bool more) {
-            if (BUFFERS == 3 && more) begin();
+        // `behind`: tiles behind the next one
+        auto turn = [&](const att_f32x16 &s, const att_f32x16 &ds, att_f32x16 &next_s, att_f32x16 &next_ds, int behind) {
+            if (BUFFERS > 2 && behind >= AHEAD) begin();
             const att_lds_byte *q_tile = lds + 2 * then() * TILE;
             att_row_scores<T, DP, true>(next_s, next_ds, key, value, q_tile, q_tile + TILE, lane, [&](int q) { make_quad(s, ds, q); });
             products();
             if (BUFFERS == 2) {
                 __syncthreads();
-                if (more) begin();
+                if (behind >= AHEAD) begin();
             }
-            if (more) finish();
+            if (behind > 0) finish(behind >= AHEAD);
             __syncthreads();
             now = then();
         };
 
         __syncthreads();                // an entry before this one is done with the buffers
-        begin();
-        finish();
-        if (count > 1) {
-            begin();
-            finish();
+        if constexpr (Tile::DIRECT) {
+            for (int i = 0; i < count && i < 2 + AHEAD - 1; ++i) begin();
+            finish(false);
+        } else {
+            for (int i = 0; i < count && i < 2; ++i) {
+                begin();
+                finish(false);
+            }
         }
         __syncthreads();
         att_row_scores<T, DP, false>(s_a, ds_a, key, value, lds, lds + TILE, lane, [](int) {});
         for (int i = 1; i < count; i += 2) {
-            turn(s_a, ds_a, s_b, ds_b, i + 1 < count);
+            turn(s_a, ds_a, s_b, ds_b, count - 1 - i);
             if (i + 1 < count) {
-                turn(s_b, ds_b, s_a, ds_a, i + 2 < count);
+                turn(s_b, ds_b, s_a, ds_a, count - 2 - i);
             } else {
                 s_a = s_b;
                 ds_a = ds_b;

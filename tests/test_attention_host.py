@@ -158,8 +158,8 @@ def test_the_library_refuses_gradients_before_any_device_call(change):
     params = _plan_attention_grad(make(2, 5, 4, 24), make(2, 5, 4, 16), make(2, 7, 2, 16), make(2, 7, 2, 24), make(2, 5, 4, 24), make(2, 5, 4), None, None, None,
                                   require_device=False).params
     needed = _backend.attention_gradient_workspace_bytes(params)
-    assert needed >= 8 * 2 * 5 * 4
-    for workspace, nbytes in ((None, needed), (1 << 20, 8 * 2 * 5 * 4 - 1), ((1 << 20) + 4, needed)):
+    assert needed >= 8 * (2 * 5 * 4 + 1)
+    for workspace, nbytes in ((None, needed), (1 << 20, 8 * (2 * 5 * 4 + 1) - 1), ((1 << 20) + 4, needed)):
         params.workspace, params.workspace_bytes = workspace, nbytes
         with pytest.raises(_backend.BackendError, match="workspace"):
             _backend.attention_gradient(params, None)
