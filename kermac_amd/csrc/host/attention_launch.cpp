@@ -24,6 +24,9 @@ constexpr int MAX_WIDTH = 256;
 constexpr int MAX_KEYS = 0x7fffffff - 1024;         // a tile behind the last key still has a number
 int element_size(int type) { return type == KMC_FP32 ? 4 : 2; }
 
+// Features that the kernels are compiled for.
+int padded_width(int features) { return features <= 64 ? 64 : features <= 96 ? 96 : features <= 128 ? 128 : 256; }
+
 // Whether rows can be read and written 16 bytes at a time: the address, and the stride of every dimension that is walked.  The tokens of a
 // tile are read through one buffer descriptor, which wants rows that do not overlap and a tile that it can number in 31 bits.
 struct Layout {
@@ -80,8 +83,7 @@ constexpr int ROWS_PER_WORKGROUP = 128;
 // 32 x 4000 x 16 heads of 64 features with lengths 82.9 / 75.7 (4 parts), best 73.3 (6); 128 x 1000 x 16 heads 92.1 uncut, 99.7 in 2 parts.
 double time_of_parts(int splits, int64_t base, int64_t rows_total, int64_t keys, bool own_keys, const kmc_attention_params *p, bool joined, double beside_us)
 {
-    const int features = std::max(p->k, p->o);
-    const double size = p->type == KMC_FP32 ? 4.0 : 2.0, width = features <= 64 ? 64 : features <= 96 ? 96 : features <= 128 ? 128 : 256;
+    const double size = element_size(p->type), width = padded_width(std::max(p->k, p->o));
     const int64_t workgroups = base * splits, least = own_keys ? 128 : 64;
     const double steps = static_cast<double>((keys + least * splits - 1) / (least * splits));
     const double join_us = (splits > 1 || joined ? rows_total * p->o * 8.0 / 4.0e6 * splits : 0.0) + (splits > 1 && !joined ? 5.0 : 0.0);
@@ -225,16 +227,23 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
     return KMC_OK;
 }
 
-constexpr int WANTED_WORKGROUPS = 512;              // two per CU
-constexpr int MIN_KEYS = 256;                       // that a part of the queries' kernel walks at least
-constexpr int MAX_PARTS = 128;
+constexpr int MAX_PARTS = 64;
 
-// Parts that `base` workgroups of `extent` steps each are cut into, `least` steps to a part.
-int parts(int64_t base, int64_t extent, int64_t least)
+// Parts that `base` workgroups of `steps` tiles each are cut into, by a model of the launch in microseconds: whole rounds of `slots` workgroups, each of
+// which takes `step_us` per tile and 3 us around them, and the sum of the parts, which costs a launch and writing and reading `elements` per part.
+int parts(int64_t base, int64_t slots, int64_t steps, double step_us, double elements)
 {
-    if (base == 0) return 1;
-    const int64_t wanted = std::min<int64_t>({(WANTED_WORKGROUPS + base / 2) / base, (extent + least - 1) / least, MAX_PARTS});
-    return static_cast<int>(std::max<int64_t>(wanted, 1));
+    int best = 1;
+    double best_us = 0;
+    for (int splits = 1; splits <= MAX_PARTS && (splits == 1 || splits <= steps); ++splits) {
+        const double rounds = static_cast<double>((base * splits + slots - 1) / slots);
+        const double us = rounds * ((steps + splits - 1) / splits * step_us + 3.0) + (splits > 1 ? 5.0 + splits * elements * 8.0 / 4.0e6 : 0.0);
+        if (splits == 1 || us < best_us) {
+            best_us = us;
+            best = splits;
+        }
+    }
+    return best;
 }
 
 struct GradPlan {
@@ -243,8 +252,6 @@ struct GradPlan {
     int64_t stats_bytes, q_bytes, k_bytes, v_bytes;
     int64_t bytes() const { return stats_bytes + q_bytes + k_bytes + v_bytes; }
 };
-
-constexpr int MIN_ROW_TILES = 4;                    // tiles of rows that a part of the keys' kernel walks at least
 
 int prepare(const kmc_attention_gradient_params *p, bool may_cut, GradPlan *plan)
 {
@@ -287,11 +294,16 @@ int prepare(const kmc_attention_gradient_params *p, bool may_cut, GradPlan *plan
     const int64_t rows = static_cast<int64_t>(p->m) * args.r;
     args.q_row_tiles = static_cast<int>((rows + 127) / 128);
     const int64_t q_base = static_cast<int64_t>(p->l) * p->g * args.q_row_tiles;
-    args.q_splits = may_cut ? parts(q_base, p->n, MIN_KEYS) : 1;
+    // a tile of the queries' kernel is 64 keys (32 of rows above 256 bytes), of the keys' kernel 32 rows; two workgroups share a CU where rows have at most
+    // 256 bytes (queries) or 128 (keys)
+    const double width = padded_width(std::max(p->k, p->o)), slower = p->type == KMC_FP32 ? 7.0 : 1.0;
+    const int64_t row_bytes = static_cast<int64_t>(width) * element_size(p->type), q_tile = row_bytes <= 256 ? 64 : 32;
+    const double q_elements = static_cast<double>(p->l) * p->m * p->h * p->k, k_elements = static_cast<double>(p->key_entries) * p->n * p->g * (p->k + p->o);
+    args.q_splits = may_cut ? parts(q_base, row_bytes <= 256 ? 512 : 256, (p->n + q_tile - 1) / q_tile, 2.4 * width / 128 * slower * (row_bytes <= 256 ? 1.0 : 0.3), q_elements) : 1;
     args.key_tiles = (p->n + 127) / 128;
     const int64_t k_base = static_cast<int64_t>(p->key_entries) * p->g * args.key_tiles;
     const int64_t tiles_of_rows = static_cast<int64_t>(args.r) * ((p->m + 31) / 32) * (p->key_entries == p->l ? 1 : p->l);
-    args.k_splits = may_cut ? parts(k_base, tiles_of_rows, MIN_ROW_TILES) : 1;
+    args.k_splits = may_cut ? parts(k_base, row_bytes <= 128 ? 512 : 256, tiles_of_rows, 1.2 * width / 128 * slower * (row_bytes <= 128 ? 1.6 : 1.0), k_elements) : 1;
     const int64_t q_workgroups = q_base * args.q_splits, k_workgroups = k_base * args.k_splits;
     if (std::max(q_workgroups, k_workgroups) > 0x7ffffff0ll) return fail(KMC_ERR_INVALID_ARGUMENT, "more workgroups than a launch holds");
     args.q_workgroups = static_cast<int>(q_workgroups);

@@ -59,13 +59,18 @@ struct AttentionGradArgs {
     int partial_k_width, partial_o_width;
 };
 
-// The sum of partial results, times a factor, in the operands' type.
-struct AttentionSumArgs {
+// Sums of partial results, times a factor, in the operands' type: up to three results in one launch.
+struct AttentionSum {
     const float *partial;
     void *out;
     i64 rows;
     int splits, width, partial_width;
     float factor;
+};
+
+struct AttentionSumArgs {
+    AttentionSum part[3];
+    i64 first[4];                           // elements in front of each part, of all
 };
 
 }  // namespace kmc

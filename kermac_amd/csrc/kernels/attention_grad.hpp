@@ -436,12 +436,17 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
 template <typename T>
 __global__ __launch_bounds__(256) void attention_sum(const AttentionSumArgs args)
 {
-    const i64 count = args.rows * args.width, step = static_cast<i64>(gridDim.x) * 256;
-    for (i64 i = static_cast<i64>(blockIdx.x) * 256 + threadIdx.x; i < count; i += step) {
-        const float *from = args.partial + i / args.width * args.partial_width + i % args.width;
-        float sum = 0.0f;
-        for (int part = 0; part < args.splits; ++part) sum += from[part * args.rows * args.partial_width];
-        static_cast<T *>(args.out)[i] = static_cast<T>(sum * args.factor);
+    const i64 step = static_cast<i64>(gridDim.x) * 256;
+    for (i64 i = static_cast<i64>(blockIdx.x) * 256 + threadIdx.x; i < args.first[3]; i += step) {
+        const int which = i >= args.first[2] ? 2 : i >= args.first[1] ? 1 : 0;
+        const AttentionSum &sum = args.part[which];
+        const i64 at = i - args.first[which];
+        const float *from = sum.partial + at / sum.width * sum.partial_width + at % sum.width;
+        const i64 stride = sum.rows * sum.partial_width;
+        float total = 0.0f;
+#pragma unroll 8
+        for (int part = 0; part < sum.splits; ++part) total += from[part * stride];
+        static_cast<T *>(sum.out)[at] = static_cast<T>(total * sum.factor);
     }
 }
 

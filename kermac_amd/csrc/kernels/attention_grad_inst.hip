@@ -29,13 +29,6 @@ hipError_t gradient(const kmc::AttentionGradArgs &args, bool aligned, hipStream_
     return aligned ? gradient<DP, true>(args, stream) : gradient<DP, false>(args, stream);
 }
 
-hipError_t sum(const float *partial, void *out, kmc::i64 rows, int splits, int width, int partial_width, float factor, hipStream_t stream)
-{
-    const kmc::AttentionSumArgs args = {partial, out, rows, splits, width, partial_width, factor};
-    const kmc::i64 blocks = (rows * width + 255) / 256;
-    return launch(kmc::attention_sum<Element>, dim3(static_cast<unsigned>(blocks < 16384 ? blocks : 16384)), dim3(256), stream, args);
-}
-
 }  // namespace
 
 #define KMC_ATT_NAME_2(name, type) name##_##type
@@ -48,14 +41,20 @@ hipError_t KMC_ATT_NAME(launch_attention_gradient)(const kmc::AttentionGradArgs 
                         : width <= 96  ? gradient<96>(args, aligned, stream)
                         : width <= 128 ? gradient<128>(args, aligned, stream)
                                        : gradient<256>(args, aligned, stream);
+    if (status != hipSuccess || (args.q_splits == 1 && args.k_splits == 1)) return status;
     const kmc::i64 q_rows = static_cast<kmc::i64>(args.l) * args.m * args.g * args.r;
-    const kmc::i64 k_rows = static_cast<kmc::i64>(args.key_entries) * args.keys.n * args.g;
-    if (status == hipSuccess && args.q_splits > 1)
-        status = sum(args.partial_q, args.grad_q, q_rows, args.q_splits, args.k, args.partial_k_width, args.scale, stream);
-    if (status == hipSuccess && args.k_splits > 1)
-        status = sum(args.partial_k, args.grad_k, k_rows, args.k_splits, args.k, args.partial_k_width, args.scale, stream);
-    if (status == hipSuccess && args.k_splits > 1)
-        status = sum(args.partial_v, args.grad_v, k_rows, args.k_splits, args.o, args.partial_o_width, 1.0f, stream);
+    const kmc::i64 k_rows = args.k_splits > 1 ? static_cast<kmc::i64>(args.key_entries) * args.keys.n * args.g : 0;
+    const kmc::AttentionSum parts[3] = {
+        {args.partial_q, args.grad_q, args.q_splits > 1 ? q_rows : 0, args.q_splits, args.k, args.partial_k_width, args.scale},
+        {args.partial_k, args.grad_k, k_rows, args.k_splits, args.k, args.partial_k_width, args.scale},
+        {args.partial_v, args.grad_v, k_rows, args.k_splits, args.o, args.partial_o_width, 1.0f}};
+    kmc::AttentionSumArgs sums = {};
+    for (int i = 0; i < 3; ++i) {
+        sums.part[i] = parts[i];
+        sums.first[i + 1] = sums.first[i] + parts[i].rows * parts[i].width;
+    }
+    const kmc::i64 blocks = (sums.first[3] + 255) / 256;
+    if (blocks > 0) status = launch(kmc::attention_sum<Element>, dim3(static_cast<unsigned>(blocks < 16384 ? blocks : 16384)), dim3(256), stream, sums);
     return status;
 }
 
