@@ -36,19 +36,19 @@ _GRADIENT_PARAMS = struct.Struct(_backend.struct_format(_backend.AttentionGradie
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(L, M, N, H, G, K, O, P, causal):
-    """kmc_attention_workspace_bytes: a function of the extents alone."""
+def _workspace_bytes(element, L, M, N, H, G, K, O, P, causal, with_lengths):
+    """kmc_attention_workspace_bytes: a function of these alone."""
     one = 16                            # stands for any address: nothing is read
     return _backend.attention_workspace_bytes(_backend.AttentionParams(
-        _backend.FP32, 0, L, M, N, H, G, K, O, 1.0, q=one, key=one, value=one, out=one, key_lengths=one, prefix_n=P, causal=causal,
+        element, 0, L, M, N, H, G, K, O, 1.0, q=one, key=one, value=one, out=one, key_lengths=one if with_lengths else None, prefix_n=P, causal=causal,
         prefix_key=one, prefix_value=one))
 
 
 @functools.lru_cache(maxsize=4096)
-def _gradient_workspace_bytes(L, M, N, H, G, K, O, key_entries):
+def _gradient_workspace_bytes(element, L, M, N, H, G, K, O, key_entries):
     one = 16
     return _backend.attention_gradient_workspace_bytes(_backend.AttentionGradientParams(
-        _backend.FP32, 0, L, M, N, H, G, K, O, key_entries, 1.0, q=one, key=one, value=one, out=one, grad_out=one, lse=one, grad_q=one, grad_key=one,
+        element, 0, L, M, N, H, G, K, O, key_entries, 1.0, q=one, key=one, value=one, out=one, grad_out=one, lse=one, grad_q=one, grad_key=one,
         grad_value=one))
 
 
@@ -179,7 +179,7 @@ def _plan_attention(queries, keys, values, out, scale, key_lengths, key_mask, re
         plan.lse = torch.empty((L, M, H), dtype=torch.float32, device=device)
         lse_ptr = plan.lse.data_ptr()
     plan.out, plan.device = out, device
-    plan.extents = (L, M, N, H, G, K, O, P, causal)
+    plan.extents = (element, L, M, N, H, G, K, O, P, causal, lengths_ptr != 0)
     plan.fields = (element, 0, L, M, N, H, G, K, O, scale, queries.data_ptr(), q_ls, q_ms, q_hs, keys.data_ptr(), k_ls, k_ns, k_gs,
                    values.data_ptr(), v_ls, v_ns, v_gs, out.data_ptr(), o_ls, o_ms, o_hs, lse_ptr, lengths_ptr, mask_ptr, mask_ls, mask_ns, P, causal,
                    pk_ptr, pk_ns, pk_gs, pv_ptr, pv_ns, pv_gs)
@@ -253,7 +253,7 @@ def _plan_attention_grad(grad_out, queries, keys, values, out, lse, scale, key_l
     if out is None:
         raise TypeError("out must be a PyTorch tensor")
     of = _plan_attention(queries, keys, values, out, scale, key_lengths, key_mask, False, require_device=require_device)
-    L, M, N, H, G, K, O, _, _ = of.extents
+    element, L, M, N, H, G, K, O = of.extents[:8]
     device, dtype = of.device, queries.dtype
     L_d, M_d, H_d, O_d, d_ls, d_ms, d_hs = _operand("grad_out", grad_out, device, dtype)
     if (L_d, M_d, H_d, O_d) != (L, M, H, O):
@@ -268,7 +268,7 @@ def _plan_attention_grad(grad_out, queries, keys, values, out, lse, scale, key_l
     grad_k, grad_v = make(keys, memory_format=contiguous), make(values, memory_format=contiguous)
     plan = _GradientPlan()
     plan.out, plan.device = (grad_q, grad_k, grad_v), device
-    plan.extents = (L, M, N, H, G, K, O, key_entries)
+    plan.extents = (element, L, M, N, H, G, K, O, key_entries)
     # type .. o of the forward block, key_entries, scale, then its operands up to out's strides
     plan.fields = (*of.fields[:9], key_entries, *of.fields[9:26], grad_out.data_ptr(), d_ls, d_ms, d_hs, lse.data_ptr(), *of.fields[27:31],
                    grad_q.data_ptr(), grad_k.data_ptr(), grad_v.data_ptr())
@@ -311,7 +311,7 @@ def cross_attention_grad(
     if needed:
         workspace = _scratch.allocate(needed, plan.device)
         if workspace is None:           # refused: uncut launches, with room for the sums of a row
-            L, M, _, H = plan.extents[:4]
+            _, L, M, _, H = plan.extents[:5]
             needed = (8 * L * M * H + 8 + 15) // 16 * 16
             workspace = _scratch.allocate(needed, plan.device)
         if workspace is None:

@@ -188,3 +188,19 @@ def test_header_and_binding_agree(tmp_path):
         for field, _ in binding._fields_:
             assert re.search(rf"^{c_name} {field} {getattr(binding, field).offset}$", printed, re.M), f"{c_name}.{field}"
     assert f"types {_backend.FP32} {_backend.FP16} {_backend.BF16}\n" in printed
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("L, M, N, H, G, K, P, lengths", [(1, 1, 5000, 8, 8, 64, None, False), (3, 1, 4000, 16, 4, 128, None, True), (2, 300, 700, 4, 2, 80, None, False),
+                                                          (64, 1, 500, 8, 2, 128, 8192, True), (2, 50, 60, 8, 1, 256, 1000, True)])
+def test_the_workspace_that_is_asked_for_is_what_the_call_uses(dtype, L, M, N, H, G, K, P, lengths):
+    """The sizes are asked for once per shape, by a call of that shape with other addresses: they have to be those of the call itself."""
+    import importlib
+    attention = importlib.import_module("kermac_amd.attention")
+    q, k, v = make(L, M, H, K, dtype=dtype), make(L, N, G, K, dtype=dtype), make(L, N, G, K, dtype=dtype)
+    prefix = (make(P, G, K, dtype=dtype), make(P, G, K, dtype=dtype)) if P else None
+    of = plan(q, k, v, key_lengths=torch.zeros(L, dtype=torch.int32) if lengths else None, prefix=prefix)
+    assert attention._workspace_bytes(*of.extents) == _backend.attention_workspace_bytes(of.params)
+    if prefix is None:
+        of = _plan_attention_grad(q, q, k, v, q, make(L, M, H), None, None, None, require_device=False)
+        assert attention._gradient_workspace_bytes(*of.extents) == _backend.attention_gradient_workspace_bytes(of.params)
