@@ -69,8 +69,8 @@ void set_scale(float scale, float *scale_log2, float *query_factor)
     *query_factor = to_base_2 > 0.0f ? (scale < 0.0f ? -1.0f : 1.0f) : 0.0f;
 }
 
-constexpr int ROWS_OF_OWN_KEYS = 32;                // up to here every wave walks keys of its own
 constexpr int ROWS_PER_WORKGROUP = 128;
+constexpr int ROWS_OF_OWN_KEYS = 32;                // up to here every wave walks keys of its own
 
 // How many parts the keys are cut into: the number with the smallest modelled time, in microseconds, fitted to sweeps of 1 .. 64 parts.
 //   Tiles of rows (bound by the matrix cores): 128 rows meet 64 keys in 2.1 us per 128 features in 16 bits (fp32: 7 times as long) while two
@@ -186,6 +186,25 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
     own.n = p->n;
     own.causal = p->causal != 0;
 
+    Layout layout{element_size(p->type)};
+    layout.operand(p->q, p->k);
+    layout.operand(p->out, p->o);
+    layout.stride(p->l, p->q_ls); layout.stride(p->m, p->q_ms); layout.stride(p->h, p->q_hs);
+    layout.stride(p->l, p->out_ls); layout.stride(p->m, p->out_ms); layout.stride(p->h, p->out_hs);
+    if (p->n > 0) {
+        layout.operand(p->key, p->k);
+        layout.operand(p->value, p->o);
+        layout.stride(p->l, p->key_ls); layout.tokens(p->n, p->key_ns, p->k); layout.stride(p->g, p->key_gs);
+        layout.stride(p->l, p->value_ls); layout.tokens(p->n, p->value_ns, p->o); layout.stride(p->g, p->value_gs);
+    }
+    if (prefixed) {
+        layout.operand(p->prefix_key, p->k);
+        layout.operand(p->prefix_value, p->o);
+        layout.tokens(p->prefix_n, p->prefix_key_ns, p->k); layout.stride(p->g, p->prefix_key_gs);
+        layout.tokens(p->prefix_n, p->prefix_value_ns, p->o); layout.stride(p->g, p->prefix_value_gs);
+    }
+    plan->aligned = layout.aligned && !(p->flags & KMC_FLAG_FORCE_SCALAR_ACCESS);
+
     const int64_t rows = static_cast<int64_t>(p->m) * args.r;
     bool fits = true;
     if (with_workspace && prefixed) {
@@ -206,24 +225,6 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
     if (!fits) return fail(KMC_ERR_INVALID_ARGUMENT, "more workgroups than a launch holds");
     plan->bytes = partial_bytes(args);
 
-    Layout layout{element_size(p->type)};
-    layout.operand(p->q, p->k);
-    layout.operand(p->out, p->o);
-    layout.stride(p->l, p->q_ls); layout.stride(p->m, p->q_ms); layout.stride(p->h, p->q_hs);
-    layout.stride(p->l, p->out_ls); layout.stride(p->m, p->out_ms); layout.stride(p->h, p->out_hs);
-    if (p->n > 0) {
-        layout.operand(p->key, p->k);
-        layout.operand(p->value, p->o);
-        layout.stride(p->l, p->key_ls); layout.tokens(p->n, p->key_ns, p->k); layout.stride(p->g, p->key_gs);
-        layout.stride(p->l, p->value_ls); layout.tokens(p->n, p->value_ns, p->o); layout.stride(p->g, p->value_gs);
-    }
-    if (prefixed) {
-        layout.operand(p->prefix_key, p->k);
-        layout.operand(p->prefix_value, p->o);
-        layout.tokens(p->prefix_n, p->prefix_key_ns, p->k); layout.stride(p->g, p->prefix_key_gs);
-        layout.tokens(p->prefix_n, p->prefix_value_ns, p->o); layout.stride(p->g, p->prefix_value_gs);
-    }
-    plan->aligned = layout.aligned && !(p->flags & KMC_FLAG_FORCE_SCALAR_ACCESS);
     return KMC_OK;
 }
 

@@ -56,8 +56,17 @@ __device__ __forceinline__ att_f32x16 att_mma(att_vec8<float> a, att_vec8<float>
 // Register i of a 32 x 32 result holds row att_row(i, half wave) of column lane % 32.
 __device__ __forceinline__ constexpr int att_row(int i, int half) { return 8 * (i / 4) + 4 * half + i % 4; }
 
-// The sum or maximum of a value over the two lanes of a column.
-__device__ __forceinline__ float att_other_half(float x) { return __shfl_xor(x, 32); }
+// The sum and the maximum of a value over the two lanes of a column.
+__device__ __forceinline__ float att_sum_of_halves(float x)
+{
+    const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+    return __builtin_bit_cast(float, static_cast<unsigned>(both[0])) + __builtin_bit_cast(float, static_cast<unsigned>(both[1]));
+}
+__device__ __forceinline__ float att_max_of_halves(float x)
+{
+    const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+    return fmaxf(__builtin_bit_cast(float, static_cast<unsigned>(both[0])), __builtin_bit_cast(float, static_cast<unsigned>(both[1])));
+}
 
 // A tile of rows of DP elements in LDS, read both ways: 16 bytes of a row per lane, 16 rows at a time, and transposed, which touches 4 rows x 64 bytes per
 // half wave.  Row r holds its 16-byte piece c in place c ^ swizzle(r) / 16: sixteen consecutive rows then have a given piece in different banks, and four
@@ -273,6 +282,12 @@ __device__ __forceinline__ void att_clear(att_lds_byte *tile, att_u64 kept, int 
         if (!(kept >> (i / PIECES) & 1)) *reinterpret_cast<att_u32x4 *>(tile + Lds::offset(i / PIECES, i % PIECES)) = att_u32x4{0, 0, 0, 0};
 }
 
+// The low `count` bits, count clamped to 0 .. 64.
+__device__ __forceinline__ att_u64 att_low_bits(int count)
+{
+    return count >= 64 ? ~0ull : count <= 0 ? 0ull : (1ull << count) - 1;
+}
+
 // One bit per key n0 .. n0 + 63: the key exists and takes part.  The same in all waves of a workgroup.
 __device__ __forceinline__ att_u64 att_kept_keys(const AttentionKeys &keys, int entry, int n0, int end, int lane)
 {
@@ -347,57 +362,57 @@ __device__ __forceinline__ void att_read_columns(att_vec8<T> (&f)[DP / 32], cons
     for (int o = 0; o < DP / 32; ++o) f[o] = att_read_transposed<T, DP>(tile, row, 32 * o, lane);
 }
 
-// s^T of a tile of KT keys in LDS and the 32 rows whose queries are in `query`.  Blocks of 32 keys take turns: a matrix instruction that adds to the
-// result of the one before waits for it.
+// s^T of a tile of KT keys in LDS and the 32 rows whose queries are in `query`, and the largest of each lane's scores.  One block of 32 keys after the
+// other; the maximum over a block is taken beside the matrix instructions of the next.
 template <typename T, int DP, int KT>
-__device__ __forceinline__ void att_scores(att_f32x16 (&s)[KT / 32], const att_vec8<T> (&query)[DP / 16], const att_lds_byte *keys, int lane)
+__device__ __forceinline__ float att_scores(att_f32x16 (&s)[KT / 32], const att_vec8<T> (&query)[DP / 16], const att_lds_byte *keys, int lane)
 {
     typedef AttGroups<T, DP> G;
-    constexpr int BLOCKS = KT / 32, AT_ONCE = BLOCKS == 1 ? G::GROUP : 2, ALL = G::STEPS / AT_ONCE;
-    att_vec8<T> f[2][AT_ONCE][BLOCKS];
-    auto read = [&](att_vec8<T> (&to)[AT_ONCE][BLOCKS], int i) {
+    constexpr int ALL = KT / 32 * G::GROUPS, EACH = 16 / G::GROUPS;
+    att_vec8<T> f[2][G::GROUP];
+    att_read_group<T, DP>(f[0], keys, 0, 0, lane);
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j)
-#pragma unroll
-            for (int b = 0; b < BLOCKS; ++b) to[j][b] = att_read_row<T, DP>(keys, 32 * b, 16 * (AT_ONCE * i + j), lane);
-    };
-    read(f[0], 0);
-#pragma unroll
-    for (int b = 0; b < BLOCKS; ++b) s[b] = att_f32x16{0};
+    for (int b = 0; b < KT / 32; ++b) s[b] = att_f32x16{0};
+    float top = -__builtin_inff();
     att_region();
 #pragma unroll
     for (int i = 0; i < ALL; ++i) {
-        if (i + 1 < ALL) read(f[(i + 1) & 1], i + 1);
+        const int b = i / G::GROUPS, group = i % G::GROUPS;
+        if (i + 1 < ALL) att_read_group<T, DP>(f[(i + 1) & 1], keys, 32 * ((i + 1) / G::GROUPS), (i + 1) % G::GROUPS, lane);
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j)
+        for (int j = 0; j < G::GROUP; ++j) s[b] = att_mma(f[i & 1][j], query[G::GROUP * group + j], s[b]);
+        if (b > 0)
 #pragma unroll
-            for (int b = 0; b < BLOCKS; ++b) s[b] = att_mma(f[i & 1][j][b], query[AT_ONCE * i + j], s[b]);
-        att_order<AT_ONCE * BLOCKS * G::READS_ROW, AT_ONCE * BLOCKS * G::MMAS, 0>();
+            for (int j = EACH * group; j < (group + 1 == G::GROUPS ? 16 : EACH * (group + 1)); ++j) top = fmaxf(top, s[b - 1][j]);
+        att_order<G::GROUP * G::READS_ROW, G::GROUP * G::MMAS, 0>();
         att_region();
     }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) top = fmaxf(top, s[KT / 32 - 1][j]);
+    return top;
 }
 
 // Masks a tile's scores (`kept` has a bit per key for this lane's row) and, where they pass the wave's base by 2^8, moves it.  Bases are whole
 // numbers, so that what was made below the old one is rescaled without rounding: output and sum, and `weights` that wait for their product.
 template <typename T, int DP, int KT>
-__device__ __forceinline__ void att_rebase(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], att_f32x16 (&s)[KT / 32], float scale_log2, att_u64 kept, int lane)
+__device__ __forceinline__ void att_rebase(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], att_f32x16 (&s)[KT / 32], float top, float scale_log2, att_u64 kept,
+                                           int lane)
 {
     const att_u64 all = KT == 64 ? ~0ull : (1ull << KT) - 1;
     if (!__all((kept & all) == all)) {
         att_rare();
+        top = -__builtin_inff();
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b) {
             const unsigned mine = static_cast<unsigned>(kept >> (32 * b)) >> (4 * (lane >> 5));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[b][i] = mine >> att_row(i, 0) & 1 ? s[b][i] : -__builtin_inff();
+            for (int i = 0; i < 16; ++i) {
+                s[b][i] = mine >> att_row(i, 0) & 1 ? s[b][i] : -__builtin_inff();
+                top = fmaxf(top, s[b][i]);
+            }
         }
     }
-    float top = s[0][0];
-#pragma unroll
-    for (int b = 0; b < KT / 32; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-    top = fmaxf(top, att_other_half(top)) * scale_log2;
+    top = att_max_of_halves(top) * scale_log2;
     if (!__all(top <= state.base + ATT_HEADROOM)) {
         att_rare();
         const float base = fmaxf(state.base, __builtin_ceilf(top));
@@ -432,7 +447,7 @@ __device__ __forceinline__ att_vec8<T> att_weights(AttState<DP> &state, const at
 
 // out^T += V^T p^T over the KT keys of a tile; with NEXT, the weights give way to those of the scores s.
 template <typename T, int DP, int KT, bool NEXT>
-__device__ __forceinline__ void att_add_values(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], const att_lds_byte *values, att_vec8<T> (&first)[DP / 32],
+__device__ __forceinline__ void att_add_values(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], const att_lds_byte *values, const att_vec8<T> (&first)[DP / 32],
                                                const att_f32x16 (&s)[KT / 32], float scale_log2, float base, int lane)
 {
     typedef AttGroups<T, DP> G;
@@ -445,7 +460,7 @@ __device__ __forceinline__ void att_add_values(AttState<DP> &state, att_vec8<T> 
 #pragma unroll
         for (int o = 0; o < DP / 32; ++o) state.out[o] = att_mma(f[step & 1][o], weights[step], state.out[o]);
         if (NEXT) weights[step] = att_weights<T, DP, KT>(state, s, step, scale_log2, base);
-        att_order<DP / 32 * G::READS_T, DP / 32 * G::MMAS, NEXT ? (DP <= 64 ? 14 : DP <= 128 ? 7 : 4) : 0>();
+        att_order<DP / 32 * G::READS_T, DP / 32 * G::MMAS, NEXT ? (G::MMAS > 1 ? 1 : DP <= 64 ? 14 : DP <= 128 ? 7 : 4) : 0>();
         att_region();
     }
 }
@@ -463,12 +478,6 @@ __device__ __forceinline__ void att_range(int length, int tile, int split, int s
     *end = length - *begin < per_split ? length : static_cast<int>(*begin + per_split);
 }
 
-// The low `count` bits, count clamped to 0 .. 64.
-__device__ __forceinline__ att_u64 att_low_bits(int count)
-{
-    return count >= 64 ? ~0ull : count <= 0 ? 0ull : (1ull << count) - 1;
-}
-
 // Where row `row` of a problem's entry lives.
 struct AttRow { int entry, query, head; };
 __device__ __forceinline__ AttRow att_find_row(const AttentionArgs &args, int first_entry, int g, int row)
@@ -481,20 +490,22 @@ __device__ __forceinline__ AttRow att_find_row(const AttentionArgs &args, int fi
     return at;
 }
 
+// What a workgroup holds in LDS.
 template <typename T, int DP>
 struct AttForwardShape {
-    // Rows per workgroup and keys per tile where waves share the keys; waves and keys per tile where each wave has keys of its own.
-    static constexpr int ROW_WAVES = 4;
-    static constexpr int SHARED_KEYS = DP * sizeof(T) <= 512 ? 64 : 32;
+    static constexpr int WAVES = 4;
+    static constexpr int ROW_BYTES = AttLds<T, DP>::STRIDE;
+    // Waves that share the keys: a ring of two tiles of keys and one of two tiles of values.
+    static constexpr int SHARED_KEYS = ROW_BYTES <= 512 ? 64 : 32;
+    static constexpr int SHARED_BYTES = 4 * SHARED_KEYS * ROW_BYTES;
+    // Waves with keys of their own.
     static constexpr int OWN_KEYS = 32;
-    static constexpr int OWN_WAVES = DP * sizeof(T) <= 512 ? 4 : 2;      // 1 KB rows: two waves' tiles fill LDS
-    static constexpr int WAVES_PER_SIMD = DP * sizeof(T) <= 256 ? 2 : 1;
-    static constexpr int KEY_BYTES = AttLds<T, DP>::STRIDE;
-    static constexpr int SHARED_BYTES = 4 * SHARED_KEYS * KEY_BYTES;     // keys and values, two tiles of each
-    static constexpr int OWN_BYTES = 2 * OWN_WAVES * OWN_KEYS * KEY_BYTES;
-    static constexpr int JOIN_BYTES = (OWN_WAVES - 1) * (DP * 32 + 64) * 4 + 512;
+    static constexpr int OWN_WAVES = ROW_BYTES <= 512 ? WAVES : 2;      // 1 KB rows: two waves' tiles fill LDS
+    static constexpr int OWN_BYTES = 2 * OWN_WAVES * OWN_KEYS * ROW_BYTES;
+    static constexpr int JOIN_BYTES = (OWN_WAVES - 1) * (DP * 32 + 64) * 4 + 128 * OWN_WAVES;
     static constexpr int BYTES_1 = SHARED_BYTES > OWN_BYTES ? SHARED_BYTES : OWN_BYTES;
     static constexpr int BYTES = BYTES_1 > JOIN_BYTES ? BYTES_1 : JOIN_BYTES;
+    static constexpr int WAVES_PER_SIMD = ROW_BYTES <= 256 ? 2 : 1;
 };
 
 // A lane's column of results [DP, 32] as the row of `width` elements that it is in memory, times a factor.
@@ -577,6 +588,7 @@ template <typename T, int DP, bool ALIGNED>
 __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void attention_forward(const AttentionArgs args)
 {
     typedef AttForwardShape<T, DP> Shape;
+    constexpr int WAVES = Shape::WAVES, THREADS = 64 * WAVES;
     __shared__ __attribute__((aligned(1024))) att_lds_byte lds[Shape::BYTES];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -607,32 +619,30 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
     const int entry = id;
 
     AttState<DP> state;
+    att_vec8<T> query[DP / 16];
 #pragma unroll
     for (int o = 0; o < DP / 32; ++o) state.out[o] = att_f32x16{0};
     state.base = -__builtin_inff();
     state.sum = 0.0f;
-    att_vec8<T> query[DP / 16];
 
     if (!job.own_keys) {
-        constexpr int KT = Shape::SHARED_KEYS;
-        constexpr int TILE = KT * Shape::KEY_BYTES;
-        att_lds_byte *key_tile = lds, *value_tile = lds + 2 * TILE;
-        const int first_row = row_tile * 32 * Shape::ROW_WAVES + 32 * wave;
-        const int row = first_row + lane % 32;
+        constexpr int KT = Shape::SHARED_KEYS, TILE = KT * Shape::ROW_BYTES, ROWS = 32 * WAVES;
+        const int first_row = row_tile * ROWS + 32 * wave, row = first_row + lane % 32;
         const bool works = first_row < job.rows;
         att_load_queries<T, DP, ALIGNED>(args, job, entry, g, row, lane, query);
         att_wait_for_loads();
         for (int segment = job.first_segment; segment < job.last_segment; ++segment) {
             const AttentionKeys &keys = args.keys[segment];
+            const i64 k_stride = keys.k_ns, v_stride = keys.v_ns;
+            const bool masked = keys.mask != nullptr;
             const int length = att_length(keys, entry);
             int begin, end;
             att_range(length, KT, split, job.splits, &begin, &end);
             // query i of a sequence's last m tokens sees the tokens up to its own
-            int limit = 0x7fffffff;
+            int limit;
+            limit = keys.causal ? length - args.m + 1 + (row) / args.r : 0x7fffffff;
             if (keys.causal) {
-                limit = length - args.m + 1 + row / args.r % args.m;
-                int last_row = (row_tile + 1) * 32 * Shape::ROW_WAVES - 1;
-                last_row = last_row < job.rows ? last_row : job.rows - 1;
+                const int last_row = (row_tile + 1) * ROWS < job.rows ? (row_tile + 1) * ROWS - 1 : job.rows - 1;
                 const int last_limit = length - args.m + 1 + last_row / args.r;
                 end = end < last_limit ? end : last_limit;
             }
@@ -640,78 +650,83 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
             const T *v = static_cast<const T *>(keys.v) + entry * keys.v_ls + g * keys.v_gs;
             if (begin >= end) continue;
             // Iteration i: scores of tile i, then the values of tile i - 1 times their weights while the exponentials of tile i are made: the matrix
-            // cores and the vector units work at the same time.  Keys are staged one tile in front of the values, in two buffers each: one barrier.
-            AttTile<T, DP, KT, 256, ALIGNED> next_k, next_v;
+            // cores and the vector units work at the same time.  It asks for the keys of tile i + 1 and the values of tile i.
+            typedef AttTile<T, DP, KT, THREADS, ALIGNED> Tile;
+            att_lds_byte *key_ring = lds, *value_ring = lds + 2 * TILE;
+            Tile next_k, next_v;
             att_f32x16 s[KT / 32];
             att_vec8<T> weights[KT / 16], first[DP / 32];
+            float top, base;
 #pragma unroll
-            for (int step = 0; step < KT / 16; ++step) weights[step] = att_vec8<T>{0};
-            __syncthreads();
-            next_k.begin(k + begin * keys.k_ns, keys.k_ns, end - begin, args.k, key_tile, threadIdx.x);
-            next_k.finish(key_tile, threadIdx.x);
-            __syncthreads();
-            int odd = 0;
-            auto stage = [&](int n) {
-                if (n + KT < end) {
-                    const i64 at = n + KT;
-                    next_k.begin(k + at * keys.k_ns, keys.k_ns, end - static_cast<int>(at), args.k, key_tile + (odd ^ 1) * TILE, threadIdx.x);
-                }
-                next_v.begin(v + n * keys.v_ns, keys.v_ns, end - n, args.o, value_tile + odd * TILE, threadIdx.x);
+                for (int step = 0; step < KT / 16; ++step) weights[step] = att_vec8<T>{0};
+            const float scale_log2 = args.scale_log2;
+            const int k_width = args.k, v_width = args.o;
+            int now = 0;                                // which of two tiles
+            auto ask_keys = [&](int n, int slot) { next_k.begin(k + n * k_stride, k_stride, end - n, k_width, key_ring + slot * TILE, threadIdx.x); };
+            auto ask = [&](int n) {
+                if (n + KT < end) ask_keys(n + KT, now ^ 1);
+                next_v.begin(v + n * v_stride, v_stride, end - n, v_width, value_ring + now * TILE, threadIdx.x);
             };
-            auto staged = [&](int n, att_u64 kept) {
-                if (n + KT < end) next_k.finish(key_tile + (odd ^ 1) * TILE, threadIdx.x);
-                next_v.finish(value_tile + odd * TILE, threadIdx.x);
+            auto got = [&](int n, att_u64 kept) {       // the keys of the next tile and the values of this one have arrived
+                if (n + KT < end) next_k.finish(key_ring + (now ^ 1) * TILE, threadIdx.x);
+                next_v.finish(value_ring + now * TILE, threadIdx.x);
                 __syncthreads();
-                if (keys.mask && kept != ~0ull) {
+                if (masked && kept != ~0ull) {
                     att_rare();
-                    att_clear<T, DP, KT, 256>(value_tile + odd * TILE, kept, threadIdx.x);
+                    att_clear<T, DP, KT, THREADS>(value_ring + now * TILE, kept, threadIdx.x);
                     __syncthreads();
                 }
-                odd ^= 1;
+                now ^= 1;
             };
-            att_u64 kept = att_kept_keys(keys, entry, begin, end, lane);
-            stage(begin);
+            __syncthreads();                            // a segment before this one is done with the buffers
+            ask_keys(begin, 0);
+            next_k.finish(key_ring, threadIdx.x);
+            __syncthreads();
+            auto rebase = [&](int n, att_u64 kept) {
+                att_rebase<T, DP, KT>(state, weights, s, top, scale_log2, kept & att_low_bits(limit - n), lane);
+                base = att_finite_base(state.base);
+            };
+            att_u64 kept = masked ? att_kept_keys(keys, entry, begin, end, lane) : att_low_bits(end - begin);
+            ask(begin);
             if (works) {
-                att_scores<T, DP, KT>(s, query, key_tile, lane);
-                att_rebase<T, DP, KT>(state, weights, s, args.scale_log2, kept & att_low_bits(limit - begin), lane);
-                const float base = att_finite_base(state.base);
+                top = att_scores<T, DP, KT>(s, query, key_ring, lane);
+                rebase(begin, kept);
 #pragma unroll
-                for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, args.scale_log2, base);
+                    for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, scale_log2, base);
             }
-            staged(begin, kept);
+            got(begin, kept);
             for (int n = begin + KT; n < end; n += KT) {
-                kept = att_kept_keys(keys, entry, n, end, lane);
-                stage(n);
+                kept = masked ? att_kept_keys(keys, entry, n, end, lane) : att_low_bits(end - n);
+                ask(n);
                 if (works) {
-                    const att_lds_byte *before = value_tile + (odd ^ 1) * TILE;
-                    att_scores<T, DP, KT>(s, query, key_tile + odd * TILE, lane);
-                    att_read_columns<T, DP>(first, before, 0, lane);
-                    att_rebase<T, DP, KT>(state, weights, s, args.scale_log2, kept & att_low_bits(limit - n), lane);
-                    att_add_values<T, DP, KT, true>(state, weights, before, first, s, args.scale_log2, att_finite_base(state.base), lane);
+                    const att_lds_byte *values = value_ring + (now ^ 1) * TILE;
+                    top = att_scores<T, DP, KT>(s, query, key_ring + now * TILE, lane);
+                    att_read_columns<T, DP>(first, values, 0, lane);
+                    rebase(n, kept);
+                    att_add_values<T, DP, KT, true>(state, weights, values, first, s, scale_log2, base, lane);
                 }
-                staged(n, kept);
+                got(n, kept);
             }
             if (works) {
-                const att_lds_byte *before = value_tile + (odd ^ 1) * TILE;
-                att_read_columns<T, DP>(first, before, 0, lane);
-                att_add_values<T, DP, KT, false>(state, weights, before, first, s, 0.0f, 0.0f, lane);
+                const att_lds_byte *values = value_ring + (now ^ 1) * TILE;
+                att_read_columns<T, DP>(first, values, 0, lane);
+                att_add_values<T, DP, KT, false>(state, weights, values, first, s, 0.0f, base, lane);
             }
         }
         if (!works) return;
-        const float sum = state.sum + att_other_half(state.sum);
-        att_forward_write<T, DP, ALIGNED>(args, job, state, sum, entry, g, row, split, lane);
+            att_forward_write<T, DP, ALIGNED>(args, job, state, att_sum_of_halves(state.sum), entry, g, row, split, lane);
     } else {
-        constexpr int KT = Shape::OWN_KEYS, WAVES = Shape::OWN_WAVES;
-        att_lds_byte *key_tile = lds + 2 * wave * KT * Shape::KEY_BYTES, *value_tile = key_tile + KT * Shape::KEY_BYTES;
+        constexpr int KT = Shape::OWN_KEYS, OWN = Shape::OWN_WAVES;
+        att_lds_byte *key_tile = lds + 2 * wave * KT * Shape::ROW_BYTES, *value_tile = key_tile + KT * Shape::ROW_BYTES;
         const int row = lane % 32;                                      // at most 32 rows: one tile
-        if (wave < WAVES) {
+        if (wave < OWN) {
             att_load_queries<T, DP, ALIGNED>(args, job, entry, g, row, lane, query);
             for (int segment = job.first_segment; segment < job.last_segment; ++segment) {
                 const AttentionKeys &keys = args.keys[segment];
                 const int length = att_length(keys, entry);
                 int begin, end;
                 att_range(length, KT, split, job.splits, &begin, &end);
-                const int limit = keys.causal ? length - args.m + 1 + row / args.r % args.m : 0x7fffffff;
+                const int limit = keys.causal ? length - args.m + 1 + row / args.r : 0x7fffffff;
                 const T *k = static_cast<const T *>(keys.k) + entry * keys.k_ls + g * keys.k_gs;
                 const T *v = static_cast<const T *>(keys.v) + entry * keys.v_ls + g * keys.v_gs;
                 AttTile<T, DP, KT, 64, ALIGNED> next_k, next_v;
@@ -720,7 +735,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                     next_k.begin(k + n * keys.k_ns, keys.k_ns, end - static_cast<int>(n), args.k, key_tile, lane);
                     next_v.begin(v + n * keys.v_ns, keys.v_ns, end - static_cast<int>(n), args.o, value_tile, lane);
                 }
-                for (; n < end; n += KT * WAVES) {
+                for (; n < end; n += KT * OWN) {
                     const att_u64 kept = att_kept_keys(keys, entry, static_cast<int>(n), end, lane);
                     next_k.finish(key_tile, lane);
                     next_v.finish(value_tile, lane);
@@ -729,43 +744,42 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                         att_clear<T, DP, KT, 64>(value_tile, kept, lane);
                         att_wave_sync();
                     }
-                    const i64 at = n + KT * WAVES;
+                    const i64 at = n + KT * OWN;
                     if (at < end) {
                         next_k.begin(k + at * keys.k_ns, keys.k_ns, end - static_cast<int>(at), args.k, key_tile, lane);
                         next_v.begin(v + at * keys.v_ns, keys.v_ns, end - static_cast<int>(at), args.o, value_tile, lane);
                     }
                     att_f32x16 s[KT / 32];
-                    att_vec8<T> weights[KT / 16] = {};
-                    att_scores<T, DP, KT>(s, query, key_tile, lane);
-                    att_rebase<T, DP, KT>(state, weights, s, args.scale_log2, kept & att_low_bits(limit - static_cast<int>(n)), lane);
+                    att_vec8<T> weights[KT / 16] = {}, first[DP / 32];
+                    const float top = att_scores<T, DP, KT>(s, query, key_tile, lane);
+                    att_rebase<T, DP, KT>(state, weights, s, top, args.scale_log2, kept & att_low_bits(limit - static_cast<int>(n)), lane);
                     const float base = att_finite_base(state.base);
 #pragma unroll
                     for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, args.scale_log2, base);
-                    att_vec8<T> first[DP / 32];
                     att_read_columns<T, DP>(first, value_tile, 0, lane);
-                    att_add_values<T, DP, KT, false>(state, weights, value_tile, first, s, 0.0f, 0.0f, lane);
+                    att_add_values<T, DP, KT, false>(state, weights, value_tile, first, s, 0.0f, base, lane);
                     att_wave_sync();
                 }
             }
         }
         // join the waves: sums and outputs below one common maximum, added in the order of the waves
-        float sum = state.sum + att_other_half(state.sum);
-        float *bases = reinterpret_cast<float *>(lds);                   // [WAVES][32], then (WAVES - 1) waves' sums and outputs
-        float *others = bases + 128;
+        float sum = att_sum_of_halves(state.sum);
+        float *bases = reinterpret_cast<float *>(lds);                   // [OWN][32], then (OWN - 1) waves' sums and outputs
+        float *others = bases + 32 * OWN;
         __syncthreads();
-        static_assert(WAVES * 32 <= 128, "room for the bases");
-        if (wave < WAVES && lane < 32) bases[wave * 32 + lane] = state.base;
+        static_assert(OWN * 32 <= 256, "room for the bases");
+        if (wave < OWN && lane < 32) bases[wave * 32 + lane] = state.base;
         __syncthreads();
         float base = -__builtin_inff();
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) base = fmaxf(base, bases[w * 32 + lane % 32]);
+        for (int w = 0; w < OWN; ++w) base = fmaxf(base, bases[w * 32 + lane % 32]);
         __syncthreads();
         const float shrink = base == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(state.base - base);
         state.base = base;
         sum *= shrink;
 #pragma unroll
         for (int o = 0; o < DP / 32; ++o) state.out[o] *= shrink;
-        if (wave > 0 && wave < WAVES) {
+        if (wave > 0 && wave < OWN) {
             float *mine = others + (wave - 1) * (DP * 32 + 64);
 #pragma unroll
             for (int o = 0; o < DP / 32; ++o)
@@ -775,8 +789,8 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
         }
         __syncthreads();
         if (wave > 0) return;
-#pragma unroll
-        for (int w = 0; w < WAVES - 1; ++w) {
+#pragma unroll 1
+        for (int w = 0; w < OWN - 1; ++w) {
             const float *from = others + w * (DP * 32 + 64);
 #pragma unroll
             for (int o = 0; o < DP / 32; ++o)

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
 #pragma unroll
         for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(static_cast<float>(grad[step][j]), static_cast<float>(result[j]), delta);
     }
-    delta += att_other_half(delta);
+    delta = att_sum_of_halves(delta);
     float lse2 = att_lse2(args.lse[at]);
 
     att_f32x16 acc[DP / 32];
@@ -121,8 +121,8 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
                 inner = __builtin_fmaf(p, ds[i], inner);
             }
         }
-        total += att_other_half(total);
-        inner += att_other_half(inner);
+        total = att_sum_of_halves(total);
+        inner = att_sum_of_halves(inner);
         if (total > 0.0f) {
             delta = inner / total;
             if (length > 1) lse2 += __builtin_amdgcn_logf(total);
