@@ -34,6 +34,43 @@ __device__ __forceinline__ float att_weight(float s, float scale_log2, float lse
 // lse to base 2 for the exponentials; a row without keys gets +inf, which makes all its weights 0.
 __device__ __forceinline__ float att_lse2(float lse) { return lse == -__builtin_inff() ? __builtin_inff() : lse * ATT_LOG2_E; }
 
+// Two products of 32 rows of two tiles in LDS with operands of the wave's own, by turns: s (scores) and ds (gradients of the result times values).
+// Between the matrix instructions, with VECTOR, the vector work of the scores before: `quad(q)` makes the weights and gradients of
+// registers 4 q .. 4 q + 3.
+template <typename T, int DP, bool VECTOR, typename Quad>
+__device__ __forceinline__ void att_two_scores(att_f32x16 &s, att_f32x16 &ds, const att_lds_byte *s_tile, const att_vec8<T> (&s_own)[DP / 16],
+                                               const att_lds_byte *ds_tile, const att_vec8<T> (&ds_own)[DP / 16], int lane, Quad quad)
+{
+    typedef AttGroups<T, DP> G;
+    constexpr int AT_ONCE = 2, ALL = G::STEPS / AT_ONCE;
+    att_vec8<T> f[2][2 * AT_ONCE];
+    auto read = [&](att_vec8<T> (&to)[2 * AT_ONCE], int i) {
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            to[2 * j] = att_read_row<T, DP>(s_tile, 0, 16 * (AT_ONCE * i + j), lane);
+            to[2 * j + 1] = att_read_row<T, DP>(ds_tile, 0, 16 * (AT_ONCE * i + j), lane);
+        }
+    };
+    read(f[0], 0);
+    s = ds = att_f32x16{0};
+    att_region();
+#pragma unroll
+    for (int i = 0; i < ALL; ++i) {
+        if (i + 1 < ALL) read(f[(i + 1) & 1], i + 1);
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            s = att_mma(f[i & 1][2 * j], s_own[AT_ONCE * i + j], s);
+            ds = att_mma(f[i & 1][2 * j + 1], ds_own[AT_ONCE * i + j], ds);
+        }
+        if (VECTOR)
+#pragma unroll
+            for (int q = 4 * i / ALL; q < 4 * (i + 1) / ALL; ++q) quad(q);
+        att_order<2 * AT_ONCE * G::READS_ROW, 2 * AT_ONCE * G::MMAS, VECTOR ? (sizeof(T) == 4 ? 1 : 4 * 4 / ALL + 1) : 0>();
+        att_region();
+    }
+}
+
+// A workgroup per (batch entry, head of keys, range of keys, 128 rows); a wave per 32 rows, whose queries and gradients it keeps in registers.
 template <typename T, int DP, bool ALIGNED>
 __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void attention_grad_queries(const AttentionGradArgs args)
 {
@@ -139,18 +176,22 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     }
     int odd = 0;
     att_wait_for_loads();
+    const i64 k_stride = keys.k_ns, v_stride = keys.v_ns;
+    const int k_width = args.k, v_width = args.o;
+    const bool masked = keys.mask != nullptr;
+    const float scale_log2 = args.scale_log2;
     if (begin < end) {
         __syncthreads();
-        next_k.begin(k + begin * keys.k_ns, keys.k_ns, end - begin, args.k, lds, threadIdx.x);
-        next_v.begin(v + begin * keys.v_ns, keys.v_ns, end - begin, args.o, lds + TILE, threadIdx.x);
+        next_k.begin(k + begin * k_stride, k_stride, end - begin, k_width, lds, threadIdx.x);
+        next_v.begin(v + begin * v_stride, v_stride, end - begin, v_width, lds + TILE, threadIdx.x);
     }
     for (int n = begin; n < end; n += KT, odd ^= 1) {
-        const att_u64 kept = att_kept_keys(keys, entry, n, end, lane);
+        const att_u64 kept = masked ? att_kept_keys(keys, entry, n, end, lane) : att_low_bits(end - n);
         att_lds_byte *key_tile = lds + 2 * odd * TILE, *value_tile = key_tile + TILE;
         next_k.finish(key_tile, threadIdx.x);
         next_v.finish(value_tile, threadIdx.x);
         __syncthreads();
-        if (keys.mask && kept != ~0ull) {
+        if (masked && kept != ~0ull) {
             att_clear<T, DP, KT, 256>(key_tile, kept, threadIdx.x);
             att_clear<T, DP, KT, 256>(value_tile, kept, threadIdx.x);
             __syncthreads();
@@ -158,35 +199,35 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
         if (n + KT < end) {
             const i64 next = n + KT;
             att_lds_byte *to = lds + 2 * (odd ^ 1) * TILE;
-            next_k.begin(k + next * keys.k_ns, keys.k_ns, end - static_cast<int>(next), args.k, to, threadIdx.x);
-            next_v.begin(v + next * keys.v_ns, keys.v_ns, end - static_cast<int>(next), args.o, to + TILE, threadIdx.x);
+            next_k.begin(k + next * k_stride, k_stride, end - static_cast<int>(next), k_width, to, threadIdx.x);
+            next_v.begin(v + next * v_stride, v_stride, end - static_cast<int>(next), v_width, to + TILE, threadIdx.x);
         }
         if (!works) continue;
+        // (overlapping the blocks, as the keys' kernel does with its tiles, takes more registers than two waves per SIMD have: 1.77 instead of 1.53 ms at
+        // 4 x 4096 x 4096 x 32 heads of 128)
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b) {
-            att_f32x16 s = {0}, ds = {0};
+            constexpr int BLOCK = 32 * AttLds<T, DP>::STRIDE;
+            att_f32x16 s, ds;
+            att_vec8<T> x[2], f[2][DP / 32];
+            att_two_scores<T, DP, false>(s, ds, key_tile + b * BLOCK, query, value_tile + b * BLOCK, grad, lane, [](int) {});
+            att_read_columns<T, DP>(f[0], key_tile + b * BLOCK, 0, lane);
 #pragma unroll
-            for (int step = 0; step < DP / 16; ++step)
-                s = att_mma(att_read_row<T, DP>(key_tile, 32 * b, 16 * step, lane), query[step], s);
-#pragma unroll
-            for (int step = 0; step < DP / 16; ++step)
-                ds = att_mma(att_read_row<T, DP>(value_tile, 32 * b, 16 * step, lane), grad[step], ds);
+            for (int i = 0; i < 16; ++i) ds[i] = att_weight(s[i], scale_log2, lse2) * (ds[i] - delta);
             const unsigned here = static_cast<unsigned>(kept >> (32 * b));
-#pragma unroll
-            for (int i = 0; i < 16; ++i) ds[i] = att_weight(s[i], args.scale_log2, lse2) * (ds[i] - delta);
             if (here != ~0u) {
                 att_rare();
                 const unsigned mine = here >> (4 * half);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) ds[i] = mine >> att_row(i, 0) & 1 ? ds[i] : 0.0f;
             }
+            x[0] = att_operand<T>(ds, 0);
+            x[1] = att_operand<T>(ds, 1);
+            att_read_columns<T, DP>(f[1], key_tile + b * BLOCK, 16, lane);
 #pragma unroll
-            for (int step = 0; step < 2; ++step) {
-                const att_vec8<T> x = att_operand<T>(ds, step);
+            for (int step = 0; step < 2; ++step)
 #pragma unroll
-                for (int o = 0; o < DP / 32; ++o)
-                    acc[o] = att_mma(att_read_transposed<T, DP>(key_tile, 32 * b + 16 * step, 32 * o, lane), x, acc[o]);
-            }
+                for (int o = 0; o < DP / 32; ++o) acc[o] = att_mma(f[step][o], x[step], acc[o]);
         }
     }
     if (row >= rows) return;
@@ -201,41 +242,6 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     }
     T *to = static_cast<T *>(args.grad_q) + at * args.k;
     att_store_columns<T, DP, ALIGNED>(to, acc, args.scale, args.k, half);
-}
-
-// s of 32 rows in LDS against a wave's keys and d v^T against its values, by turns.  Between the matrix instructions, with VECTOR, the vector work of the
-// tile before: `quad(q)` makes the weights and gradients of the scores of its rows 8 q + 4 h + 0..3.
-template <typename T, int DP, bool VECTOR, typename Quad>
-__device__ __forceinline__ void att_row_scores(att_f32x16 &s, att_f32x16 &ds, const att_vec8<T> (&key)[DP / 16], const att_vec8<T> (&value)[DP / 16],
-                                               const att_lds_byte *q_tile, const att_lds_byte *d_tile, int lane, Quad quad)
-{
-    typedef AttGroups<T, DP> G;
-    constexpr int AT_ONCE = 2, ALL = G::STEPS / AT_ONCE;
-    att_vec8<T> f[2][2 * AT_ONCE];
-    auto read = [&](att_vec8<T> (&to)[2 * AT_ONCE], int i) {
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-            to[2 * j] = att_read_row<T, DP>(q_tile, 0, 16 * (AT_ONCE * i + j), lane);
-            to[2 * j + 1] = att_read_row<T, DP>(d_tile, 0, 16 * (AT_ONCE * i + j), lane);
-        }
-    };
-    read(f[0], 0);
-    s = ds = att_f32x16{0};
-    att_region();
-#pragma unroll
-    for (int i = 0; i < ALL; ++i) {
-        if (i + 1 < ALL) read(f[(i + 1) & 1], i + 1);
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-            s = att_mma(f[i & 1][2 * j], key[AT_ONCE * i + j], s);
-            ds = att_mma(f[i & 1][2 * j + 1], value[AT_ONCE * i + j], ds);
-        }
-        if (VECTOR)
-#pragma unroll
-            for (int q = 4 * i / ALL; q < 4 * (i + 1) / ALL; ++q) quad(q);
-        att_order<2 * AT_ONCE * G::READS_ROW, 2 * AT_ONCE * G::MMAS, VECTOR ? (sizeof(T) == 4 ? 1 : 4 * 4 / ALL + 1) : 0>();
-        att_region();
-    }
 }
 
 // A workgroup per (entry of the keys, head of keys, part of the rows, 128 keys); a wave per 32 keys, whose keys and values it keeps in registers.
@@ -289,6 +295,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
     const i64 per_entry = static_cast<i64>(args.r) * tiles_m;
     const int entries = args.key_entries == args.l ? 1 : args.l;
     const i64 per_split = (per_entry * entries + args.k_splits - 1) / args.k_splits;
+    const float scale_log2 = args.scale_log2;
     const i64 part_first = split * per_split, part_last = part_first + per_split;
     const i64 rows_total = static_cast<i64>(args.l) * args.m * args.g * args.r;
 
@@ -304,29 +311,31 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
 
         Tile next_q, next_d;
         int head = first / tiles_m, m0 = first % tiles_m * RT, to = 0;          // of the next tile to load
+        // (behind the last tile: nothing is read)
+        const i64 q_ms = args.q_ms, q_hs = args.q_hs, d_ms = args.grad_out_ms, d_hs = args.grad_out_hs;
+        const T *q_entry = static_cast<const T *>(args.q) + entry * args.q_ls + g * args.r * q_hs;
+        const T *d_entry = static_cast<const T *>(args.grad_out) + entry * args.grad_out_ls + g * args.r * d_hs;
+        const float *stats_entry = args.stats + (static_cast<i64>(entry) * args.g + g) * args.r * args.m + (lane < RT ? 0 : rows_total) + lane % RT;
+        const float *stats_behind = args.stats + 2 * rows_total + (lane < RT ? 0 : 1);
+        const int m = args.m, q_width = args.k, d_width = args.o;
+        int left = count;
         auto begin = [&]() {
-            const int some = args.m - m0, h = g * args.r + head;
+            const int some = left > 0 ? m - m0 : 0;
             att_lds_byte *q_tile = lds + 2 * to * TILE;
-            next_q.begin(static_cast<const T *>(args.q) + entry * args.q_ls + m0 * args.q_ms + h * args.q_hs, args.q_ms, some, args.k, q_tile, threadIdx.x);
-            next_d.begin(static_cast<const T *>(args.grad_out) + entry * args.grad_out_ls + m0 * args.grad_out_ms + h * args.grad_out_hs, args.grad_out_ms, some,
-                         args.o, q_tile + TILE, threadIdx.x);
+            next_q.begin(q_entry + m0 * q_ms + head * q_hs, q_ms, some, q_width, q_tile, threadIdx.x);
+            next_d.begin(d_entry + m0 * d_ms + head * d_hs, d_ms, some, d_width, q_tile + TILE, threadIdx.x);
             // (all waves load the same: they count the same loads; rows that do not exist get the pair behind all others)
-            const int i = lane % RT;
-            const i64 at = i < some ? (static_cast<i64>(entry) * args.g * args.r + h) * args.m + m0 + i + (lane < RT ? 0 : rows_total)
-                                    : 2 * rows_total + (lane < RT ? 0 : 1);
-            att_load_words(args.stats + at, all_stats[to]);
+            att_load_words(lane % RT < some ? stats_entry + static_cast<i64>(head) * m + m0 : stats_behind, all_stats[to]);
+            --left;
             m0 += RT;
-            if (m0 >= args.m) {
-                m0 = 0;
-                ++head;
-            }
+            head = m0 >= m ? head + 1 : head;
+            m0 = m0 >= m ? 0 : m0;
             if (Tile::DIRECT) to = to + 1 == BUFFERS ? 0 : to + 1;
         };
-        // The tile asked for longest ago has arrived; `some`: AHEAD - 1 others are on their way.
-        auto finish = [&](bool some) {
+        // The tile asked for longest ago has arrived; AHEAD - 1 others may be on their way.
+        auto finish = [&]() {
             if constexpr (Tile::DIRECT) {
-                if (some) att_wait_for_loads<(AHEAD - 1) * LOADS>();
-                else att_wait_for_loads();
+                att_wait_for_loads<(AHEAD - 1) * LOADS>();
             } else {
                 att_wait_for_loads();
                 att_lds_byte *q_tile = lds + 2 * to * TILE;
@@ -345,7 +354,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
             const att_f32x4 delta = *reinterpret_cast<const att_f32x4 *>(stats + RT + 8 * q + 4 * half);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float weight = att_weight(s[4 * q + j], args.scale_log2, lse2[j]);
+                const float weight = att_weight(s[4 * q + j], scale_log2, lse2[j]);
                 p[q / 2][4 * (q % 2) + j] = static_cast<T>(weight);
                 x[q / 2][4 * (q % 2) + j] = static_cast<T>(weight * (ds[4 * q + j] - delta[j]));
             }
@@ -373,37 +382,33 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
                 att_region();
             }
         };
-        // `behind`: tiles behind the next one
-        auto turn = [&](const att_f32x16 &s, const att_f32x16 &ds, att_f32x16 &next_s, att_f32x16 &next_ds, int behind) {
-            if (BUFFERS > 2 && behind >= AHEAD) begin();
+        auto turn = [&](const att_f32x16 &s, const att_f32x16 &ds, att_f32x16 &next_s, att_f32x16 &next_ds) {
+            if (BUFFERS > 2) begin();
             const att_lds_byte *q_tile = lds + 2 * then() * TILE;
-            att_row_scores<T, DP, true>(next_s, next_ds, key, value, q_tile, q_tile + TILE, lane, [&](int q) { make_quad(s, ds, q); });
+            att_two_scores<T, DP, true>(next_s, next_ds, q_tile, key, q_tile + TILE, value, lane, [&](int q) { make_quad(s, ds, q); });
             products();
             if (BUFFERS == 2) {
                 __syncthreads();
-                if (behind >= AHEAD) begin();
+                begin();
             }
-            if (behind > 0) finish(behind >= AHEAD);
+            finish();
             __syncthreads();
             now = then();
         };
 
         __syncthreads();                // an entry before this one is done with the buffers
-        if constexpr (Tile::DIRECT) {
-            for (int i = 0; i < count && i < 2 + AHEAD - 1; ++i) begin();
-            finish(false);
-        } else {
-            for (int i = 0; i < count && i < 2; ++i) {
-                begin();
-                finish(false);
-            }
+#pragma unroll 1
+        for (int i = 0; i < 1 + AHEAD; ++i) {
+            begin();
+            if (!Tile::DIRECT) finish();
         }
+        att_wait_for_loads();
         __syncthreads();
-        att_row_scores<T, DP, false>(s_a, ds_a, key, value, lds, lds + TILE, lane, [](int) {});
+        att_two_scores<T, DP, false>(s_a, ds_a, lds, key, lds + TILE, value, lane, [](int) {});
         for (int i = 1; i < count; i += 2) {
-            turn(s_a, ds_a, s_b, ds_b, count - 1 - i);
+            turn(s_a, ds_a, s_b, ds_b);
             if (i + 1 < count) {
-                turn(s_b, ds_b, s_a, ds_a, count - 2 - i);
+                turn(s_b, ds_b, s_a, ds_a);
             } else {
                 s_a = s_b;
                 ds_a = ds_b;
@@ -412,6 +417,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
 #pragma unroll
         for (int q = 0; q < 4; ++q) make_quad(s_a, ds_a, q);
         products();
+        att_wait_for_loads();
     }
     if (!exists) return;
     const i64 at = (static_cast<i64>(key_entry) * keys.n + n) * args.g + g;
