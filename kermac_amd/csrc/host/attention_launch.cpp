@@ -43,9 +43,12 @@ struct Layout {
     void tokens(int extent, int64_t stride, int width)
     {
         this->stride(extent, stride);
-        aligned = aligned && (extent <= 1 || stride >= width) && stride * size < (1 << 24);
+        if (extent > 1) aligned = aligned && stride >= width && stride < (1 << 24) / size;
     }
 };
+
+// The stride of tokens that a tile is read with.  That of a single token means nothing, and a small one would put the rows behind it on top of it.
+int64_t token_stride(int extent, int64_t stride, int width) { return extent > 1 ? stride : width; }
 
 int check_extents(int type, int l, int m, int n, int h, int g, int k, int o, float scale)
 {
@@ -75,7 +78,7 @@ constexpr int ROWS_OF_OWN_KEYS = 32;                // up to here every wave wal
 // How many parts the keys are cut into: the number with the smallest modelled time, in microseconds, fitted to sweeps of 1 .. 64 parts.
 //   Tiles of rows (bound by the matrix cores): 128 rows meet 64 keys in 2.1 us per 128 features in 16 bits (fp32: 7 times as long) while two
 //   workgroups share a CU, in 0.65 of that alone; a launch of more workgroups than fit waits for half of one at its end.
-//   Beside another job (`beside_us` of its own) the two share the chip.
+//   Beside another job (`beside_us` of its own) the two share the chip.  Rows of more than 256 bytes let one workgroup on a CU.
 //   Single tokens (bound by memory): keys and values at 4.7 TB/s, but no workgroup faster than 4 us and 1.05 us per 128 keys of 128 features, and
 //   3.5 us of its place for a workgroup; the launch waits for the last ones, with lengths that differ for the longest.
 //   Joining the parts costs a launch, 5 us, and writing and reading a partial result per part.
@@ -94,6 +97,8 @@ double time_of_parts(int splits, int64_t base, int64_t rows_total, int64_t keys,
     }
     const double tile_us = 2.1 * width / 128 * (p->type == KMC_FP32 ? 7.0 : 1.0), one = steps * tile_us;
     if (beside_us > 0) return join_us + std::max(one, workgroups * one / 512 + beside_us);
+    // rows of more than 256 bytes: one workgroup per CU, whole rounds of which the last one counts
+    if (width * size > 256) return join_us + 0.55 * one * ((workgroups + 255) / 256);
     return join_us + (workgroups <= 256 ? 0.65 * one : workgroups <= 512 ? one : workgroups * one / 512 + 0.5 * one);
 }
 
@@ -175,12 +180,12 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
     const bool prefixed = p->prefix_n > 0;
     kmc::AttentionKeys &prefix = args.keys[0], &own = args.keys[prefixed ? 1 : 0];
     if (prefixed) {
-        prefix.k = p->prefix_key; prefix.k_ns = p->prefix_key_ns; prefix.k_gs = p->prefix_key_gs;
-        prefix.v = p->prefix_value; prefix.v_ns = p->prefix_value_ns; prefix.v_gs = p->prefix_value_gs;
+        prefix.k = p->prefix_key; prefix.k_ns = token_stride(p->prefix_n, p->prefix_key_ns, p->k); prefix.k_gs = p->prefix_key_gs;
+        prefix.v = p->prefix_value; prefix.v_ns = token_stride(p->prefix_n, p->prefix_value_ns, p->o); prefix.v_gs = p->prefix_value_gs;
         prefix.n = p->prefix_n;
     }
-    own.k = p->key; own.k_ls = p->key_ls; own.k_ns = p->key_ns; own.k_gs = p->key_gs;
-    own.v = p->value; own.v_ls = p->value_ls; own.v_ns = p->value_ns; own.v_gs = p->value_gs;
+    own.k = p->key; own.k_ls = p->key_ls; own.k_ns = token_stride(p->n, p->key_ns, p->k); own.k_gs = p->key_gs;
+    own.v = p->value; own.v_ls = p->value_ls; own.v_ns = token_stride(p->n, p->value_ns, p->o); own.v_gs = p->value_gs;
     own.lengths = p->key_lengths;
     own.mask = p->key_mask; own.mask_ls = p->key_mask_ls; own.mask_ns = p->key_mask_ns;
     own.n = p->n;
@@ -274,13 +279,13 @@ int prepare(const kmc_attention_gradient_params *p, bool may_cut, GradPlan *plan
         return fail(KMC_ERR_INVALID_ARGUMENT, "null key / value / grad_key / grad_value pointer");
 
     kmc::AttentionGradArgs &args = plan->args;
-    args.q = p->q; args.q_ls = p->q_ls; args.q_ms = p->q_ms; args.q_hs = p->q_hs;
+    args.q = p->q; args.q_ls = p->q_ls; args.q_ms = token_stride(p->m, p->q_ms, p->k); args.q_hs = p->q_hs;
     args.out = p->out; args.out_ls = p->out_ls; args.out_ms = p->out_ms; args.out_hs = p->out_hs;
-    args.grad_out = p->grad_out; args.grad_out_ls = p->grad_out_ls; args.grad_out_ms = p->grad_out_ms; args.grad_out_hs = p->grad_out_hs;
+    args.grad_out = p->grad_out; args.grad_out_ls = p->grad_out_ls; args.grad_out_ms = token_stride(p->m, p->grad_out_ms, p->o); args.grad_out_hs = p->grad_out_hs;
     args.lse = p->lse;
     kmc::AttentionKeys &keys = args.keys;
-    keys.k = p->key; keys.k_ls = p->key_ls; keys.k_ns = p->key_ns; keys.k_gs = p->key_gs;
-    keys.v = p->value; keys.v_ls = p->value_ls; keys.v_ns = p->value_ns; keys.v_gs = p->value_gs;
+    keys.k = p->key; keys.k_ls = p->key_ls; keys.k_ns = token_stride(p->n, p->key_ns, p->k); keys.k_gs = p->key_gs;
+    keys.v = p->value; keys.v_ls = p->value_ls; keys.v_ns = token_stride(p->n, p->value_ns, p->o); keys.v_gs = p->value_gs;
     keys.lengths = p->key_lengths;
     keys.mask = p->key_mask; keys.mask_ls = p->key_mask_ls; keys.mask_ns = p->key_mask_ns;
     keys.n = p->n;
