@@ -212,11 +212,11 @@ __device__ __forceinline__ void att_wait_for_loads()
 
 // A tile of ROWS rows of DP elements on its way from memory to LDS.  begin() asks for it, finish() has it written.  DIRECT: from memory straight into LDS, 1 KB per
 // wave and instruction, each lane fetching the piece that belongs where its 16 bytes end up; no register waits for it.  Otherwise (unaligned rows,
-// tiles of one wave) through registers.
+// tiles of one wave, whose next tile waits in registers while LDS holds the current one, unless a row of 1 KB asks too many) through registers.
 template <typename T, int DP, int ROWS, int THREADS, bool ALIGNED>
 struct AttTile {
     typedef AttLds<T, DP> Lds;
-    static constexpr bool DIRECT = ALIGNED && THREADS > 64;
+    static constexpr bool DIRECT = ALIGNED && (THREADS > 64 || Lds::STRIDE == 1024);
     static constexpr int SLOTS = Lds::STRIDE / 16;                      // threads of a row
     static constexpr int ROW_STEP = THREADS / SLOTS;
     static constexpr int PER_THREAD = ROWS / ROW_STEP;                  // loads of a thread
@@ -325,17 +325,25 @@ constexpr float ATT_HEADROOM = 8.0f;
 
 // Fragments are read from LDS a group ahead of the matrix instructions that use them.  The compiler, left alone, reads each one in front of its
 // use and waits for it; these fix the order within a region: READS reads, then the matrix instructions, each followed by VALU vector instructions.
-template <int READS, int MMAS, int VALU>
+// Not above 128 features: those kernels have more values than registers, and with a fixed order around the spilled ones the compiler's code
+// for fp32 gave gradients of the queries that were off by 9 % (right without, and in every kernel that spills nothing).
+template <int DP, int READS, int MMAS, int VALU>
 __device__ __forceinline__ void att_order()
 {
-    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    if constexpr (DP <= 128) {
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
 #pragma unroll
-    for (int i = 0; i < MMAS; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if (VALU > 0) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+        for (int i = 0; i < MMAS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (VALU > 0) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+        }
     }
 }
-__device__ __forceinline__ void att_region() { __builtin_amdgcn_sched_barrier(0); }
+template <int DP>
+__device__ __forceinline__ void att_region()
+{
+    if constexpr (DP <= 128) __builtin_amdgcn_sched_barrier(0);
+}
 
 template <typename T, int DP>
 struct AttGroups {
@@ -345,6 +353,8 @@ struct AttGroups {
     static constexpr int MMAS = sizeof(T) == 4 ? 8 : 1;                 // matrix instructions per fragment
     static constexpr int READS_ROW = sizeof(T) == 4 ? 2 : 1;
     static constexpr int READS_T = sizeof(T) == 4 ? 8 : 2;
+    static constexpr int COLUMNS = DP / 32 <= 4 ? DP / 32 : sizeof(T) == 4 ? 2 : 4;     // fragments of a group of transposed ones
+    static constexpr int COLUMN_GROUPS = DP / 32 / COLUMNS;             // for all columns of 16 rows
 };
 
 template <typename T, int DP, int GROUP>
@@ -354,12 +364,12 @@ __device__ __forceinline__ void att_read_group(att_vec8<T> (&f)[GROUP], const at
     for (int i = 0; i < GROUP; ++i) f[i] = att_read_row<T, DP>(tile, row, 16 * (GROUP * group + i), lane);
 }
 
-// All DP columns of 16 rows, transposed.
-template <typename T, int DP>
-__device__ __forceinline__ void att_read_columns(att_vec8<T> (&f)[DP / 32], const att_lds_byte *tile, int row, int lane)
+// Group `group` of the columns of 16 rows, transposed.
+template <typename T, int DP, int COLUMNS>
+__device__ __forceinline__ void att_read_columns(att_vec8<T> (&f)[COLUMNS], const att_lds_byte *tile, int row, int group, int lane)
 {
 #pragma unroll
-    for (int o = 0; o < DP / 32; ++o) f[o] = att_read_transposed<T, DP>(tile, row, 32 * o, lane);
+    for (int o = 0; o < COLUMNS; ++o) f[o] = att_read_transposed<T, DP>(tile, row, 32 * (COLUMNS * group + o), lane);
 }
 
 // s^T of a tile of KT keys in LDS and the 32 rows whose queries are in `query`, and the largest of each lane's scores.  One block of 32 keys after the
@@ -374,7 +384,7 @@ __device__ __forceinline__ float att_scores(att_f32x16 (&s)[KT / 32], const att_
 #pragma unroll
     for (int b = 0; b < KT / 32; ++b) s[b] = att_f32x16{0};
     float top = -__builtin_inff();
-    att_region();
+    att_region<DP>();
 #pragma unroll
     for (int i = 0; i < ALL; ++i) {
         const int b = i / G::GROUPS, group = i % G::GROUPS;
@@ -384,8 +394,8 @@ __device__ __forceinline__ float att_scores(att_f32x16 (&s)[KT / 32], const att_
         if (b > 0)
 #pragma unroll
             for (int j = EACH * group; j < (group + 1 == G::GROUPS ? 16 : EACH * (group + 1)); ++j) top = fmaxf(top, s[b - 1][j]);
-        att_order<G::GROUP * G::READS_ROW, G::GROUP * G::MMAS, 0>();
-        att_region();
+        att_order<DP, G::GROUP * G::READS_ROW, G::GROUP * G::MMAS, 0>();
+        att_region<DP>();
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j) top = fmaxf(top, s[KT / 32 - 1][j]);
@@ -445,23 +455,30 @@ __device__ __forceinline__ att_vec8<T> att_weights(AttState<DP> &state, const at
     return weights;
 }
 
-// out^T += V^T p^T over the KT keys of a tile; with NEXT, the weights give way to those of the scores s.
+// out^T += V^T p^T over the KT keys of a tile; with NEXT, the weights give way to those of the scores s.  `first`: the first group of V's columns.
 template <typename T, int DP, int KT, bool NEXT>
-__device__ __forceinline__ void att_add_values(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], const att_lds_byte *values, const att_vec8<T> (&first)[DP / 32],
-                                               const att_f32x16 (&s)[KT / 32], float scale_log2, float base, int lane)
+__device__ __forceinline__ void att_add_values(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], const att_lds_byte *values,
+                                               const att_vec8<T> (&first)[AttGroups<T, DP>::COLUMNS], const att_f32x16 (&s)[KT / 32], float scale_log2, float base,
+                                               int lane)
 {
     typedef AttGroups<T, DP> G;
-    att_vec8<T> f[2][DP / 32];
+    constexpr int ALL = KT / 16 * G::COLUMN_GROUPS;
+    att_vec8<T> f[2][G::COLUMNS];
 #pragma unroll
-    for (int o = 0; o < DP / 32; ++o) f[0][o] = first[o];
+    for (int o = 0; o < G::COLUMNS; ++o) f[0][o] = first[o];
 #pragma unroll
-    for (int step = 0; step < KT / 16; ++step) {
-        if (step + 1 < KT / 16) att_read_columns<T, DP>(f[(step + 1) & 1], values, 16 * (step + 1), lane);
+    for (int i = 0; i < ALL; ++i) {
+        const int step = i / G::COLUMN_GROUPS, group = i % G::COLUMN_GROUPS;
+        if (i + 1 < ALL) att_read_columns<T, DP>(f[(i + 1) & 1], values, 16 * ((i + 1) / G::COLUMN_GROUPS), (i + 1) % G::COLUMN_GROUPS, lane);
 #pragma unroll
-        for (int o = 0; o < DP / 32; ++o) state.out[o] = att_mma(f[step & 1][o], weights[step], state.out[o]);
-        if (NEXT) weights[step] = att_weights<T, DP, KT>(state, s, step, scale_log2, base);
-        att_order<DP / 32 * G::READS_T, DP / 32 * G::MMAS, NEXT ? (G::MMAS > 1 ? 1 : DP <= 64 ? 14 : DP <= 128 ? 7 : 4) : 0>();
-        att_region();
+        for (int o = 0; o < G::COLUMNS; ++o) {
+            att_f32x16 &out = state.out[G::COLUMNS * group + o];
+            out = att_mma(f[i & 1][o], weights[step], out);
+        }
+        const bool last = group + 1 == G::COLUMN_GROUPS;
+        if (NEXT && last) weights[step] = att_weights<T, DP, KT>(state, s, step, scale_log2, base);
+        att_order<DP, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, NEXT ? (G::MMAS > 1 ? 1 : DP <= 64 ? 14 : 7) : 0>();
+        att_region<DP>();
     }
 }
 
@@ -655,7 +672,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
             att_lds_byte *key_ring = lds, *value_ring = lds + 2 * TILE;
             Tile next_k, next_v;
             att_f32x16 s[KT / 32];
-            att_vec8<T> weights[KT / 16], first[DP / 32];
+            att_vec8<T> weights[KT / 16], first[AttGroups<T, DP>::COLUMNS];
             float top, base;
 #pragma unroll
                 for (int step = 0; step < KT / 16; ++step) weights[step] = att_vec8<T>{0};
@@ -701,7 +718,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                 if (works) {
                     const att_lds_byte *values = value_ring + (now ^ 1) * TILE;
                     top = att_scores<T, DP, KT>(s, query, key_ring + now * TILE, lane);
-                    att_read_columns<T, DP>(first, values, 0, lane);
+                    att_read_columns<T, DP>(first, values, 0, 0, lane);
                     rebase(n, kept);
                     att_add_values<T, DP, KT, true>(state, weights, values, first, s, scale_log2, base, lane);
                 }
@@ -709,7 +726,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
             }
             if (works) {
                 const att_lds_byte *values = value_ring + (now ^ 1) * TILE;
-                att_read_columns<T, DP>(first, values, 0, lane);
+                att_read_columns<T, DP>(first, values, 0, 0, lane);
                 att_add_values<T, DP, KT, false>(state, weights, values, first, s, 0.0f, base, lane);
             }
         }
@@ -729,14 +746,19 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                 const int limit = keys.causal ? length - args.m + 1 + row / args.r : 0x7fffffff;
                 const T *k = static_cast<const T *>(keys.k) + entry * keys.k_ls + g * keys.k_gs;
                 const T *v = static_cast<const T *>(keys.v) + entry * keys.v_ls + g * keys.v_gs;
-                AttTile<T, DP, KT, 64, ALIGNED> next_k, next_v;
+                typedef AttTile<T, DP, KT, 64, ALIGNED> Tile;
+                Tile next_k, next_v;
                 i64 n = begin + wave * KT;
-                if (n < end) {
+                if (!Tile::DIRECT && n < end) {
                     next_k.begin(k + n * keys.k_ns, keys.k_ns, end - static_cast<int>(n), args.k, key_tile, lane);
                     next_v.begin(v + n * keys.v_ns, keys.v_ns, end - static_cast<int>(n), args.o, value_tile, lane);
                 }
                 for (; n < end; n += KT * OWN) {
                     const att_u64 kept = att_kept_keys(keys, entry, static_cast<int>(n), end, lane);
+                    if (Tile::DIRECT) {
+                        next_k.begin(k + n * keys.k_ns, keys.k_ns, end - static_cast<int>(n), args.k, key_tile, lane);
+                        next_v.begin(v + n * keys.v_ns, keys.v_ns, end - static_cast<int>(n), args.o, value_tile, lane);
+                    }
                     next_k.finish(key_tile, lane);
                     next_v.finish(value_tile, lane);
                     att_wave_sync();
@@ -745,18 +767,18 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                         att_wave_sync();
                     }
                     const i64 at = n + KT * OWN;
-                    if (at < end) {
+                    if (!Tile::DIRECT && at < end) {
                         next_k.begin(k + at * keys.k_ns, keys.k_ns, end - static_cast<int>(at), args.k, key_tile, lane);
                         next_v.begin(v + at * keys.v_ns, keys.v_ns, end - static_cast<int>(at), args.o, value_tile, lane);
                     }
                     att_f32x16 s[KT / 32];
-                    att_vec8<T> weights[KT / 16] = {}, first[DP / 32];
+                    att_vec8<T> weights[KT / 16] = {}, first[AttGroups<T, DP>::COLUMNS];
                     const float top = att_scores<T, DP, KT>(s, query, key_tile, lane);
                     att_rebase<T, DP, KT>(state, weights, s, top, args.scale_log2, kept & att_low_bits(limit - static_cast<int>(n)), lane);
                     const float base = att_finite_base(state.base);
 #pragma unroll
                     for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, args.scale_log2, base);
-                    att_read_columns<T, DP>(first, value_tile, 0, lane);
+                    att_read_columns<T, DP>(first, value_tile, 0, 0, lane);
                     att_add_values<T, DP, KT, false>(state, weights, value_tile, first, s, 0.0f, base, lane);
                     att_wave_sync();
                 }

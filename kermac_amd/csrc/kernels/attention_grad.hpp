@@ -53,7 +53,7 @@ __device__ __forceinline__ void att_two_scores(att_f32x16 &s, att_f32x16 &ds, co
     };
     read(f[0], 0);
     s = ds = att_f32x16{0};
-    att_region();
+    att_region<DP>();
 #pragma unroll
     for (int i = 0; i < ALL; ++i) {
         if (i + 1 < ALL) read(f[(i + 1) & 1], i + 1);
@@ -65,8 +65,8 @@ __device__ __forceinline__ void att_two_scores(att_f32x16 &s, att_f32x16 &ds, co
         if (VECTOR)
 #pragma unroll
             for (int q = 4 * i / ALL; q < 4 * (i + 1) / ALL; ++q) quad(q);
-        att_order<2 * AT_ONCE * G::READS_ROW, 2 * AT_ONCE * G::MMAS, VECTOR ? (sizeof(T) == 4 ? 1 : 4 * 4 / ALL + 1) : 0>();
-        att_region();
+        att_order<DP, 2 * AT_ONCE * G::READS_ROW, 2 * AT_ONCE * G::MMAS, VECTOR ? (sizeof(T) == 4 ? 1 : 4 * 4 / ALL + 1) : 0>();
+        att_region<DP>();
     }
 }
 
@@ -209,9 +209,11 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
         for (int b = 0; b < KT / 32; ++b) {
             constexpr int BLOCK = 32 * AttLds<T, DP>::STRIDE;
             att_f32x16 s, ds;
-            att_vec8<T> x[2], f[2][DP / 32];
-            att_two_scores<T, DP, false>(s, ds, key_tile + b * BLOCK, query, value_tile + b * BLOCK, grad, lane, [](int) {});
-            att_read_columns<T, DP>(f[0], key_tile + b * BLOCK, 0, lane);
+            typedef AttGroups<T, DP> G;
+            att_vec8<T> x[2], f[2][G::COLUMNS];
+            const att_lds_byte *block = key_tile + b * BLOCK;
+            att_two_scores<T, DP, false>(s, ds, block, query, value_tile + b * BLOCK, grad, lane, [](int) {});
+            att_read_columns<T, DP>(f[0], block, 0, 0, lane);
 #pragma unroll
             for (int i = 0; i < 16; ++i) ds[i] = att_weight(s[i], scale_log2, lse2) * (ds[i] - delta);
             const unsigned here = static_cast<unsigned>(kept >> (32 * b));
@@ -223,11 +225,18 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
             }
             x[0] = att_operand<T>(ds, 0);
             x[1] = att_operand<T>(ds, 1);
-            att_read_columns<T, DP>(f[1], key_tile + b * BLOCK, 16, lane);
 #pragma unroll
-            for (int step = 0; step < 2; ++step)
+            for (int i = 0; i < 2 * G::COLUMN_GROUPS; ++i) {
+                const int step = i / G::COLUMN_GROUPS, group = i % G::COLUMN_GROUPS;
+                if (i + 1 < 2 * G::COLUMN_GROUPS)
+                    att_read_columns<T, DP>(f[(i + 1) & 1], block, 16 * ((i + 1) / G::COLUMN_GROUPS), (i + 1) % G::COLUMN_GROUPS, lane);
 #pragma unroll
-                for (int o = 0; o < DP / 32; ++o) acc[o] = att_mma(f[step][o], x[step], acc[o]);
+                for (int o = 0; o < G::COLUMNS; ++o) acc[G::COLUMNS * group + o] = att_mma(f[i & 1][o], x[step], acc[G::COLUMNS * group + o]);
+                if (G::COLUMN_GROUPS > 1) {
+                    att_order<DP, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, 0>();
+                    att_region<DP>();
+                }
+            }
         }
     }
     if (row >= rows) return;
@@ -367,19 +376,26 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
                 p[step] = __builtin_bit_cast(att_vec8<T>, __builtin_bit_cast(words, p[step]) & keep);
                 x[step] = __builtin_bit_cast(att_vec8<T>, __builtin_bit_cast(words, x[step]) & keep);
             }
-            att_vec8<T> f[2][DP / 32];
-            att_read_columns<T, DP>(f[0], d_tile, 0, lane);
-            att_region();
+            // four steps of 16 rows: two of the gradients, two of the queries
+            constexpr int ALL = 4 * G::COLUMN_GROUPS;
+            att_vec8<T> f[2][G::COLUMNS];
+            auto read = [&](att_vec8<T> (&to)[G::COLUMNS], int i) {
+                const int step = i / G::COLUMN_GROUPS;
+                att_read_columns<T, DP>(to, step < 2 ? d_tile : q_tile, 16 * (step % 2), i % G::COLUMN_GROUPS, lane);
+            };
+            read(f[0], 0);
+            att_region<DP>();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (i < 3) att_read_columns<T, DP>(f[(i + 1) & 1], i == 0 ? d_tile : q_tile, i == 1 ? 0 : 16, lane);
+            for (int i = 0; i < ALL; ++i) {
+                const int step = i / G::COLUMN_GROUPS, group = i % G::COLUMN_GROUPS;
+                if (i + 1 < ALL) read(f[(i + 1) & 1], i + 1);
 #pragma unroll
-                for (int o = 0; o < DP / 32; ++o) {
-                    if (i < 2) acc_v[o] = att_mma(f[i & 1][o], p[i], acc_v[o]);
-                    else acc_k[o] = att_mma(f[i & 1][o], x[i - 2], acc_k[o]);
+                for (int o = 0; o < G::COLUMNS; ++o) {
+                    att_f32x16 &to = step < 2 ? acc_v[G::COLUMNS * group + o] : acc_k[G::COLUMNS * group + o];
+                    to = att_mma(f[i & 1][o], step < 2 ? p[step] : x[step - 2], to);
                 }
-                att_order<DP / 32 * G::READS_T, DP / 32 * G::MMAS, 0>();
-                att_region();
+                att_order<DP, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, 0>();
+                att_region<DP>();
             }
         };
         auto turn = [&](const att_f32x16 &s, const att_f32x16 &ds, att_f32x16 &next_s, att_f32x16 &next_ds) {
