@@ -210,6 +210,15 @@ __device__ __forceinline__ void att_wait_for_loads()
     asm volatile("" : : : "memory");
 }
 
+// No read of LDS is outstanding: what is asked for next may overwrite what was read, and a read whose register is not used yet may not have been made.
+// (A barrier waits for that by itself.)
+__device__ __forceinline__ void att_wait_for_reads()
+{
+    asm volatile("" : : : "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);         // lgkmcnt 0, the other counters as they are
+    asm volatile("" : : : "memory");
+}
+
 // A tile of ROWS rows of DP elements on its way from memory to LDS.  begin() asks for it, finish() has it written.  DIRECT: from memory straight into LDS, 1 KB per
 // wave and instruction, each lane fetching the piece that belongs where its 16 bytes end up; no register waits for it.  Otherwise (unaligned rows,
 // tiles of one wave, whose next tile waits in registers while LDS holds the current one, unless a row of 1 KB asks too many) through registers.
@@ -599,8 +608,16 @@ __device__ __forceinline__ void att_load_queries(const AttentionArgs &args, cons
 
 // A workgroup per (batch entry, head of keys, range of keys, tile of rows).
 //
-// More than 32 rows: ROW_WAVES waves of 32 rows each share the tiles of keys and values.  At most 32 rows (single tokens): reading keys
-// and values is all the work, so every wave walks tiles of its own without waiting for the others, and the waves' results are joined at the end.
+// More than 32 rows: WAVES waves of 32 rows each share the tiles of keys and values.  Bound by the matrix cores, which what feeds them keeps from their
+// rate: with 128 features in 16 bits, the fragments of keys and values that a wave reads from LDS take as long as the products that it makes of them.
+// 8 entries x 4096 queries x 8192 keys x 32 heads on 8 x 128 bf16: 4.0 ms, 1.1 PFLOP/s (the matrix cores are busy half of the time; a large
+// bf16 matrix product of the library's reaches 1.24).  Measured and left out: 64 rows per wave (half the reads from LDS, one wave per SIMD: 7.0 ms), 8
+// waves that share a tile (the same time), tiles of 32 keys in deeper rings (4.8 ms).  fp32 is bound by its products: 72 useful TFLOP/s of 154 at
+// 2 x 1000 x 2900 x 8 heads of 64, of which 80 % of the keys take part.
+//
+// At most 32 rows (single tokens): reading keys and values is all the work, so every wave walks tiles of its own without waiting for the others,
+// and the waves' results are joined at the end.  32 entries x 1 query x up to 4000 keys x 16 heads of 64 bf16: 89 us, 4.4 TB/s (a large copy
+// reaches 4.8); 4 x 32768 keys x 16 heads of 128: 194 us, 5.5 TB/s.
 template <typename T, int DP, bool ALIGNED>
 __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void attention_forward(const AttentionArgs args)
 {
@@ -656,8 +673,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
             int begin, end;
             att_range(length, KT, split, job.splits, &begin, &end);
             // query i of a sequence's last m tokens sees the tokens up to its own
-            int limit;
-            limit = keys.causal ? length - args.m + 1 + (row) / args.r : 0x7fffffff;
+            const int limit = keys.causal ? length - args.m + 1 + row / args.r : 0x7fffffff;
             if (keys.causal) {
                 const int last_row = (row_tile + 1) * ROWS < job.rows ? (row_tile + 1) * ROWS - 1 : job.rows - 1;
                 const int last_limit = length - args.m + 1 + last_row / args.r;
@@ -675,7 +691,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
             att_vec8<T> weights[KT / 16], first[AttGroups<T, DP>::COLUMNS];
             float top, base;
 #pragma unroll
-                for (int step = 0; step < KT / 16; ++step) weights[step] = att_vec8<T>{0};
+            for (int step = 0; step < KT / 16; ++step) weights[step] = att_vec8<T>{0};
             const float scale_log2 = args.scale_log2;
             const int k_width = args.k, v_width = args.o;
             int now = 0;                                // which of two tiles
@@ -709,7 +725,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                 top = att_scores<T, DP, KT>(s, query, key_ring, lane);
                 rebase(begin, kept);
 #pragma unroll
-                    for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, scale_log2, base);
+                for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, scale_log2, base);
             }
             got(begin, kept);
             for (int n = begin + KT; n < end; n += KT) {
@@ -731,7 +747,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
             }
         }
         if (!works) return;
-            att_forward_write<T, DP, ALIGNED>(args, job, state, att_sum_of_halves(state.sum), entry, g, row, split, lane);
+        att_forward_write<T, DP, ALIGNED>(args, job, state, att_sum_of_halves(state.sum), entry, g, row, split, lane);
     } else {
         constexpr int KT = Shape::OWN_KEYS, OWN = Shape::OWN_WAVES;
         att_lds_byte *key_tile = lds + 2 * wave * KT * Shape::ROW_BYTES, *value_tile = key_tile + KT * Shape::ROW_BYTES;
@@ -756,6 +772,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                 for (; n < end; n += KT * OWN) {
                     const att_u64 kept = att_kept_keys(keys, entry, static_cast<int>(n), end, lane);
                     if (Tile::DIRECT) {
+                        att_wait_for_reads();
                         next_k.begin(k + n * keys.k_ns, keys.k_ns, end - static_cast<int>(n), args.k, key_tile, lane);
                         next_v.begin(v + n * keys.v_ns, keys.v_ns, end - static_cast<int>(n), args.o, value_tile, lane);
                     }
