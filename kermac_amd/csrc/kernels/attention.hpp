@@ -325,7 +325,7 @@ __device__ __forceinline__ void att_wave_sync()
 template <int DP>
 struct AttState {
     att_f32x16 out[DP / 32];
-    float base, sum;             // a whole number near the largest score so far and the sum of this lane's exponentials relative to it, to base 2
+    float base, sum;             // a score near the largest so far and the sum of this lane's exponentials relative to it, to base 2
 };
 
 // Outputs and sums are rescaled only when a score passes the one they are relative to by 2^8: exponentials stay below 256, far inside every type,
@@ -411,8 +411,9 @@ __device__ __forceinline__ float att_scores(att_f32x16 (&s)[KT / 32], const att_
     return top;
 }
 
-// Masks a tile's scores (`kept` has a bit per key for this lane's row) and, where they pass the wave's base by 2^8, moves it.  Bases are whole
-// numbers, so that what was made below the old one is rescaled without rounding: output and sum, and `weights` that wait for their product.
+// Masks a tile's scores (`kept` has a bit per key for this lane's row) and, where they pass the wave's base by 2^8, moves it to the largest, whose weight is
+// then exactly 1 (a row of one key gets its value without a rounding).  What was made below the old base is rescaled: output and sum, and `weights`
+// that wait for their product and are rounded once more.
 template <typename T, int DP, int KT>
 __device__ __forceinline__ void att_rebase(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], att_f32x16 (&s)[KT / 32], float top, float scale_log2, att_u64 kept,
                                            int lane)
@@ -434,7 +435,7 @@ __device__ __forceinline__ void att_rebase(AttState<DP> &state, att_vec8<T> (&we
     top = att_max_of_halves(top) * scale_log2;
     if (!__all(top <= state.base + ATT_HEADROOM)) {
         att_rare();
-        const float base = fmaxf(state.base, __builtin_ceilf(top));
+        const float base = fmaxf(state.base, top);
         const float shrink = __builtin_amdgcn_exp2f(state.base - (base == -__builtin_inff() ? 0.0f : base));
         state.base = base;
         state.sum *= shrink;

@@ -219,3 +219,24 @@ def test_prefix_of_a_generation(device, dtype):
         # both are within one bound of the same truth
         assert torch.allclose(out.double(), whole[:, at - step:at].double(), rtol=8 * reference.UNIT[dtype], atol=8 * reference.UNIT[dtype] * 4)
     assert at == N
+
+
+@pytest.mark.parametrize("dtype", TYPES[:2], ids=str)
+@pytest.mark.parametrize("M", [1, 8, 40, 300])
+@pytest.mark.parametrize("scale", [None, 0.3, -7.0])
+def test_one_key_is_its_value(device, dtype, M, scale):
+    """A softmax over one key is 1: the values come back bit for bit, alone, behind masked keys and through a length.
+
+    Its weight is 1 up to fp32's rounding of the exponent (|scale q k| below 2^9 here, so off by less than 2^-14), which is less than
+    half a step beside 1 of either type, and so is what the division by the sum leaves beside the value before it is rounded.
+    """
+    q, k, v = operands(2, M, 200, 4, 2, 64, 64, dtype, device)
+    one = v[:, :1].repeat_interleave(2, 2).expand(2, M, 4, 64)
+    assert torch.equal(kermac.cross_attention(q, k[:, :1], v[:, :1], scale=scale), one)
+    lengths = torch.ones(2, dtype=torch.int32, device=device)
+    assert torch.equal(kermac.cross_attention(q, k, v, scale=scale, key_lengths=lengths), one)
+    mask = torch.zeros(200, dtype=torch.bool, device=device)
+    mask[150] = True
+    assert torch.equal(kermac.cross_attention(q, k, v, scale=scale, key_mask=mask), v[:, 150:151].repeat_interleave(2, 2).expand(2, M, 4, 64))
+    nothing = torch.zeros(2, dtype=torch.int32, device=device)
+    assert torch.equal(kermac.prefix_attention(q, k[0, :1], v[0, :1], k, v, nothing, scale=scale), v[:1, :1].repeat_interleave(2, 2).expand(2, M, 4, 64))
