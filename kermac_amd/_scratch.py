@@ -18,7 +18,8 @@ coefficient product.  All of it goes through this module, which offers two contr
     calls that share it must be ordered on one stream, and its contents mean nothing between calls.
 
 A route that is refused its memory falls back to the kernels that need none; results keep their
-tolerance, and for a given shape and setting the choice is always the same.
+tolerance, and for a given shape and setting the choice is always the same.  One operator has no such
+kernels: ``cross_attention_grad`` raises where the 8 bytes per row that it cannot do without are refused.
 """
 from __future__ import annotations
 

@@ -15,7 +15,6 @@ step calls ``cross_attention_grad`` with the result and the row sums that ``cros
 from __future__ import annotations
 
 import functools
-import math
 import struct
 from typing import Optional
 
@@ -28,6 +27,7 @@ from .build_a_kernel import _current_stream_for
 _TYPES = {torch.float32: _backend.FP32, torch.float16: _backend.FP16, torch.bfloat16: _backend.BF16}
 _MAX_WIDTH = 256
 _MAX_EXTENT = 2_000_000_000
+_MAX_SCALE = 2e38                       # times log2(e) still a number of fp32
 
 # A call on one token costs the GPU a few microseconds, so its host side counts: the parameter blocks are packed in one step (a field by
 # field structure takes four times as long), and what a shape asks of the workspace is asked of the library once.
@@ -137,8 +137,8 @@ def _plan_attention(queries, keys, values, out, scale, key_lengths, key_mask, re
     if L * M * H > _MAX_EXTENT or max(L, M, N, H) > _MAX_EXTENT:
         raise ValueError(f"at most {_MAX_EXTENT} keys, and rows over the batch and the heads: got N={N}, L={L}, M={M}, H={H}")
     scale = K ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
+    if not abs(scale) <= _MAX_SCALE:
+        raise ValueError(f"scale must be finite and at most {_MAX_SCALE:g}, got {scale}")
     lengths_ptr = mask_ptr = mask_ls = mask_ns = 0
     if key_lengths is not None:
         name = "key_lengths" if prefix is None else "lengths"
@@ -221,7 +221,7 @@ def cross_attention(
     values of batch size 1 serve all entries of the batch.
 
     Args:
-        scale: ``K ** -0.5`` when None; any finite number.
+        scale: ``K ** -0.5`` when None; any number up to 2e38 in magnitude.
         key_lengths: int32 ``[L]``: the first so many keys of an entry take part (taken as 0 .. N where outside).
         key_mask: bool ``[N]`` or ``[L, N]``: the keys that take part.  With both, a key has to pass both.
         out: optional result, ``[L, M, H, O]``, written in place and returned; it must not share memory with the inputs.
@@ -233,7 +233,7 @@ def cross_attention(
 
     Raises:
         TypeError: non-tensor inputs or a wrong dtype.
-        ValueError: bad shapes, strides, batch sizes or devices, a scale that is not finite.
+        ValueError: bad shapes, strides, batch sizes or devices, a scale that is not finite or beyond 2e38.
     """
     plan = _plan_attention(queries, keys, values, out, scale, key_lengths, key_mask, return_lse)
     _launch(plan, debug)
@@ -302,7 +302,7 @@ def cross_attention_grad(
 
     Raises:
         TypeError: non-tensor inputs or a wrong dtype.
-        ValueError: bad shapes, strides, batch sizes or devices, a scale that is not finite.
+        ValueError: bad shapes, strides, batch sizes or devices, a scale that is not finite or beyond 2e38.
         RuntimeError: the limit on scratch memory, or the supplied buffer, does not allow those bytes.
     """
     plan = _plan_attention_grad(grad_out, queries, keys, values, out, lse, scale, key_lengths, key_mask)
@@ -341,7 +341,8 @@ def prefix_attention(
     ``lengths[l]`` rows of ``keys[l]`` and ``values[l]``.  Its queries are its last ``M`` tokens: query ``m`` is its own token
     ``lengths[l] - M + m`` and meets the whole prefix and its own tokens up to itself.  ``M = 1`` is one step of generation, a
     larger ``M`` a prompt behind the prefix.  Where ``lengths[l] < M``, the first queries are tokens that do not exist: they meet
-    the prefix alone.  What ``keys`` and ``values`` hold behind ``lengths[l]`` does not matter.
+    the prefix alone.  What ``keys`` and ``values`` hold behind ``lengths[l]`` does not matter.  (In front of it it does: an infinity or NaN among
+    the values of a sequence's own token may reach its queries in front of that token too, whose weight for it is 0.)
 
     Types, heads, ``scale``, ``out`` and errors are those of ``cross_attention``; ``lengths`` is int32, taken as 0 .. N where outside.
     Returns ``out`` (allocated ``[L, M, H, O]`` when None).

@@ -21,6 +21,7 @@ KMC_DECLARE_ATTENTION(2)
 namespace {
 
 constexpr int MAX_WIDTH = 256;
+constexpr double MAX_SCALE = 2.0e38;  // times log2(e) still a number of fp32
 constexpr int MAX_KEYS = 0x7fffffff - 1024;         // a tile behind the last key still has a number
 int element_size(int type) { return type == KMC_FP32 ? 4 : 2; }
 
@@ -58,7 +59,7 @@ int check_extents(int type, int l, int m, int n, int h, int g, int k, int o, flo
     if (h > 0 && (g == 0 || h % g != 0)) return fail(KMC_ERR_INVALID_ARGUMENT, "h=%d is no multiple of g=%d", h, g);
     if (k < 1 || k > MAX_WIDTH || o < 1 || o > MAX_WIDTH)
         return fail(KMC_ERR_INVALID_ARGUMENT, "k=%d and o=%d must be in 1 .. %d", k, o, MAX_WIDTH);
-    if (!std::isfinite(scale)) return fail(KMC_ERR_INVALID_ARGUMENT, "scale must be finite");
+    if (!(std::fabs(scale) <= MAX_SCALE)) return fail(KMC_ERR_INVALID_ARGUMENT, "scale must be finite and at most %g", MAX_SCALE);
     // rows of a head of keys over the batch, and rows times heads over the batch, are numbered in 31 bits
     if (static_cast<double>(l) * m * h > 2.0e9) return fail(KMC_ERR_INVALID_ARGUMENT, "l m h = %.0f is beyond 2e9 rows", static_cast<double>(l) * m * h);
     return KMC_OK;
@@ -153,7 +154,6 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
     const int status = check_extents(p->type, p->l, p->m, p->n, p->h, p->g, p->k, p->o, p->scale);
     if (status != KMC_OK) return status;
     if (p->prefix_n < 0 || p->prefix_n > MAX_KEYS) return fail(KMC_ERR_INVALID_ARGUMENT, "prefix_n=%d is outside 0 .. %d", p->prefix_n, MAX_KEYS);
-    if (p->causal && !p->key_lengths) return fail(KMC_ERR_INVALID_ARGUMENT, "causal needs key_lengths");
     if ((p->causal || p->prefix_n > 0) && p->key_mask) return fail(KMC_ERR_INVALID_ARGUMENT, "key_mask does not go with a prefix");
     const int64_t strides[] = {p->q_ls, p->q_ms, p->q_hs, p->key_ls, p->key_ns, p->key_gs, p->value_ls, p->value_ns, p->value_gs,
                                p->out_ls, p->out_ms, p->out_hs, p->key_mask_ls, p->key_mask_ns, p->prefix_key_ns, p->prefix_key_gs,
@@ -163,6 +163,7 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
     plan->bytes = 0;
     plan->empty = p->l == 0 || p->m == 0 || p->h == 0;
     if (plan->empty) return KMC_OK;
+    if (p->causal && !p->key_lengths) return fail(KMC_ERR_INVALID_ARGUMENT, "causal needs key_lengths");
     if (!p->q || !p->out) return fail(KMC_ERR_INVALID_ARGUMENT, "null q / out pointer");
     if (p->n > 0 && (!p->key || !p->value)) return fail(KMC_ERR_INVALID_ARGUMENT, "null key / value pointer");
     if (p->prefix_n > 0 && (!p->prefix_key || !p->prefix_value)) return fail(KMC_ERR_INVALID_ARGUMENT, "null prefix_key / prefix_value pointer");

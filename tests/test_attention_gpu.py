@@ -240,3 +240,10 @@ def test_one_key_is_its_value(device, dtype, M, scale):
     assert torch.equal(kermac.cross_attention(q, k, v, scale=scale, key_mask=mask), v[:, 150:151].repeat_interleave(2, 2).expand(2, M, 4, 64))
     nothing = torch.zeros(2, dtype=torch.int32, device=device)
     assert torch.equal(kermac.prefix_attention(q, k[0, :1], v[0, :1], k, v, nothing, scale=scale), v[:1, :1].repeat_interleave(2, 2).expand(2, M, 4, 64))
+
+
+def test_prefix_of_no_sequences(device):
+    q, pk, pv, k, v = prefix_operands(1, 3, 50, 7, 4, 2, 64, 64, torch.bfloat16, device)
+    lengths = torch.zeros(1, dtype=torch.int32, device=device)
+    assert kermac.prefix_attention(q[:0], pk, pv, k[:0], v[:0], lengths[:0]).shape == (0, 3, 4, 64)
+    assert kermac.prefix_attention(q[:, :0], pk, pv, k, v, lengths).shape == (1, 0, 4, 64)

@@ -204,3 +204,38 @@ def test_the_workspace_that_is_asked_for_is_what_the_call_uses(dtype, L, M, N, H
     if prefix is None:
         of = _plan_attention_grad(q, q, k, v, q, make(L, M, H), None, None, None, require_device=False)
         assert attention._gradient_workspace_bytes(*of.extents) == _backend.attention_gradient_workspace_bytes(of.params)
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, 3e38, -math.inf])
+def test_scales_that_fp32_does_not_hold_to_base_2(scale):
+    """Scores are taken to base 2: a scale is refused where fp32 does not hold its product with log2(e), in Python and in the library."""
+    q, k, v = make(2, 5, 4, 16), make(2, 7, 2, 16), make(2, 7, 2, 24)
+    with pytest.raises(ValueError, match="scale"):
+        plan(q, k, v, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        _plan_attention_grad(make(2, 5, 4, 24), q, k, v, make(2, 5, 4, 24), make(2, 5, 4), scale, None, None, require_device=False)
+    assert plan(q, k, v, scale=-1.9e38).params.scale < -1.8e38
+    assert _backend.attention_workspace_bytes(library_parameters(scale=-1.9e38)) > 0
+    params = library_parameters(scale=scale)
+    with pytest.raises(_backend.BackendError, match="scale"):
+        _backend.attention(params, None)
+
+
+def test_a_batch_of_no_sequences():
+    """Empty tensors have no address, the lengths of a batch of none among them: the library takes that for a call with nothing to do."""
+    params = plan(make(0, 5, 4, 16), make(0, 7, 2, 16), make(0, 7, 2, 24), key_lengths=torch.zeros(0, dtype=torch.int32), prefix=(make(9, 2, 16), make(9, 2, 24))).params
+    assert params.key_lengths is None and params.causal == 1
+    assert _backend.attention_workspace_bytes(params) == 0
+    _backend.attention(params, None)
+
+
+def test_operands_on_another_device_are_refused():
+    q, k, v = make(2, 5, 4, 16), make(2, 7, 2, 16), make(2, 7, 2, 24)
+    elsewhere = torch.device("meta")
+    for change in (dict(k=k.to(elsewhere)), dict(v=v.to(elsewhere)), dict(out=make(2, 5, 4, 24).to(elsewhere)),
+                   dict(key_lengths=torch.zeros(2, dtype=torch.int32, device=elsewhere)), dict(key_mask=torch.zeros(7, dtype=torch.bool, device=elsewhere)),
+                   dict(prefix=(make(9, 2, 16).to(elsewhere), make(9, 2, 24)), key_lengths=torch.zeros(2, dtype=torch.int32))):
+        with pytest.raises(ValueError, match="same CUDA device"):
+            plan(**{**dict(q=q, k=k, v=v), **change})
+    with pytest.raises(ValueError, match="same CUDA device"):
+        _plan_attention_grad(make(2, 5, 4, 24), q, k, v, make(2, 5, 4, 24), make(2, 5, 4).to(elsewhere), None, None, None, require_device=False)
