@@ -527,9 +527,11 @@ struct AttForwardShape {
     static constexpr int SHARED_BYTES = 4 * SHARED_KEYS * ROW_BYTES;
     // Waves with keys of their own.
     static constexpr int OWN_KEYS = 32;
-    static constexpr int OWN_WAVES = ROW_BYTES <= 512 ? WAVES : 2;      // 1 KB rows: two waves' tiles fill LDS
-    static constexpr int OWN_BYTES = 2 * OWN_WAVES * OWN_KEYS * ROW_BYTES;
-    static constexpr int JOIN_BYTES = (OWN_WAVES - 1) * (DP * 32 + 64) * 4 + 128 * OWN_WAVES;
+    // Rows of 1 KB: two tiles for every wave do not fit LDS, and half of the waves would leave half of the matrix cores idle, which in fp32 take longer than
+    // the memory.  Keys and values take turns in one tile then (1 token x 20000 keys x 8 heads of 256 fp32: 136 us, with two waves of two tiles 151).
+    static constexpr bool OWN_TURNS = ROW_BYTES > 512;
+    static constexpr int OWN_BYTES = (OWN_TURNS ? 1 : 2) * WAVES * OWN_KEYS * ROW_BYTES;
+    static constexpr int JOIN_BYTES = (WAVES - 1) * (DP * 32 + 64) * 4 + 128 * WAVES;
     static constexpr int BYTES_1 = SHARED_BYTES > OWN_BYTES ? SHARED_BYTES : OWN_BYTES;
     static constexpr int BYTES = BYTES_1 > JOIN_BYTES ? BYTES_1 : JOIN_BYTES;
     static constexpr int WAVES_PER_SIMD = ROW_BYTES <= 256 ? 2 : 1;
@@ -750,76 +752,86 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
         if (!works) return;
         att_forward_write<T, DP, ALIGNED>(args, job, state, att_sum_of_halves(state.sum), entry, g, row, split, lane);
     } else {
-        constexpr int KT = Shape::OWN_KEYS, OWN = Shape::OWN_WAVES;
-        att_lds_byte *key_tile = lds + 2 * wave * KT * Shape::ROW_BYTES, *value_tile = key_tile + KT * Shape::ROW_BYTES;
+        constexpr int KT = Shape::OWN_KEYS;
+        constexpr bool TURNS = Shape::OWN_TURNS;
+        att_lds_byte *key_tile = lds + (TURNS ? 1 : 2) * wave * KT * Shape::ROW_BYTES, *value_tile = TURNS ? key_tile : key_tile + KT * Shape::ROW_BYTES;
         const int row = lane % 32;                                      // at most 32 rows: one tile
-        if (wave < OWN) {
-            att_load_queries<T, DP, ALIGNED>(args, job, entry, g, row, lane, query);
-            for (int segment = job.first_segment; segment < job.last_segment; ++segment) {
-                const AttentionKeys &keys = args.keys[segment];
-                const int length = att_length(keys, entry);
-                int begin, end;
-                att_range(length, KT, split, job.splits, &begin, &end);
-                const int limit = keys.causal ? length - args.m + 1 + row / args.r : 0x7fffffff;
-                const T *k = static_cast<const T *>(keys.k) + entry * keys.k_ls + g * keys.k_gs;
-                const T *v = static_cast<const T *>(keys.v) + entry * keys.v_ls + g * keys.v_gs;
-                typedef AttTile<T, DP, KT, 64, ALIGNED> Tile;
-                Tile next_k, next_v;
-                i64 n = begin + wave * KT;
-                if (!Tile::DIRECT && n < end) {
-                    next_k.begin(k + n * keys.k_ns, keys.k_ns, end - static_cast<int>(n), args.k, key_tile, lane);
-                    next_v.begin(v + n * keys.v_ns, keys.v_ns, end - static_cast<int>(n), args.o, value_tile, lane);
+        att_load_queries<T, DP, ALIGNED>(args, job, entry, g, row, lane, query);
+        for (int segment = job.first_segment; segment < job.last_segment; ++segment) {
+            const AttentionKeys &keys = args.keys[segment];
+            const int length = att_length(keys, entry);
+            int begin, end;
+            att_range(length, KT, split, job.splits, &begin, &end);
+            const int limit = keys.causal ? length - args.m + 1 + row / args.r : 0x7fffffff;
+            const T *k = static_cast<const T *>(keys.k) + entry * keys.k_ls + g * keys.k_gs;
+            const T *v = static_cast<const T *>(keys.v) + entry * keys.v_ls + g * keys.v_gs;
+            typedef AttTile<T, DP, KT, 64, ALIGNED> Tile;
+            static_assert(TURNS || !Tile::DIRECT, "the next tile waits in registers");
+            Tile next_k, next_v;
+            auto ask_keys = [&](i64 n) { next_k.begin(k + n * keys.k_ns, keys.k_ns, end - static_cast<int>(n), args.k, key_tile, lane); };
+            auto ask_values = [&](i64 n) { next_v.begin(v + n * keys.v_ns, keys.v_ns, end - static_cast<int>(n), args.o, value_tile, lane); };
+            i64 n = begin + wave * KT;
+            if (!TURNS && n < end) {
+                ask_keys(n);
+                ask_values(n);
+            }
+            for (; n < end; n += KT * WAVES) {
+                const att_u64 kept = att_kept_keys(keys, entry, static_cast<int>(n), end, lane);
+                att_f32x16 s[KT / 32];
+                att_vec8<T> weights[KT / 16] = {}, first[AttGroups<T, DP>::COLUMNS];
+                float top;
+                if (TURNS) {
+                    att_wait_for_reads();                   // those of the values before
+                    ask_keys(n);
                 }
-                for (; n < end; n += KT * OWN) {
-                    const att_u64 kept = att_kept_keys(keys, entry, static_cast<int>(n), end, lane);
-                    if (Tile::DIRECT) {
-                        att_wait_for_reads();
-                        next_k.begin(k + n * keys.k_ns, keys.k_ns, end - static_cast<int>(n), args.k, key_tile, lane);
-                        next_v.begin(v + n * keys.v_ns, keys.v_ns, end - static_cast<int>(n), args.o, value_tile, lane);
-                    }
-                    next_k.finish(key_tile, lane);
-                    next_v.finish(value_tile, lane);
+                next_k.finish(key_tile, lane);
+                if (TURNS) {
                     att_wave_sync();
-                    if (keys.mask && (kept & 0xffffffffull) != 0xffffffffull) {
-                        att_clear<T, DP, KT, 64>(value_tile, kept, lane);
-                        att_wave_sync();
+                    top = att_scores<T, DP, KT>(s, query, key_tile, lane);
+                    att_wave_sync();
+                    att_wait_for_reads();
+                    ask_values(n);
+                }
+                next_v.finish(value_tile, lane);
+                att_wave_sync();
+                if (keys.mask && (kept & 0xffffffffull) != 0xffffffffull) {
+                    att_clear<T, DP, KT, 64>(value_tile, kept, lane);
+                    att_wave_sync();
+                }
+                if (!TURNS) {
+                    const i64 at = n + KT * WAVES;
+                    if (at < end) {
+                        ask_keys(at);
+                        ask_values(at);
                     }
-                    const i64 at = n + KT * OWN;
-                    if (!Tile::DIRECT && at < end) {
-                        next_k.begin(k + at * keys.k_ns, keys.k_ns, end - static_cast<int>(at), args.k, key_tile, lane);
-                        next_v.begin(v + at * keys.v_ns, keys.v_ns, end - static_cast<int>(at), args.o, value_tile, lane);
-                    }
-                    att_f32x16 s[KT / 32];
-                    att_vec8<T> weights[KT / 16] = {}, first[AttGroups<T, DP>::COLUMNS];
-                    const float top = att_scores<T, DP, KT>(s, query, key_tile, lane);
-                    att_rebase<T, DP, KT>(state, weights, s, top, args.scale_log2, kept & att_low_bits(limit - static_cast<int>(n)), lane);
-                    const float base = att_finite_base(state.base);
+                    top = att_scores<T, DP, KT>(s, query, key_tile, lane);
+                }
+                att_rebase<T, DP, KT>(state, weights, s, top, args.scale_log2, kept & att_low_bits(limit - static_cast<int>(n)), lane);
+                const float base = att_finite_base(state.base);
 #pragma unroll
-                    for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, args.scale_log2, base);
-                    att_read_columns<T, DP>(first, value_tile, 0, 0, lane);
-                    att_add_values<T, DP, KT, false>(state, weights, value_tile, first, s, 0.0f, base, lane);
-                    att_wave_sync();
-                }
+                for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, args.scale_log2, base);
+                att_read_columns<T, DP>(first, value_tile, 0, 0, lane);
+                att_add_values<T, DP, KT, false>(state, weights, value_tile, first, s, 0.0f, base, lane);
+                att_wave_sync();
             }
         }
         // join the waves: sums and outputs below one common maximum, added in the order of the waves
         float sum = att_sum_of_halves(state.sum);
-        float *bases = reinterpret_cast<float *>(lds);                   // [OWN][32], then (OWN - 1) waves' sums and outputs
-        float *others = bases + 32 * OWN;
+        float *bases = reinterpret_cast<float *>(lds);                   // [WAVES][32], then (WAVES - 1) waves' sums and outputs
+        float *others = bases + 32 * WAVES;
         __syncthreads();
-        static_assert(OWN * 32 <= 256, "room for the bases");
-        if (wave < OWN && lane < 32) bases[wave * 32 + lane] = state.base;
+        if (lane < 32) bases[wave * 32 + lane] = state.base;
         __syncthreads();
         float base = -__builtin_inff();
 #pragma unroll
-        for (int w = 0; w < OWN; ++w) base = fmaxf(base, bases[w * 32 + lane % 32]);
+        for (int w = 0; w < WAVES; ++w) base = fmaxf(base, bases[w * 32 + lane % 32]);
         __syncthreads();
         const float shrink = base == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(state.base - base);
         state.base = base;
         sum *= shrink;
 #pragma unroll
         for (int o = 0; o < DP / 32; ++o) state.out[o] *= shrink;
-        if (wave > 0 && wave < OWN) {
+        if (wave > 0) {
             float *mine = others + (wave - 1) * (DP * 32 + 64);
 #pragma unroll
             for (int o = 0; o < DP / 32; ++o)
@@ -830,7 +842,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
         __syncthreads();
         if (wave > 0) return;
 #pragma unroll 1
-        for (int w = 0; w < OWN - 1; ++w) {
+        for (int w = 0; w < WAVES - 1; ++w) {
             const float *from = others + w * (DP * 32 + 64);
 #pragma unroll
             for (int o = 0; o < DP / 32; ++o)
