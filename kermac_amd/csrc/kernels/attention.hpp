@@ -183,20 +183,34 @@ typedef int att_s32x4 __attribute__((ext_vector_type(4)));
 // The rows of a tile in memory: rows 0 .. rows - 1 of base, `width` elements each, `stride` apart; what lies outside reads as zero without a branch
 // per load.
 template <typename T>
-__device__ __forceinline__ att_s32x4 att_descriptor(const T *base, int step, int rows, int width)
+__device__ __forceinline__ att_s32x4 att_descriptor(att_u64 address, int step, int rows, int width)
 {
     const int bytes = rows > 0 ? (rows - 1) * step + width * static_cast<int>(sizeof(T)) : 0;
-    const att_u64 address = reinterpret_cast<att_u64>(base);
     return att_s32x4{__builtin_amdgcn_readfirstlane(static_cast<int>(address)), __builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32) & 0xffff),
                      __builtin_amdgcn_readfirstlane(bytes), ATT_BUFFER_FORMAT};
 }
 
-// 4 bytes per lane from memory straight into LDS: lane l's to to + 4 l.
-__device__ __forceinline__ void att_load_words(const float *from, const float *to)
+// An address that is the same in all lanes, in scalar registers.
+template <typename T>
+__device__ __forceinline__ att_u64 att_uniform(const T *p)
+{
+    const att_u64 address = reinterpret_cast<att_u64>(p);
+    const unsigned low = __builtin_amdgcn_readfirstlane(static_cast<int>(address)), high = __builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32));
+    return static_cast<att_u64>(high) << 32 | low;
+}
+
+template <typename T>
+__device__ __forceinline__ unsigned att_lds_address(const T *p)
+{
+    return static_cast<unsigned>(reinterpret_cast<size_t>((const __attribute__((address_space(3))) T *)p));
+}
+
+// 4 bytes per lane from memory straight into LDS: lane l's to the address `to` + 4 l.
+__device__ __forceinline__ void att_load_words(const float *from, unsigned to)
 {
     typedef const __attribute__((address_space(1))) float *global_float;
-    const unsigned lds = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(reinterpret_cast<size_t>((const __attribute__((address_space(3))) float *)to)));
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"((global_float)from), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
+                 : : "v"((global_float)from), "s"(__builtin_amdgcn_readfirstlane(to)) : "memory", "m0");
 }
 
 // At most IN_FLIGHT loads are outstanding, and the compiler knows: it would otherwise wait, in front of the first use of a register that was loaded
@@ -232,20 +246,27 @@ struct AttTile {
     static_assert(THREADS % SLOTS == 0 && ROWS % ROW_STEP == 0 && PER_THREAD > 0, "whole rows per step");
     att_u32x4 held[DIRECT ? 1 : PER_THREAD];
 
+    // DIRECT, from a tile's descriptor
+    __device__ __forceinline__ void begin_at(att_s32x4 from, int step, int width, att_lds_byte *tile, int thread)
+    {
+        constexpr int SIZE = static_cast<int>(sizeof(T));
+        const int row = thread / SLOTS;
+        const unsigned to = att_lds_address(tile) + __builtin_amdgcn_readfirstlane(thread / 64) * (64 / SLOTS * Lds::STRIDE);
+#pragma unroll
+        for (int j = 0; j < PER_THREAD; ++j) {
+            const int r = row + j * ROW_STEP, at = (16 * (thread % SLOTS) ^ Lds::swizzle(row) ^ Lds::swizzle(j * ROW_STEP)) / SIZE;
+            const unsigned offset = at < width ? static_cast<unsigned>(r * step + at * SIZE) : 0x80000000u;
+            const unsigned lds = __builtin_amdgcn_readfirstlane(to + j * ROW_STEP * Lds::STRIDE);
+            asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(offset), "s"(from), "s"(lds) : "memory", "m0");
+        }
+    }
+
     __device__ __forceinline__ void begin(const T *base, i64 stride, int rows, int width, att_lds_byte *tile, int thread)
     {
         constexpr int SIZE = static_cast<int>(sizeof(T));
         const int row = thread / SLOTS, step = static_cast<int>(stride) * SIZE;
         if constexpr (DIRECT) {
-            const att_s32x4 from = att_descriptor(base, step, rows < ROWS ? rows : ROWS, width);
-            const unsigned to = static_cast<unsigned>(reinterpret_cast<size_t>((__attribute__((address_space(3))) att_lds_byte *)tile));
-#pragma unroll
-            for (int j = 0; j < PER_THREAD; ++j) {
-                const int r = row + j * ROW_STEP, at = (16 * (thread % SLOTS) ^ Lds::swizzle(row) ^ Lds::swizzle(j * ROW_STEP)) / SIZE;
-                const unsigned offset = at < width ? static_cast<unsigned>(r * step + at * SIZE) : 0x80000000u;
-                const unsigned lds = __builtin_amdgcn_readfirstlane(to + (thread / 64 * (64 / SLOTS) + j * ROW_STEP) * Lds::STRIDE);
-                asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(offset), "s"(from), "s"(lds) : "memory", "m0");
-            }
+            begin_at(att_descriptor<T>(reinterpret_cast<att_u64>(base), step, rows < ROWS ? rows : ROWS, width), step, width, tile, thread);
         } else if constexpr (ALIGNED) {
             const int some = rows < ROWS ? rows : ROWS, bytes = some > 0 ? (some - 1) * step + width * SIZE : 0;
             const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, bytes, ATT_BUFFER_FORMAT);

@@ -35,8 +35,8 @@ __device__ __forceinline__ float att_weight(float s, float scale_log2, float lse
 __device__ __forceinline__ float att_lse2(float lse) { return lse == -__builtin_inff() ? __builtin_inff() : lse * ATT_LOG2_E; }
 
 // Two products of 32 rows of two tiles in LDS with operands of the wave's own, by turns: s (scores) and ds (gradients of the result times values).
-// Between the matrix instructions, with VECTOR, the vector work of the scores before: `quad(q)` makes the weights and gradients of
-// registers 4 q .. 4 q + 3.
+// Between the matrix instructions, with VECTOR, the vector work of the scores before: `quad(q)` makes the weights of registers
+// 4 q .. 4 q + 3.
 template <typename T, int DP, bool VECTOR, typename Quad>
 __device__ __forceinline__ void att_two_scores(att_f32x16 &s, att_f32x16 &ds, const att_lds_byte *s_tile, const att_vec8<T> (&s_own)[DP / 16],
                                                const att_lds_byte *ds_tile, const att_vec8<T> (&ds_own)[DP / 16], int lane, Quad quad)
@@ -65,7 +65,7 @@ __device__ __forceinline__ void att_two_scores(att_f32x16 &s, att_f32x16 &ds, co
         if (VECTOR)
 #pragma unroll
             for (int q = 4 * i / ALL; q < 4 * (i + 1) / ALL; ++q) quad(q);
-        att_order<DP, 2 * AT_ONCE * G::READS_ROW, 2 * AT_ONCE * G::MMAS, VECTOR ? (sizeof(T) == 4 ? 1 : 4 * 4 / ALL + 1) : 0>();
+        att_order<DP, 2 * AT_ONCE * G::READS_ROW, 2 * AT_ONCE * G::MMAS, VECTOR ? (sizeof(T) == 4 ? 1 : 48 / (2 * G::STEPS) + 1) : 0>();
         att_region<DP>();
     }
 }
@@ -268,10 +268,13 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
     constexpr int RT = Shape::ROWS, TILE = RT * AttLds<T, DP>::STRIDE;
     typedef AttTile<T, DP, RT, 256, ALIGNED> Tile;
     constexpr int BUFFERS = Tile::DIRECT || Shape::DEEP == 2 ? Shape::DEEP : 3;
-    constexpr int AHEAD = BUFFERS == 2 ? 1 : BUFFERS - 2;              // tiles on their way behind the two in use
+    constexpr bool OVERLAP = DP <= 128;                                 // (wider rows leave no registers for the scores of two tiles)
+    constexpr int AHEAD = BUFFERS - (OVERLAP ? 2 : 1);                  // tiles on their way behind those in use
+    static_assert(AHEAD > 0, "a tile on its way");
     constexpr int LOADS = 2 * Tile::PER_THREAD + 1;                     // of a wave for a tile
     __shared__ __attribute__((aligned(1024))) att_lds_byte lds[2 * BUFFERS * TILE];     // queries and gradients of the result
     __shared__ __attribute__((aligned(256))) float all_stats[BUFFERS][2 * RT];           // lse to base 2 and delta of a tile's rows
+    const unsigned stats_lds = att_lds_address(all_stats);
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int id = (blockIdx.x & 7) * (args.k_grid >> 3) + (blockIdx.x >> 3);
@@ -309,6 +312,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
     const float scale_log2 = args.scale_log2;
     const i64 part_first = split * per_split, part_last = part_first + per_split;
     const i64 rows_total = static_cast<i64>(args.l) * args.m * args.g * args.r;
+    bool ever_kept = false;
 
     for (int e = static_cast<int>(part_first / per_entry); e < entries && e * per_entry < part_last; ++e) {
         const int entry = key_entry + e;
@@ -316,31 +320,43 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
         const int count = static_cast<int>((part_last < (e + 1) * per_entry ? part_last - e * per_entry : per_entry) - first);
         const int length = att_length(keys, entry);
         if (!(att_kept_keys(keys, entry, first_key, length, lane) | att_kept_keys(keys, entry, first_key + 64, length, lane))) continue;
-        // (the gradient of a key that does not take part is cleared where it would enter the products: what the key holds may be anything)
+        // A key that does not take part has a column of the products of its own, whatever it holds: its gradient is set to zero at the end, unless another entry
+        // that shares it adds to it.
         const bool kept = exists && n < length && (!keys.mask || keys.mask[entry * keys.mask_ls + n * keys.mask_ns] != 0);
-        const unsigned keep = kept ? ~0u : 0u;
+        const bool clear = entries > 1 && !__all(kept);
+        ever_kept |= kept;
 
+        // What moves from tile to tile: addresses in scalar registers that grow by one of two steps.
         Tile next_q, next_d;
-        int head = first / tiles_m, m0 = first % tiles_m * RT, to = 0;          // of the next tile to load
-        // (behind the last tile: nothing is read)
-        const i64 q_ms = args.q_ms, q_hs = args.q_hs, d_ms = args.grad_out_ms, d_hs = args.grad_out_hs;
-        const T *q_entry = static_cast<const T *>(args.q) + entry * args.q_ls + g * args.r * q_hs;
-        const T *d_entry = static_cast<const T *>(args.grad_out) + entry * args.grad_out_ls + g * args.r * d_hs;
-        const float *stats_entry = args.stats + (static_cast<i64>(entry) * args.g + g) * args.r * args.m + (lane < RT ? 0 : rows_total) + lane % RT;
-        const float *stats_behind = args.stats + 2 * rows_total + (lane < RT ? 0 : 1);
+        constexpr int SIZE = static_cast<int>(sizeof(T));
         const int m = args.m, q_width = args.k, d_width = args.o;
-        int left = count;
+        int m0 = first % tiles_m * RT, to = 0, left = count;                    // of the next tile to load
+        const int head = g * args.r + first / tiles_m, last_m0 = (tiles_m - 1) * RT;
+        att_u64 q_at = att_uniform(static_cast<const T *>(args.q) + entry * args.q_ls + m0 * args.q_ms + head * args.q_hs);
+        att_u64 d_at = att_uniform(static_cast<const T *>(args.grad_out) + entry * args.grad_out_ls + m0 * args.grad_out_ms + head * args.grad_out_hs);
+        const i64 q_next = RT * args.q_ms * SIZE, q_wrap = (args.q_hs - last_m0 * args.q_ms) * SIZE;
+        const i64 d_next = RT * args.grad_out_ms * SIZE, d_wrap = (args.grad_out_hs - last_m0 * args.grad_out_ms) * SIZE;
+        const int q_step = static_cast<int>(args.q_ms) * SIZE, d_step = static_cast<int>(args.grad_out_ms) * SIZE;
+        const float *stats_at = args.stats + (static_cast<i64>(entry) * args.g * args.r + head) * m + m0 + (lane < RT ? 0 : rows_total) + lane % RT;
+        const float *const stats_behind = args.stats + 2 * rows_total + (lane < RT ? 0 : 1);
         auto begin = [&]() {
-            const int some = left > 0 ? m - m0 : 0;
+            const bool last = m0 == last_m0;
+            const int some = left <= 0 ? 0 : last ? m - last_m0 : RT;           // (behind the last tile: nothing is read)
             att_lds_byte *q_tile = lds + 2 * to * TILE;
-            next_q.begin(q_entry + m0 * q_ms + head * q_hs, q_ms, some, q_width, q_tile, threadIdx.x);
-            next_d.begin(d_entry + m0 * d_ms + head * d_hs, d_ms, some, d_width, q_tile + TILE, threadIdx.x);
+            if constexpr (Tile::DIRECT) {
+                next_q.begin_at(att_descriptor<T>(q_at, q_step, some, q_width), q_step, q_width, q_tile, threadIdx.x);
+                next_d.begin_at(att_descriptor<T>(d_at, d_step, some, d_width), d_step, d_width, q_tile + TILE, threadIdx.x);
+            } else {
+                next_q.begin(reinterpret_cast<const T *>(q_at), args.q_ms, some, q_width, q_tile, threadIdx.x);
+                next_d.begin(reinterpret_cast<const T *>(d_at), args.grad_out_ms, some, d_width, q_tile + TILE, threadIdx.x);
+            }
             // (all waves load the same: they count the same loads; rows that do not exist get the pair behind all others)
-            att_load_words(lane % RT < some ? stats_entry + static_cast<i64>(head) * m + m0 : stats_behind, all_stats[to]);
+            att_load_words(lane % RT < some ? stats_at : stats_behind, stats_lds + 8 * RT * to);
             --left;
-            m0 += RT;
-            head = m0 >= m ? head + 1 : head;
-            m0 = m0 >= m ? 0 : m0;
+            m0 = last ? 0 : m0 + RT;
+            q_at += last ? q_wrap : q_next;
+            d_at += last ? d_wrap : d_next;
+            stats_at += last ? m - last_m0 : RT;
             if (Tile::DIRECT) to = to + 1 == BUFFERS ? 0 : to + 1;
         };
         // The tile asked for longest ago has arrived; AHEAD - 1 others may be on their way.
@@ -359,24 +375,30 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
         auto then = [&]() { return now + 1 == BUFFERS ? 0 : now + 1; };
         att_f32x16 s_a, ds_a, s_b, ds_b;
         att_vec8<T> p[2], x[2];
-        auto make_quad = [&](const att_f32x16 &s, const att_f32x16 &ds, int q) {
-            const float *stats = all_stats[now];
-            const att_f32x4 lse2 = *reinterpret_cast<const att_f32x4 *>(stats + 8 * q + 4 * half);
-            const att_f32x4 delta = *reinterpret_cast<const att_f32x4 *>(stats + RT + 8 * q + 4 * half);
+        float weight[16];
+        auto make_weights = [&](const att_f32x16 &s, int q) {
+            const att_f32x4 lse2 = *reinterpret_cast<const att_f32x4 *>(all_stats[now] + 8 * q + 4 * half);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float weight = att_weight(s[4 * q + j], scale_log2, lse2[j]);
-                p[q / 2][4 * (q % 2) + j] = static_cast<T>(weight);
-                x[q / 2][4 * (q % 2) + j] = static_cast<T>(weight * (ds[4 * q + j] - delta[j]));
+                weight[4 * q + j] = att_weight(s[4 * q + j], scale_log2, lse2[j]);
+                p[q / 2][4 * (q % 2) + j] = static_cast<T>(weight[4 * q + j]);
             }
         };
-        auto products = [&]() {
-            const att_lds_byte *q_tile = lds + 2 * now * TILE, *d_tile = q_tile + TILE;
-            typedef unsigned words __attribute__((ext_vector_type(sizeof(att_vec8<T>) / 4)));
+        auto make_gradients = [&](const att_f32x16 &ds, int q) {
+            const att_f32x4 delta = *reinterpret_cast<const att_f32x4 *>(all_stats[now] + RT + 8 * q + 4 * half);
 #pragma unroll
-            for (int step = 0; step < 2; ++step) {
-                p[step] = __builtin_bit_cast(att_vec8<T>, __builtin_bit_cast(words, p[step]) & keep);
-                x[step] = __builtin_bit_cast(att_vec8<T>, __builtin_bit_cast(words, x[step]) & keep);
+            for (int j = 0; j < 4; ++j) x[q / 2][4 * (q % 2) + j] = static_cast<T>(weight[4 * q + j] * (ds[4 * q + j] - delta[j]));
+        };
+        auto products = [&](const att_f32x16 &ds) {
+            const att_lds_byte *q_tile = lds + 2 * now * TILE, *d_tile = q_tile + TILE;
+            if (clear) {
+                unsigned keep = kept ? ~0u : 0u;
+                asm volatile("" : "+v"(keep));              // (nothing of this is made in front of the branch)
+                typedef unsigned words __attribute__((ext_vector_type(sizeof(att_vec8<T>) / 4)));
+#pragma unroll
+                for (int step = 0; step < 2; ++step) p[step] = __builtin_bit_cast(att_vec8<T>, __builtin_bit_cast(words, p[step]) & keep);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) weight[i] = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, weight[i]) & keep);
             }
             // four steps of 16 rows: two of the gradients, two of the queries
             constexpr int ALL = 4 * G::COLUMN_GROUPS;
@@ -396,48 +418,70 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
                     att_f32x16 &to = step < 2 ? acc_v[G::COLUMNS * group + o] : acc_k[G::COLUMNS * group + o];
                     to = att_mma(f[i & 1][o], step < 2 ? p[step] : x[step - 2], to);
                 }
-                att_order<DP, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, 0>();
+                if (step < 2 && group == 0) {
+                    make_gradients(ds, 2 * step);
+                    make_gradients(ds, 2 * step + 1);
+                    att_order<DP, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, (G::MMAS > 1 ? 2 : 24 / G::COLUMNS)>();
+                } else {
+                    att_order<DP, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, 0>();
+                }
                 att_region<DP>();
             }
         };
-        auto turn = [&](const att_f32x16 &s, const att_f32x16 &ds, att_f32x16 &next_s, att_f32x16 &next_ds) {
-            if (BUFFERS > 2) begin();
-            const att_lds_byte *q_tile = lds + 2 * then() * TILE;
-            att_two_scores<T, DP, true>(next_s, next_ds, q_tile, key, q_tile + TILE, value, lane, [&](int q) { make_quad(s, ds, q); });
-            products();
-            if (BUFFERS == 2) {
-                __syncthreads();
-                begin();
-            }
+        auto next_tile = [&]() {
             finish();
             __syncthreads();
             now = then();
         };
+        auto turn = [&](const att_f32x16 &s, const att_f32x16 &ds, att_f32x16 &next_s, att_f32x16 &next_ds) {
+            begin();
+            const att_lds_byte *q_tile = lds + 2 * then() * TILE;
+            att_two_scores<T, DP, true>(next_s, next_ds, q_tile, key, q_tile + TILE, value, lane, [&](int q) { make_weights(s, q); });
+            products(ds);
+            next_tile();
+        };
 
         __syncthreads();                // an entry before this one is done with the buffers
 #pragma unroll 1
-        for (int i = 0; i < 1 + AHEAD; ++i) {
+        for (int i = 0; i < BUFFERS - 1; ++i) {
             begin();
             if (!Tile::DIRECT) finish();
         }
         att_wait_for_loads();
         __syncthreads();
-        att_two_scores<T, DP, false>(s_a, ds_a, lds, key, lds + TILE, value, lane, [](int) {});
-        for (int i = 1; i < count; i += 2) {
-            turn(s_a, ds_a, s_b, ds_b);
-            if (i + 1 < count) {
+        if constexpr (OVERLAP) {
+            att_two_scores<T, DP, false>(s_a, ds_a, lds, key, lds + TILE, value, lane, [](int) {});
+            int i = 1;
+            for (; i + 1 < count; i += 2) {
+                turn(s_a, ds_a, s_b, ds_b);
                 turn(s_b, ds_b, s_a, ds_a);
-            } else {
+            }
+            if (i < count) {
+                turn(s_a, ds_a, s_b, ds_b);
                 s_a = s_b;
                 ds_a = ds_b;
             }
-        }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) make_quad(s_a, ds_a, q);
-        products();
+            for (int q = 0; q < 4; ++q) make_weights(s_a, q);
+            products(ds_a);
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < count; ++i) {
+                begin();
+                const att_lds_byte *q_tile = lds + 2 * now * TILE;
+                att_two_scores<T, DP, false>(s_a, ds_a, q_tile, key, q_tile + TILE, value, lane, [](int) {});
+#pragma unroll
+                for (int q = 0; q < 4; ++q) make_weights(s_a, q);
+                products(ds_a);
+                next_tile();
+            }
+        }
         att_wait_for_loads();
     }
     if (!exists) return;
+    if (!ever_kept)
+#pragma unroll
+        for (int o = 0; o < DP / 32; ++o) acc_k[o] = acc_v[o] = att_f32x16{0};
     const i64 at = (static_cast<i64>(key_entry) * keys.n + n) * args.g + g;
     if (args.k_splits > 1) {
         const i64 slot = split * (static_cast<i64>(args.key_entries) * keys.n * args.g) + at;
