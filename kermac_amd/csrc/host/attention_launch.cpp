@@ -126,6 +126,7 @@ bool plan_job(kmc::AttentionJob *job, int first_segment, int last_segment, int64
 {
     job->first_segment = first_segment;
     job->last_segment = last_segment;
+    job->entries = static_cast<int>(entries);
     job->rows = static_cast<int>(rows);
     job->own_keys = rows <= ROWS_OF_OWN_KEYS;
     job->row_tiles = job->own_keys ? 1 : static_cast<int>((rows + ROWS_PER_WORKGROUP - 1) / ROWS_PER_WORKGROUP);

@@ -662,19 +662,19 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
     if (id >= job.workgroups) return;
     const int row_tile = id % job.row_tiles;
     id /= job.row_tiles;
-    int g, split;
+    int g, split, entry;
     if (job.own_keys) {             // the heads of the same tokens, which stand side by side in memory, at the same time
         g = id % args.g;
         id /= args.g;
         split = id % job.splits;
         id /= job.splits;
-    } else {
+        entry = id;
+    } else {                        // one head of all entries, whose lengths differ, on an XCD
         split = id % job.splits;
         id /= job.splits;
-        g = id % args.g;
-        id /= args.g;
+        entry = id % job.entries;
+        g = id / job.entries;
     }
-    const int entry = id;
 
     AttState<DP> state;
     att_vec8<T> query[DP / 16];

@@ -21,7 +21,7 @@ struct AttentionKeys {
 // A list of workgroups: (batch entry, head of keys, range of keys, tile of rows), the tile of rows fastest.
 struct AttentionJob {
     int first_segment, last_segment;
-    int rows, row_tiles, splits;
+    int entries, rows, row_tiles, splits;
     int slot;                               // of its first partial result
     int partial, own_keys;
     int workgroups, grid;                   // grid: workgroups rounded up to a multiple of the 8 XCDs

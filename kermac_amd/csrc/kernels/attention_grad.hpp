@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     id /= args.q_row_tiles;
     const int split = id % args.q_splits;
     id /= args.q_splits;
-    const int g = id % args.g, entry = id / args.g;
+    const int entry = id % args.l, g = id / args.l;             // one head of all entries, whose lengths differ, on an XCD
 
     const int rows = args.m * args.r;
     const int first_row = row_tile * 128 + 32 * wave, row = first_row + lane % 32;
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
     id /= args.key_tiles;
     const int split = id % args.k_splits;
     id /= args.k_splits;
-    const int g = id % args.g, key_entry = id / args.g;
+    const int key_entry = id % args.key_entries, g = id / args.key_entries;
 
     const AttentionKeys &keys = args.keys;
     const int first_key = key_tile * 128, n = first_key + 32 * wave + lane % 32;
