@@ -467,7 +467,7 @@ typedef struct kmc_attention_params {
     int32_t l, m, n;            /* batch entries, queries and keys of each */
     int32_t h, g;               /* heads of queries, heads of keys and values; h a multiple of g */
     int32_t k, o;               /* features of queries and keys, of values; 1 .. 256 */
-    float scale;
+    float scale;                /* of magnitude 2e38 at most */
     const void *q; int64_t q_ls, q_ms, q_hs;                    /* [l, m, h, k] */
     const void *key; int64_t key_ls, key_ns, key_gs;            /* [l, n, g, k] */
     const void *value; int64_t value_ls, value_ns, value_gs;    /* [l, n, g, o] */

@@ -3,7 +3,8 @@
 ``import kermac_amd as kermac`` gives the reference's names:
 ``cdist``, ``cdist_grad``, ``run_kernel``, ``pre_compile_descriptors``,
 ``KernelDescriptor``, the enums, the predefined descriptors, ``ModuleCache``
-and the helpers of ``common``.
+and the helpers of ``common``.  Beside them stands attention, a kernel matrix whose rows are
+divided by their sums times values: ``cross_attention``, ``cross_attention_grad``, ``prefix_attention``.
 """
 from .common import (Alignment, CudaTimer, FillMode, Majorness, PyTorchStreamWrapper, TensorStats, ceil_div,
                      merge_batch_size, tensor_stats)
