@@ -392,7 +392,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[q / 2][4 * (q % 2) + j] = static_cast<T>(weight[4 * q + j] * (ds[4 * q + j] - delta[j]));
         };
-        auto products = [&](const att_f32x16 &ds) {
+        auto products = [&](att_f32x16 &ds) {
             const att_lds_byte *q_tile = lds + 2 * now * TILE, *d_tile = q_tile + TILE;
             if (clear) {
                 unsigned keep = kept ? ~0u : 0u;
@@ -401,7 +401,11 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
 #pragma unroll
                 for (int step = 0; step < 2; ++step) p[step] = __builtin_bit_cast(att_vec8<T>, __builtin_bit_cast(words, p[step]) & keep);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) weight[i] = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, weight[i]) & keep);
+                for (int i = 0; i < 16; ++i) {
+                    const float w = weight[i], d = ds[i];               // (of an element of a vector, the builtin takes the first)
+                    weight[i] = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, w) & keep);
+                    ds[i] = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, d) & keep);
+                }
             }
             // four steps of 16 rows: two of the gradients, two of the queries
             constexpr int ALL = 4 * G::COLUMN_GROUPS;
@@ -436,7 +440,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
             __syncthreads();
             now = then();
         };
-        auto turn = [&](const att_f32x16 &s, const att_f32x16 &ds, att_f32x16 &next_s, att_f32x16 &next_ds) {
+        auto turn = [&](const att_f32x16 &s, att_f32x16 &ds, att_f32x16 &next_s, att_f32x16 &next_ds) {
             begin();
             const att_lds_byte *q_tile = lds + 2 * then() * TILE;
             att_two_scores<T, DP, true>(next_s, next_ds, q_tile, key, q_tile + TILE, value, lane, [&](int q) { make_weights(s, q); });

@@ -166,3 +166,22 @@ def test_against_differences(device):
         got = (grads[which].cpu().double() * direction).sum()
         allowed = (bounds[which] * direction.abs()).sum() + (whole - half).abs() + 1e-11 * weights.abs().sum()
         assert (got - half).abs() <= allowed, (which, got.item(), half.item(), allowed.item())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("K, O", [(64, 64), (128, 96), (200, 256), (33, 64)])
+@pytest.mark.parametrize("kind", ["lengths", "holes", "both"])
+def test_what_takes_no_part_may_hold_anything(device, dtype, K, O, kind):
+    """Keys left out of every entry hold infinities and NaN, for entries with keys of their own and for a source that they share; those that one
+    entry leaves out and another one meets are numbers.  M and the heads end inside tiles and parts."""
+    L, M, N = 3, 45, 300
+    lengths = torch.tensor([290, 129, 7], dtype=torch.int32) if kind != "holes" else None
+    mask = torch.rand(L, N, generator=torch.Generator().manual_seed(8)) < 0.4 if kind != "lengths" else None
+    keep = reference.keep_of(L, 1, N, lengths, mask)[:, 0]
+    for key_batch in (L, 1):
+        q, k, v = operands(L, M, N, 6, 2, K, O, dtype, device, key_batch=key_batch)
+        unused = ~keep if key_batch == L else ~keep.any(0, keepdim=True)
+        k[unused], v[unused] = math.nan, math.inf
+        masks = dict(key_lengths=None if lengths is None else lengths.to(device), key_mask=None if mask is None else mask.to(device))
+        grads = check(q, k, v, f"{kind} of {key_batch}", **masks)
+        assert grads[1].cpu()[unused].eq(0).all() and grads[2].cpu()[unused].eq(0).all()
