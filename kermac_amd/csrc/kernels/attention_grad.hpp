@@ -37,18 +37,18 @@ __device__ __forceinline__ float att_lse2(float lse) { return lse == -__builtin_
 // Two products of 32 rows of two tiles in LDS with operands of the wave's own, by turns: s (scores) and ds (gradients of the result times values).
 // Between the matrix instructions, with VECTOR, the vector work of the scores before: `quad(q)` makes the weights of registers
 // 4 q .. 4 q + 3.
-template <typename T, int DP, bool VECTOR, typename Quad>
+template <typename T, int DP, bool VECTOR, bool BOTH = true, typename Quad>
 __device__ __forceinline__ void att_two_scores(att_f32x16 &s, att_f32x16 &ds, const att_lds_byte *s_tile, const att_vec8<T> (&s_own)[DP / 16],
                                                const att_lds_byte *ds_tile, const att_vec8<T> (&ds_own)[DP / 16], int lane, Quad quad)
 {
     typedef AttGroups<T, DP> G;
-    constexpr int AT_ONCE = 2, ALL = G::STEPS / AT_ONCE;
+    constexpr int AT_ONCE = DP * sizeof(T) > 512 ? 1 : 2, ALL = G::STEPS / AT_ONCE;
     att_vec8<T> f[2][2 * AT_ONCE];
     auto read = [&](att_vec8<T> (&to)[2 * AT_ONCE], int i) {
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
             to[2 * j] = att_read_row<T, DP>(s_tile, 0, 16 * (AT_ONCE * i + j), lane);
-            to[2 * j + 1] = att_read_row<T, DP>(ds_tile, 0, 16 * (AT_ONCE * i + j), lane);
+            if (BOTH) to[2 * j + 1] = att_read_row<T, DP>(ds_tile, 0, 16 * (AT_ONCE * i + j), lane);
         }
     };
     read(f[0], 0);
@@ -60,7 +60,7 @@ __device__ __forceinline__ void att_two_scores(att_f32x16 &s, att_f32x16 &ds, co
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
             s = att_mma(f[i & 1][2 * j], s_own[AT_ONCE * i + j], s);
-            ds = att_mma(f[i & 1][2 * j + 1], ds_own[AT_ONCE * i + j], ds);
+            if (BOTH) ds = att_mma(f[i & 1][2 * j + 1], ds_own[AT_ONCE * i + j], ds);
         }
         if (VECTOR)
 #pragma unroll
@@ -263,17 +263,24 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
 // bounds it with 128 features is LDS: every wave reads each tile twice by rows and twice by columns, as long as its products take.  Waves with 64 keys
 // would halve that, and have no registers for it (3.4 ms, with spills whose reloads wait for the tiles on their way); a barrier after two tiles instead of
 // one changes nothing.  With 64 features it is the vector work: 8 x 1000 x 1500 keys at most x 16 heads 113 us.
-template <typename T, int DP, bool ALIGNED>
+//
+// In fp32, 32 keys and values of more than 128 features and their gradients are 512 registers by themselves.  There a launch makes one of the two gradients, and
+// the scores are computed twice (2 x 1000 x 1500 x 8 heads of 256: 814 us for both, 1180 in one launch with its spills).
+enum AttKeysPart { ATT_BOTH, ATT_GRAD_KEYS, ATT_GRAD_VALUES };
+
+template <typename T, int DP, bool ALIGNED, AttKeysPart PART>
 __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void attention_grad_keys(const AttentionGradArgs args)
 {
     typedef AttGradShape<T, DP> Shape;
     typedef AttGroups<T, DP> G;
     constexpr int RT = Shape::ROWS, TILE = RT * AttLds<T, DP>::STRIDE;
     typedef AttTile<T, DP, RT, 256, ALIGNED> Tile;
+    constexpr bool OF_KEYS = PART != ATT_GRAD_VALUES, OF_VALUES = PART != ATT_GRAD_KEYS;
     constexpr int BUFFERS = Tile::DIRECT || Shape::DEEP == 2 ? Shape::DEEP : 3;
     constexpr bool OVERLAP = DP <= 128;                                 // (wider rows leave no registers for the scores of two tiles)
     constexpr int AHEAD = BUFFERS - (OVERLAP ? 2 : 1);                  // tiles on their way behind those in use
     static_assert(AHEAD > 0, "a tile on its way");
+    static_assert(!OVERLAP || PART == ATT_BOTH, "a part walks one tile at a time");
     constexpr int LOADS = 2 * Tile::PER_THREAD + 1;                     // of a wave for a tile
     __shared__ __attribute__((aligned(1024))) att_lds_byte lds[2 * BUFFERS * TILE];     // queries and gradients of the result
     __shared__ __attribute__((aligned(256))) float all_stats[BUFFERS][2 * RT];           // lse to base 2 and delta of a tile's rows
@@ -300,7 +307,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
         if (args.query_factor != 1.0f)
 #pragma unroll
             for (int j = 0; j < 8; ++j) key[step][j] = static_cast<T>(static_cast<float>(key[step][j]) * args.query_factor);
-        value[step] = att_load8<T, ALIGNED>(v, 16 * step + 8 * half, args.o);
+        if (OF_KEYS) value[step] = att_load8<T, ALIGNED>(v, 16 * step + 8 * half, args.o);
     }
     att_wait_for_loads();
     att_f32x16 acc_k[DP / 32], acc_v[DP / 32];
@@ -408,16 +415,19 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
                 }
             }
             // four steps of 16 rows: two of the gradients, two of the queries
-            constexpr int ALL = 4 * G::COLUMN_GROUPS;
+            constexpr int FIRST = OF_VALUES ? 0 : 2 * G::COLUMN_GROUPS, ALL = OF_KEYS ? 4 * G::COLUMN_GROUPS : 2 * G::COLUMN_GROUPS;
+            if (!OF_VALUES)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) make_gradients(ds, q);
             att_vec8<T> f[2][G::COLUMNS];
             auto read = [&](att_vec8<T> (&to)[G::COLUMNS], int i) {
                 const int step = i / G::COLUMN_GROUPS;
                 att_read_columns<T, DP>(to, step < 2 ? d_tile : q_tile, 16 * (step % 2), i % G::COLUMN_GROUPS, lane);
             };
-            read(f[0], 0);
+            read(f[0], FIRST);
             att_region<DP>();
 #pragma unroll
-            for (int i = 0; i < ALL; ++i) {
+            for (int i = FIRST; i < ALL; ++i) {
                 const int step = i / G::COLUMN_GROUPS, group = i % G::COLUMN_GROUPS;
                 if (i + 1 < ALL) read(f[(i + 1) & 1], i + 1);
 #pragma unroll
@@ -425,7 +435,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
                     att_f32x16 &to = step < 2 ? acc_v[G::COLUMNS * group + o] : acc_k[G::COLUMNS * group + o];
                     to = att_mma(f[i & 1][o], step < 2 ? p[step] : x[step - 2], to);
                 }
-                if (step < 2 && group == 0) {
+                if (OF_KEYS && step < 2 && group == 0) {
                     make_gradients(ds, 2 * step);
                     make_gradients(ds, 2 * step + 1);
                     att_order<DP, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, (G::MMAS > 1 ? 2 : 24 / G::COLUMNS)>();
@@ -476,7 +486,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
             for (int i = 0; i < count; ++i) {
                 begin();
                 const att_lds_byte *q_tile = lds + 2 * now * TILE;
-                att_two_scores<T, DP, false>(s_a, ds_a, q_tile, key, q_tile + TILE, value, lane, [](int) {});
+                att_two_scores<T, DP, false, OF_KEYS>(s_a, ds_a, q_tile, key, q_tile + TILE, value, lane, [](int) {});
 #pragma unroll
                 for (int q = 0; q < 4; ++q) make_weights(s_a, q);
                 products(ds_a);
@@ -498,13 +508,13 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int column = 32 * o + att_row(i, half);
-                if (column < args.k) to_k[column] = acc_k[o][i];
-                if (column < args.o) to_v[column] = acc_v[o][i];
+                if (OF_KEYS && column < args.k) to_k[column] = acc_k[o][i];
+                if (OF_VALUES && column < args.o) to_v[column] = acc_v[o][i];
             }
         return;
     }
-    att_store_columns<T, DP, ALIGNED>(static_cast<T *>(args.grad_k) + at * args.k, acc_k, args.scale, args.k, half);
-    att_store_columns<T, DP, ALIGNED>(static_cast<T *>(args.grad_v) + at * args.o, acc_v, 1.0f, args.o, half);
+    if (OF_KEYS) att_store_columns<T, DP, ALIGNED>(static_cast<T *>(args.grad_k) + at * args.k, acc_k, args.scale, args.k, half);
+    if (OF_VALUES) att_store_columns<T, DP, ALIGNED>(static_cast<T *>(args.grad_v) + at * args.o, acc_v, 1.0f, args.o, half);
 }
 
 // The parts of a cut gradient, added in their order.
