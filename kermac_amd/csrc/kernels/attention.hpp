@@ -56,6 +56,13 @@ __device__ __forceinline__ att_f32x16 att_mma(att_vec8<float> a, att_vec8<float>
 // Register i of a 32 x 32 result holds row att_row(i, half wave) of column lane % 32.
 __device__ __forceinline__ constexpr int att_row(int i, int half) { return 8 * (i / 4) + 4 * half + i % 4; }
 
+// Whether bit att_row(i, half) of `rows`, the same in all lanes, is set: a mask in scalar registers, so that a selection is one vector instruction.
+__device__ __forceinline__ bool att_has_row(unsigned rows, int i)
+{
+    const int low = static_cast<int>(rows << (31 - att_row(i, 0))) >> 31, high = static_cast<int>(rows << (31 - att_row(i, 1))) >> 31;
+    return __builtin_amdgcn_inverse_ballot_w64(static_cast<att_u64>(static_cast<unsigned>(high)) << 32 | static_cast<unsigned>(low));
+}
+
 // The sum and the maximum of a value over the two lanes of a column.
 __device__ __forceinline__ float att_sum_of_halves(float x)
 {
@@ -244,10 +251,13 @@ struct AttTile {
     static constexpr int ROW_STEP = THREADS / SLOTS;
     static constexpr int PER_THREAD = ROWS / ROW_STEP;                  // loads of a thread
     static_assert(THREADS % SLOTS == 0 && ROWS % ROW_STEP == 0 && PER_THREAD > 0, "whole rows per step");
+    static_assert(ROW_STEP <= 32, "has_row shifts 32 bits");
     att_u32x4 held[DIRECT ? 1 : PER_THREAD];
 
+    static __device__ __forceinline__ bool has_row(att_u64 kept, int row, int j) { return static_cast<unsigned>(kept >> (j * ROW_STEP)) >> row & 1; }
+
     // DIRECT, from a tile's descriptor
-    __device__ __forceinline__ void begin_at(att_s32x4 from, int step, int width, att_lds_byte *tile, int thread)
+    __device__ __forceinline__ void begin_at(att_s32x4 from, int step, int width, att_lds_byte *tile, int thread, att_u64 kept = ~0ull)
     {
         constexpr int SIZE = static_cast<int>(sizeof(T));
         const int row = thread / SLOTS;
@@ -255,18 +265,19 @@ struct AttTile {
 #pragma unroll
         for (int j = 0; j < PER_THREAD; ++j) {
             const int r = row + j * ROW_STEP, at = (16 * (thread % SLOTS) ^ Lds::swizzle(row) ^ Lds::swizzle(j * ROW_STEP)) / SIZE;
-            const unsigned offset = at < width ? static_cast<unsigned>(r * step + at * SIZE) : 0x80000000u;
+            const unsigned offset = at < width && has_row(kept, row, j) ? static_cast<unsigned>(r * step + at * SIZE) : 0x80000000u;
             const unsigned lds = __builtin_amdgcn_readfirstlane(to + j * ROW_STEP * Lds::STRIDE);
             asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(offset), "s"(from), "s"(lds) : "memory", "m0");
         }
     }
 
-    __device__ __forceinline__ void begin(const T *base, i64 stride, int rows, int width, att_lds_byte *tile, int thread)
+    // Rows whose bit in `kept` is not set become zeros: nothing is read of them.
+    __device__ __forceinline__ void begin(const T *base, i64 stride, int rows, int width, att_lds_byte *tile, int thread, att_u64 kept = ~0ull)
     {
         constexpr int SIZE = static_cast<int>(sizeof(T));
         const int row = thread / SLOTS, step = static_cast<int>(stride) * SIZE;
         if constexpr (DIRECT) {
-            begin_at(att_descriptor<T>(reinterpret_cast<att_u64>(base), step, rows < ROWS ? rows : ROWS, width), step, width, tile, thread);
+            begin_at(att_descriptor<T>(reinterpret_cast<att_u64>(base), step, rows < ROWS ? rows : ROWS, width), step, width, tile, thread, kept);
         } else if constexpr (ALIGNED) {
             const int some = rows < ROWS ? rows : ROWS, bytes = some > 0 ? (some - 1) * step + width * SIZE : 0;
             const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, bytes, ATT_BUFFER_FORMAT);
@@ -274,7 +285,7 @@ struct AttTile {
             unsigned offset = at < width ? static_cast<unsigned>(row * step + at * SIZE) : 0x80000000u;
 #pragma unroll
             for (int j = 0; j < PER_THREAD; ++j) {
-                held[j] = __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0);
+                held[j] = __builtin_amdgcn_raw_buffer_load_b128(from, has_row(kept, row, j) ? offset : 0x80000000u, 0, 0);
                 offset += ROW_STEP * step;
             }
         } else {
@@ -282,7 +293,7 @@ struct AttTile {
 #pragma unroll
             for (int j = 0; j < PER_THREAD; ++j) {
                 held[j] = att_u32x4{0, 0, 0, 0};
-                if (row + j * ROW_STEP < rows) held[j] = att_load16<T, false>(p, thread % SLOTS * Lds::PIECE, width);
+                if (row + j * ROW_STEP < rows && has_row(kept, row, j)) held[j] = att_load16<T, false>(p, thread % SLOTS * Lds::PIECE, width);
                 p += ROW_STEP * stride;
             }
         }
@@ -302,29 +313,25 @@ struct AttTile {
     }
 };
 
-// Rows of a tile in LDS whose bit in `kept` is not set become zeros.  Between barriers.
-template <typename T, int DP, int ROWS, int THREADS>
-__device__ __forceinline__ void att_clear(att_lds_byte *tile, att_u64 kept, int thread)
-{
-    typedef AttLds<T, DP> Lds;
-    constexpr int PIECES = DP / Lds::PIECE;
-    for (int i = thread; i < ROWS * PIECES; i += THREADS)
-        if (!(kept >> (i / PIECES) & 1)) *reinterpret_cast<att_u32x4 *>(tile + Lds::offset(i / PIECES, i % PIECES)) = att_u32x4{0, 0, 0, 0};
-}
-
 // The low `count` bits, count clamped to 0 .. 64.
 __device__ __forceinline__ att_u64 att_low_bits(int count)
 {
     return count >= 64 ? ~0ull : count <= 0 ? 0ull : (1ull << count) - 1;
 }
 
+// Not 0 if key n0 + lane exists and takes part.  Asked for a tile ahead: a wait for it in front of every tile takes as long as the tile's products do.
+__device__ __forceinline__ int att_ask_kept(const AttentionKeys &keys, int entry, int n0, int end, int lane)
+{
+    const int n = n0 + lane;
+    int kept = n < end;
+    if (kept && keys.mask) kept = keys.mask[entry * keys.mask_ls + n * keys.mask_ns];
+    return kept;
+}
+
 // One bit per key n0 .. n0 + 63: the key exists and takes part.  The same in all waves of a workgroup.
 __device__ __forceinline__ att_u64 att_kept_keys(const AttentionKeys &keys, int entry, int n0, int end, int lane)
 {
-    const int n = n0 + lane;
-    bool kept = n < end;
-    if (kept && keys.mask) kept = keys.mask[entry * keys.mask_ls + n * keys.mask_ns] != 0;
-    return __ballot(kept);
+    return __ballot(att_ask_kept(keys, entry, n0, end, lane) != 0);
 }
 
 __device__ __forceinline__ int att_length(const AttentionKeys &keys, int entry)
@@ -432,26 +439,37 @@ __device__ __forceinline__ float att_scores(att_f32x16 (&s)[KT / 32], const att_
     return top;
 }
 
-// Masks a tile's scores (`kept` has a bit per key for this lane's row) and, where they pass the wave's base by 2^8, moves it to the largest, whose weight is
+// Masks a tile's scores (`kept` has a bit per key, the same in all lanes; with `causal`, this lane's row meets the first `limit` of them only) and, where they pass the wave's base by 2^8, moves it to the largest, whose weight is
 // then exactly 1 (a row of one key gets its value without a rounding).  What was made below the old base is rescaled: output and sum, and `weights`
 // that wait for their product and are rounded once more.
 template <typename T, int DP, int KT>
 __device__ __forceinline__ void att_rebase(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], att_f32x16 (&s)[KT / 32], float top, float scale_log2, att_u64 kept,
-                                           int lane)
+                                           bool causal, int limit, int lane)
 {
     const att_u64 all = KT == 64 ? ~0ull : (1ull << KT) - 1;
-    if (!__all((kept & all) == all)) {
+    if ((kept & all) != all) {
         att_rare();
         top = -__builtin_inff();
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b) {
-            const unsigned mine = static_cast<unsigned>(kept >> (32 * b)) >> (4 * (lane >> 5));
+            const unsigned rows = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(kept >> (32 * b)));
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[b][i] = mine >> att_row(i, 0) & 1 ? s[b][i] : -__builtin_inff();
+                s[b][i] = att_has_row(rows, i) ? s[b][i] : -__builtin_inff();
                 top = fmaxf(top, s[b][i]);
             }
         }
+    }
+    if (causal && !__all(limit >= KT)) {
+        att_rare();
+        top = -__builtin_inff();
+#pragma unroll
+        for (int b = 0; b < KT / 32; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[b][i] = 32 * b + att_row(i, 0) < limit - 4 * (lane >> 5) ? s[b][i] : -__builtin_inff();
+                top = fmaxf(top, s[b][i]);
+            }
     }
     top = att_max_of_halves(top) * scale_log2;
     if (!__all(top <= state.base + ATT_HEADROOM)) {
@@ -692,7 +710,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
         for (int segment = job.first_segment; segment < job.last_segment; ++segment) {
             const AttentionKeys &keys = args.keys[segment];
             const i64 k_stride = keys.k_ns, v_stride = keys.v_ns;
-            const bool masked = keys.mask != nullptr;
+            const bool masked = keys.mask != nullptr, causal = keys.causal;
             const int length = att_length(keys, entry);
             int begin, end;
             att_range(length, KT, split, job.splits, &begin, &end);
@@ -720,19 +738,18 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
             const int k_width = args.k, v_width = args.o;
             int now = 0;                                // which of two tiles
             auto ask_keys = [&](int n, int slot) { next_k.begin(k + n * k_stride, k_stride, end - n, k_width, key_ring + slot * TILE, threadIdx.x); };
-            auto ask = [&](int n) {
+            auto ask = [&](int n, att_u64 kept) {
                 if (n + KT < end) ask_keys(n + KT, now ^ 1);
-                next_v.begin(v + n * v_stride, v_stride, end - n, v_width, value_ring + now * TILE, threadIdx.x);
+                if (masked) {
+                    next_v.begin(v + n * v_stride, v_stride, end - n, v_width, value_ring + now * TILE, threadIdx.x, kept);
+                } else {
+                    next_v.begin(v + n * v_stride, v_stride, end - n, v_width, value_ring + now * TILE, threadIdx.x);
+                }
             };
-            auto got = [&](int n, att_u64 kept) {       // the keys of the next tile and the values of this one have arrived
+            auto got = [&](int n) {                     // the keys of the next tile and the values of this one have arrived
                 if (n + KT < end) next_k.finish(key_ring + (now ^ 1) * TILE, threadIdx.x);
                 next_v.finish(value_ring + now * TILE, threadIdx.x);
                 __syncthreads();
-                if (masked && kept != ~0ull) {
-                    att_rare();
-                    att_clear<T, DP, KT, THREADS>(value_ring + now * TILE, kept, threadIdx.x);
-                    __syncthreads();
-                }
                 now ^= 1;
             };
             __syncthreads();                            // a segment before this one is done with the buffers
@@ -740,21 +757,29 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
             next_k.finish(key_ring, threadIdx.x);
             __syncthreads();
             auto rebase = [&](int n, att_u64 kept) {
-                att_rebase<T, DP, KT>(state, weights, s, top, scale_log2, kept & att_low_bits(limit - n), lane);
+                att_rebase<T, DP, KT>(state, weights, s, top, scale_log2, kept, causal, limit - n, lane);
                 base = att_finite_base(state.base);
             };
-            att_u64 kept = masked ? att_kept_keys(keys, entry, begin, end, lane) : att_low_bits(end - begin);
-            ask(begin);
+            int next_kept = 0;
+            auto kept_keys = [&](int n) {
+                if (!masked) return att_low_bits(end - n);
+                const att_u64 kept = __ballot(next_kept != 0);
+                next_kept = n + KT < end ? att_ask_kept(keys, entry, n + KT, end, lane) : 0;
+                return kept;
+            };
+            if (masked) next_kept = att_ask_kept(keys, entry, begin, end, lane);
+            att_u64 kept = kept_keys(begin);
+            ask(begin, kept);
             if (works) {
                 top = att_scores<T, DP, KT>(s, query, key_ring, lane);
                 rebase(begin, kept);
 #pragma unroll
                 for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, scale_log2, base);
             }
-            got(begin, kept);
+            got(begin);
             for (int n = begin + KT; n < end; n += KT) {
-                kept = masked ? att_kept_keys(keys, entry, n, end, lane) : att_low_bits(end - n);
-                ask(n);
+                kept = kept_keys(n);
+                ask(n, kept);
                 if (works) {
                     const att_lds_byte *values = value_ring + (now ^ 1) * TILE;
                     top = att_scores<T, DP, KT>(s, query, key_ring + now * TILE, lane);
@@ -762,7 +787,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                     rebase(n, kept);
                     att_add_values<T, DP, KT, true>(state, weights, values, first, s, scale_log2, base, lane);
                 }
-                got(n, kept);
+                got(n);
             }
             if (works) {
                 const att_lds_byte *values = value_ring + (now ^ 1) * TILE;
@@ -790,14 +815,25 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
             static_assert(TURNS || !Tile::DIRECT, "the next tile waits in registers");
             Tile next_k, next_v;
             auto ask_keys = [&](i64 n) { next_k.begin(k + n * keys.k_ns, keys.k_ns, end - static_cast<int>(n), args.k, key_tile, lane); };
-            auto ask_values = [&](i64 n) { next_v.begin(v + n * keys.v_ns, keys.v_ns, end - static_cast<int>(n), args.o, value_tile, lane); };
+            auto ask_values = [&](i64 n, att_u64 kept) {
+                if (keys.mask) {
+                    next_v.begin(v + n * keys.v_ns, keys.v_ns, end - static_cast<int>(n), args.o, value_tile, lane, kept);
+                } else {
+                    next_v.begin(v + n * keys.v_ns, keys.v_ns, end - static_cast<int>(n), args.o, value_tile, lane);
+                }
+            };
             i64 n = begin + wave * KT;
+            auto ask_kept = [&](i64 n) { return n < end ? att_ask_kept(keys, entry, static_cast<int>(n), end, lane) : 0; };
+            att_u64 kept = __ballot(ask_kept(n) != 0);
+            int next_kept = ask_kept(n + KT * WAVES);
             if (!TURNS && n < end) {
                 ask_keys(n);
-                ask_values(n);
+                ask_values(n, kept);
             }
             for (; n < end; n += KT * WAVES) {
-                const att_u64 kept = att_kept_keys(keys, entry, static_cast<int>(n), end, lane);
+                const i64 at = n + KT * WAVES;
+                const att_u64 then_kept = __ballot(next_kept != 0);
+                next_kept = ask_kept(at + KT * WAVES);
                 att_f32x16 s[KT / 32];
                 att_vec8<T> weights[KT / 16] = {}, first[AttGroups<T, DP>::COLUMNS];
                 float top;
@@ -811,29 +847,25 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                     top = att_scores<T, DP, KT>(s, query, key_tile, lane);
                     att_wave_sync();
                     att_wait_for_reads();
-                    ask_values(n);
+                    ask_values(n, kept);
                 }
                 next_v.finish(value_tile, lane);
                 att_wave_sync();
-                if (keys.mask && (kept & 0xffffffffull) != 0xffffffffull) {
-                    att_clear<T, DP, KT, 64>(value_tile, kept, lane);
-                    att_wave_sync();
-                }
                 if (!TURNS) {
-                    const i64 at = n + KT * WAVES;
                     if (at < end) {
                         ask_keys(at);
-                        ask_values(at);
+                        ask_values(at, then_kept);
                     }
                     top = att_scores<T, DP, KT>(s, query, key_tile, lane);
                 }
-                att_rebase<T, DP, KT>(state, weights, s, top, args.scale_log2, kept & att_low_bits(limit - static_cast<int>(n)), lane);
+                att_rebase<T, DP, KT>(state, weights, s, top, args.scale_log2, kept, keys.causal, limit - static_cast<int>(n), lane);
                 const float base = att_finite_base(state.base);
 #pragma unroll
                 for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, args.scale_log2, base);
                 att_read_columns<T, DP>(first, value_tile, 0, 0, lane);
                 att_add_values<T, DP, KT, false>(state, weights, value_tile, first, s, 0.0f, base, lane);
                 att_wave_sync();
+                kept = then_kept;
             }
         }
         // join the waves: sums and outputs below one common maximum, added in the order of the waves

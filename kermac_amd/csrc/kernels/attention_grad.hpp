@@ -131,16 +131,11 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
         // Few keys: delta from the rounded result would be off by as much as ds is large, so it is summed from the weights themselves,
         // which are normalised again while they are at hand (a single key's weight is exactly 1, its ds exactly 0).
         const att_u64 kept = att_kept_keys(keys, entry, begin, end, lane);
-        next_k.begin(k, keys.k_ns, end, args.k, lds, threadIdx.x);
-        next_v.begin(v, keys.v_ns, end, args.o, lds + TILE, threadIdx.x);
+        next_k.begin(k, keys.k_ns, end, args.k, lds, threadIdx.x, kept);
+        next_v.begin(v, keys.v_ns, end, args.o, lds + TILE, threadIdx.x, kept);
         next_k.finish(lds, threadIdx.x);
         next_v.finish(lds + TILE, threadIdx.x);
         __syncthreads();
-        if (keys.mask && kept != ~0ull) {
-            att_clear<T, DP, KT, 256>(lds, kept, threadIdx.x);
-            att_clear<T, DP, KT, 256>(lds + TILE, kept, threadIdx.x);
-            __syncthreads();
-        }
         float total = 0.0f, inner = 0.0f;
 #pragma unroll 1
         for (int b = 0; b < KT / 32; ++b) {
@@ -181,28 +176,31 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     const int k_width = args.k, v_width = args.o;
     const bool masked = keys.mask != nullptr;
     const float scale_log2 = args.scale_log2;
+    auto ask = [&](i64 n, att_lds_byte *to, att_u64 kept) {
+        const int some = end - static_cast<int>(n);
+        if (masked) {
+            next_k.begin(k + n * k_stride, k_stride, some, k_width, to, threadIdx.x, kept);
+            next_v.begin(v + n * v_stride, v_stride, some, v_width, to + TILE, threadIdx.x, kept);
+        } else {
+            next_k.begin(k + n * k_stride, k_stride, some, k_width, to, threadIdx.x);
+            next_v.begin(v + n * v_stride, v_stride, some, v_width, to + TILE, threadIdx.x);
+        }
+    };
+    auto ask_kept = [&](i64 n) { return masked && n < end ? att_ask_kept(keys, entry, static_cast<int>(n), end, lane) : 0; };
+    att_u64 kept = masked ? __ballot(ask_kept(begin) != 0) : att_low_bits(end - begin), then_kept;
+    int next_kept = ask_kept(static_cast<i64>(begin) + KT);
     if (begin < end) {
         __syncthreads();
-        next_k.begin(k + begin * k_stride, k_stride, end - begin, k_width, lds, threadIdx.x);
-        next_v.begin(v + begin * v_stride, v_stride, end - begin, v_width, lds + TILE, threadIdx.x);
+        ask(begin, lds, kept);
     }
-    for (int n = begin; n < end; n += KT, odd ^= 1) {
-        const att_u64 kept = masked ? att_kept_keys(keys, entry, n, end, lane) : att_low_bits(end - n);
+    for (int n = begin; n < end; n += KT, odd ^= 1, kept = then_kept) {
+        then_kept = masked ? __ballot(next_kept != 0) : att_low_bits(end - n - KT);
+        next_kept = ask_kept(static_cast<i64>(n) + 2 * KT);
         att_lds_byte *key_tile = lds + 2 * odd * TILE, *value_tile = key_tile + TILE;
         next_k.finish(key_tile, threadIdx.x);
         next_v.finish(value_tile, threadIdx.x);
         __syncthreads();
-        if (masked && kept != ~0ull) {
-            att_clear<T, DP, KT, 256>(key_tile, kept, threadIdx.x);
-            att_clear<T, DP, KT, 256>(value_tile, kept, threadIdx.x);
-            __syncthreads();
-        }
-        if (n + KT < end) {
-            const i64 next = n + KT;
-            att_lds_byte *to = lds + 2 * (odd ^ 1) * TILE;
-            next_k.begin(k + next * k_stride, k_stride, end - static_cast<int>(next), k_width, to, threadIdx.x);
-            next_v.begin(v + next * v_stride, v_stride, end - static_cast<int>(next), v_width, to + TILE, threadIdx.x);
-        }
+        if (n + KT < end) ask(n + KT, lds + 2 * (odd ^ 1) * TILE, then_kept);
         if (!works) continue;
         // (overlapping the blocks, as the keys' kernel does with its tiles, takes more registers than two waves per SIMD have: 1.77 instead of 1.53 ms at
         // 4 x 4096 x 4096 x 32 heads of 128)
@@ -220,9 +218,9 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
             const unsigned here = static_cast<unsigned>(kept >> (32 * b));
             if (here != ~0u) {
                 att_rare();
-                const unsigned mine = here >> (4 * half);
+                const unsigned rows = __builtin_amdgcn_readfirstlane(here);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) ds[i] = mine >> att_row(i, 0) & 1 ? ds[i] : 0.0f;
+                for (int i = 0; i < 16; ++i) ds[i] = att_has_row(rows, i) ? ds[i] : 0.0f;
             }
             x[0] = att_operand<T>(ds, 0);
             x[1] = att_operand<T>(ds, 1);
