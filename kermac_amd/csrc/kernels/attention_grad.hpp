@@ -138,7 +138,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
         __syncthreads();
         float total = 0.0f, inner = 0.0f;
 #pragma unroll 1
-        for (int b = 0; b < KT / 32; ++b) {
+        for (int b = 0; b < KT / 32 && 32 * b < end; ++b) {
             att_f32x16 s = {0}, ds = {0};
 #pragma unroll
             for (int step = 0; step < DP / 16; ++step) {
@@ -206,6 +206,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
         // 4 x 4096 x 4096 x 32 heads of 128)
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b) {
+            if (b > 0 && 32 * b >= end - n) break;
             constexpr int BLOCK = 32 * AttLds<T, DP>::STRIDE;
             att_f32x16 s, ds;
             typedef AttGroups<T, DP> G;
