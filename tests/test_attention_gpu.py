@@ -247,3 +247,21 @@ def test_prefix_of_no_sequences(device):
     lengths = torch.zeros(1, dtype=torch.int32, device=device)
     assert kermac.prefix_attention(q[:0], pk, pv, k[:0], v[:0], lengths[:0]).shape == (0, 3, 4, 64)
     assert kermac.prefix_attention(q[:, :0], pk, pv, k, v, lengths).shape == (1, 0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("K, O", [(96, 80), (128, 128), (256, 200), (33, 7)])
+@pytest.mark.parametrize("M", [1, 9, 150])
+def test_masked_keys_of_any_width_may_hold_anything(device, dtype, K, O, M):
+    """Keys left out one by one, whole tiles of them, and all of an entry: what they hold stays out, in aligned rows and in others."""
+    L, N = 4, 500
+    mask = torch.rand(L, N, generator=torch.Generator().manual_seed(8)) < 0.6
+    mask[1, 40:333], mask[2] = False, False
+    mask[3] = torch.arange(N) == 499
+    for pad in (0, 1):
+        q, k, v = operands(L, M, N, 4, 2, K + pad, O + pad, dtype, device)
+        q, k, v = q[..., pad:], k[..., pad:], v[..., pad:]
+        k[~mask], v[~mask] = math.nan, math.inf
+        out = check_cross(q, k, v, f"pad={pad}", key_mask=mask.to(device))
+        assert out[2].eq(0).all()
+        check_cross(q, k, v, f"pad={pad} and lengths", key_mask=mask.to(device), key_lengths=torch.tensor([350, 500, 2, 0], dtype=torch.int32, device=device))
