@@ -439,9 +439,9 @@ __device__ __forceinline__ float att_scores(att_f32x16 (&s)[KT / 32], const att_
     return top;
 }
 
-// Masks a tile's scores (`kept` has a bit per key, the same in all lanes; with `causal`, this lane's row meets the first `limit` of them only) and, where they pass the wave's base by 2^8, moves it to the largest, whose weight is
-// then exactly 1 (a row of one key gets its value without a rounding).  What was made below the old base is rescaled: output and sum, and `weights`
-// that wait for their product and are rounded once more.
+// Masks a tile's scores (`kept` has a bit per key, the same in all lanes; with `causal`, this lane's row meets the first `limit` of them only) and, where
+// they pass the wave's base by 2^8, moves it to the largest, whose weight is then exactly 1 (a row of one key gets its value without a rounding).  What was
+// made below the old base is rescaled: output and sum, and `weights` that wait for their product and are rounded once more.
 template <typename T, int DP, int KT>
 __device__ __forceinline__ void att_rebase(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], att_f32x16 (&s)[KT / 32], float top, float scale_log2, att_u64 kept,
                                            bool causal, int limit, int lane)

@@ -185,3 +185,15 @@ def test_what_takes_no_part_may_hold_anything(device, dtype, K, O, kind):
         masks = dict(key_lengths=None if lengths is None else lengths.to(device), key_mask=None if mask is None else mask.to(device))
         grads = check(q, k, v, f"{kind} of {key_batch}", **masks)
         assert grads[1].cpu()[unused].eq(0).all() and grads[2].cpu()[unused].eq(0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("K, O", [(64, 64), (80, 96), (128, 128), (128, 40), (256, 256)])
+@pytest.mark.parametrize("M, N", [(5, 700), (200, 150), (333, 31)])
+def test_rows_at_odd_addresses(device, dtype, K, O, M, N):
+    """Rows that start and end between 16-byte pieces are read by elements, in kernels of their own."""
+    q, k, v = (x[..., 1:] for x in operands(2, M, N, 4, 2, K + 1, O + 1, dtype, device))
+    lengths = torch.tensor([N, N - 20], dtype=torch.int32, device=device)
+    check(q, k, v, "odd", key_lengths=lengths)
+    out = torch.empty(2, M, 4, O + 1, dtype=dtype, device=device)[..., 1:]
+    assert torch.equal(kermac.cross_attention(q, k, v, out, key_lengths=lengths), kermac.cross_attention(q, k, v, key_lengths=lengths))
