@@ -147,7 +147,7 @@ struct Plan {
     int64_t bytes;              // of workspace
 };
 
-int64_t partial_bytes(const kmc::AttentionArgs &args) { return args.slots * args.rows_total * (4ll * args.partial_width + 4); }
+int64_t partial_bytes(const kmc::AttentionArgs &args) { return args.slots * args.rows_total * (4ll * args.partial_width + 8); }
 
 int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
 {
@@ -371,7 +371,8 @@ int kmc_attention(const kmc_attention_params *params, void *stream)
     if (plan.bytes > 0) {
         if (!aligned16(params->workspace)) return fail(KMC_ERR_INVALID_ARGUMENT, "workspace is not aligned to 16 bytes");
         args.partial_out = static_cast<float *>(params->workspace);
-        args.partial_lse = args.partial_out + args.slots * args.rows_total * args.partial_width;
+        args.partial_shift = args.partial_out + args.slots * args.rows_total * args.partial_width;
+        args.partial_lse = args.partial_shift + args.slots * args.rows_total;
     }
     const int width = std::max(params->k, params->o);
     const hipStream_t on = static_cast<hipStream_t>(stream);

@@ -349,12 +349,36 @@ __device__ __forceinline__ void att_wave_sync()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// What a wave carries along the keys for its 32 rows.
+// What a wave carries along the keys for its 32 rows.  The weight of a score s (a product, not scaled yet) is exp2((s - shift) scale_log2 - base): 1 for the
+// score that the row's weights are relative to, one of the largest so far.
 template <int DP>
 struct AttState {
     att_f32x16 out[DP / 32];
-    float base, sum;             // a score near the largest so far and the sum of this lane's exponentials relative to it, to base 2
+    float shift, base, sum;      // shift is -inf before the first key; sum of this lane's weights
+    bool shifted;                // a row of the wave has a shift
 };
+
+// What weights relative to the score `top` take.  In 16 bits, base = top scale_log2 rounded to fp32 and no shift, one instruction less per weight: the weight of `top` is
+// then exp2 of that rounding's error, below 2^-12 up to a base of 2^12, which the rounding to the operands' type takes away.  Where the base is larger (that error
+// grows to any size: at 2^30 a weight would be 2^32, or 0 in every type) and in fp32, top is subtracted first, and its weight is exactly 1.
+constexpr float ATT_LARGEST_BASE = 4096.0f;
+
+template <typename T>
+__device__ __forceinline__ void att_relative_to(float top, float scale_log2, float *shift, float *base)
+{
+    const float product = top * scale_log2;
+    const bool shifted = sizeof(T) == 4 || !(fabsf(product) < ATT_LARGEST_BASE);
+    *shift = shifted ? top : 0.0f;
+    *base = shifted ? 0.0f : product;
+}
+
+// The log of a row's sum of exponentials from that relative to the shift, to base 2.  -inf stands for a row without keys and for no other.
+__device__ __forceinline__ float att_natural_lse(float shift, float lse2, float scale_log2)
+{
+    if (lse2 == -__builtin_inff()) return lse2;
+    const float lse = __builtin_fmaf(lse2, ATT_LN_2, shift * (scale_log2 * ATT_LN_2));
+    return lse == -__builtin_inff() ? -__FLT_MAX__ : lse;
+}
 
 // Outputs and sums are rescaled only when a score passes the one they are relative to by 2^8: exponentials stay below 256, far inside every type,
 // and after the first tiles the 64 or more multiplications per tile are not made.
@@ -440,8 +464,9 @@ __device__ __forceinline__ float att_scores(att_f32x16 (&s)[KT / 32], const att_
 }
 
 // Masks a tile's scores (`kept` has a bit per key, the same in all lanes; with `causal`, this lane's row meets the first `limit` of them only) and, where
-// they pass the wave's base by 2^8, moves it to the largest, whose weight is then exactly 1 (a row of one key gets its value without a rounding).  What was
-// made below the old base is rescaled: output and sum, and `weights` that wait for their product and are rounded once more.
+// the weight of one would pass 2^8, makes the weights relative to the largest, whose own is then 1 in the operands' type (a row of one key gets its value without
+// a rounding).  What was made before is rescaled: output and sum, and `weights` that wait for their product and are rounded once more.  Shifts are
+// subtracted from the scores.
 template <typename T, int DP, int KT>
 __device__ __forceinline__ void att_rebase(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], att_f32x16 (&s)[KT / 32], float top, float scale_log2, att_u64 kept,
                                            bool causal, int limit, int lane)
@@ -471,12 +496,18 @@ __device__ __forceinline__ void att_rebase(AttState<DP> &state, att_vec8<T> (&we
                 top = fmaxf(top, s[b][i]);
             }
     }
-    top = att_max_of_halves(top) * scale_log2;
-    if (!__all(top <= state.base + ATT_HEADROOM)) {
+    top = att_max_of_halves(top);
+    const float above = __builtin_fmaf(top - state.shift, scale_log2, -state.base);     // the largest weight, to base 2; not a number without keys
+    if (__any(above > ATT_HEADROOM)) {
         att_rare();
-        const float base = fmaxf(state.base, top);
-        const float shrink = __builtin_amdgcn_exp2f(state.base - (base == -__builtin_inff() ? 0.0f : base));
-        state.base = base;
+        float shift, base, shrink = 1.0f;
+        att_relative_to<T>(top, scale_log2, &shift, &base);
+        if (above > 0.0f) {
+            shrink = __builtin_amdgcn_exp2f(__builtin_fmaf(state.shift - shift, scale_log2, state.base - base));
+            state.shift = shift;
+            state.base = base;
+        }
+        state.shifted = __any(state.shift != 0.0f && state.shift != -__builtin_inff());
         state.sum *= shrink;
 #pragma unroll
         for (int o = 0; o < DP / 32; ++o) state.out[o] *= shrink;
@@ -485,9 +516,15 @@ __device__ __forceinline__ void att_rebase(AttState<DP> &state, att_vec8<T> (&we
 #pragma unroll
             for (int j = 0; j < 8; ++j) weights[step][j] = static_cast<T>(static_cast<float>(weights[step][j]) * shrink);
     }
+    if (sizeof(T) == 4 || state.shifted) {
+        if (sizeof(T) != 4) att_rare();
+        const float shift = state.shift == -__builtin_inff() ? 0.0f : state.shift;
+#pragma unroll
+        for (int b = 0; b < KT / 32; ++b) s[b] -= shift;
+    }
 }
 
-// exp(s - base) of 16 keys, in the operands' type.
+// The weights of 16 keys, in the operands' type.
 template <typename T, int DP, int KT>
 __device__ __forceinline__ att_vec8<T> att_weights(AttState<DP> &state, const att_f32x16 (&s)[KT / 32], int step, float scale_log2, float base)
 {
@@ -531,9 +568,6 @@ __device__ __forceinline__ void att_add_values(AttState<DP> &state, att_vec8<T> 
     }
 }
 
-// Below a base of -inf (no key of this row yet) every exponential is that of -inf, 0.
-__device__ __forceinline__ float att_finite_base(float base) { return base == -__builtin_inff() ? 0.0f : base; }
-
 // Keys [begin, end) of a segment for split `split` of `splits`, in whole tiles.
 __device__ __forceinline__ void att_range(int length, int tile, int split, int splits, int *begin, int *end)
 {
@@ -570,7 +604,7 @@ struct AttForwardShape {
     // the memory.  Keys and values take turns in one tile then (1 token x 20000 keys x 8 heads of 256 fp32: 136 us, with two waves of two tiles 151).
     static constexpr bool OWN_TURNS = ROW_BYTES > 512;
     static constexpr int OWN_BYTES = (OWN_TURNS ? 1 : 2) * WAVES * OWN_KEYS * ROW_BYTES;
-    static constexpr int JOIN_BYTES = (WAVES - 1) * (DP * 32 + 64) * 4 + 128 * WAVES;
+    static constexpr int JOIN_BYTES = (WAVES - 1) * (DP * 32 + 64) * 4 + 256 * WAVES;
     static constexpr int BYTES_1 = SHARED_BYTES > OWN_BYTES ? SHARED_BYTES : OWN_BYTES;
     static constexpr int BYTES = BYTES_1 > JOIN_BYTES ? BYTES_1 : JOIN_BYTES;
     static constexpr int WAVES_PER_SIMD = ROW_BYTES <= 256 ? 2 : 1;
@@ -599,7 +633,7 @@ __device__ __forceinline__ void att_store_columns(T *to, const att_f32x16 (&x)[D
         }
 }
 
-// Writes a wave's 32 rows: the result itself, or a partial result and its lse (to base 2) for att_join.
+// Writes a wave's 32 rows: the result itself, or for attention_join a partial result, its shift and its lse beside the shift (to base 2).
 template <typename T, int DP, bool ALIGNED>
 __device__ __forceinline__ void att_forward_write(const AttentionArgs &args, const AttentionJob &job, const AttState<DP> &state, float sum, int entry, int g,
                                                   int row, int split, int lane)
@@ -612,7 +646,10 @@ __device__ __forceinline__ void att_forward_write(const AttentionArgs &args, con
     const float lse2 = sum == 0.0f ? -__builtin_inff() : state.base + __builtin_amdgcn_logf(sum);
     if (job.partial) {
         const i64 slot = static_cast<i64>(job.slot + split) * args.rows_total + id;
-        if (half == 0) args.partial_lse[slot] = lse2;
+        if (half == 0) {
+            args.partial_shift[slot] = sum == 0.0f ? -__builtin_inff() : state.shift;
+            args.partial_lse[slot] = lse2;
+        }
         if (sum == 0.0f) return;                                                    // nobody reads it
         float *to = args.partial_out + slot * args.partial_width;
 #pragma unroll
@@ -628,7 +665,7 @@ __device__ __forceinline__ void att_forward_write(const AttentionArgs &args, con
             }
         return;
     }
-    if (args.lse && half == 0) args.lse[id] = lse2 * ATT_LN_2;
+    if (args.lse && half == 0) args.lse[id] = att_natural_lse(state.shift, lse2, args.scale_log2);
     att_store_columns<T, DP, ALIGNED>(static_cast<T *>(args.out) + at.entry * args.out_ls + at.query * args.out_ms + at.head * args.out_hs, state.out, inverse,
                                       args.o, half);
 }
@@ -698,8 +735,9 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
     att_vec8<T> query[DP / 16];
 #pragma unroll
     for (int o = 0; o < DP / 32; ++o) state.out[o] = att_f32x16{0};
-    state.base = -__builtin_inff();
-    state.sum = 0.0f;
+    state.shift = -__builtin_inff();
+    state.base = state.sum = 0.0f;
+    state.shifted = false;
 
     if (!job.own_keys) {
         constexpr int KT = Shape::SHARED_KEYS, TILE = KT * Shape::ROW_BYTES, ROWS = 32 * WAVES;
@@ -758,7 +796,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
             __syncthreads();
             auto rebase = [&](int n, att_u64 kept) {
                 att_rebase<T, DP, KT>(state, weights, s, top, scale_log2, kept, causal, limit - n, lane);
-                base = att_finite_base(state.base);
+                base = state.base;
             };
             int next_kept = 0;
             auto kept_keys = [&](int n) {
@@ -859,7 +897,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                     top = att_scores<T, DP, KT>(s, query, key_tile, lane);
                 }
                 att_rebase<T, DP, KT>(state, weights, s, top, args.scale_log2, kept, keys.causal, limit - static_cast<int>(n), lane);
-                const float base = att_finite_base(state.base);
+                const float base = state.base;
 #pragma unroll
                 for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, args.scale_log2, base);
                 att_read_columns<T, DP>(first, value_tile, 0, 0, lane);
@@ -868,18 +906,28 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                 kept = then_kept;
             }
         }
-        // join the waves: sums and outputs below one common maximum, added in the order of the waves
+        // join the waves: sums and outputs relative to the largest score that one of them has, added in the order of the waves
         float sum = att_sum_of_halves(state.sum);
-        float *bases = reinterpret_cast<float *>(lds);                   // [WAVES][32], then (WAVES - 1) waves' sums and outputs
+        float *shifts = reinterpret_cast<float *>(lds), *bases = shifts + 32 * WAVES;      // [WAVES][32] each, then (WAVES - 1) waves' sums and outputs
         float *others = bases + 32 * WAVES;
         __syncthreads();
-        if (lane < 32) bases[wave * 32 + lane] = state.base;
+        if (lane < 32) {
+            shifts[wave * 32 + lane] = state.shift;
+            bases[wave * 32 + lane] = state.base;
+        }
         __syncthreads();
-        float base = -__builtin_inff();
+        float shift = shifts[lane % 32], base = bases[lane % 32];
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) base = fmaxf(base, bases[w * 32 + lane % 32]);
+        for (int w = 1; w < WAVES; ++w) {
+            const float other_shift = shifts[w * 32 + lane % 32], other_base = bases[w * 32 + lane % 32];
+            // a shift above 0 is larger than every base without one, and a shift below 0 smaller
+            const bool larger = other_shift > shift || (other_shift == shift && other_base > base);
+            shift = larger ? other_shift : shift;
+            base = larger ? other_base : base;
+        }
         __syncthreads();
-        const float shrink = base == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(state.base - base);
+        const float shrink = state.shift == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(state.shift - shift, args.scale_log2, state.base - base));
+        state.shift = shift;
         state.base = base;
         sum *= shrink;
 #pragma unroll
@@ -908,7 +956,8 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
 }
 
 // The partial results of one row, weighted by exp(lse of the part - lse of all).  A wave per row, the parts in their order.  The weights come
-// first, a lane per part, so that the loads of the results, eight parts at a time, do not wait for them one by one.
+// first, a lane per part, so that the loads of the results, eight parts at a time, do not wait for them one by one.  They are relative to the part with the
+// largest shift, and the largest lse among those (without keys both are -inf).
 template <typename T>
 __global__ __launch_bounds__(256) void attention_join(const AttentionArgs args)
 {
@@ -916,13 +965,22 @@ __global__ __launch_bounds__(256) void attention_join(const AttentionArgs args)
     const i64 id = static_cast<i64>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (id >= args.rows_total) return;
     static_assert(ATT_MAX_SLOTS == 128, "two parts per lane");
-    const float first = lane < args.slots ? args.partial_lse[lane * args.rows_total + id] : -__builtin_inff();
-    const float second = 64 + lane < args.slots ? args.partial_lse[(64 + lane) * args.rows_total + id] : -__builtin_inff();
-    float top = fmaxf(first, second);
+    float shifts[2], lses[2], weight[2];
 #pragma unroll
-    for (int step = 32; step > 0; step >>= 1) top = fmaxf(top, __shfl_xor(top, step));
-    const float base = top == -__builtin_inff() ? 0.0f : top;
-    const float weight[2] = {__builtin_amdgcn_exp2f(first - base), __builtin_amdgcn_exp2f(second - base)};
+    for (int j = 0; j < 2; ++j) {
+        const bool part = 64 * j + lane < args.slots;
+        shifts[j] = part ? args.partial_shift[(64 * j + lane) * args.rows_total + id] : -__builtin_inff();
+        lses[j] = part ? args.partial_lse[(64 * j + lane) * args.rows_total + id] : -__builtin_inff();
+    }
+    float shift = fmaxf(shifts[0], shifts[1]);
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1) shift = fmaxf(shift, __shfl_xor(shift, step));
+    float base = fmaxf(shifts[0] == shift ? lses[0] : -__builtin_inff(), shifts[1] == shift ? lses[1] : -__builtin_inff());
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1) base = fmaxf(base, __shfl_xor(base, step));
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        weight[j] = shifts[j] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(shifts[j] - shift, args.scale_log2, lses[j] - base));
     float sum = weight[0] + weight[1];
 #pragma unroll
     for (int step = 32; step > 0; step >>= 1) sum += __shfl_xor(sum, step);
@@ -946,7 +1004,7 @@ __global__ __launch_bounds__(256) void attention_join(const AttentionArgs args)
     const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
     const i64 token = id / (static_cast<i64>(args.g) * args.r);
     const int head = static_cast<int>(id % (static_cast<i64>(args.g) * args.r));
-    if (args.lse && lane == 0) args.lse[id] = sum == 0.0f ? -__builtin_inff() : (base + __builtin_amdgcn_logf(sum)) * ATT_LN_2;
+    if (args.lse && lane == 0) args.lse[id] = att_natural_lse(shift, sum == 0.0f ? -__builtin_inff() : base + __builtin_amdgcn_logf(sum), args.scale_log2);
     T *to = static_cast<T *>(args.out) + token / args.m * args.out_ls + token % args.m * args.out_ms + head * args.out_hs;
 #pragma unroll
     for (int j = 0; j < 4; ++j)

@@ -38,7 +38,8 @@ struct AttentionArgs {
     int m, g, r, k, o;
     float scale_log2;                       // |scale| log2(e), above 0
     float query_factor;                     // 1; -1 for a negative scale; 0 for a scale of 0
-    float *partial_out, *partial_lse;       // [slots, rows_total, partial_width], [slots, rows_total] to base 2
+    float *partial_out;                     // [slots, rows_total, partial_width]
+    float *partial_shift, *partial_lse;     // [slots, rows_total]: a score that was subtracted (-inf: no keys), and the lse beside it to base 2
     int slots, partial_width;
     i64 rows_total;                         // l m g r
 };
