@@ -505,7 +505,8 @@ typedef struct kmc_attention_gradient_params {
     const uint8_t *key_mask; int64_t key_mask_ls, key_mask_ns;
     void *grad_q, *grad_key, *grad_value;       /* [l, m, h, k], [key_entries, n, g, k], [key_entries, n, g, o] */
     /* What kmc_attention_gradient_workspace_bytes asks for, 16-byte aligned; at least 8 l m h + 8 bytes, rounded up to a multiple of 16,
-     * with which no work is cut. */
+     * with which no work is cut.  Rows whose lse is 2839 or larger in magnitude want another 4 (l m h + l g ceil(m h / g / 128)) bytes, rounded up likewise:
+     * without them p is off by the relative 2^-23 |lse|, as fp32 holds the lse, and from some 10^8 on means nothing. */
     void *workspace; int64_t workspace_bytes;
 } kmc_attention_gradient_params;
 int kmc_attention_gradient(const kmc_attention_gradient_params *params, void *stream);

@@ -298,7 +298,8 @@ def cross_attention_grad(
     numbers of that type, so gradients far below 1e-4 want a loss scale.
 
     Returns ``(grad_queries, grad_keys, grad_values)``, new contiguous tensors with the shapes of the inputs.  Takes 8 bytes of
-    scratch memory per row at least.
+    scratch memory per row at least.  Scores of any size want 4 more (and 4 per 128 rows): where a limit leaves only those 8, weights of a row
+    whose ``lse`` is 2839 or larger in magnitude are off by the relative ``2**-23 * |lse|``, as fp32 holds it.
 
     Raises:
         TypeError: non-tensor inputs or a wrong dtype.
@@ -310,10 +311,13 @@ def cross_attention_grad(
     needed, workspace = _gradient_workspace_bytes(*plan.extents), None
     if needed:
         workspace = _scratch.allocate(needed, plan.device)
-        if workspace is None:           # refused: uncut launches, with room for the sums of a row
-            _, L, M, _, H = plan.extents[:5]
-            needed = (8 * L * M * H + 8 + 15) // 16 * 16
-            workspace = _scratch.allocate(needed, plan.device)
+        if workspace is None:           # refused: uncut launches, with room for the sums of a row, and for a shift of its scores if there is
+            _, L, M, _, H, G = plan.extents[:6]
+            least, shifts = (8 * L * M * H + 8 + 15) // 16 * 16, (4 * L * M * H + 4 * L * G * -(-M * (H // G) // 128) + 15) // 16 * 16
+            for needed in (least + shifts, least):
+                workspace = _scratch.allocate(needed, plan.device)
+                if workspace is not None:
+                    break
         if workspace is None:
             raise RuntimeError(f"cross_attention_grad needs {needed} bytes of scratch memory: the limit, the supplied buffer or the device does not allow them")
     if debug:

@@ -257,8 +257,8 @@ int parts(int64_t base, int64_t slots, int64_t steps, double step_us, double ele
 struct GradPlan {
     kmc::AttentionGradArgs args;
     bool aligned, empty;
-    int64_t stats_bytes, q_bytes, k_bytes, v_bytes;
-    int64_t bytes() const { return stats_bytes + q_bytes + k_bytes + v_bytes; }
+    int64_t stats_bytes, shift_bytes, q_bytes, k_bytes, v_bytes;
+    int64_t bytes() const { return stats_bytes + shift_bytes + q_bytes + k_bytes + v_bytes; }
 };
 
 int prepare(const kmc_attention_gradient_params *p, bool may_cut, GradPlan *plan)
@@ -321,6 +321,7 @@ int prepare(const kmc_attention_gradient_params *p, bool may_cut, GradPlan *plan
 
     const int64_t q_rows = static_cast<int64_t>(p->l) * p->m * p->h, k_rows = static_cast<int64_t>(p->key_entries) * p->n * p->g;
     plan->stats_bytes = (8 * q_rows + 8 + 15) / 16 * 16;
+    plan->shift_bytes = (4 * q_rows + 4 * q_base + 15) / 16 * 16;
     if (args.q_splits > 1) plan->q_bytes = 4ll * args.q_splits * q_rows * args.partial_k_width;
     if (args.k_splits > 1) {
         plan->k_bytes = 4ll * args.k_splits * k_rows * args.partial_k_width;
@@ -402,6 +403,7 @@ int kmc_attention_gradient(const kmc_attention_gradient_params *params, void *st
     if (!params->workspace || params->workspace_bytes < plan.bytes()) {
         status = prepare(params, false, &plan);
         if (status != KMC_OK) return status;
+        if (params->workspace_bytes < plan.bytes()) plan.shift_bytes = 0;
         if (!params->workspace || params->workspace_bytes < plan.bytes())
             return fail(KMC_ERR_INVALID_ARGUMENT, "the gradient of attention needs a workspace of %lld bytes", static_cast<long long>(plan.bytes()));
     }
@@ -411,7 +413,12 @@ int kmc_attention_gradient(const kmc_attention_gradient_params *params, void *st
     kmc::AttentionGradArgs &args = plan.args;
     char *at = static_cast<char *>(params->workspace);
     args.stats = reinterpret_cast<float *>(at);
-    args.partial_q = reinterpret_cast<float *>(at += plan.stats_bytes);
+    at += plan.stats_bytes;
+    if (plan.shift_bytes > 0) {
+        args.row_shift = reinterpret_cast<float *>(at);
+        args.row_flags = reinterpret_cast<int *>(at) + static_cast<int64_t>(args.l) * args.m * args.g * args.r;
+    }
+    args.partial_q = reinterpret_cast<float *>(at += plan.shift_bytes);
     args.partial_k = reinterpret_cast<float *>(at += plan.q_bytes);
     args.partial_v = reinterpret_cast<float *>(at += plan.k_bytes);
     const int width = std::max(params->k, params->o);

@@ -28,8 +28,13 @@ struct AttGradShape {
     static constexpr int DEEP = PAIR <= 16384 ? 6 : PAIR <= 32768 ? 4 : 2;      // buffers for them that fit LDS (twice, where two workgroups share a CU)
 };
 
-// ds of a 32 x 32 result from scores, d v^T, and the row's statistics: p comes back in `s`.
+// p of a score from the row's statistics.
 __device__ __forceinline__ float att_weight(float s, float scale_log2, float lse2) { return __builtin_amdgcn_exp2f(__builtin_fmaf(s, scale_log2, -lse2)); }
+
+// An lse of this size or more (4096 to base 2) is not exact enough for p = exp(s - lse): fp32 rounds it, and its product with log2(e), to 2^-12 or worse each, which
+// p is then off by as a factor; at 2^30 that factor is any power of two up to 2^64.  The queries' kernel walks the keys of such rows once more in front, for the
+// largest score, the sum of the exponentials relative to it and delta; p is then exp2((s - largest) scale_log2 - log2(sum)), as in the forward kernel.
+constexpr float ATT_LARGEST_LSE = ATT_LARGEST_BASE * ATT_LN_2;
 
 // lse to base 2 for the exponentials; a row without keys gets +inf, which makes all its weights 0.
 __device__ __forceinline__ float att_lse2(float lse) { return lse == -__builtin_inff() ? __builtin_inff() : lse * ATT_LOG2_E; }
@@ -79,6 +84,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     constexpr int KT = Shape::KEYS;
     constexpr int TILE = KT * AttLds<T, DP>::STRIDE;
     __shared__ __attribute__((aligned(1024))) att_lds_byte lds[4 * TILE];       // keys and values, two tiles of each
+    __shared__ float shifts[128];               // with `large`, of the rows: not in a register that the loop holds
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int id = (blockIdx.x & 7) * (args.q_grid >> 3) + (blockIdx.x >> 3);
@@ -112,11 +118,16 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
         for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(static_cast<float>(grad[step][j]), static_cast<float>(result[j]), delta);
     }
     delta = att_sum_of_halves(delta);
-    float lse2 = att_lse2(args.lse[at]);
-
-    att_f32x16 acc[DP / 32];
+    float lse2 = att_lse2(args.lse[at]), shift = 0.0f;
+    // whether one of the workgroup's 128 rows has a large lse: every wave looks at all of them
+    bool large = false;
+    if (args.row_shift)
 #pragma unroll
-    for (int o = 0; o < DP / 32; ++o) acc[o] = att_f32x16{0};
+        for (int j = 0; j < 2; ++j) {
+            const int other = row_tile * 128 + 64 * j + lane;
+            const float lse = other < rows ? args.lse[(static_cast<i64>(entry) * args.m + other / args.r) * (static_cast<i64>(args.g) * args.r) + g * args.r + other % args.r] : 0.0f;
+            large = __any(!(fabsf(lse) < ATT_LARGEST_LSE) && lse != -__builtin_inff()) || large;
+        }
 
     const AttentionKeys &keys = args.keys;
     const int length = att_length(keys, entry);
@@ -127,40 +138,59 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     const T *k = static_cast<const T *>(keys.k) + entry * keys.k_ls + g * keys.k_gs;
     const T *v = static_cast<const T *>(keys.v) + entry * keys.v_ls + g * keys.v_gs;
     AttTile<T, DP, KT, 256, ALIGNED> next_k, next_v;
-    if (one_tile && begin < end) {
+    if ((one_tile || large) && begin < end) {
         // Few keys: delta from the rounded result would be off by as much as ds is large, so it is summed from the weights themselves,
         // which are normalised again while they are at hand (a single key's weight is exactly 1, its ds exactly 0).
-        const att_u64 kept = att_kept_keys(keys, entry, begin, end, lane);
-        next_k.begin(k, keys.k_ns, end, args.k, lds, threadIdx.x, kept);
-        next_v.begin(v, keys.v_ns, end, args.o, lds + TILE, threadIdx.x, kept);
-        next_k.finish(lds, threadIdx.x);
-        next_v.finish(lds + TILE, threadIdx.x);
-        __syncthreads();
-        float total = 0.0f, inner = 0.0f;
+        float top = -__builtin_inff(), total = 0.0f, inner = 0.0f;
 #pragma unroll 1
-        for (int b = 0; b < KT / 32 && 32 * b < end; ++b) {
-            att_f32x16 s = {0}, ds = {0};
+        for (int n = 0; n < length; n += KT) {
+            const att_u64 kept = att_kept_keys(keys, entry, n, length, lane);
+            if (n > 0) __syncthreads();                 // the tile before has been read
+            next_k.begin(k + n * keys.k_ns, keys.k_ns, length - n, args.k, lds, threadIdx.x, kept);
+            next_v.begin(v + n * keys.v_ns, keys.v_ns, length - n, args.o, lds + TILE, threadIdx.x, kept);
+            next_k.finish(lds, threadIdx.x);
+            next_v.finish(lds + TILE, threadIdx.x);
+            __syncthreads();
+#pragma unroll 1
+            for (int b = 0; b < KT / 32 && 32 * b < length - n; ++b) {
+                att_f32x16 s = {0}, ds = {0};
 #pragma unroll
-            for (int step = 0; step < DP / 16; ++step) {
-                s = att_mma(att_read_row<T, DP>(lds, 32 * b, 16 * step, lane), query[step], s);
-                ds = att_mma(att_read_row<T, DP>(lds + TILE, 32 * b, 16 * step, lane), grad[step], ds);
-            }
-            const unsigned mine = static_cast<unsigned>(kept >> (32 * b)) >> (4 * half);
+                for (int step = 0; step < DP / 16; ++step) {
+                    s = att_mma(att_read_row<T, DP>(lds, 32 * b, 16 * step, lane), query[step], s);
+                    ds = att_mma(att_read_row<T, DP>(lds + TILE, 32 * b, 16 * step, lane), grad[step], ds);
+                }
+                const unsigned mine = static_cast<unsigned>(kept >> (32 * b)) >> (4 * half);
+                float block_top = -__builtin_inff();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const bool counts = mine >> att_row(i, 0) & 1;
-                const float p = !counts ? 0.0f : length == 1 ? 1.0f : att_weight(s[i], args.scale_log2, lse2);
-                total += p;
-                inner = __builtin_fmaf(p, ds[i], inner);
+                for (int i = 0; i < 16; ++i) block_top = fmaxf(block_top, mine >> att_row(i, 0) & 1 ? s[i] : -__builtin_inff());
+                block_top = att_max_of_halves(block_top);
+                if (block_top > top) {
+                    const float shrink = __builtin_amdgcn_exp2f((top - block_top) * args.scale_log2);
+                    total *= shrink;
+                    inner *= shrink;
+                    top = block_top;
+                }
+                const float from = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const bool counts = mine >> att_row(i, 0) & 1;
+                    const float p = counts ? __builtin_amdgcn_exp2f((s[i] - from) * args.scale_log2) : 0.0f;
+                    total += p;
+                    inner = counts ? __builtin_fmaf(p, ds[i], inner) : inner;
+                }
             }
         }
         total = att_sum_of_halves(total);
         inner = att_sum_of_halves(inner);
-        if (total > 0.0f) {
+        if (total == 0.0f) {
+            lse2 = __builtin_inff();
+        } else {
             delta = inner / total;
-            if (length > 1) lse2 += __builtin_amdgcn_logf(total);
+            shift = large ? top : 0.0f;
+            lse2 = large ? __builtin_amdgcn_logf(total) : __builtin_fmaf(top, args.scale_log2, __builtin_amdgcn_logf(total));
         }
     }
+    if (lse2 == __builtin_inff()) delta = 0.0f;         // (no key: the gradient is 0 whatever that of the result is)
     if (blockIdx.x == 0 && threadIdx.x == 0) {          // for rows that do not exist: weights of 0
         args.stats[2 * rows_total] = __builtin_inff();
         args.stats[2 * rows_total + 1] = 0.0f;
@@ -169,7 +199,13 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
         float *stats = args.stats + (static_cast<i64>(entry) * args.g * args.r + head) * args.m + token;
         stats[0] = lse2;
         stats[rows_total] = delta;
+        if (args.row_shift) args.row_shift[stats - args.stats] = shift;
     }
+    if (args.row_flags && split == 0 && threadIdx.x == 0) args.row_flags[(static_cast<i64>(entry) * args.g + g) * args.q_row_tiles + row_tile] = large;
+    att_f32x16 acc[DP / 32];
+#pragma unroll
+    for (int o = 0; o < DP / 32; ++o) acc[o] = att_f32x16{0};
+    if (large && half == 0) shifts[32 * wave + lane] = shift;
     int odd = 0;
     att_wait_for_loads();
     const i64 k_stride = keys.k_ns, v_stride = keys.v_ns;
@@ -214,15 +250,19 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
             const att_lds_byte *block = key_tile + b * BLOCK;
             att_two_scores<T, DP, false>(s, ds, block, query, value_tile + b * BLOCK, grad, lane, [](int) {});
             att_read_columns<T, DP>(f[0], block, 0, 0, lane);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) ds[i] = att_weight(s[i], scale_log2, lse2) * (ds[i] - delta);
             const unsigned here = static_cast<unsigned>(kept >> (32 * b));
-            if (here != ~0u) {
+            if (large || here != ~0u) {
                 att_rare();
                 const unsigned rows = __builtin_amdgcn_readfirstlane(here);
+                if (large) s -= shifts[32 * wave + lane % 32];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) ds[i] = att_has_row(rows, i) ? ds[i] : 0.0f;
+                for (int i = 0; i < 16; ++i) {
+                    s[i] = att_has_row(rows, i) ? s[i] : -__builtin_inff();
+                    ds[i] = att_has_row(rows, i) ? ds[i] : 0.0f;
+                }
             }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ds[i] = att_weight(s[i], scale_log2, lse2) * (ds[i] - delta);
             x[0] = att_operand<T>(ds, 0);
             x[1] = att_operand<T>(ds, 1);
 #pragma unroll
@@ -334,6 +374,10 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
         const bool kept = exists && n < length && (!keys.mask || keys.mask[entry * keys.mask_ls + n * keys.mask_ns] != 0);
         const bool clear = entries > 1 && !__all(kept);
         ever_kept |= kept;
+        bool large = false;                                 // a row of this entry and head of keys has a shift
+        if (args.row_flags)
+            for (int i = 0; i < args.q_row_tiles; i += 64)
+                large = __any(i + lane < args.q_row_tiles && args.row_flags[(static_cast<i64>(entry) * args.g + g) * args.q_row_tiles + i + lane] != 0) || large;
 
         // What moves from tile to tile: addresses in scalar registers that grow by one of two steps.
         Tile next_q, next_d;
@@ -385,6 +429,18 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
         att_f32x16 s_a, ds_a, s_b, ds_b;
         att_vec8<T> p[2], x[2];
         float weight[16];
+        // of the tile whose weights are made next
+        int shift_m0 = m0;
+        const float *shift_at = args.row_shift + (static_cast<i64>(entry) * args.g * args.r + head) * m + m0;
+        auto shift_scores = [&](att_f32x16 &s) {
+            if (!large) return;
+            att_rare();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] -= shift_m0 + att_row(i, half) < m ? shift_at[att_row(i, half)] : 0.0f;
+            const bool last = shift_m0 == last_m0;
+            shift_at += last ? m - last_m0 : RT;
+            shift_m0 = last ? 0 : shift_m0 + RT;
+        };
         auto make_weights = [&](const att_f32x16 &s, int q) {
             const att_f32x4 lse2 = *reinterpret_cast<const att_f32x4 *>(all_stats[now] + 8 * q + 4 * half);
 #pragma unroll
@@ -449,7 +505,8 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
             __syncthreads();
             now = then();
         };
-        auto turn = [&](const att_f32x16 &s, att_f32x16 &ds, att_f32x16 &next_s, att_f32x16 &next_ds) {
+        auto turn = [&](att_f32x16 &s, att_f32x16 &ds, att_f32x16 &next_s, att_f32x16 &next_ds) {
+            shift_scores(s);
             begin();
             const att_lds_byte *q_tile = lds + 2 * then() * TILE;
             att_two_scores<T, DP, true>(next_s, next_ds, q_tile, key, q_tile + TILE, value, lane, [&](int q) { make_weights(s, q); });
@@ -477,6 +534,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
                 s_a = s_b;
                 ds_a = ds_b;
             }
+            shift_scores(s_a);
 #pragma unroll
             for (int q = 0; q < 4; ++q) make_weights(s_a, q);
             products(ds_a);
@@ -486,6 +544,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
                 begin();
                 const att_lds_byte *q_tile = lds + 2 * now * TILE;
                 att_two_scores<T, DP, false, OF_KEYS>(s_a, ds_a, q_tile, key, q_tile + TILE, value, lane, [](int) {});
+                shift_scores(s_a);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) make_weights(s_a, q);
                 products(ds_a);

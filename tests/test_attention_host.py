@@ -239,3 +239,11 @@ def test_operands_on_another_device_are_refused():
             plan(**{**dict(q=q, k=k, v=v), **change})
     with pytest.raises(ValueError, match="same CUDA device"):
         _plan_attention_grad(make(2, 5, 4, 24), q, k, v, make(2, 5, 4, 24), make(2, 5, 4).to(elsewhere), None, None, None, require_device=False)
+
+
+def test_the_workspace_of_a_gradient_has_room_for_shifts():
+    """12 bytes per row and 4 per 128 rows of a head of keys: row statistics, and what is subtracted from the scores of rows whose lse is large."""
+    plan = _plan_attention_grad(make(3, 50, 8, 24), make(3, 50, 8, 16), make(3, 7, 2, 16), make(3, 7, 2, 24), make(3, 50, 8, 24), make(3, 50, 8), None, None, None,
+                                require_device=False)
+    rows = 3 * 50 * 8
+    assert _backend.attention_gradient_workspace_bytes(plan.params) >= 8 * rows + 16 + (4 * rows + 4 * 3 * 2 * 2 + 15) // 16 * 16

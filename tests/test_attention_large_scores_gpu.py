@@ -137,3 +137,108 @@ def test_one_key_is_its_value(device, dtype, M, scale):
     assert torch.equal(kermac.cross_attention(q, k, v, scale=scale, key_lengths=lengths), one)
     nothing = torch.zeros(2, dtype=torch.int32, device=device)
     assert torch.equal(kermac.prefix_attention(q, k[0, :1], v[0, :1], k, v, nothing, scale=scale), v[:1, :1].repeat_interleave(2, 2).expand(2, M, 4, 64))
+
+
+# ------------------------------------------------------------------------------------------------ gradients
+
+def check_gradients(grads, d, q, k, v, keep, scale, what):
+    """Against the formulas in 64 bits.  Scores are exact; weights are off by 2^-10 of themselves at most where the lse is below 4096 to base 2 (fp32 rounds it, and its
+    product with log2(e), to 2^-13 each) and by a few roundings where it is larger.  What passes the operands' type may come back as an infinity, not as NaN."""
+    unit, floor = UNIT[q.dtype], reference.FLOOR[q.dtype]
+    L, M, H, _ = q.shape
+    N, G, O = v.shape[1:]
+    R, shared = H // G, k.shape[0] == 1 and L > 1
+    p, lse = softmax(q, k, keep, scale)
+    scale = torch.tensor(scale, dtype=torch.float32).double()
+    k, v = (x.cpu().double().expand(L, -1, -1, -1).repeat_interleave(R, 2).transpose(1, 2).contiguous() for x in (k, v))
+    q, d = (x.cpu().double().transpose(1, 2).contiguous() for x in (q, d))
+    near = (lse.abs() < 4096 * math.log(2))[..., None]
+    E = torch.where(near, 2.0 ** -10, 256 * E32)
+    A = torch.matmul(p, v.abs())
+    out = torch.matmul(p, v)
+    dp, dp_magnitude = torch.matmul(d, v.transpose(2, 3)), torch.matmul(d.abs(), v.abs().transpose(2, 3))
+    delta = (d * out).sum(-1, keepdim=True)
+    delta_error = (d.abs() * (unit * 1.01 * (out.abs() + A) + 2 * (E + (N + 16) * E32) * A + floor)).sum(-1, keepdim=True) + (O + N + 16) * E32 * (d.abs() * A).sum(-1, keepdim=True)
+    alone = p.amax(-1, keepdim=True) == 1.0                   # all weight on one key: its dp is delta, so that ds is 0, to the last bit
+    ds = torch.where(alone, 0.0, p * (dp - delta))
+    ds_error = E * p * (dp - delta).abs() + p * ((O + 16) * E32 * dp_magnitude + delta_error)
+    ds_error = torch.where(alone, 0.0, ds_error + unit * 1.01 * (ds.abs() + ds_error) + floor * (p > 0))
+    p_error = torch.where(alone, 0.0, E * p + unit * 1.01 * p + floor * (p > 0))
+    if alone.any():
+        assert grads[0].cpu().transpose(1, 2)[alone[..., 0] & ~near[..., 0]].eq(0).all(), what + ": the gradient of a query with one key is 0"
+
+    def over_rows(x):
+        x = x.reshape(L, G, R, N, -1).sum(2).transpose(1, 2)
+        return x.sum(0, keepdim=True) if shared else x
+
+    rows = M * R * (L if shared else 1) + 16
+    values = ((scale * torch.matmul(ds, k)).transpose(1, 2), over_rows(scale * torch.matmul(ds.transpose(2, 3), q)), over_rows(torch.matmul(p.transpose(2, 3), d)))
+    bounds = (scale.abs() * (torch.matmul(ds_error, k.abs()) + (N + 16) * E32 * torch.matmul(ds.abs(), k.abs())).transpose(1, 2),
+              over_rows(scale.abs() * (torch.matmul(ds_error.transpose(2, 3), q.abs()) + rows * E32 * torch.matmul(ds.abs().transpose(2, 3), q.abs()))),
+              over_rows(torch.matmul(p_error.transpose(2, 3), d.abs()) + rows * E32 * torch.matmul(p.transpose(2, 3), d.abs())))
+    largest = torch.finfo(grads[0].dtype).max
+    for name, got, truth, bound in zip(("queries", "keys", "values"), grads, values, bounds):
+        bound = bound + unit * 1.01 * (truth.abs() + bound) + floor
+        beyond = truth.abs() + bound > 0.99 * largest
+        assert not got.isnan().any(), f"{what}: NaN in the gradient of {name}"
+        reference.assert_within(got.masked_fill(beyond.to(got.device), 0.0), truth.masked_fill(beyond, 0.0), bound, f"{what} grad of {name}")
+
+
+def step(d, q, k, v, **masks):
+    out, lse = kermac.cross_attention(q, k, v, return_lse=True, **masks)
+    return kermac.cross_attention_grad(d, q, k, v, out, lse, **masks)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("scale", SCALES)
+@pytest.mark.parametrize("L, M, N, keys", [(2, 3, 20, 2), (2, 1, 5000, 2), (3, 40, 200, 3), (3, 40, 200, 1), (1, 200, 1001, 1)])
+def test_gradient(device, dtype, scale, L, M, N, keys):
+    """One tile of keys and many, whole and cut, sources of their own and a shared one; masks and a row without keys."""
+    q, k = whole(L, M, 4, 64, dtype=dtype, device=device, seed=1), whole(keys, N, 2, 64, dtype=dtype, device=device, seed=2)
+    v, d = normal(keys, N, 2, 64, dtype=dtype, seed=3).to(device), normal(L, M, 4, 64, dtype=dtype, seed=9).to(device)
+    check_gradients(step(d, q, k, v, scale=scale), d, q, k, v, reference.keep_of(L, M, N), scale, "all")
+    mask = (torch.rand(L, N, generator=torch.Generator().manual_seed(5)) < 0.3).to(device)
+    lengths = torch.tensor([N // 2, 0, N][:L], dtype=torch.int32, device=device)
+    check_gradients(step(d, q, k, v, scale=scale, key_mask=mask, key_lengths=lengths), d, q, k, v, reference.keep_of(L, M, N, lengths, mask), scale, "masked")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("width", [64, 80, 128, 256])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("M, N", [(1, 30), (40, 300), (130, 900)])
+def test_gradient_of_scores_far_from_zero(device, dtype, width, sign, M, N):
+    """Rows far away beside ordinary ones, in aligned rows and in others."""
+    L = 2
+    for pad in (0, 1):
+        q, k = torch.zeros(L, M, 2, width + pad, dtype=dtype, device=device)[..., pad:], torch.zeros(L, N, 1, width + pad, dtype=dtype, device=device)[..., pad:]
+        few_q, few_k, _ = far_operands(L, M, N, dtype, device, sign)
+        q[..., :2], k[..., :2] = few_q[..., :2], few_k[..., :2]
+        q[:, 1::2, :, 0] = 0.0
+        v, d = normal(L, N, 1, width, dtype=dtype, seed=3).to(device), normal(L, M, 2, width, dtype=dtype, seed=9).to(device)
+        mask = (torch.rand(L, N, generator=torch.Generator().manual_seed(5)) < 0.7).to(device)
+        for masks in ({}, dict(key_mask=mask)):
+            check_gradients(step(d, q, k, v, scale=1.0, **masks), d, q, k, v, reference.keep_of(L, M, N, **masks), 1.0, f"pad={pad} {list(masks)}")
+
+
+def test_gradient_with_the_least_scratch_memory(device):
+    """Without room for shifts, ordinary rows have the gradients that they have with it."""
+    q, k, v, d = (normal(2, n, h, 64, dtype=torch.bfloat16, seed=i).to(device) for i, (n, h) in enumerate(((40, 4), (130, 2), (130, 2), (40, 4))))
+    q[0, 3] *= 1000.0
+    out, lse = kermac.cross_attention(q, k, v, return_lse=True)
+    assert lse.abs().max() > 2839 and lse[1].abs().max() < 2839
+    roomy = kermac.cross_attention_grad(d, q, k, v, out, lse)
+    kermac.set_max_scratch_bytes(8 * 2 * 40 * 4 + 16)
+    try:
+        least = kermac.cross_attention_grad(d, q, k, v, out, lse)
+    finally:
+        kermac.set_max_scratch_bytes(None)
+    assert all(torch.equal(a[1], b[1]) for a, b in zip(roomy, least))
+
+
+def test_a_row_without_keys_has_no_gradient(device):
+    """Whatever the gradient of its result is."""
+    q, k, v = (normal(2, n, 2, 64, dtype=torch.bfloat16, seed=i).to(device) for i, n in enumerate((5, 200, 200)))
+    d = torch.full_like(q, math.inf)
+    mask = torch.zeros(2, 200, dtype=torch.bool, device=device)
+    for grad in step(d, q, k, v, key_mask=mask) + step(d, q, k, v, key_lengths=torch.zeros(2, dtype=torch.int32, device=device)):
+        assert grad.eq(0).all()
