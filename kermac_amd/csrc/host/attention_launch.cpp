@@ -155,7 +155,8 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
     const int status = check_extents(p->type, p->l, p->m, p->n, p->h, p->g, p->k, p->o, p->scale);
     if (status != KMC_OK) return status;
     if (p->prefix_n < 0 || p->prefix_n > MAX_KEYS) return fail(KMC_ERR_INVALID_ARGUMENT, "prefix_n=%d is outside 0 .. %d", p->prefix_n, MAX_KEYS);
-    if ((p->causal || p->prefix_n > 0) && p->key_mask) return fail(KMC_ERR_INVALID_ARGUMENT, "key_mask does not go with a prefix");
+    const bool causal = p->causal != 0 || p->prefix_n > 0;              // own keys behind a prefix are met up to the query's own
+    if (causal && p->key_mask) return fail(KMC_ERR_INVALID_ARGUMENT, "key_mask does not go with a prefix");
     const int64_t strides[] = {p->q_ls, p->q_ms, p->q_hs, p->key_ls, p->key_ns, p->key_gs, p->value_ls, p->value_ns, p->value_gs,
                                p->out_ls, p->out_ms, p->out_hs, p->key_mask_ls, p->key_mask_ns, p->prefix_key_ns, p->prefix_key_gs,
                                p->prefix_value_ns, p->prefix_value_gs};
@@ -164,7 +165,7 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
     plan->bytes = 0;
     plan->empty = p->l == 0 || p->m == 0 || p->h == 0;
     if (plan->empty) return KMC_OK;
-    if (p->causal && !p->key_lengths) return fail(KMC_ERR_INVALID_ARGUMENT, "causal needs key_lengths");
+    if (causal && !p->key_lengths) return fail(KMC_ERR_INVALID_ARGUMENT, "a prefix, or causal, needs key_lengths");
     if (!p->q || !p->out) return fail(KMC_ERR_INVALID_ARGUMENT, "null q / out pointer");
     if (p->n > 0 && (!p->key || !p->value)) return fail(KMC_ERR_INVALID_ARGUMENT, "null key / value pointer");
     if (p->prefix_n > 0 && (!p->prefix_key || !p->prefix_value)) return fail(KMC_ERR_INVALID_ARGUMENT, "null prefix_key / prefix_value pointer");
@@ -191,7 +192,7 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
     own.lengths = p->key_lengths;
     own.mask = p->key_mask; own.mask_ls = p->key_mask_ls; own.mask_ns = p->key_mask_ns;
     own.n = p->n;
-    own.causal = p->causal != 0;
+    own.causal = causal;
 
     Layout layout{element_size(p->type)};
     layout.operand(p->q, p->k);

@@ -247,3 +247,11 @@ def test_the_workspace_of_a_gradient_has_room_for_shifts():
                                 require_device=False)
     rows = 3 * 50 * 8
     assert _backend.attention_gradient_workspace_bytes(plan.params) >= 8 * rows + 16 + (4 * rows + 4 * 3 * 2 * 2 + 15) // 16 * 16
+
+
+def test_a_prefix_alone_makes_the_own_keys_causal():
+    """prefix_n > 0 with causal = 0 is the header's "prefix_n > 0 or causal": lengths are needed and a mask is refused, as with causal = 1."""
+    assert _backend.attention_workspace_bytes(library_parameters(causal=0)) == _backend.attention_workspace_bytes(library_parameters()) > 0
+    for change in (dict(key_lengths=None), dict(key_mask=16)):
+        with pytest.raises(_backend.BackendError, match="prefix"):
+            _backend.attention_workspace_bytes(library_parameters(causal=0, **change))

@@ -166,3 +166,18 @@ def test_a_training_step_of_a_layer(device):
     for name, got, weight in zip("qkv", grads, weights):
         error = (got.cpu().double() - weight.grad).norm() / weight.grad.norm()
         assert error < 6 * math.sqrt(max(width, L * N)) * 2.0 ** -24 * 8, (name, error.item())
+
+
+@pytest.mark.parametrize("L, M, P, N", [(2, 5, 100, 40), (1, 70, 30, 90)])
+def test_a_prefix_through_the_c_abi_is_causal_by_itself(device, L, M, P, N):
+    """A C caller who sets prefix_n alone gets what one gets who sets causal too: no query meets the tokens behind it."""
+    from kermac_amd import _backend
+    from kermac_amd.attention import _plan_attention
+    q, pk, pv, k, v = prefix_operands(L, M, P, N, 4, 2, 64, 64, torch.bfloat16, device)
+    lengths = torch.full((L,), N - 3, dtype=torch.int32, device=device)
+    plan = _plan_attention(q, k, v, torch.empty_like(q), None, lengths, None, False, prefix=(pk, pv))
+    params = plan.params
+    params.causal = 0
+    _backend.attention(params, torch.cuda.current_stream().cuda_stream)
+    truth, bound = reference.prefix(q, pk, pv, k, v, lengths, 64 ** -0.5)
+    reference.assert_within(plan.out, truth, bound, "prefix_n alone")
