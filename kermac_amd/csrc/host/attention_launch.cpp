@@ -120,7 +120,7 @@ int choose_parts(int64_t base, int64_t rows_total, int64_t keys, bool own_keys, 
 }
 static_assert(2 * 64 <= kmc::ATT_MAX_SLOTS, "the parts of two jobs");
 
-// false: more workgroups than a launch holds
+// false: more workgroups than the kernels count (two jobs in 31 bits)
 bool plan_job(kmc::AttentionJob *job, int first_segment, int last_segment, int64_t entries, int64_t rows, int keys, bool may_cut, bool joined,
               const kmc_attention_params *p, double *us)
 {
@@ -230,7 +230,7 @@ int prepare(const kmc_attention_params *p, bool with_workspace, Plan *plan)
             args.slots = args.job[0].splits;
         }
     }
-    if (!fits) return fail(KMC_ERR_INVALID_ARGUMENT, "more workgroups than a launch holds");
+    if (!fits) return with_workspace ? prepare(p, false, plan) : fail(KMC_ERR_INVALID_ARGUMENT, "more workgroups than the kernels count");
     plan->bytes = partial_bytes(args);
 
     return KMC_OK;
@@ -314,7 +314,7 @@ int prepare(const kmc_attention_gradient_params *p, bool may_cut, GradPlan *plan
     const int64_t tiles_of_rows = static_cast<int64_t>(args.r) * ((p->m + 31) / 32) * (p->key_entries == p->l ? 1 : p->l);
     args.k_splits = may_cut ? parts(k_base, row_bytes <= 128 ? 512 : 256, tiles_of_rows, 1.2 * width / 128 * slower * (row_bytes <= 128 ? 1.6 : 1.0), k_elements) : 1;
     const int64_t q_workgroups = q_base * args.q_splits, k_workgroups = k_base * args.k_splits;
-    if (std::max(q_workgroups, k_workgroups) > 0x7ffffff0ll) return fail(KMC_ERR_INVALID_ARGUMENT, "more workgroups than a launch holds");
+    if (std::max(q_workgroups, k_workgroups) > 0x7ffffff0ll) return fail(KMC_ERR_INVALID_ARGUMENT, "more workgroups than the kernels count");
     args.q_workgroups = static_cast<int>(q_workgroups);
     args.q_grid = static_cast<int>((q_workgroups + 7) / 8 * 8);
     args.k_workgroups = static_cast<int>(k_workgroups);

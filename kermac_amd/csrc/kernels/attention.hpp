@@ -709,7 +709,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
     // The prefix's workgroups come first: they are bound by the matrix cores and are about as many as fit the chip at most, so those of the sequences'
     // own keys, bound by memory, run beside and behind them (128 sequences behind 65536 tokens: 233 us, with the two kinds alternating 276).
     // XCD x gets a contiguous part of a job's list, in which the tiles of rows of one set of keys stand together: they share its L2.
-    int id = blockIdx.x;
+    int id = static_cast<int>(blockIdx.x) + args.first_block;
     const bool second = id >= args.job[0].grid;
     const AttentionJob &job = args.job[second];
     if (second) id -= args.job[0].grid;
@@ -962,53 +962,53 @@ template <typename T>
 __global__ __launch_bounds__(256) void attention_join(const AttentionArgs args)
 {
     const int lane = threadIdx.x & 63;
-    const i64 id = static_cast<i64>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (id >= args.rows_total) return;
     static_assert(ATT_MAX_SLOTS == 128, "two parts per lane");
-    float shifts[2], lses[2], weight[2];
+    for (i64 id = static_cast<i64>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); id < args.rows_total; id += static_cast<i64>(gridDim.x) * 4) {
+        float shifts[2], lses[2], weight[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const bool part = 64 * j + lane < args.slots;
-        shifts[j] = part ? args.partial_shift[(64 * j + lane) * args.rows_total + id] : -__builtin_inff();
-        lses[j] = part ? args.partial_lse[(64 * j + lane) * args.rows_total + id] : -__builtin_inff();
-    }
-    float shift = fmaxf(shifts[0], shifts[1]);
-#pragma unroll
-    for (int step = 32; step > 0; step >>= 1) shift = fmaxf(shift, __shfl_xor(shift, step));
-    float base = fmaxf(shifts[0] == shift ? lses[0] : -__builtin_inff(), shifts[1] == shift ? lses[1] : -__builtin_inff());
-#pragma unroll
-    for (int step = 32; step > 0; step >>= 1) base = fmaxf(base, __shfl_xor(base, step));
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-        weight[j] = shifts[j] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(shifts[j] - shift, args.scale_log2, lses[j] - base));
-    float sum = weight[0] + weight[1];
-#pragma unroll
-    for (int step = 32; step > 0; step >>= 1) sum += __shfl_xor(sum, step);
-    float out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int AT_ONCE = 8;
-    for (int part = 0; part < args.slots; part += AT_ONCE) {
-        float x[AT_ONCE][4];
-#pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u) {
-            const i64 slot = (part + u < args.slots ? part + u : 0) * args.rows_total + id;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[u][j] = 64 * j + lane < args.o ? args.partial_out[slot * args.partial_width + 64 * j + lane] : 0.0f;
+        for (int j = 0; j < 2; ++j) {
+            const bool part = 64 * j + lane < args.slots;
+            shifts[j] = part ? args.partial_shift[(64 * j + lane) * args.rows_total + id] : -__builtin_inff();
+            lses[j] = part ? args.partial_lse[(64 * j + lane) * args.rows_total + id] : -__builtin_inff();
         }
+        float shift = fmaxf(shifts[0], shifts[1]);
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u) {
-            const float w = part + u < args.slots ? __shfl(weight[part >= 64], (part + u) & 63) : 0.0f;
+        for (int step = 32; step > 0; step >>= 1) shift = fmaxf(shift, __shfl_xor(shift, step));
+        float base = fmaxf(shifts[0] == shift ? lses[0] : -__builtin_inff(), shifts[1] == shift ? lses[1] : -__builtin_inff());
 #pragma unroll
-            for (int j = 0; j < 4; ++j) out[j] += w != 0.0f ? w * x[u][j] : 0.0f;         // a part without keys wrote nothing
+        for (int step = 32; step > 0; step >>= 1) base = fmaxf(base, __shfl_xor(base, step));
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            weight[j] = shifts[j] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(shifts[j] - shift, args.scale_log2, lses[j] - base));
+        float sum = weight[0] + weight[1];
+#pragma unroll
+        for (int step = 32; step > 0; step >>= 1) sum += __shfl_xor(sum, step);
+        float out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr int AT_ONCE = 8;
+        for (int part = 0; part < args.slots; part += AT_ONCE) {
+            float x[AT_ONCE][4];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const i64 slot = (part + u < args.slots ? part + u : 0) * args.rows_total + id;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[u][j] = 64 * j + lane < args.o ? args.partial_out[slot * args.partial_width + 64 * j + lane] : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const float w = part + u < args.slots ? __shfl(weight[part >= 64], (part + u) & 63) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) out[j] += w != 0.0f ? w * x[u][j] : 0.0f;         // a part without keys wrote nothing
+            }
         }
-    }
-    const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-    const i64 token = id / (static_cast<i64>(args.g) * args.r);
-    const int head = static_cast<int>(id % (static_cast<i64>(args.g) * args.r));
-    if (args.lse && lane == 0) args.lse[id] = att_natural_lse(shift, sum == 0.0f ? -__builtin_inff() : base + __builtin_amdgcn_logf(sum), args.scale_log2);
-    T *to = static_cast<T *>(args.out) + token / args.m * args.out_ls + token % args.m * args.out_ms + head * args.out_hs;
+        const float inverse = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+        const i64 token = id / (static_cast<i64>(args.g) * args.r);
+        const int head = static_cast<int>(id % (static_cast<i64>(args.g) * args.r));
+        if (args.lse && lane == 0) args.lse[id] = att_natural_lse(shift, sum == 0.0f ? -__builtin_inff() : base + __builtin_amdgcn_logf(sum), args.scale_log2);
+        T *to = static_cast<T *>(args.out) + token / args.m * args.out_ls + token % args.m * args.out_ms + head * args.out_hs;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (64 * j + lane < args.o) to[64 * j + lane] = static_cast<T>(out[j] * inverse);
+        for (int j = 0; j < 4; ++j)
+            if (64 * j + lane < args.o) to[64 * j + lane] = static_cast<T>(out[j] * inverse);
+    }
 }
 
 }  // namespace kmc

@@ -6,6 +6,8 @@ namespace kmc {
 typedef long long i64;
 
 constexpr int ATT_MAX_SLOTS = 128;          // partial results of a row
+// A dimension of a grid holds fewer than 2^32 threads, so this many workgroups of 256; larger grids are several launches, each a multiple of the 8 XCDs.
+constexpr int ATT_MAX_BLOCKS = (1 << 24) - 8;
 
 // Keys and values of one segment; strides in elements.
 struct AttentionKeys {
@@ -35,6 +37,7 @@ struct AttentionArgs {
     float *lse;                             // [l, m, g r], or null
     AttentionKeys keys[2];
     AttentionJob job[2];
+    int first_block;                        // of this launch
     int m, g, r, k, o;
     float scale_log2;                       // |scale| log2(e), above 0
     float query_factor;                     // 1; -1 for a negative scale; 0 for a scale of 0
@@ -50,6 +53,7 @@ struct AttentionGradArgs {
     const float *lse;                       // [l, m, g r]
     AttentionKeys keys;
     void *grad_q, *grad_k, *grad_v;         // contiguous [l, m, g r, k], [key_entries, n, g, k], [key_entries, n, g, o]
+    int first_block;                        // of this launch
     int l, m, g, r, k, o;
     int key_entries;                        // l, or 1: one source for all entries
     float scale, scale_log2, query_factor;

@@ -87,7 +87,8 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     __shared__ float shifts[128];               // with `large`, of the rows: not in a register that the loop holds
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int id = (blockIdx.x & 7) * (args.q_grid >> 3) + (blockIdx.x >> 3);
+    const int block = static_cast<int>(blockIdx.x) + args.first_block;
+    int id = (block & 7) * (args.q_grid >> 3) + (block >> 3);
     if (id >= args.q_workgroups) return;
     const int row_tile = id % args.q_row_tiles;
     id /= args.q_row_tiles;
@@ -191,7 +192,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
         }
     }
     if (lse2 == __builtin_inff()) delta = 0.0f;         // (no key: the gradient is 0 whatever that of the result is)
-    if (blockIdx.x == 0 && threadIdx.x == 0) {          // for rows that do not exist: weights of 0
+    if (block == 0 && threadIdx.x == 0) {               // for rows that do not exist: weights of 0
         args.stats[2 * rows_total] = __builtin_inff();
         args.stats[2 * rows_total + 1] = 0.0f;
     }
@@ -326,7 +327,8 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
     const unsigned stats_lds = att_lds_address(all_stats);
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int id = (blockIdx.x & 7) * (args.k_grid >> 3) + (blockIdx.x >> 3);
+    const int block = static_cast<int>(blockIdx.x) + args.first_block;
+    int id = (block & 7) * (args.k_grid >> 3) + (block >> 3);
     if (id >= args.k_workgroups) return;
     const int key_tile = id % args.key_tiles;
     id /= args.key_tiles;

@@ -18,14 +18,14 @@ template <int DP, bool ALIGNED>
 hipError_t gradient(const kmc::AttentionGradArgs &args, hipStream_t stream)
 {
     // the queries' kernel writes delta, which the keys' kernel reads
-    const hipError_t status = launch(kmc::attention_grad_queries<Element, DP, ALIGNED>, dim3(args.q_grid), dim3(256), stream, args);
+    const hipError_t status = launch_in_parts(kmc::attention_grad_queries<Element, DP, ALIGNED>, args.q_grid, kmc::ATT_MAX_BLOCKS, dim3(256), stream, args);
     if (status != hipSuccess || args.k_grid == 0) return status;
     if constexpr (DP * sizeof(Element) > 512) {
-        const hipError_t first = launch(kmc::attention_grad_keys<Element, DP, ALIGNED, kmc::ATT_GRAD_KEYS>, dim3(args.k_grid), dim3(256), stream, args);
+        const hipError_t first = launch_in_parts(kmc::attention_grad_keys<Element, DP, ALIGNED, kmc::ATT_GRAD_KEYS>, args.k_grid, kmc::ATT_MAX_BLOCKS, dim3(256), stream, args);
         if (first != hipSuccess) return first;
-        return launch(kmc::attention_grad_keys<Element, DP, ALIGNED, kmc::ATT_GRAD_VALUES>, dim3(args.k_grid), dim3(256), stream, args);
+        return launch_in_parts(kmc::attention_grad_keys<Element, DP, ALIGNED, kmc::ATT_GRAD_VALUES>, args.k_grid, kmc::ATT_MAX_BLOCKS, dim3(256), stream, args);
     } else {
-        return launch(kmc::attention_grad_keys<Element, DP, ALIGNED, kmc::ATT_BOTH>, dim3(args.k_grid), dim3(256), stream, args);
+        return launch_in_parts(kmc::attention_grad_keys<Element, DP, ALIGNED, kmc::ATT_BOTH>, args.k_grid, kmc::ATT_MAX_BLOCKS, dim3(256), stream, args);
     }
 }
 

@@ -17,9 +17,8 @@ typedef __bf16 Element;
 template <int DP>
 hipError_t forward(const kmc::AttentionArgs &args, bool aligned, hipStream_t stream)
 {
-    const dim3 grid(static_cast<unsigned>(args.job[0].grid + args.job[1].grid));
-    return aligned ? launch(kmc::attention_forward<Element, DP, true>, grid, dim3(256), stream, args)
-                   : launch(kmc::attention_forward<Element, DP, false>, grid, dim3(256), stream, args);
+    return launch_in_parts(aligned ? kmc::attention_forward<Element, DP, true> : kmc::attention_forward<Element, DP, false>, args.job[0].grid + args.job[1].grid,
+                           kmc::ATT_MAX_BLOCKS, dim3(256), stream, args);
 }
 
 }  // namespace
@@ -36,8 +35,8 @@ hipError_t KMC_ATT_NAME(launch_attention_forward)(const kmc::AttentionArgs &args
         if (status != hipSuccess) return status;
     }
     if (args.slots == 0) return hipSuccess;
-    const dim3 grid(static_cast<unsigned>((args.rows_total + 3) / 4));
-    return launch(kmc::attention_join<Element>, grid, dim3(256), stream, args);
+    const kmc::i64 blocks = (args.rows_total + 3) / 4;
+    return launch(kmc::attention_join<Element>, dim3(static_cast<unsigned>(blocks < kmc::ATT_MAX_BLOCKS ? blocks : kmc::ATT_MAX_BLOCKS)), dim3(256), stream, args);
 }
 
 }  // namespace kmc_host

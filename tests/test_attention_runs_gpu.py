@@ -181,3 +181,40 @@ def test_a_prefix_through_the_c_abi_is_causal_by_itself(device, L, M, P, N):
     _backend.attention(params, torch.cuda.current_stream().cuda_stream)
     truth, bound = reference.prefix(q, pk, pv, k, v, lengths, 64 ** -0.5)
     reference.assert_within(plan.out, truth, bound, "prefix_n alone")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=str)
+def test_more_workgroups_than_a_launch_holds(device, dtype):
+    """2^24 workgroups of 256 threads are one more than a grid takes: the first, the last and the entries around the border of the launches are looked at."""
+    L, N, K = (1 << 24) + 77, 3, 8
+    q = torch.randn(L, 1, 1, K, device=device, dtype=dtype, generator=torch.Generator(device=device).manual_seed(1))
+    k, v = normal(1, N, 1, K, dtype=dtype, seed=2).to(device), normal(1, N, 1, K, dtype=dtype, seed=3).to(device)
+    out, lse = kermac.cross_attention(q, k, v, return_lse=True)
+    grads = kermac.cross_attention_grad(out, q, k, v, out, lse)
+    border = (1 << 24) - 8
+    for some in (slice(0, 50), slice(border // 8 - 20, border // 8 + 20), slice(border - 20, border + 20), slice(L - 50, L)):
+        part, part_lse = kermac.cross_attention(q[some], k, v, return_lse=True)
+        assert torch.equal(out[some], part) and torch.equal(lse[some], part_lse)
+        # (a row's gradient of its query is its own)
+        assert torch.equal(grads[0][some], kermac.cross_attention_grad(part, q[some], k, v, part, part_lse)[0])
+    scores = (q.double() * K ** -0.5 @ k[0, :, 0].double().t()).squeeze(2)
+    truth = torch.softmax(scores, -1) @ v[0, :, 0].double()
+    unit = reference.UNIT[dtype]
+    assert ((out.double() - truth[:, :, None].reshape(out.shape)).abs() <= 2 * unit * v.double().abs().max() + 2.0 ** -18).all()
+
+
+def test_more_rows_than_a_launch_of_the_join_holds(device):
+    """2^26 rows, whose parts one wave each joins, behind a prefix that all of them share."""
+    L, M, P, N, K = 2, (1 << 25) + 3, 5, 2, 8
+    make = torch.Generator(device=device).manual_seed(1)
+    q = torch.randn(L, M, 1, K, device=device, dtype=torch.float16, generator=make)
+    pk, pv = normal(P, 1, K, dtype=torch.float16, seed=4).to(device), normal(P, 1, K, dtype=torch.float16, seed=5).to(device)
+    k, v = normal(L, N, 1, K, dtype=torch.float16, seed=2).to(device), normal(L, N, 1, K, dtype=torch.float16, seed=3).to(device)
+    lengths = torch.tensor([0, 2], dtype=torch.int32, device=device)
+    out = kermac.prefix_attention(q, pk, pv, k, v, lengths)
+    # the queries in front of an entry's own tokens meet the prefix alone
+    shared = kermac.cross_attention(q.reshape(1, L * M, 1, K), pk, pv).reshape(L, M, 1, K)
+    far = 2 * reference.UNIT[torch.float16] * pv.float().abs().max()
+    assert ((out[:, :-2].float() - shared[:, :-2].float()).abs() <= far).all()
+    last = kermac.prefix_attention(q[:, -2:].contiguous(), pk, pv, k, v, lengths)
+    assert ((out[:, -2:].float() - last.float()).abs() <= 2 * reference.UNIT[torch.float16] * max(pv.float().abs().max(), v.float().abs().max())).all()
