@@ -349,7 +349,7 @@ __device__ __forceinline__ void att_wave_sync()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// What a wave carries along the keys for its 32 rows.  The weight of a score s (a product, not scaled yet) is exp2((s - shift) scale_log2 - base): 1 for the
+// What a wave carries along the keys for its 32 rows.  The weight of a score s (a product, not scaled yet) is exp2((s - shift) scale_log2 - base): 2^LIFT for the
 // score that the row's weights are relative to, one of the largest so far.
 template <int DP>
 struct AttState {
@@ -358,9 +358,14 @@ struct AttState {
     bool shifted;                // a row of the wave has a shift
 };
 
+// Weights in fp16 are 2^7 times what they are in the other types.  With ATT_HEADROOM they reach 2^15 of the type's 2^16, and at the other end a weight keeps bits down to
+// 2^-31 of the largest: behind one key that stands out by 18 (to base e), the others' weights of 2^-26 would be 0, whatever their number.  Sum and output keep
+// the factor, which the division takes out.
+template <typename T> constexpr float ATT_LIFT = std::is_same<T, _Float16>::value ? 7.0f : 0.0f;
+
 // What weights relative to the score `top` take.  In 16 bits, base = top scale_log2 rounded to fp32 and no shift, one instruction less per weight: the weight of `top` is
-// then exp2 of that rounding's error, below 2^-12 up to a base of 2^12, which the rounding to the operands' type takes away.  Where the base is larger (that error
-// grows to any size: at 2^30 a weight would be 2^32, or 0 in every type) and in fp32, top is subtracted first, and its weight is exactly 1.
+// then 2^LIFT times exp2 of that rounding's error, at most 2^-12 up to a base of 2^12, which the rounding to the operands' type takes away.  Where the base is larger (that error
+// grows to any size: at 2^30 a weight would be 2^32, or 0 in every type) and in fp32, top is subtracted first, and its weight is exactly 2^LIFT.
 constexpr float ATT_LARGEST_BASE = 4096.0f;
 
 template <typename T>
@@ -369,7 +374,7 @@ __device__ __forceinline__ void att_relative_to(float top, float scale_log2, flo
     const float product = top * scale_log2;
     const bool shifted = sizeof(T) == 4 || !(fabsf(product) < ATT_LARGEST_BASE);
     *shift = shifted ? top : 0.0f;
-    *base = shifted ? 0.0f : product;
+    *base = shifted ? -ATT_LIFT<T> : __builtin_fmaf(top, scale_log2, -ATT_LIFT<T>);
 }
 
 // The log of a row's sum of exponentials from that relative to the shift, to base 2.  -inf stands for a row without keys and for no other.
@@ -380,7 +385,7 @@ __device__ __forceinline__ float att_natural_lse(float shift, float lse2, float 
     return lse == -__builtin_inff() ? -__FLT_MAX__ : lse;
 }
 
-// Outputs and sums are rescaled only when a score passes the one they are relative to by 2^8: exponentials stay below 256, far inside every type,
+// Outputs and sums are rescaled only when a score passes the one they are relative to by 2^8: weights stay below 2^(8 + LIFT), inside every type,
 // and after the first tiles the 64 or more multiplications per tile are not made.
 constexpr float ATT_HEADROOM = 8.0f;
 
@@ -464,8 +469,8 @@ __device__ __forceinline__ float att_scores(att_f32x16 (&s)[KT / 32], const att_
 }
 
 // Masks a tile's scores (`kept` has a bit per key, the same in all lanes; with `causal`, this lane's row meets the first `limit` of them only) and, where
-// the weight of one would pass 2^8, makes the weights relative to the largest, whose own is then 1 in the operands' type (a row of one key gets its value without
-// a rounding).  What was made before is rescaled: output and sum, and `weights` that wait for their product and are rounded once more.  Shifts are
+// the weight of one would pass 2^(8 + LIFT), makes the weights relative to the largest, whose own is then 2^LIFT in the operands' type (a row of one key gets its value
+// without a rounding).  What was made before is rescaled: output and sum, and `weights` that wait for their product and are rounded once more.  Shifts are
 // subtracted from the scores.
 template <typename T, int DP, int KT>
 __device__ __forceinline__ void att_rebase(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], att_f32x16 (&s)[KT / 32], float top, float scale_log2, att_u64 kept,
@@ -498,11 +503,11 @@ __device__ __forceinline__ void att_rebase(AttState<DP> &state, att_vec8<T> (&we
     }
     top = att_max_of_halves(top);
     const float above = __builtin_fmaf(top - state.shift, scale_log2, -state.base);     // the largest weight, to base 2; not a number without keys
-    if (__any(above > ATT_HEADROOM)) {
+    if (__any(above > ATT_HEADROOM + ATT_LIFT<T>)) {
         att_rare();
         float shift, base, shrink = 1.0f;
         att_relative_to<T>(top, scale_log2, &shift, &base);
-        if (above > 0.0f) {
+        if (above > ATT_LIFT<T>) {
             shrink = __builtin_amdgcn_exp2f(__builtin_fmaf(state.shift - shift, scale_log2, state.base - base));
             state.shift = shift;
             state.base = base;
