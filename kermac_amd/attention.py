@@ -294,8 +294,9 @@ def cross_attention_grad(
     ``out`` and ``lse`` are what ``cross_attention(..., return_lse=True)`` returned for the same tensors, scale, lengths and
     mask.  The gradient of a head of keys and values is the sum over the heads of queries that share it; that of keys and
     values of batch size 1 is the sum over the batch.  Keys that do not take part have a gradient of zero, and so has a query without
-    keys.  Sums are fp32 in an order that does not depend on timing; in fp16 the products of weights and gradients are
-    numbers of that type, so gradients far below 1e-4 want a loss scale.
+    keys.  Sums are fp32 in an order that does not depend on timing.  In fp16, the gradients of the scores, ``p * (d v - sum p d v)`` with
+    ``d`` the gradient of the result and without ``scale``, are numbers of that type: what passes 65504 becomes infinite, what is below ``6e-8`` is lost,
+    and a loss scale has to bring them in between.
 
     Returns ``(grad_queries, grad_keys, grad_values)``, new contiguous tensors with the shapes of the inputs.  Takes 8 bytes of
     scratch memory per row at least.  Scores of any size want 4 more (and 4 per 128 rows): where a limit leaves only those 8, weights of a row

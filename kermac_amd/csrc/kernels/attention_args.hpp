@@ -57,7 +57,7 @@ struct AttentionGradArgs {
     int l, m, g, r, k, o;
     int key_entries;                        // l, or 1: one source for all entries
     float scale, scale_log2, query_factor;
-    float *stats;                           // [2, l, g r, m]: lse to base 2 (+inf without keys) and delta, from the first kernel for the second; behind them +inf and 0
+    float *stats;                           // [2, l, g r, m]: lse to base 2 (+inf without keys) and delta, for weights times a power of two, from the first kernel for the second; behind them +inf and 0
     // For rows of large scores, or null: [l, g r, m], what is subtracted from a row's scores in front of the scale, and [l, g, q_row_tiles], whether a tile of 128 rows
     // has such rows (their lse is the one beside the shift).
     float *row_shift;

@@ -10,7 +10,8 @@
 //
 // As in the forward kernel, a product's result registers are the next product's operand: the rows' kernel computes s^T[n, row]
 // and multiplies K^T ds^T, the keys' kernel computes s[row, n] and multiplies d^T p and q^T ds.  p and ds are rounded to the
-// operands' type for that (ds in fp16 keeps numbers down to 6e-8: gradients far below 1e-4 want the usual loss scaling).
+// operands' type for that.  In fp16, p is 2^15 times itself there, so that many keys of small weights keep their bits; ds, which is as it stands above, without the
+// scale, has to lie between 6e-8 and 65504 in magnitude: gradients of the result want a loss scale that brings them there.
 #pragma once
 
 #include "attention.hpp"
@@ -35,6 +36,10 @@ __device__ __forceinline__ float att_weight(float s, float scale_log2, float lse
 // p is then off by as a factor; at 2^30 that factor is any power of two up to 2^64.  The queries' kernel walks the keys of such rows once more in front, for the
 // largest score, the sum of the exponentials relative to it and delta; p is then exp2((s - largest) scale_log2 - log2(sum)), as in the forward kernel.
 constexpr float ATT_LARGEST_LSE = ATT_LARGEST_BASE * ATT_LN_2;
+
+// Powers of two in the keys' kernel, where p is an operand: p times 2^LIFT, which is at most 2^15 in fp16; the sums of grad_v and the factor of ds take it out.
+template <typename T> constexpr float ATT_GRAD_LIFT = std::is_same<T, _Float16>::value ? 15.0f : 0.0f;
+template <typename T> constexpr float ATT_GRAD_LOWER = std::is_same<T, _Float16>::value ? 0x1p-15f : 1.0f;
 
 // lse to base 2 for the exponentials; a row without keys gets +inf, which makes all its weights 0.
 __device__ __forceinline__ float att_lse2(float lse) { return lse == -__builtin_inff() ? __builtin_inff() : lse * ATT_LOG2_E; }
@@ -198,8 +203,8 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     }
     if (split == 0 && row < rows && half == 0) {
         float *stats = args.stats + (static_cast<i64>(entry) * args.g * args.r + head) * args.m + token;
-        stats[0] = lse2;
-        stats[rows_total] = delta;
+        stats[0] = lse2 - ATT_GRAD_LIFT<T>;
+        stats[rows_total] = delta * ATT_GRAD_LOWER<T>;
         if (args.row_shift) args.row_shift[stats - args.stats] = shift;
     }
     if (args.row_flags && split == 0 && threadIdx.x == 0) args.row_flags[(static_cast<i64>(entry) * args.g + g) * args.q_row_tiles + row_tile] = large;
@@ -454,7 +459,8 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
         auto make_gradients = [&](const att_f32x16 &ds, int q) {
             const att_f32x4 delta = *reinterpret_cast<const att_f32x4 *>(all_stats[now] + RT + 8 * q + 4 * half);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[q / 2][4 * (q % 2) + j] = static_cast<T>(weight[4 * q + j] * (ds[4 * q + j] - delta[j]));
+            for (int j = 0; j < 4; ++j)
+                x[q / 2][4 * (q % 2) + j] = static_cast<T>(weight[4 * q + j] * __builtin_fmaf(ds[4 * q + j], ATT_GRAD_LOWER<T>, -delta[j]));
         };
         auto products = [&](att_f32x16 &ds) {
             const att_lds_byte *q_tile = lds + 2 * now * TILE, *d_tile = q_tile + TILE;
@@ -574,7 +580,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
         return;
     }
     if (OF_KEYS) att_store_columns<T, DP, ALIGNED>(static_cast<T *>(args.grad_k) + at * args.k, acc_k, args.scale, args.k, half);
-    if (OF_VALUES) att_store_columns<T, DP, ALIGNED>(static_cast<T *>(args.grad_v) + at * args.o, acc_v, 1.0f, args.o, half);
+    if (OF_VALUES) att_store_columns<T, DP, ALIGNED>(static_cast<T *>(args.grad_v) + at * args.o, acc_v, ATT_GRAD_LOWER<T>, args.o, half);
 }
 
 // The parts of a cut gradient, added in their order.

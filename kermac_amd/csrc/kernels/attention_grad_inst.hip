@@ -53,7 +53,7 @@ hipError_t KMC_ATT_NAME(launch_attention_gradient)(const kmc::AttentionGradArgs 
     const kmc::AttentionSum parts[3] = {
         {args.partial_q, args.grad_q, args.q_splits > 1 ? q_rows : 0, args.q_splits, args.k, args.partial_k_width, args.scale},
         {args.partial_k, args.grad_k, k_rows, args.k_splits, args.k, args.partial_k_width, args.scale},
-        {args.partial_v, args.grad_v, k_rows, args.k_splits, args.o, args.partial_o_width, 1.0f}};
+        {args.partial_v, args.grad_v, k_rows, args.k_splits, args.o, args.partial_o_width, kmc::ATT_GRAD_LOWER<Element>}};
     kmc::AttentionSumArgs sums = {};
     for (int i = 0; i < 3; ++i) {
         sums.part[i] = parts[i];
