@@ -7,6 +7,7 @@ library travels with the source tree; nothing is installed elsewhere.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -90,6 +91,17 @@ def _jobs():
     return jobs
 
 
+def ordered_kernels_that_spill(remarks: str) -> list:
+    """The attention kernels with a fixed order of instructions (their last template argument is true) that the compiler's
+    -Rpass-analysis=kernel-resource-usage reports with vector registers in memory."""
+    spilling = []
+    for block in remarks.split("Function Name: ")[1:]:
+        name, spilled = block.split(maxsplit=1)[0], re.search(r"VGPRs Spill: (\d+)", block)
+        if re.search(r"Lb1E+v", name) and (spilled is None or int(spilled.group(1)) > 0):
+            spilling.append(name)
+    return spilling
+
+
 def _newest_source_mtime() -> float:
     newest = 0.0
     for path in list(CSRC.rglob("*")) + [Path(__file__), PACKAGE_DIR.parent / "include" / "kermac_amd.h"]:
@@ -118,12 +130,18 @@ def build(force: bool = True, verbose: bool = False, workers: int | None = None,
         src, obj, defines = job
         if not force and obj.exists() and obj.stat().st_mtime > newest:
             return obj
-        cmd = [hipcc, *HIPCC_FLAGS, *extra_flags, *defines, "-c", str(src), "-o", str(obj)]
+        attention = src.name.startswith("attention") and src.suffix == ".hip"
+        remarks = ["-Rpass-analysis=kernel-resource-usage"] if attention else []
+        cmd = [hipcc, *HIPCC_FLAGS, *remarks, *extra_flags, *defines, "-c", str(src), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd), flush=True)
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError(f"hipcc failed for {src.name} {defines}:\n{proc.stdout}\n{proc.stderr}")
+        spilling = ordered_kernels_that_spill(proc.stderr) if attention else []
+        if spilling:
+            obj.unlink()
+            raise RuntimeError(f"{src.name} {defines}: kernels with a fixed order of instructions spill registers: {', '.join(spilling)}")
         return obj
 
     workers = workers or min(8, os.cpu_count() or 1)

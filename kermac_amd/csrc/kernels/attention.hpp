@@ -391,12 +391,14 @@ constexpr float ATT_HEADROOM = 8.0f;
 
 // Fragments are read from LDS a group ahead of the matrix instructions that use them.  The compiler, left alone, reads each one in front of its
 // use and waits for it; these fix the order within a region: READS reads, then the matrix instructions, each followed by VALU vector instructions.
-// Not above 128 features: those kernels have more values than registers, and with a fixed order around the spilled ones the compiler's code
-// for fp32 gave gradients of the queries that were off by 9 % (right without, and in every kernel that spills nothing).
-template <int DP, int READS, int MMAS, int VALU>
+// Only in kernels that have registers for all their values: with a fixed order around spilled ones, the compiler's code for fp32 of 256 features
+// gave gradients of the queries that were off by 9 % (right without).  The build refuses an ORDERED kernel that spills.
+template <typename T, int DP, bool ALIGNED> constexpr bool ATT_ORDERED = ALIGNED && DP <= 128;
+
+template <bool ORDERED, int READS, int MMAS, int VALU>
 __device__ __forceinline__ void att_order()
 {
-    if constexpr (DP <= 128) {
+    if constexpr (ORDERED) {
         __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
 #pragma unroll
         for (int i = 0; i < MMAS; ++i) {
@@ -405,10 +407,10 @@ __device__ __forceinline__ void att_order()
         }
     }
 }
-template <int DP>
+template <bool ORDERED>
 __device__ __forceinline__ void att_region()
 {
-    if constexpr (DP <= 128) __builtin_amdgcn_sched_barrier(0);
+    if constexpr (ORDERED) __builtin_amdgcn_sched_barrier(0);
 }
 
 template <typename T, int DP>
@@ -440,7 +442,7 @@ __device__ __forceinline__ void att_read_columns(att_vec8<T> (&f)[COLUMNS], cons
 
 // s^T of a tile of KT keys in LDS and the 32 rows whose queries are in `query`, and the largest of each lane's scores.  One block of 32 keys after the
 // other; the maximum over a block is taken beside the matrix instructions of the next.
-template <typename T, int DP, int KT>
+template <typename T, int DP, int KT, bool ORDERED>
 __device__ __forceinline__ float att_scores(att_f32x16 (&s)[KT / 32], const att_vec8<T> (&query)[DP / 16], const att_lds_byte *keys, int lane)
 {
     typedef AttGroups<T, DP> G;
@@ -450,7 +452,7 @@ __device__ __forceinline__ float att_scores(att_f32x16 (&s)[KT / 32], const att_
 #pragma unroll
     for (int b = 0; b < KT / 32; ++b) s[b] = att_f32x16{0};
     float top = -__builtin_inff();
-    att_region<DP>();
+    att_region<ORDERED>();
 #pragma unroll
     for (int i = 0; i < ALL; ++i) {
         const int b = i / G::GROUPS, group = i % G::GROUPS;
@@ -460,8 +462,8 @@ __device__ __forceinline__ float att_scores(att_f32x16 (&s)[KT / 32], const att_
         if (b > 0)
 #pragma unroll
             for (int j = EACH * group; j < (group + 1 == G::GROUPS ? 16 : EACH * (group + 1)); ++j) top = fmaxf(top, s[b - 1][j]);
-        att_order<DP, G::GROUP * G::READS_ROW, G::GROUP * G::MMAS, 0>();
-        att_region<DP>();
+        att_order<ORDERED, G::GROUP * G::READS_ROW, G::GROUP * G::MMAS, 0>();
+        att_region<ORDERED>();
     }
 #pragma unroll
     for (int j = 0; j < 16; ++j) top = fmaxf(top, s[KT / 32 - 1][j]);
@@ -547,7 +549,7 @@ __device__ __forceinline__ att_vec8<T> att_weights(AttState<DP> &state, const at
 }
 
 // out^T += V^T p^T over the KT keys of a tile; with NEXT, the weights give way to those of the scores s.  `first`: the first group of V's columns.
-template <typename T, int DP, int KT, bool NEXT>
+template <typename T, int DP, int KT, bool NEXT, bool ORDERED>
 __device__ __forceinline__ void att_add_values(AttState<DP> &state, att_vec8<T> (&weights)[KT / 16], const att_lds_byte *values,
                                                const att_vec8<T> (&first)[AttGroups<T, DP>::COLUMNS], const att_f32x16 (&s)[KT / 32], float scale_log2, float base,
                                                int lane)
@@ -568,8 +570,8 @@ __device__ __forceinline__ void att_add_values(AttState<DP> &state, att_vec8<T> 
         }
         const bool last = group + 1 == G::COLUMN_GROUPS;
         if (NEXT && last) weights[step] = att_weights<T, DP, KT>(state, s, step, scale_log2, base);
-        att_order<DP, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, NEXT ? (G::MMAS > 1 ? 1 : DP <= 64 ? 14 : 7) : 0>();
-        att_region<DP>();
+        att_order<ORDERED, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, NEXT ? (G::MMAS > 1 ? 1 : DP <= 64 ? 14 : 7) : 0>();
+        att_region<ORDERED>();
     }
 }
 
@@ -702,7 +704,7 @@ __device__ __forceinline__ void att_load_queries(const AttentionArgs &args, cons
 // At most 32 rows (single tokens): reading keys and values is all the work, so every wave walks tiles of its own without waiting for the others,
 // and the waves' results are joined at the end.  32 entries x 1 query x up to 4000 keys x 16 heads of 64 bf16: 89 us, 4.4 TB/s (a large copy
 // reaches 4.8); 4 x 32768 keys x 16 heads of 128: 194 us, 5.5 TB/s.
-template <typename T, int DP, bool ALIGNED>
+template <typename T, int DP, bool ALIGNED, bool ORDERED = ATT_ORDERED<T, DP, ALIGNED>>
 __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void attention_forward(const AttentionArgs args)
 {
     typedef AttForwardShape<T, DP> Shape;
@@ -814,7 +816,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
             att_u64 kept = kept_keys(begin);
             ask(begin, kept);
             if (works) {
-                top = att_scores<T, DP, KT>(s, query, key_ring, lane);
+                top = att_scores<T, DP, KT, ORDERED>(s, query, key_ring, lane);
                 rebase(begin, kept);
 #pragma unroll
                 for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, scale_log2, base);
@@ -825,17 +827,17 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                 ask(n, kept);
                 if (works) {
                     const att_lds_byte *values = value_ring + (now ^ 1) * TILE;
-                    top = att_scores<T, DP, KT>(s, query, key_ring + now * TILE, lane);
+                    top = att_scores<T, DP, KT, ORDERED>(s, query, key_ring + now * TILE, lane);
                     att_read_columns<T, DP>(first, values, 0, 0, lane);
                     rebase(n, kept);
-                    att_add_values<T, DP, KT, true>(state, weights, values, first, s, scale_log2, base, lane);
+                    att_add_values<T, DP, KT, true, ORDERED>(state, weights, values, first, s, scale_log2, base, lane);
                 }
                 got(n);
             }
             if (works) {
                 const att_lds_byte *values = value_ring + (now ^ 1) * TILE;
                 att_read_columns<T, DP>(first, values, 0, 0, lane);
-                att_add_values<T, DP, KT, false>(state, weights, values, first, s, 0.0f, base, lane);
+                att_add_values<T, DP, KT, false, ORDERED>(state, weights, values, first, s, 0.0f, base, lane);
             }
         }
         if (!works) return;
@@ -887,7 +889,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                 next_k.finish(key_tile, lane);
                 if (TURNS) {
                     att_wave_sync();
-                    top = att_scores<T, DP, KT>(s, query, key_tile, lane);
+                    top = att_scores<T, DP, KT, ORDERED>(s, query, key_tile, lane);
                     att_wave_sync();
                     att_wait_for_reads();
                     ask_values(n, kept);
@@ -899,14 +901,14 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
                         ask_keys(at);
                         ask_values(at, then_kept);
                     }
-                    top = att_scores<T, DP, KT>(s, query, key_tile, lane);
+                    top = att_scores<T, DP, KT, ORDERED>(s, query, key_tile, lane);
                 }
                 att_rebase<T, DP, KT>(state, weights, s, top, args.scale_log2, kept, keys.causal, limit - static_cast<int>(n), lane);
                 const float base = state.base;
 #pragma unroll
                 for (int step = 0; step < KT / 16; ++step) weights[step] = att_weights<T, DP, KT>(state, s, step, args.scale_log2, base);
                 att_read_columns<T, DP>(first, value_tile, 0, 0, lane);
-                att_add_values<T, DP, KT, false>(state, weights, value_tile, first, s, 0.0f, base, lane);
+                att_add_values<T, DP, KT, false, ORDERED>(state, weights, value_tile, first, s, 0.0f, base, lane);
                 att_wave_sync();
                 kept = then_kept;
             }

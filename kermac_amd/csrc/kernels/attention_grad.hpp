@@ -47,7 +47,7 @@ __device__ __forceinline__ float att_lse2(float lse) { return lse == -__builtin_
 // Two products of 32 rows of two tiles in LDS with operands of the wave's own, by turns: s (scores) and ds (gradients of the result times values).
 // Between the matrix instructions, with VECTOR, the vector work of the scores before: `quad(q)` makes the weights of registers
 // 4 q .. 4 q + 3.
-template <typename T, int DP, bool VECTOR, bool BOTH = true, typename Quad>
+template <typename T, int DP, bool ORDERED, bool VECTOR, bool BOTH = true, typename Quad>
 __device__ __forceinline__ void att_two_scores(att_f32x16 &s, att_f32x16 &ds, const att_lds_byte *s_tile, const att_vec8<T> (&s_own)[DP / 16],
                                                const att_lds_byte *ds_tile, const att_vec8<T> (&ds_own)[DP / 16], int lane, Quad quad)
 {
@@ -63,7 +63,7 @@ __device__ __forceinline__ void att_two_scores(att_f32x16 &s, att_f32x16 &ds, co
     };
     read(f[0], 0);
     s = ds = att_f32x16{0};
-    att_region<DP>();
+    att_region<ORDERED>();
 #pragma unroll
     for (int i = 0; i < ALL; ++i) {
         if (i + 1 < ALL) read(f[(i + 1) & 1], i + 1);
@@ -75,14 +75,14 @@ __device__ __forceinline__ void att_two_scores(att_f32x16 &s, att_f32x16 &ds, co
         if (VECTOR)
 #pragma unroll
             for (int q = 4 * i / ALL; q < 4 * (i + 1) / ALL; ++q) quad(q);
-        att_order<DP, 2 * AT_ONCE * G::READS_ROW, 2 * AT_ONCE * G::MMAS, VECTOR ? (sizeof(T) == 4 ? 1 : 48 / (2 * G::STEPS) + 1) : 0>();
-        att_region<DP>();
+        att_order<ORDERED, 2 * AT_ONCE * G::READS_ROW, 2 * AT_ONCE * G::MMAS, VECTOR ? (sizeof(T) == 4 ? 1 : 48 / (2 * G::STEPS) + 1) : 0>();
+        att_region<ORDERED>();
     }
 }
 
 // A workgroup per (batch entry, head of keys, range of keys, 128 rows); a wave per 32 rows, whose queries and gradients it keeps in registers.
 // Three products, two of which share what is read of a tile: 1.45 ms at 4 x 4096 x 4096, 32 heads on 8 x 128 bf16, the matrix cores busy 60 % of the time.
-template <typename T, int DP, bool ALIGNED>
+template <typename T, int DP, bool ALIGNED, bool ORDERED = ATT_ORDERED<T, DP, ALIGNED>>
 __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void attention_grad_queries(const AttentionGradArgs args)
 {
     typedef AttGradShape<T, DP> Shape;
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
             typedef AttGroups<T, DP> G;
             att_vec8<T> x[2], f[2][G::COLUMNS];
             const att_lds_byte *block = key_tile + b * BLOCK;
-            att_two_scores<T, DP, false>(s, ds, block, query, value_tile + b * BLOCK, grad, lane, [](int) {});
+            att_two_scores<T, DP, ORDERED, false>(s, ds, block, query, value_tile + b * BLOCK, grad, lane, [](int) {});
             att_read_columns<T, DP>(f[0], block, 0, 0, lane);
             const unsigned here = static_cast<unsigned>(kept >> (32 * b));
             if (large || here != ~0u) {
@@ -279,8 +279,8 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
 #pragma unroll
                 for (int o = 0; o < G::COLUMNS; ++o) acc[G::COLUMNS * group + o] = att_mma(f[i & 1][o], x[step], acc[G::COLUMNS * group + o]);
                 if (G::COLUMN_GROUPS > 1) {
-                    att_order<DP, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, 0>();
-                    att_region<DP>();
+                    att_order<ORDERED, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, 0>();
+                    att_region<ORDERED>();
                 }
             }
         }
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
 // the scores are computed twice (2 x 1000 x 1500 x 8 heads of 256: 814 us for both, 1180 in one launch with its spills).
 enum AttKeysPart { ATT_BOTH, ATT_GRAD_KEYS, ATT_GRAD_VALUES };
 
-template <typename T, int DP, bool ALIGNED, AttKeysPart PART>
+template <typename T, int DP, bool ALIGNED, AttKeysPart PART, bool ORDERED = ATT_ORDERED<T, DP, ALIGNED>>
 __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void attention_grad_keys(const AttentionGradArgs args)
 {
     typedef AttGradShape<T, DP> Shape;
@@ -375,10 +375,11 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
         const int first = static_cast<int>(part_first > e * per_entry ? part_first - e * per_entry : 0);
         const int count = static_cast<int>((part_last < (e + 1) * per_entry ? part_last - e * per_entry : per_entry) - first);
         const int length = att_length(keys, entry);
-        if (!(att_kept_keys(keys, entry, first_key, length, lane) | att_kept_keys(keys, entry, first_key + 64, length, lane))) continue;
+        const att_u64 kept_keys[2] = {att_kept_keys(keys, entry, first_key, length, lane), att_kept_keys(keys, entry, first_key + 64, length, lane)};
+        if (!(kept_keys[0] | kept_keys[1])) continue;
         // A key that does not take part has a column of the products of its own, whatever it holds: its gradient is set to zero at the end, unless another entry
         // that shares it adds to it.
-        const bool kept = exists && n < length && (!keys.mask || keys.mask[entry * keys.mask_ls + n * keys.mask_ns] != 0);
+        const bool kept = static_cast<unsigned>(kept_keys[wave >> 1] >> (32 * (wave & 1))) >> (lane & 31) & 1;
         const bool clear = entries > 1 && !__all(kept);
         ever_kept |= kept;
         bool large = false;                                 // a row of this entry and head of keys has a shift
@@ -488,7 +489,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
                 att_read_columns<T, DP>(to, step < 2 ? d_tile : q_tile, 16 * (step % 2), i % G::COLUMN_GROUPS, lane);
             };
             read(f[0], FIRST);
-            att_region<DP>();
+            att_region<ORDERED>();
 #pragma unroll
             for (int i = FIRST; i < ALL; ++i) {
                 const int step = i / G::COLUMN_GROUPS, group = i % G::COLUMN_GROUPS;
@@ -501,11 +502,11 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
                 if (OF_KEYS && step < 2 && group == 0) {
                     make_gradients(ds, 2 * step);
                     make_gradients(ds, 2 * step + 1);
-                    att_order<DP, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, (G::MMAS > 1 ? 2 : 24 / G::COLUMNS)>();
+                    att_order<ORDERED, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, (G::MMAS > 1 ? 2 : 24 / G::COLUMNS)>();
                 } else {
-                    att_order<DP, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, 0>();
+                    att_order<ORDERED, G::COLUMNS * G::READS_T, G::COLUMNS * G::MMAS, 0>();
                 }
-                att_region<DP>();
+                att_region<ORDERED>();
             }
         };
         auto next_tile = [&]() {
@@ -517,7 +518,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
             shift_scores(s);
             begin();
             const att_lds_byte *q_tile = lds + 2 * then() * TILE;
-            att_two_scores<T, DP, true>(next_s, next_ds, q_tile, key, q_tile + TILE, value, lane, [&](int q) { make_weights(s, q); });
+            att_two_scores<T, DP, ORDERED, true>(next_s, next_ds, q_tile, key, q_tile + TILE, value, lane, [&](int q) { make_weights(s, q); });
             products(ds);
             next_tile();
         };
@@ -531,7 +532,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
         att_wait_for_loads();
         __syncthreads();
         if constexpr (OVERLAP) {
-            att_two_scores<T, DP, false>(s_a, ds_a, lds, key, lds + TILE, value, lane, [](int) {});
+            att_two_scores<T, DP, ORDERED, false>(s_a, ds_a, lds, key, lds + TILE, value, lane, [](int) {});
             int i = 1;
             for (; i + 1 < count; i += 2) {
                 turn(s_a, ds_a, s_b, ds_b);
@@ -551,7 +552,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
             for (int i = 0; i < count; ++i) {
                 begin();
                 const att_lds_byte *q_tile = lds + 2 * now * TILE;
-                att_two_scores<T, DP, false, OF_KEYS>(s_a, ds_a, q_tile, key, q_tile + TILE, value, lane, [](int) {});
+                att_two_scores<T, DP, ORDERED, false, OF_KEYS>(s_a, ds_a, q_tile, key, q_tile + TILE, value, lane, [](int) {});
                 shift_scores(s_a);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) make_weights(s_a, q);
