@@ -79,12 +79,15 @@ constexpr int ROWS_OF_OWN_KEYS = 32;                // up to here every wave wal
 // How many parts the keys are cut into: the number with the smallest modelled time, in microseconds, fitted to sweeps of 1 .. 64 parts.
 //   Tiles of rows (bound by the matrix cores): 128 rows meet 64 keys in 2.1 us per 128 features in 16 bits (fp32: 7 times as long) while two
 //   workgroups share a CU, in 0.65 of that alone; a launch of more workgroups than fit waits for half of one at its end.
-//   Beside another job (`beside_us` of its own) the two share the chip.  Rows of more than 256 bytes let one workgroup on a CU.
+//   Beside another job (`beside_us` of its own) the two share the chip, and half of that job's time is in the way.  Rows of more than 256 bytes let one workgroup on a CU.
 //   Single tokens (bound by memory): keys and values at 4.7 TB/s, but no workgroup faster than 4 us and 1.05 us per 128 keys of 128 features, and
-//   3.5 us of its place for a workgroup; the launch waits for the last ones, with lengths that differ for the longest.
+//   3.5 us of its place for a workgroup; the launch waits for the last ones.
 //   Joining the parts costs a launch, 5 us, and writing and reading a partial result per part.
-// 1 token against 32000 keys of 8 heads: 257 us in 1 part, 34.6 in the 32 of this rule, 32.2 in the best number, 16; 200 queries against 3000 keys 49.9 / 16.1;
-// 32 x 4000 x 16 heads of 64 features with lengths 82.9 / 75.7 (4 parts), best 73.3 (6); 128 x 1000 x 16 heads 92.1 uncut, 99.7 in 2 parts.
+// How many of the keys take part is not known here: it plans for all of them, whether there are lengths or not (an entry's own length is cut into the parts evenly).
+// 1 token against 32000 keys of 8 heads: 257 us in 1 part, 34.8 in the 32 of this rule, 32.8 in the best number, 16; 4 x 200 queries against 3000 keys of 4 heads 47.3 in 4, the best;
+// 256 x 1000 x 4 heads uncut 100, the best.  11 shapes with lengths of about 5, 25, 50, 75 and 100 % of the keys: above the best number of parts of each by 19, 5, 6, 6 and 5 %
+// in the geometric mean (planned for three quarters of the keys where there are lengths: 32, 8, 7, 6 and 5 %).  8 shapes behind a prefix, with about 10, 50, 75 and 100 % of the own keys:
+// 15, 7, 5 and 7 % above the best numbers of both (with all of the other job's time in the way and that plan 26, 14, 10 and 11 %).
 double time_of_parts(int splits, int64_t base, int64_t rows_total, int64_t keys, bool own_keys, const kmc_attention_params *p, bool joined, double beside_us)
 {
     const double size = element_size(p->type), width = padded_width(std::max(p->k, p->o));
@@ -93,11 +96,11 @@ double time_of_parts(int splits, int64_t base, int64_t rows_total, int64_t keys,
     const double join_us = (splits > 1 || joined ? rows_total * p->o * 8.0 / 4.0e6 * splits : 0.0) + (splits > 1 && !joined ? 5.0 : 0.0);
     if (own_keys) {
         const double one = 4.0 + steps * 1.05 * width / 128 * (p->type == KMC_FP32 ? 5.5 : 1.0);
-        const double memory = keys * static_cast<double>(base) * (p->k + p->o) * size / 4.7e6 * (p->key_lengths ? 0.75 : 1.0);
-        return join_us + std::max(memory, one) + workgroups * 3.5 / 512 + one * (p->key_lengths ? 1.0 : 0.3);
+        const double memory = keys * static_cast<double>(base) * (p->k + p->o) * size / 4.7e6;
+        return join_us + std::max(memory, one) + workgroups * 3.5 / 512 + one * 0.3;
     }
     const double tile_us = 2.1 * width / 128 * (p->type == KMC_FP32 ? 7.0 : 1.0), one = steps * tile_us;
-    if (beside_us > 0) return join_us + std::max(one, workgroups * one / 512 + beside_us);
+    if (beside_us > 0) return join_us + std::max(one, workgroups * one / 512 + 0.5 * beside_us);
     // rows of more than 256 bytes: one workgroup per CU, whole rounds of which the last one counts
     if (width * size > 256) return join_us + 0.55 * one * ((workgroups + 255) / 256);
     return join_us + (workgroups <= 256 ? 0.65 * one : workgroups <= 512 ? one : workgroups * one / 512 + 0.5 * one);

@@ -255,3 +255,12 @@ def test_a_prefix_alone_makes_the_own_keys_causal():
     for change in (dict(key_lengths=None), dict(key_mask=16)):
         with pytest.raises(_backend.BackendError, match="prefix"):
             _backend.attention_workspace_bytes(library_parameters(causal=0, **change))
+
+
+@pytest.mark.parametrize("L, M, N, H, G", [(8, 1, 32000, 32, 8), (16, 1, 8192, 32, 8), (1, 1, 32000, 8, 8), (128, 1, 8192, 32, 8), (2, 200, 3000, 8, 8)])
+def test_lengths_do_not_change_the_parts(L, M, N, H, G):
+    """How full the keys are is not known when the work is cut: a call with lengths is cut as one without."""
+    q, k = make(1, M, H, 128, dtype=torch.bfloat16).expand(L, M, H, 128), make(1, N, G, 128, dtype=torch.bfloat16).expand(L, N, G, 128)
+    out = torch.empty(L, M, H, 128, dtype=torch.bfloat16)
+    with_lengths, without = (_backend.attention_workspace_bytes(plan(q, k, k, out=out, key_lengths=lengths).params) for lengths in (torch.zeros(L, dtype=torch.int32), None))
+    assert with_lengths == without
