@@ -17,7 +17,11 @@ def llvm(tool):
 
 
 def spills(tmp_path):
-    """{kernel: spilled vector registers} from the metadata of the library's code objects."""
+    return {name: count for name, (count, _) in metadata(tmp_path, b"attention_").items()}
+
+
+def metadata(tmp_path, part):
+    """{kernel: (spilled vector registers, accumulation registers)} from the library's code objects that hold `part`."""
     fat = tmp_path / "fat"
     subprocess.run([llvm("llvm-objcopy"), f"--dump-section=.hip_fatbin={fat}", str(_backend.LIB_PATH), str(tmp_path / "copy.so")], check=True)
     blob, found = fat.read_bytes(), {}
@@ -29,12 +33,13 @@ def spills(tmp_path):
             target = blob[entry + 24:entry + 24 + length].decode()
             entry += 24 + length
             code = blob[at + start:at + start + size]
-            if "gfx950" in target and b"attention_" in code:
+            if "gfx950" in target and part in code:
                 path = tmp_path / f"{at}.co"
                 path.write_bytes(code)
                 notes = subprocess.run([llvm("llvm-readelf"), "--notes", str(path)], check=True, capture_output=True, text=True).stdout
                 for kernel in re.split(r"\n\s+- \.agpr_count", notes)[1:]:
-                    found[re.search(r"\.name:\s+(\S+)", kernel).group(1)] = int(re.search(r"\.vgpr_spill_count:\s+(\d+)", kernel).group(1))
+                    found[re.search(r"\.name:\s+(\S+)", kernel).group(1)] = (int(re.search(r"\.vgpr_spill_count:\s+(\d+)", kernel).group(1)),
+                                                                               int(re.match(r":\s+(\d+)", kernel).group(1)))
     return found
 
 
@@ -55,3 +60,19 @@ def test_the_build_refuses_an_ordered_kernel_that_spills():
     ordered, free = "_ZN3kmc17attention_forwardIfLi64ELb1ELb1EEEvNS_13AttentionArgsE", "_ZN3kmc17attention_forwardIfLi256ELb1ELb0EEEvNS_13AttentionArgsE"
     assert _build.ordered_kernels_that_spill(remark(ordered, 0) + remark(free, 80)) == []
     assert _build.ordered_kernels_that_spill(remark(free, 0) + remark(ordered, 1)) == [ordered]
+
+
+def test_spilled_values_stay_out_of_accumulation_registers():
+    """The compiler loses registers of values that it spills partly to accumulation registers: the units whose kernels spill with such registers are built without.
+
+    All other kernels of the library that spill have none of them."""
+    attention = [src for src, _, _ in _build._jobs() if _build.is_attention(src)]
+    assert len(attention) == 6
+    at = _build.ATTENTION_FLAGS.index("-amdgpu-spill-vgpr-to-agpr=0")
+    assert _build.ATTENTION_FLAGS[at - 1] == "-mllvm"
+
+
+def test_other_kernels_that_spill_have_no_accumulation_registers(tmp_path):
+    """(the count of these registers that a kernel's metadata gives, beside its spills)"""
+    for name, (count, accumulation) in metadata(tmp_path, b"").items():
+        assert "attention_" in name or count == 0 or accumulation == 0, name
