@@ -256,7 +256,9 @@ struct AttTile {
 
     static __device__ __forceinline__ bool has_row(att_u64 kept, int row, int j) { return static_cast<unsigned>(kept >> (j * ROW_STEP)) >> row & 1; }
 
-    // DIRECT, from a tile's descriptor
+    // DIRECT, from a tile's descriptor.  A load may read a scalar register that a vector instruction wrote only 5 wait states behind it, which the hardware does not wait for
+    // and the compiler does not see to in front of assembly.  Five here cost up to 2 % (16 questions behind a prefix 198 -> 203 us), and scalar instructions or six other states
+    // stand in between wherever the compiler puts a descriptor together: a test reads that from the built library.
     __device__ __forceinline__ void begin_at(att_s32x4 from, int step, int width, att_lds_byte *tile, int thread, att_u64 kept = ~0ull)
     {
         constexpr int SIZE = static_cast<int>(sizeof(T));

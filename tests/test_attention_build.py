@@ -76,3 +76,77 @@ def test_other_kernels_that_spill_have_no_accumulation_registers(tmp_path):
     """(the count of these registers that a kernel's metadata gives, beside its spills)"""
     for name, (count, accumulation) in metadata(tmp_path, b"").items():
         assert "attention_" in name or count == 0 or accumulation == 0, name
+
+
+def vector_written_scalars(op, args):
+    """Scalar registers that a vector instruction writes."""
+    if op.startswith(("v_readfirstlane", "v_readlane", "v_cmp")):
+        return scalars(args[0])
+    if op.startswith(("v_mad_u64", "v_mad_i64", "v_div_scale", "v_add_co", "v_addc_co", "v_sub_co", "v_subb_co")):
+        return scalars(args[1])
+    return set()
+
+
+def scalars(operand):
+    one, many = re.fullmatch(r"s(\d+)", operand), re.fullmatch(r"s\[(\d+):(\d+)\]", operand)
+    return {int(one.group(1))} if one else set(range(int(many.group(1)), int(many.group(2)) + 1)) if many else set()
+
+
+def short_waits(lines, needed):
+    """Loads into LDS that read a scalar register less than `needed` wait states behind a vector instruction that wrote it; the hardware does not wait, and the
+    compiler, which does elsewhere, does not look into the assembly statements that these loads are written in."""
+    found, at_target = set(), {}
+    for _ in range(2):                                                  # twice: backward branches bring their state to labels that were passed
+        pending = {}                                                    # register: wait states since
+        for address, op, args, target in lines:
+            for register, age in at_target.get(address, {}).items():
+                pending[register] = min(age, pending.get(register, needed))
+            if op.startswith("buffer_load") and "lds" in args[-1].split():
+                if any(register in pending for register in scalars(args[1])):
+                    found.add(address)
+            states = int(args[0], 0) + 1 if op == "s_nop" else 1
+            pending = {register: age + states for register, age in pending.items() if age + states < needed}
+            for register in vector_written_scalars(op, args):
+                pending[register] = 0
+            if op.startswith("s_") and not op.startswith(("s_cmp", "s_cbranch", "s_nop", "s_waitcnt")) and args:
+                for register in scalars(args[0]):
+                    pending.pop(register, None)
+            if target is not None:
+                known = at_target.setdefault(target, {})
+                for register, age in pending.items():
+                    known[register] = min(age, known.get(register, needed))
+    return found
+
+
+def test_loads_into_lds_wait_for_their_descriptors(tmp_path):
+    metadata(tmp_path, b"attention_")
+    loads = 0
+    for path in tmp_path.glob("*.co"):
+        text = subprocess.run([llvm("llvm-objdump"), "-d", "--no-show-raw-insn", str(path)], check=True, capture_output=True, text=True).stdout
+        for function in re.split(r"\n[0-9a-f]+ <(?=\w)", text)[1:]:
+            name, lines, start = function.split(">", 1)[0], [], None
+            for line in function.splitlines()[1:]:
+                parsed = re.match(r"\s+(\w+)\s*(.*?)\s*// ([0-9A-F]+):(.*)$", line)
+                if not parsed:
+                    continue
+                op, rest, address, behind = parsed.groups()
+                address = int(address, 16)
+                start = address if start is None else start
+                jump = re.search(r"<[^>+]+(?:\+0x([0-9a-f]+))?>", behind) if op.startswith(("s_branch", "s_cbranch")) else None
+                args = [x.strip() for x in re.split(r",(?![^\[]*\])", rest)] if rest else [""]
+                lines.append((address, op, args, start + int(jump.group(1) or "0", 16) if jump else None))
+                loads += op.startswith("buffer_load") and "lds" in rest.split()
+            assert not short_waits(lines, 5), name
+    assert loads > 100
+
+
+def test_short_waits_are_found():
+    def program(*texts):
+        return [(4 * i, t.split(None, 1)[0], [x.strip() for x in re.split(r",(?![^\[]*\])", t.split(None, 1)[1])], None) for i, t in enumerate(texts)]
+    load = "buffer_load_dwordx4 v5, s[12:15], 0 offen lds"
+    assert short_waits(program("v_readfirstlane_b32 s13, v0", "s_mov_b32 m0, s3", "s_nop 0", load), 5) == {12}
+    assert short_waits(program("v_readlane_b32 s15, v0, 3", "s_nop 4", load), 5) == set()
+    assert short_waits(program("v_readfirstlane_b32 s16, v0", load), 5) == set()
+    assert short_waits(program("v_readfirstlane_b32 s13, v0", "s_mov_b32 s13, s2", load), 5) == set()
+    jump = program("s_nop 0", load, "v_readfirstlane_b32 s12, v0", "s_branch 0")
+    assert short_waits(jump[:3] + [(12, "s_branch", ["0"], 0)], 5) == {4}
