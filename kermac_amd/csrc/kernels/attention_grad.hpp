@@ -90,6 +90,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     constexpr int TILE = KT * AttLds<T, DP>::STRIDE;
     __shared__ __attribute__((aligned(1024))) att_lds_byte lds[4 * TILE];       // keys and values, two tiles of each
     __shared__ float shifts[128];               // with `large`, of the rows: not in a register that the loop holds
+    __shared__ int large_rows[4];               // of the waves
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int block = static_cast<int>(blockIdx.x) + args.first_block;
@@ -110,6 +111,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     const T *d = static_cast<const T *>(args.grad_out) + entry * args.grad_out_ls + token * args.grad_out_ms + head * args.grad_out_hs;
     const T *out = static_cast<const T *>(args.out) + entry * args.out_ls + token * args.out_ms + head * args.out_hs;
 
+    const float lse = args.lse[at];
     att_vec8<T> query[DP / 16], grad[DP / 16];
     float delta = 0.0f;
 #pragma unroll
@@ -124,16 +126,14 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
         for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(static_cast<float>(grad[step][j]), static_cast<float>(result[j]), delta);
     }
     delta = att_sum_of_halves(delta);
-    float lse2 = att_lse2(args.lse[at]), shift = 0.0f;
-    // whether one of the workgroup's 128 rows has a large lse: every wave looks at all of them
-    bool large = false;
-    if (args.row_shift)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int other = row_tile * 128 + 64 * j + lane;
-            const float lse = other < rows ? args.lse[(static_cast<i64>(entry) * args.m + other / args.r) * (static_cast<i64>(args.g) * args.r) + g * args.r + other % args.r] : 0.0f;
-            large = __any(!(fabsf(lse) < ATT_LARGEST_LSE) && lse != -__builtin_inff()) || large;
-        }
+    float lse2 = att_lse2(lse), shift = 0.0f;
+    bool large = false;                         // one of the workgroup's 128 rows has a large lse
+    if (args.row_shift) {
+        const bool mine = __any(!(fabsf(lse) < ATT_LARGEST_LSE) && lse != -__builtin_inff());
+        if (lane == 0) large_rows[wave] = mine;
+        __syncthreads();
+        large = __builtin_amdgcn_readfirstlane(large_rows[0] | large_rows[1] | large_rows[2] | large_rows[3]) != 0;
+    }
 
     const AttentionKeys &keys = args.keys;
     const int length = att_length(keys, entry);
@@ -166,21 +166,25 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
                     ds = att_mma(att_read_row<T, DP>(lds + TILE, 32 * b, 16 * step, lane), grad[step], ds);
                 }
                 const unsigned mine = static_cast<unsigned>(kept >> (32 * b)) >> (4 * half);
-                float block_top = -__builtin_inff();
+                float from = 0.0f, base = lse2;
+                if (large) {                            // weights relative to the largest score so far
+                    float block_top = -__builtin_inff();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) block_top = fmaxf(block_top, mine >> att_row(i, 0) & 1 ? s[i] : -__builtin_inff());
-                block_top = att_max_of_halves(block_top);
-                if (block_top > top) {
-                    const float shrink = __builtin_amdgcn_exp2f((top - block_top) * args.scale_log2);
-                    total *= shrink;
-                    inner *= shrink;
-                    top = block_top;
+                    for (int i = 0; i < 16; ++i) block_top = fmaxf(block_top, mine >> att_row(i, 0) & 1 ? s[i] : -__builtin_inff());
+                    block_top = att_max_of_halves(block_top);
+                    if (block_top > top) {
+                        const float shrink = __builtin_amdgcn_exp2f((top - block_top) * args.scale_log2);
+                        total *= shrink;
+                        inner *= shrink;
+                        top = block_top;
+                    }
+                    from = top == -__builtin_inff() ? 0.0f : top;
+                    base = 0.0f;
                 }
-                const float from = top == -__builtin_inff() ? 0.0f : top;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const bool counts = mine >> att_row(i, 0) & 1;
-                    const float p = counts ? __builtin_amdgcn_exp2f((s[i] - from) * args.scale_log2) : 0.0f;
+                    const float p = !counts ? 0.0f : length == 1 ? 1.0f : att_weight(s[i] - from, args.scale_log2, base);
                     total += p;
                     inner = counts ? __builtin_fmaf(p, ds[i], inner) : inner;
                 }
@@ -193,7 +197,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
         } else {
             delta = inner / total;
             shift = large ? top : 0.0f;
-            lse2 = large ? __builtin_amdgcn_logf(total) : __builtin_fmaf(top, args.scale_log2, __builtin_amdgcn_logf(total));
+            lse2 = (large ? 0.0f : lse2) + (length > 1 ? __builtin_amdgcn_logf(total) : 0.0f);
         }
     }
     if (lse2 == __builtin_inff()) delta = 0.0f;         // (no key: the gradient is 0 whatever that of the result is)
@@ -211,7 +215,7 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
     att_f32x16 acc[DP / 32];
 #pragma unroll
     for (int o = 0; o < DP / 32; ++o) acc[o] = att_f32x16{0};
-    if (large && half == 0) shifts[32 * wave + lane] = shift;
+    if ((DP > 128 || large) && half == 0) shifts[32 * wave + lane] = shift;
     int odd = 0;
     att_wait_for_loads();
     const i64 k_stride = keys.k_ns, v_stride = keys.v_ns;
@@ -257,18 +261,31 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
             att_two_scores<T, DP, ORDERED, false>(s, ds, block, query, value_tile + b * BLOCK, grad, lane, [](int) {});
             att_read_columns<T, DP>(f[0], block, 0, 0, lane);
             const unsigned here = static_cast<unsigned>(kept >> (32 * b));
-            if (large || here != ~0u) {
-                att_rare();
-                const unsigned rows = __builtin_amdgcn_readfirstlane(here);
-                if (large) s -= shifts[32 * wave + lane % 32];
+            if constexpr (DP > 128) {
+                // (a branch in front of the weights costs these kernels more than 16 subtractions: 526 us instead of 590 in fp32 of 256 features, 2 x 1000 x 1500 x 8 heads)
+                s -= shifts[32 * wave + lane % 32];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[i] = att_has_row(rows, i) ? s[i] : -__builtin_inff();
-                    ds[i] = att_has_row(rows, i) ? ds[i] : 0.0f;
+                for (int i = 0; i < 16; ++i) ds[i] = att_weight(s[i], scale_log2, lse2) * (ds[i] - delta);
+                if (here != ~0u) {
+                    att_rare();
+                    const unsigned rows = __builtin_amdgcn_readfirstlane(here);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) ds[i] = att_has_row(rows, i) ? ds[i] : 0.0f;
                 }
-            }
+            } else {
+                if (large || here != ~0u) {
+                    att_rare();
+                    const unsigned rows = __builtin_amdgcn_readfirstlane(here);
+                    if (large) s -= shifts[32 * wave + lane % 32];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) ds[i] = att_weight(s[i], scale_log2, lse2) * (ds[i] - delta);
+                    for (int i = 0; i < 16; ++i) {
+                        s[i] = att_has_row(rows, i) ? s[i] : -__builtin_inff();
+                        ds[i] = att_has_row(rows, i) ? ds[i] : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) ds[i] = att_weight(s[i], scale_log2, lse2) * (ds[i] - delta);
+            }
             x[0] = att_operand<T>(ds, 0);
             x[1] = att_operand<T>(ds, 1);
 #pragma unroll
@@ -355,11 +372,6 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
             for (int j = 0; j < 8; ++j) key[step][j] = static_cast<T>(static_cast<float>(key[step][j]) * args.query_factor);
         if (OF_KEYS) value[step] = att_load8<T, ALIGNED>(v, 16 * step + 8 * half, args.o);
     }
-    att_wait_for_loads();
-    att_f32x16 acc_k[DP / 32], acc_v[DP / 32];
-#pragma unroll
-    for (int o = 0; o < DP / 32; ++o) acc_k[o] = acc_v[o] = att_f32x16{0};
-
     // the rows: entries that share the keys, their heads, 32 queries at a time; this workgroup's part of them
     const int tiles_m = (args.m + RT - 1) / RT;
     const i64 per_entry = static_cast<i64>(args.r) * tiles_m;
@@ -369,11 +381,25 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
     const i64 part_first = split * per_split, part_last = part_first + per_split;
     const i64 rows_total = static_cast<i64>(args.l) * args.m * args.g * args.r;
     bool ever_kept = false;
+    // not 0 if a row of an entry and this head of keys has a shift
+    auto ask_large = [&](int e) {
+        int some = 0;
+        if (args.row_flags && e < entries)
+            for (int i = lane; i < args.q_row_tiles; i += 64) some |= args.row_flags[(static_cast<i64>(key_entry + e) * args.g + g) * args.q_row_tiles + i];
+        return some;
+    };
+    const int first_entry = static_cast<int>(part_first / per_entry);
+    int some_large = ask_large(first_entry);
+    att_wait_for_loads();
+    att_f32x16 acc_k[DP / 32], acc_v[DP / 32];
+#pragma unroll
+    for (int o = 0; o < DP / 32; ++o) acc_k[o] = acc_v[o] = att_f32x16{0};
 
-    for (int e = static_cast<int>(part_first / per_entry); e < entries && e * per_entry < part_last; ++e) {
+    for (int e = first_entry; e < entries && e * per_entry < part_last; some_large = ask_large(++e)) {
         const int entry = key_entry + e;
         const int first = static_cast<int>(part_first > e * per_entry ? part_first - e * per_entry : 0);
         const int count = static_cast<int>((part_last < (e + 1) * per_entry ? part_last - e * per_entry : per_entry) - first);
+        const bool large = __any(some_large != 0);
         const int length = att_length(keys, entry);
         const att_u64 kept_keys[2] = {att_kept_keys(keys, entry, first_key, length, lane), att_kept_keys(keys, entry, first_key + 64, length, lane)};
         if (!(kept_keys[0] | kept_keys[1])) continue;
@@ -382,10 +408,6 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD_K)) void 
         const bool kept = static_cast<unsigned>(kept_keys[wave >> 1] >> (32 * (wave & 1))) >> (lane & 31) & 1;
         const bool clear = entries > 1 && !__all(kept);
         ever_kept |= kept;
-        bool large = false;                                 // a row of this entry and head of keys has a shift
-        if (args.row_flags)
-            for (int i = 0; i < args.q_row_tiles; i += 64)
-                large = __any(i + lane < args.q_row_tiles && args.row_flags[(static_cast<i64>(entry) * args.g + g) * args.q_row_tiles + i + lane] != 0) || large;
 
         // What moves from tile to tile: addresses in scalar registers that grow by one of two steps.
         Tile next_q, next_d;
