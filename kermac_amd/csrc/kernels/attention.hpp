@@ -657,7 +657,8 @@ __device__ __forceinline__ void att_forward_write(const AttentionArgs &args, con
     if (job.partial) {
         const i64 slot = static_cast<i64>(job.slot + split) * args.rows_total + id;
         if (half == 0) {
-            args.partial_shift[slot] = sum == 0.0f ? -__builtin_inff() : state.shift;
+            // (-inf says that the part has no keys; one whose scores are all not a number has no shift either, and stays one)
+            args.partial_shift[slot] = sum == 0.0f ? -__builtin_inff() : state.shift == -__builtin_inff() ? 0.0f : state.shift;
             args.partial_lse[slot] = lse2;
         }
         if (sum == 0.0f) return;                                                    // nobody reads it

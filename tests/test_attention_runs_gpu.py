@@ -218,3 +218,22 @@ def test_more_rows_than_a_launch_of_the_join_holds(device):
     assert ((out[:, :-2].float() - shared[:, :-2].float()).abs() <= far).all()
     last = kermac.prefix_attention(q[:, -2:].contiguous(), pk, pv, k, v, lengths)
     assert ((out[:, -2:].float() - last.float()).abs() <= 2 * reference.UNIT[torch.float16] * max(pv.float().abs().max(), v.float().abs().max())).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M, N", [(3, 5000), (200, 3001)])
+def test_not_a_number_stays_in_parts(device, dtype, M, N):
+    """Rows whose scores are all NaN, in every part that the keys are cut into, and keys whose score is NaN or infinite in one of them."""
+    q, k, v = operands(2, M, N, 2, 2, 64, 64, dtype, device)
+    q[0, 1] = math.nan
+    names = kernels_of(lambda: kermac.cross_attention(q, k, v))
+    assert any("attention_join" in name for name in names)
+    out, lse = kermac.cross_attention(q, k, v, return_lse=True)
+    assert out[0, 1].isnan().all() and lse[0, 1].isnan().all() and out.isnan().sum() == 2 * 64
+    prefixed = kermac.prefix_attention(q, k[0], v[0], k, v, torch.zeros(2, dtype=torch.int32, device=device))
+    assert prefixed[0, 1].isnan().all() and prefixed.isnan().sum() == 2 * 64
+    q[0, 1] = 1.0
+    for value in (math.nan, math.inf):
+        k[1, N - 2] = value                     # (infinity: the scores of the entry's rows are infinities of their sums' signs, or NaN)
+        out = kermac.cross_attention(q.abs() + 0.1, k, v)
+        assert out[1].isnan().all() and not out[0].isnan().any()
