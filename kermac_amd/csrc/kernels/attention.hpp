@@ -13,8 +13,8 @@
 // row of the softmax (two lanes, for alternating groups of four keys), its statistics are one register each, and the
 // registers that hold s^T are, in the order in which they stand, the operand of out^T[o, row] = V^T P^T if the
 // contraction takes the keys of a step as 4 h + {0..3}, 8 + 4 h + {0..3} for half wave h.  V^T comes from row-major tiles in
-// LDS by the transposing read (16-bit types) or by 32-bit reads (fp32).  P is rounded to the type of the values: the error of
-// a sum of many rounded weights stays below the rounding of the result itself; fp32 keeps every bit.
+// LDS by the transposing read (16-bit types) or by 32-bit reads (fp32).  P is rounded to the type of the values, half a step per
+// weight, which leaves about as large an error in the result as its own rounding does (bf16, 8 x 4096 x 8192: 2.3e-3 in all, 1.7e-3 where weights stay in 32 bits); fp32 keeps every bit.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -611,7 +611,7 @@ struct AttForwardShape {
     // Waves with keys of their own.
     static constexpr int OWN_KEYS = 32;
     // Rows of 1 KB: two tiles for every wave do not fit LDS, and half of the waves would leave half of the matrix cores idle, which in fp32 take longer than
-    // the memory.  Keys and values take turns in one tile then (1 token x 20000 keys x 8 heads of 256 fp32: 136 us, with two waves of two tiles 151).
+    // the memory.  Keys and values take turns in one tile then (1 token x 20000 keys x 8 heads of 256 fp32: 125 us, with two waves of two tiles 10 % more).
     static constexpr bool OWN_TURNS = ROW_BYTES > 512;
     static constexpr int OWN_BYTES = (OWN_TURNS ? 1 : 2) * WAVES * OWN_KEYS * ROW_BYTES;
     static constexpr int JOIN_BYTES = (WAVES - 1) * (DP * 32 + 64) * 4 + 256 * WAVES;
@@ -698,16 +698,16 @@ __device__ __forceinline__ void att_load_queries(const AttentionArgs &args, cons
 
 // A workgroup per (batch entry, head of keys, range of keys, tile of rows).
 //
-// More than 32 rows: WAVES waves of 32 rows each share the tiles of keys and values.  Bound by the matrix cores, which what feeds them keeps from their
-// rate: with 128 features in 16 bits, the fragments of keys and values that a wave reads from LDS take as long as the products that it makes of them.
-// 8 entries x 4096 queries x 8192 keys x 32 heads on 8 x 128 bf16: 4.0 ms, 1.1 PFLOP/s (the matrix cores are busy half of the time; a large
+// More than 32 rows: WAVES waves of 32 rows each share the tiles of keys and values.  With 128 features in 16 bits the matrix cores are busy 52 % of the time, under
+// the power limit, vector instructions and reads of LDS take the rest of a wave's turn.
+// 8 entries x 4096 queries x 8192 keys x 32 heads on 8 x 128 bf16: 4.1 ms, 1.1 PFLOP/s (a large
 // bf16 matrix product of the library's reaches 1.24).  Measured and left out: 64 rows per wave (half the reads from LDS, one wave per SIMD: 7.0 ms), 8
-// waves that share a tile (the same time), tiles of 32 keys in deeper rings (4.8 ms).  fp32 is bound by its products: 72 useful TFLOP/s of 154 at
-// 2 x 1000 x 2900 x 8 heads of 64, of which 80 % of the keys take part.
+// waves that share a tile (the same time), tiles of 32 keys in deeper rings (4.8 ms).  fp32: 72 useful TFLOP/s of 154 at
+// 2 x 1000 x 2900 x 8 heads of 64, of which 80 % of the keys take part; the matrix cores are busy 64 % of the time.
 //
 // At most 32 rows (single tokens): reading keys and values is all the work, so every wave walks tiles of its own without waiting for the others,
-// and the waves' results are joined at the end.  32 entries x 1 query x up to 4000 keys x 16 heads of 64 bf16: 89 us, 4.4 TB/s (a large copy
-// reaches 4.8); 4 x 32768 keys x 16 heads of 128: 194 us, 5.5 TB/s.
+// and the waves' results are joined at the end.  32 entries x 1 query x up to 4000 keys x 16 heads of 64 bf16: 90 us, 4.4 TB/s (a large copy
+// reaches 4.8); 4 x 32768 keys x 16 heads of 128: 192 us, 5.6 TB/s.
 template <typename T, int DP, bool ALIGNED, bool ORDERED = ATT_ORDERED<T, DP, ALIGNED>>
 __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void attention_forward(const AttentionArgs args)
 {
@@ -718,7 +718,7 @@ __global__ __launch_bounds__(256, (AttForwardShape<T, DP>::WAVES_PER_SIMD)) void
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     // The prefix's workgroups come first: they are bound by the matrix cores and are about as many as fit the chip at most, so those of the sequences'
-    // own keys, bound by memory, run beside and behind them (128 sequences behind 65536 tokens: 233 us, with the two kinds alternating 276).
+    // own keys, bound by memory, run beside and behind them (128 sequences behind 65536 tokens, before other steps: 233 us, with the two kinds alternating 276; now 210).
     // XCD x gets a contiguous part of a job's list, in which the tiles of rows of one set of keys stand together: they share its L2.
     int id = static_cast<int>(blockIdx.x) + args.first_block;
     const bool second = id >= args.job[0].grid;

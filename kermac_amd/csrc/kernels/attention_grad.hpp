@@ -81,7 +81,7 @@ __device__ __forceinline__ void att_two_scores(att_f32x16 &s, att_f32x16 &ds, co
 }
 
 // A workgroup per (batch entry, head of keys, range of keys, 128 rows); a wave per 32 rows, whose queries and gradients it keeps in registers.
-// Three products, two of which share what is read of a tile: 1.45 ms at 4 x 4096 x 4096, 32 heads on 8 x 128 bf16, the matrix cores busy 60 % of the time.
+// Three products, two of which share what is read of a tile: 1.47 ms at 4 x 4096 x 4096, 32 heads on 8 x 128 bf16, the matrix cores busy 59 % of the time.
 template <typename T, int DP, bool ALIGNED, bool ORDERED = ATT_ORDERED<T, DP, ALIGNED>>
 __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void attention_grad_queries(const AttentionGradArgs args)
 {
@@ -321,13 +321,13 @@ __global__ __launch_bounds__(256, (AttGradShape<T, DP>::WAVES_PER_SIMD)) void at
 // Turn i: the scores of tile i + 1 (32 rows) on the matrix cores while the vector units make the weights and gradients of tile i from its scores, then
 // the two products of tile i.  Behind the buffers of these two tiles stand as many as fit for those on their way: the workgroups of a head walk its rows in step,
 // so every tile comes from far, and one turn is shorter than that takes (4 x 4096 x 4096, 32 heads on 8 x 128 bf16: 4.2 ms with one tile on its way, 2.6
-// with four; one wave per SIMD, whose 64 KB of keys, values and their gradients fill its registers; the matrix cores are busy 40 % of the time).  What
-// bounds it with 128 features is LDS: every wave reads each tile twice by rows and twice by columns, as long as its products take.  Waves with 64 keys
-// would halve that, and have no registers for it (3.4 ms, with spills whose reloads wait for the tiles on their way); a barrier after two tiles instead of
-// one changes nothing.  With 64 features it is the vector work: 8 x 1000 x 1500 keys at most x 16 heads 113 us.
+// with four; one wave per SIMD, whose 64 KB of keys, values and their gradients fill its registers).  What bounds it with 128 features is that one wave's work follows
+// its own: the matrix cores are busy 39 % of the time, LDS, of which every wave reads each tile twice by rows and twice by columns, 24 %, vector instructions 29 %.
+// Waves with 64 keys would halve the reads, and have no registers for it (3.4 ms, with spills whose reloads wait for the tiles on their way); a barrier after two
+// tiles instead of one changes nothing.  With 64 features, 8 x 1000 x 1500 keys at most x 16 heads, 115 us: the matrix cores are busy 23 % of the time, vector instructions 28 %.
 //
 // In fp32, 32 keys and values of more than 128 features and their gradients are 512 registers by themselves.  There a launch makes one of the two gradients, and
-// the scores are computed twice (2 x 1000 x 1500 x 8 heads of 256: 814 us for both, 1180 in one launch with its spills).
+// the scores are computed twice (2 x 1000 x 1500 x 8 heads of 256: 800 us for both, 1180 in one launch with its spills).
 enum AttKeysPart { ATT_BOTH, ATT_GRAD_KEYS, ATT_GRAD_VALUES };
 
 template <typename T, int DP, bool ALIGNED, AttKeysPart PART, bool ORDERED = ATT_ORDERED<T, DP, ALIGNED>>
