@@ -228,8 +228,9 @@ def cross_attention(
         return_lse: also return ``log sum exp`` of every row, fp32 ``[L, M, H]``, for ``cross_attention_grad``.
 
     What keys and values hold where they do not take part does not matter, infinities and NaN included.  A row
-    without a key (or with scores of -inf alone) gets zeros, and -inf for its ``lse``.  Returns ``out`` (allocated
-    ``[L, M, H, O]`` when None), or ``(out, lse)``.
+    without a key (or with scores of -inf alone) gets zeros, and -inf for its ``lse``, which no other row has: one below fp32's
+    numbers is the lowest of them.  Scores of any size give a softmax, with all the weight on the largest where they are far apart.  Returns ``out``
+    (allocated ``[L, M, H, O]`` when None), or ``(out, lse)``.
 
     Raises:
         TypeError: non-tensor inputs or a wrong dtype.
